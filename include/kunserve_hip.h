@@ -218,6 +218,35 @@ int kunserve_rope_append_kv(const kunserve_kv_pool* pool, int32_t layer,
                             const float* inv_freq_dev, int32_t interleave,
                             kunserve_stream_t stream);
 
+/* Rotary embedding of the first rotary_dim dims of a head: pair j is turned by
+ * position * freq_dev[j] radians (rotary_dim / 2 fp64 frequencies, angles formed
+ * in 64 bits) and scaled by `scale`. Pairs are (j, j + rotary_dim / 2), or
+ * (2j, 2j + 1) when interleave is non-zero. rotary_dim: a multiple of 16 up
+ * to head_dim. No reference counterpart (see kunserve_rope_append_kv). */
+typedef struct {
+  const double* freq_dev;
+  int32_t rotary_dim;
+  int32_t interleave;
+  float scale;
+} kunserve_rotary;
+
+/* kunserve_rope_append_kv with rotary frequencies of this form and positions
+ * apart from the cache: token i of the step is rotated at positions_dev[i]
+ * (int32 [num_tokens]; NULL: at its place in the cache, kv_len[b] - q_len[b] +
+ * i) and appended at its place in the cache. The rotated q goes to q_out, which
+ * is q itself (in place) or apart from q, k_new and v_new. Tokens of no row
+ * are left as they are. */
+int kunserve_rotary_append_kv(const kunserve_kv_pool* pool, int32_t layer,
+                              const kunserve_page_table* table,
+                              const int32_t* q_indptr_dev, int32_t num_tokens,
+                              const kunserve_tensor3* q, kunserve_tensor3* q_out,
+                              int32_t num_qo_heads,
+                              const kunserve_tensor3* k_new,
+                              const kunserve_tensor3* v_new,
+                              const kunserve_rotary* rotary,
+                              const int32_t* positions_dev,
+                              kunserve_stream_t stream);
+
 /* ---------------------------------------------- decode attention (A4) */
 
 typedef struct {
@@ -310,6 +339,47 @@ int kunserve_paged_decode_noalloc(const kunserve_kv_pool* pool, int32_t layer,
                                   const kunserve_decode_plan_info* info,
                                   kunserve_stream_t stream);
 
+/* --------------------------- decode attention of rows that share pages */
+
+typedef struct {
+  kunserve_decode_plan_info decode; /* what the rows hold for themselves, and
+                                       the joining of all partials           */
+  int32_t num_shared;    /* work records of shared pages (incl. padding)      */
+  int32_t tiles;         /* 16-column tiles of a workgroup                    */
+  int32_t num_pairs;     /* (row, first partial) records                      */
+  int32_t num_segments;  /* runs of pages that several rows share             */
+  int32_t head_dim;      /* head_dim the plan was made for                    */
+  int32_t plan_ints;     /* int32 entries of the plan buffer in use           */
+} kunserve_shared_plan_info;
+
+/* Upper bound of the plan buffer length (int32 entries) for these lengths. */
+int64_t kunserve_shared_plan_bound(const int32_t* kv_len_host, int32_t num_seqs);
+
+/* Host-side plan of decode rows whose page lists (CSR, host arrays) may begin
+ * with the same ids: every run of at least 64 tokens of whole pages that two
+ * or more rows hold at the same place, before their new tokens' pages, is read
+ * once for those rows (a prefix tree: rows may share a prefix of a prefix).
+ * Rows that share nothing are planned as by kunserve_decode_plan_grouped. */
+int kunserve_shared_plan(const int32_t* indptr_host, const int32_t* indices_host,
+                         const int32_t* kv_len_host, int32_t num_seqs,
+                         int32_t num_qo_heads, int32_t num_kv_heads,
+                         int32_t page_size, int32_t head_dim, int32_t num_cus,
+                         int32_t* plan_host, int64_t plan_capacity,
+                         kunserve_shared_plan_info* info);
+
+/* kunserve_paged_decode on such a plan, for the table it was made from (other
+ * ids or lengths: not this plan). The workspace is 16-byte aligned and holds
+ * kunserve_decode_workspace_bytes of info->decode. */
+int kunserve_shared_decode(const kunserve_kv_pool* pool, int32_t layer,
+                           const kunserve_page_table* table,
+                           const int32_t* q_token_dev,
+                           const kunserve_tensor3* q, kunserve_tensor3* out,
+                           int32_t num_qo_heads, float sm_scale,
+                           const int32_t* plan_dev,
+                           const kunserve_shared_plan_info* info,
+                           void* workspace_dev, int64_t workspace_bytes,
+                           kunserve_stream_t stream);
+
 /* ------------------------------------- chunked-prefill attention (A5 ii) */
 
 typedef struct {
@@ -395,6 +465,74 @@ int kunserve_paged_prefill(const kunserve_kv_pool* pool, int32_t layer,
                            void* workspace_dev, int64_t workspace_bytes,
                            kunserve_stream_t stream);
 
+/* -------------------------- attention weights of the cache, eviction */
+
+/* Accumulated attention weight of every cached token and KV head (device,
+ * fp32): element (page, layer, kv_head, slot) lies at page*page_stride +
+ * layer*layer_stride + kv_head*head_stride + slot, for the pages of a pool. */
+typedef struct {
+  float* w;
+  int64_t page_stride;
+  int64_t layer_stride;
+  int64_t head_stride;
+} kunserve_kv_weights;
+
+typedef struct {
+  int64_t num_columns;   /* workspace entries (8 bytes each)                  */
+  int32_t num_items;     /* work records (row, partition)                     */
+  int32_t num_combines;  /* records of the columns' combination               */
+  int32_t window;        /* observers of a row at most                        */
+  int32_t num_qo_heads;  /* heads the plan was made for                       */
+  int32_t plan_ints;     /* int32 entries of the plan buffer in use           */
+} kunserve_weights_plan_info;
+
+/* Upper bound of the plan buffer length (int32 entries). */
+int64_t kunserve_weights_plan_bound(const int32_t* q_indptr_host,
+                                    const int32_t* kv_len_host, int32_t num_seqs,
+                                    int32_t num_qo_heads, int32_t window);
+
+/* Host-side plan of kunserve_cache_weights, shared by every layer of a step. */
+int kunserve_weights_plan(const int32_t* q_indptr_host, const int32_t* kv_len_host,
+                          int32_t num_seqs, int32_t num_qo_heads, int32_t window,
+                          int32_t* plan_host, int64_t plan_capacity,
+                          kunserve_weights_plan_info* info);
+
+int64_t kunserve_weights_workspace_bytes(const kunserve_weights_plan_info* info);
+
+/* What a step's attention says of the cache: for every row b with new tokens,
+ * cached token t and KV head g,
+ *   w := (t new ? 0 : w) + sum of softmax(q . K^T * sm_scale)[t]
+ * over the last min(q_len[b], window) new tokens of the row that see t (their
+ * positions are t or later) and the query heads of g. The step's K is in its
+ * pages already and q rotated. No page may be in two places of the table. Slots
+ * past a row's end and pages outside the pool are left as they are. */
+int kunserve_cache_weights(const kunserve_kv_pool* pool,
+                           const kunserve_kv_weights* weights, int32_t layer,
+                           const kunserve_page_table* table,
+                           const int32_t* q_indptr_dev, const kunserve_tensor3* q,
+                           int32_t num_qo_heads, float sm_scale,
+                           const int32_t* plan_dev,
+                           const kunserve_weights_plan_info* info,
+                           void* workspace_dev, int64_t workspace_bytes,
+                           kunserve_stream_t stream);
+
+/* Eviction: of row b, in every layer and KV head, the first `sinks` cached
+ * tokens, the last `recent` ones and the heaviest of those between stay, keep[b]
+ * in all (device int32; kv_len[b] and max_keep at most; below sinks + recent
+ * the first ones come first; equal weights: the lowest index; NaN: below every
+ * number). Their K, V and weights are copied in their order to the pages
+ * out_indices[out_indptr[b]..], slots 0, 1, .., which must not be pages of the
+ * table nor twice in the list; slots behind the last kept one are left as they
+ * are. kept (int32 [num_seqs][num_layers][num_kv_heads][kept_stride]) receives
+ * the kept tokens' indices, -1 behind the last. Of pages outside the pool a
+ * source counts as NaN and gives zeros, a destination is not written. */
+int kunserve_evict(const kunserve_kv_pool* pool, const kunserve_kv_weights* weights,
+                   const kunserve_page_table* table, const int32_t* out_indptr_dev,
+                   const int32_t* out_indices_dev, const int32_t* keep_dev,
+                   int32_t max_keep, int32_t sinks, int32_t recent,
+                   int32_t* kept_dev, int64_t kept_stride,
+                   kunserve_stream_t stream);
+
 /* ------------------------------------------------ a step's layers */
 
 /* One step of a batch (kunserve/worker.py:270-312), shared by its layers:
@@ -467,6 +605,32 @@ int kunserve_tensors_overlap(const kunserve_tensor3* a, int32_t heads_a,
 int kunserve_attention_step(const kunserve_step* step, int32_t layer,
                             const kunserve_step_io* io,
                             kunserve_stream_t stream);
+
+/* What a step may have beside kunserve_step. shared_info.num_segments > 0: the
+ * decode rows share pages, and run by this plan (shared_plan_dev) in place of
+ * decode_plan_dev and without counters. weights.w not NULL: the attention
+ * weights of the whole step's rows are added by this plan, after the attention,
+ * in the workspace weights_workspace_dev; the step's pages are then private,
+ * each in one place of the table. positions_dev (may be NULL): the tokens'
+ * rotary positions (kunserve_rotary_append_kv). */
+typedef struct {
+  const int32_t* shared_plan_dev;
+  kunserve_shared_plan_info shared_info;
+  kunserve_kv_weights weights;
+  const int32_t* weights_plan_dev;
+  kunserve_weights_plan_info weights_info;
+  void* weights_workspace_dev;
+  int64_t weights_workspace_bytes;
+  const int32_t* positions_dev;
+} kunserve_step_extras;
+
+/* kunserve_attention_step with extras (may be NULL). rotary (may be NULL):
+ * kunserve_rotary_append_kv, q in place, in place of io's frequencies. */
+int kunserve_attention_step_with(const kunserve_step* step,
+                                 const kunserve_step_extras* extras, int32_t layer,
+                                 const kunserve_step_io* io,
+                                 const kunserve_rotary* rotary,
+                                 kunserve_stream_t stream);
 
 /* MFMA calibration (no reference counterpart): each of num_workgroups
  * workgroups runs 8 waves (two per SIMD) of `iterations` rounds of two

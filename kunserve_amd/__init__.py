@@ -14,16 +14,21 @@ import types
 import torch
 
 from . import _lib
+from .cache_weights import KVWeights, WeightsPlan, add_weights, evict
 from .llama_op import LlamaOp, kept_layers
-from .paged_kv import (AttentionStep, DecodePlan, KVPool, PageTable, PrefillPlan, append_kv,
-                       copy_blocks, csr_from_lists, kv_lens_for_step, kv_pack, kv_scatter,
-                       paged_decode, paged_prefill, rope_append_kv, rope_inv_freq, swap)
+from .paged_kv import (AttentionStep, DecodePlan, KVPool, PageTable, PrefillPlan,
+                       SharedDecodePlan, append_kv, copy_blocks, csr_from_lists,
+                       kv_lens_for_step, kv_pack, kv_scatter, paged_decode, paged_prefill,
+                       rope_append_kv, rope_inv_freq, rotary_append_kv, shared_decode, swap)
 from .pmm import PmmPool
+from .rotary import Rotary, rotary_frequencies
 
 __all__ = [
-    "AttentionStep", "DecodePlan", "KVPool", "LlamaOp", "PageTable", "PmmPool", "PrefillPlan",
-    "append_kv", "copy_blocks", "csr_from_lists", "kv_lens_for_step", "kv_pack",
-    "kept_layers", "kv_scatter", "paged_decode", "paged_prefill", "rope_append_kv", "rope_inv_freq", "swap",
+    "AttentionStep", "DecodePlan", "KVPool", "KVWeights", "LlamaOp", "PageTable", "PmmPool",
+    "PrefillPlan", "Rotary", "SharedDecodePlan", "WeightsPlan", "add_weights", "append_kv",
+    "copy_blocks", "csr_from_lists", "evict", "kv_lens_for_step", "kv_pack", "kept_layers",
+    "kv_scatter", "paged_decode", "paged_prefill", "rope_append_kv", "rope_inv_freq",
+    "rotary_append_kv", "rotary_frequencies", "shared_decode", "swap",
     "library_path",
 ]
 

@@ -76,6 +76,36 @@ class Step(Structure):
     ]
 
 
+class SharedPlanInfo(Structure):
+    _fields_ = [("decode", DecodePlanInfo), ("num_shared", c_int32), ("tiles", c_int32),
+                ("num_pairs", c_int32), ("num_segments", c_int32), ("head_dim", c_int32),
+                ("plan_ints", c_int32)]
+
+
+class KVWeights(Structure):
+    _fields_ = [("w", c_void_p), ("page_stride", c_int64), ("layer_stride", c_int64),
+                ("head_stride", c_int64)]
+
+
+class WeightsPlanInfo(Structure):
+    _fields_ = [("num_columns", c_int64), ("num_items", c_int32), ("num_combines", c_int32),
+                ("window", c_int32), ("num_qo_heads", c_int32), ("plan_ints", c_int32)]
+
+
+class Rotary(Structure):
+    _fields_ = [("freq_dev", c_void_p), ("rotary_dim", c_int32), ("interleave", c_int32),
+                ("scale", c_float)]
+
+
+class StepExtras(Structure):
+    _fields_ = [
+        ("shared_plan_dev", c_void_p), ("shared_info", SharedPlanInfo), ("weights", KVWeights),
+        ("weights_plan_dev", c_void_p), ("weights_info", WeightsPlanInfo),
+        ("weights_workspace_dev", c_void_p), ("weights_workspace_bytes", c_int64),
+        ("positions_dev", c_void_p),
+    ]
+
+
 # kunserve_step_io as packed bytes: (data, token stride, head stride) of q, k,
 # v and out, inv_freq, interleave. Cheaper to fill per layer than a Structure.
 STEP_IO = struct.Struct("@12qqi4x")
@@ -102,6 +132,29 @@ SIGNATURES = {
     "kunserve_rope_append_kv": (c_int, [POINTER(KVPool), c_int32, POINTER(PageTable), c_void_p,
                                         c_int32, POINTER(Tensor3), c_int32, POINTER(Tensor3),
                                         POINTER(Tensor3), c_void_p, c_int32, c_void_p]),
+    "kunserve_rotary_append_kv": (c_int, [POINTER(KVPool), c_int32, POINTER(PageTable), c_void_p,
+                                          c_int32, POINTER(Tensor3), POINTER(Tensor3), c_int32,
+                                          POINTER(Tensor3), POINTER(Tensor3), POINTER(Rotary),
+                                          c_void_p, c_void_p]),
+    "kunserve_shared_plan_bound": (c_int64, [c_void_p, c_int32]),
+    "kunserve_shared_plan": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,
+                                     c_int32, c_int32, c_int32, c_void_p, c_int64,
+                                     POINTER(SharedPlanInfo)]),
+    "kunserve_shared_decode": (c_int, [POINTER(KVPool), c_int32, POINTER(PageTable), c_void_p,
+                                       POINTER(Tensor3), POINTER(Tensor3), c_int32, c_float,
+                                       c_void_p, POINTER(SharedPlanInfo), c_void_p, c_int64,
+                                       c_void_p]),
+    "kunserve_weights_plan_bound": (c_int64, [c_void_p, c_void_p, c_int32, c_int32, c_int32]),
+    "kunserve_weights_plan": (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p,
+                                      c_int64, POINTER(WeightsPlanInfo)]),
+    "kunserve_weights_workspace_bytes": (c_int64, [POINTER(WeightsPlanInfo)]),
+    "kunserve_cache_weights": (c_int, [POINTER(KVPool), POINTER(KVWeights), c_int32,
+                                       POINTER(PageTable), c_void_p, POINTER(Tensor3), c_int32,
+                                       c_float, c_void_p, POINTER(WeightsPlanInfo), c_void_p,
+                                       c_int64, c_void_p]),
+    "kunserve_evict": (c_int, [POINTER(KVPool), POINTER(KVWeights), POINTER(PageTable), c_void_p,
+                               c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_int64,
+                               c_void_p]),
     "kunserve_decode_plan_bound": (c_int64, [c_void_p, c_int32]),
     "kunserve_decode_plan": (c_int, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
                                      c_void_p, c_int64, POINTER(DecodePlanInfo)]),
@@ -137,6 +190,8 @@ SIGNATURES = {
     "kunserve_tensors_overlap": (c_int, [POINTER(Tensor3), c_int32, POINTER(Tensor3), c_int32,
                                          c_int32, c_int32]),
     "kunserve_attention_step": (c_int, [POINTER(Step), c_int32, c_void_p, c_void_p]),
+    "kunserve_attention_step_with": (c_int, [POINTER(Step), POINTER(StepExtras), c_int32, c_void_p,
+                                             POINTER(Rotary), c_void_p]),
     "kunserve_fused_pool": (c_int, [POINTER(KVPool), c_int64, c_int32, POINTER(KVPool)]),
     "kunserve_fused_page_ids": (c_int, [c_void_p, c_int64, c_int64, c_int32, c_int64,
                                         c_void_p]),

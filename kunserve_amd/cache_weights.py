@@ -1,0 +1,164 @@
+"""What attention says of the cache, and the cache made shorter by it.
+
+KVWeights holds, for every cached token and KV head, the attention weight that
+it got so far; steps made with it (AttentionStep(weights=...)) add to it. evict
+keeps the heaviest tokens of a request in pages of their own. The reference has
+no counterpart: its block manager frees whole requests
+(kunserve/block_manager.py:493-500).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Sequence, Union
+
+import numpy as np
+import torch
+
+from . import _lib
+from .paged_kv import (KVPool, PageTable, _i32, _ptr, _stream_ptr, _tensor3,
+                       _upload_packed, csr_from_lists)
+
+
+class KVWeights:
+    """Accumulated attention weights of a pool's tokens: w [num_pages, num_layers,
+    num_kv_heads, page_size], float32 with the slots contiguous. A new token's
+    weight starts at 0 in the step that appends it, so nothing has to be cleared
+    when pages are used again."""
+
+    def __init__(self, pool: KVPool, w: Optional[torch.Tensor] = None):
+        shape = (pool.num_pages, pool.num_layers, pool.num_kv_heads, pool.page_size)
+        if w is None:
+            w = torch.zeros(shape, dtype=torch.float32, device=pool.device)
+        if (tuple(w.shape) != shape or w.dtype != torch.float32 or w.stride(-1) != 1
+                or w.device != pool.device):
+            raise ValueError(f"weights must be float32 {shape} on {pool.device} with the slots "
+                             "contiguous")
+        self.w = w
+        self._desc = _lib.KVWeights(w.data_ptr(), w.stride(0), w.stride(1), w.stride(2))
+
+    def check(self, pool: KVPool) -> None:
+        shape = (pool.num_pages, pool.num_layers, pool.num_kv_heads, pool.page_size)
+        if tuple(self.w.shape) != shape or self.w.device != pool.device:
+            raise ValueError(f"the weights {tuple(self.w.shape)} on {self.w.device} are not those "
+                             f"of a pool {shape} on {pool.device}")
+
+    def plan(self, q_indptr_host, kv_len_host, num_qo_heads: int, window: int) -> "WeightsPlan":
+        """The plan of a step's rows, not yet on the device (WeightsPlan.bind)."""
+        return WeightsPlan(q_indptr_host, kv_len_host, num_qo_heads, window, self.w.device,
+                           upload=False)
+
+    def add(self, pool: KVPool, layer: int, table: PageTable, q_indptr: torch.Tensor,
+            q: torch.Tensor, plan: "WeightsPlan", sm_scale: Optional[float] = None,
+            workspace: Optional[torch.Tensor] = None) -> None:
+        """add_weights to these weights."""
+        add_weights(pool, self, layer, table, q_indptr, q, plan, sm_scale, workspace)
+
+
+class WeightsPlan:
+    """Work of add_weights for a step's rows, computed on the host once per step and
+    shared by every layer (kunserve_weights_plan)."""
+
+    def __init__(self, q_indptr_host: Sequence[int], kv_len_host: Sequence[int],
+                 num_qo_heads: int, window: int, device: torch.device, upload: bool = True):
+        qi, kv = _i32(q_indptr_host), _i32(kv_len_host)
+        n = len(kv)
+        if len(qi) != n + 1:
+            raise ValueError("q_indptr must have num_seqs + 1 entries")
+        kv_ptr = kv.ctypes.data if n else None
+        cap = int(_lib.lib().kunserve_weights_plan_bound(qi.ctypes.data, kv_ptr, n, num_qo_heads,
+                                                         window))
+        buf = np.empty(max(cap, 4), dtype=np.int32)   # the plan writes what it uses
+        self.info = _lib.WeightsPlanInfo()
+        _lib.call("kunserve_weights_plan", qi.ctypes.data, kv_ptr, n, num_qo_heads, window,
+                  buf.ctypes.data, buf.size, ctypes.byref(self.info))
+        self.plan_host = buf[: self.info.plan_ints].copy()
+        self.plan = None
+        if upload:
+            self.bind(_upload_packed(self.host_arrays(), device))
+
+    def host_arrays(self) -> list:
+        return [self.plan_host]
+
+    def bind(self, dev: Sequence[torch.Tensor]) -> None:
+        self.plan = dev[0] if self.info.plan_ints else None
+
+    def workspace_bytes(self) -> int:
+        return int(_lib.lib().kunserve_weights_workspace_bytes(ctypes.byref(self.info)))
+
+
+def add_weights(pool: KVPool, weights: KVWeights, layer: int, table: PageTable,
+                q_indptr: torch.Tensor, q: torch.Tensor, plan: WeightsPlan,
+                sm_scale: Optional[float] = None,
+                workspace: Optional[torch.Tensor] = None) -> None:
+    """Adds to `weights` what the last new tokens of every row attend to
+    (kunserve_cache_weights): q [num_tokens, Hq, D] after its rotation, the step's
+    K in its pages. No page may be in two places of the table."""
+    weights.check(pool)
+    if q.shape[2] != pool.head_dim:
+        raise ValueError(f"q shape {tuple(q.shape)} does not match head_dim {pool.head_dim}")
+    if q_indptr.numel() != table.num_seqs + 1:
+        raise ValueError("q_indptr must have num_seqs + 1 entries")
+    pool.check_dtype(q)
+    scale = sm_scale if sm_scale is not None else 1.0 / math.sqrt(pool.head_dim)
+    need = plan.workspace_bytes()
+    if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=pool.device)
+    qd = _tensor3(q)
+    _lib.call("kunserve_cache_weights", pool.desc(), ctypes.byref(weights._desc), layer,
+              table.desc(), q_indptr.data_ptr(), ctypes.byref(qd), q.shape[1],
+              ctypes.c_float(scale), _ptr(plan.plan), ctypes.byref(plan.info), _ptr(workspace),
+              0 if workspace is None else workspace.numel() * workspace.element_size(),
+              _stream_ptr(pool.device))
+
+
+def evict(pool: KVPool, weights: KVWeights, pages_of_reqs: Sequence[Sequence[int]],
+          kv_lens: Sequence[int], pages_out: Sequence[Sequence[int]],
+          budget: Union[int, Sequence[int]], sinks: int = 4, recent: int = 0) -> torch.Tensor:
+    """Shortens the cache of requests to `budget` tokens each (one number, or one
+    per request; a request that has no more keeps all): in every layer and KV head
+    the first `sinks`, the last `recent` and the heaviest of the tokens between
+    stay (equal weights: the lowest index), in their order. Their K, V and weights
+    are copied to pages_out, ceil(tokens / page_size) pages per request that are
+    no pages of the requests; the old pages are the caller's to free once the
+    stream has passed this call.
+
+    The shortened request goes on with min(budget, kv_len) cached tokens, its
+    positions where they were (AttentionStep(rope_positions=...)). Returns the
+    indices kept, int32 [requests, layers, kv_heads, most kept], -1 behind a
+    request's last."""
+    weights.check(pool)
+    kv = np.asarray(kv_lens, dtype=np.int64).reshape(-1)
+    n = len(kv)
+    if len(pages_of_reqs) != n or len(pages_out) != n:
+        raise ValueError(f"{n} kv lengths but {len(pages_of_reqs)} and {len(pages_out)} page lists")
+    budget = np.asarray(budget, dtype=np.int64)
+    if budget.ndim > 1 or (budget.ndim == 1 and len(budget) != n):
+        raise ValueError(f"budget must be one number or one per request ({n})")
+    if np.any(budget < 0) or np.any(kv < 0) or sinks < 0 or recent < 0:
+        raise ValueError("budget, kv_lens, sinks and recent must not be negative")
+    limit = 2**31 - 1   # tokens of a request are counted in int32
+    if np.any(kv > limit):
+        raise ValueError(f"a request of over {limit} tokens")
+    keep = np.minimum(np.broadcast_to(budget, kv.shape), kv)
+    indptr, indices = csr_from_lists(pages_of_reqs, kv, pool.page_size, pool.num_pages)
+    out_indptr, out_indices = csr_from_lists(pages_out, keep, pool.page_size, pool.num_pages)
+    taken = np.zeros(pool.num_pages, dtype=bool)
+    taken[indices] = True
+    if taken[out_indices].any():
+        raise ValueError(f"page {int(out_indices[taken[out_indices]][0])} of pages_out holds "
+                         "tokens of the requests")
+    if np.unique(out_indices).size != out_indices.size:
+        raise ValueError("a page is twice in pages_out")
+    most = int(keep.max()) if n else 0
+    kept = torch.empty((n, pool.num_layers, pool.num_kv_heads, most), dtype=torch.int32,
+                       device=pool.device)
+    if most == 0:
+        return kept
+    table = PageTable(indptr, indices, kv, pool.device, upload=False)
+    dev = _upload_packed(table.host_arrays() + [out_indptr, out_indices, _i32(keep)], pool.device)
+    table.bind(dev[:3])
+    _lib.call("kunserve_evict", pool.desc(), ctypes.byref(weights._desc), table.desc(),
+              dev[3].data_ptr(), dev[4].data_ptr(), dev[5].data_ptr(), most, min(sinks, limit),
+              min(recent, limit), kept.data_ptr(), most, _stream_ptr(pool.device))
+    return kept

@@ -48,8 +48,17 @@ extern "C" int kunserve_tensors_overlap(const kunserve_tensor3* a, int32_t heads
 
 extern "C" int kunserve_attention_step(const kunserve_step* step, int32_t layer,
                                        const kunserve_step_io* io, kunserve_stream_t stream) {
+  return kunserve_attention_step_with(step, nullptr, layer, io, nullptr, stream);
+}
+
+extern "C" int kunserve_attention_step_with(const kunserve_step* step,
+                                            const kunserve_step_extras* extras, int32_t layer,
+                                            const kunserve_step_io* io,
+                                            const kunserve_rotary* rotary,
+                                            kunserve_stream_t stream) {
   clear_error();
   KSV_CHECK_ARG(step && io, "null step or tensors");
+  const bool weighted = extras && extras->weights.w;
   kunserve_tensor3 q = io->q, out = io->out;
   StepFusion decode, prefill;
   decode.counters = step->counters_dev;
@@ -67,7 +76,15 @@ extern "C" int kunserve_attention_step(const kunserve_step* step, int32_t layer,
     return false;
   };
   int rc = KUNSERVE_OK;
-  if (io->inv_freq_dev) {
+  if (weighted)   // they are formed from q after out is written
+    KSV_CHECK_ARG(!kunserve_tensors_overlap(&out, step->num_qo_heads, &q, step->num_qo_heads,
+                                            step->num_tokens, step->pool.head_dim),
+                  "out overlaps q, which the attention weights are formed from");
+  if (rotary) {
+    rc = kunserve_rotary_append_kv(&step->pool, layer, &step->table, step->q_indptr_dev,
+                                   step->num_tokens, &q, &q, step->num_qo_heads, &io->k, &io->v,
+                                   rotary, extras ? extras->positions_dev : nullptr, stream);
+  } else if (io->inv_freq_dev) {
     rc = kunserve_rope_append_kv(&step->pool, layer, &step->table, step->q_indptr_dev,
                                  step->num_tokens, &q, step->num_qo_heads, &io->k, &io->v,
                                  io->inv_freq_dev, io->interleave, stream);
@@ -79,7 +96,13 @@ extern "C" int kunserve_attention_step(const kunserve_step* step, int32_t layer,
                             step->num_tokens, &io->k, &io->v, stream);
   }
   if (rc) return rc;
-  if (step->decode_table.num_seqs > 0) {
+  if (step->decode_table.num_seqs > 0 && extras && extras->shared_info.num_segments > 0) {
+    rc = shared_decode(&step->pool, layer, &step->decode_table, step->decode_q_token_dev, &q, &out,
+                       step->num_qo_heads, step->sm_scale, extras->shared_plan_dev,
+                       &extras->shared_info, step->workspace_dev, step->workspace_bytes, decode,
+                       stream);
+    if (rc) return rc;
+  } else if (step->decode_table.num_seqs > 0) {
     rc = paged_decode(&step->pool, layer, &step->decode_table, step->decode_q_token_dev, &q, &out,
                       step->num_qo_heads, step->sm_scale, step->decode_plan_dev,
                       &step->decode_info, step->workspace_dev, step->workspace_bytes, decode,
@@ -93,6 +116,12 @@ extern "C" int kunserve_attention_step(const kunserve_step* step, int32_t layer,
                        step->workspace_bytes, prefill, stream);
     if (rc) return rc;
   }
+  if (weighted)
+    return kunserve_cache_weights(&step->pool, &extras->weights, layer, &step->table,
+                                  step->q_indptr_dev, &q, step->num_qo_heads, step->sm_scale,
+                                  extras->weights_plan_dev, &extras->weights_info,
+                                  extras->weights_workspace_dev, extras->weights_workspace_bytes,
+                                  stream);
   return KUNSERVE_OK;
 }
 

@@ -1,0 +1,373 @@
+// The attention weight that each cached token gets (what an eviction goes by).
+//
+// The observers of a row are the last min(q_len, window) of its new tokens.
+// With p[i, h, t] = softmax over t <= pos(i) of q[i, h] . k[t] * sm_scale,
+//   w[t] := (t new ? 0 : w[t]) + sum over observers i and the query heads h of
+//           the KV head of p[i, h, t]
+// for every cached token of the row and every KV head, in fp32. A new token's
+// weight starts at 0, so pages that are used again need no clearing.
+//
+// Columns: the row's observers times the query heads of a KV head. Three
+// launches: the maximum and sum of every column over each partition of
+// kPartTokens tokens; their combination; and the scores once more, this time
+// as probabilities summed over the columns. The sums run in one order, with no
+// atomics, so results do not depend on timing. A workgroup keeps its partition
+// of K in registers (64 tokens a wave, as MFMA operands) and takes the columns
+// 16 at a time, so K is read once by each of the two launches.
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "common.hpp"
+
+namespace kunserve {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kSubs = 4;                            // 16-token tiles of a wave
+constexpr int kPartTokens = kWaves * kSubs * 16;    // 256
+constexpr float kNegBig = -1.0e30f;                 // finite "minus infinity" for running maxima
+
+struct WeightsArgs {
+  const f16* q;
+  int64_t q_tok, q_head;
+  const f16* k;   // pool K at the layer
+  int64_t page_stride, head_stride, token_stride;
+  float* w;       // at the layer
+  int64_t w_page, w_head;
+  int32_t num_pages, page_shift;
+  const int32_t* indptr;
+  const int32_t* indices;
+  const int32_t* kv_len;
+  const int32_t* q_indptr;
+  const int32_t* items;      // [num_items][4]: row, first token, column offset, partitions
+  const int32_t* combines;   // [num_combines][4]: row, first column, column offset, partitions
+  float2* stats;             // per row: [partitions + 1][columns]; the last: combined
+  int32_t num_qo_heads, num_kv_heads, ratio, window;
+  float scale_log2;
+};
+
+// Maximum and sum over the four 16-lane groups.
+__device__ __forceinline__ float across_groups_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float across_groups_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// ADD false: the partition's maxima and sums; true: its tokens' weights.
+template <typename T, int D, bool ADD>
+__global__ __launch_bounds__(kThreads) void weights_scores_kernel(WeightsArgs a) {
+  typedef typename Vec<T>::v8 V8;
+  constexpr int KS = D / 32;   // MFMAs of a 16-token tile
+  __shared__ float2 s_stat[2][kWaves][16];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const int j = lane & 15, tg = lane >> 4;
+  const int32_t* item = a.items + 4 * blockIdx.x;
+  const int seq = item[0], part0 = item[1], hkv = blockIdx.y;
+  const int64_t offset = item[2];
+  const int n = a.kv_len[seq], q0 = a.q_indptr[seq], q_len = a.q_indptr[seq + 1] - q0;
+  const int obs = min(q_len, a.window);       // observers
+  const int cols = obs * a.ratio;             // columns of this KV head
+  const int all = cols * a.num_kv_heads;
+  const int t0 = part0 + wave * kSubs * 16;   // first token of the wave
+  const int mask = (1 << a.page_shift) - 1;
+  const int32_t* pages = a.indices + a.indptr[seq];
+  auto page_of = [&](int t) -> int {   // -1: past the row's end or outside the pool
+    if (t >= n) return -1;
+    const int p = pages[t >> a.page_shift];
+    return p >= 0 && p < a.num_pages ? p : -1;
+  };
+
+  // K as the A operand: row j of tile `sub` is token t0 + 16 sub + j.
+  V8 k[kSubs][KS];
+  uint32_t ok = 0;   // of the lane's tokens in the result: bit 4 sub + x
+#pragma unroll
+  for (int sub = 0; sub < kSubs; ++sub) {
+    const int t = t0 + 16 * sub + j;
+    const int p = page_of(t);
+    const f16* row = a.k + int64_t(hkv) * a.head_stride + int64_t(max(p, 0)) * a.page_stride +
+                     int64_t(t & mask) * a.token_stride + 8 * tg;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) k[sub][s] = p >= 0 ? load_v8<T>(row + 32 * s) : V8{};
+    const uint64_t fine = __ballot(p >= 0);   // bit j: token t0 + 16 sub + j
+    ok |= uint32_t((fine >> (4 * tg)) & 15u) << (4 * sub);
+  }
+  float mass[kSubs][4] = {};
+  float2* stats = a.stats + offset;
+  const int64_t done = int64_t(item[3]) * all;   // the combined columns
+  int turn = 0;
+  for (int c0 = 0; c0 < cols; c0 += 16, turn ^= 1) {
+    const int c = c0 + j;
+    const int o = c / a.ratio, h = hkv * a.ratio + c % a.ratio;
+    const bool col_ok = c < cols;
+    const f16* qp = a.q + int64_t(q0 + q_len - obs + min(o, obs - 1)) * a.q_tok +
+                    int64_t(h) * a.q_head + 8 * tg;
+    V8 q[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[s] = col_ok ? load_v8<T>(qp + 32 * s) : V8{};
+    const int last = n - obs + o;   // the last token that the observer sees
+    f32x4 sc[kSubs];
+#pragma unroll
+    for (int sub = 0; sub < kSubs; ++sub) {
+      sc[sub] = f32x4{};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) sc[sub] = mfma16(k[sub][s], q[s], sc[sub]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int t = t0 + 16 * sub + 4 * tg + x;
+        const bool seen = ((ok >> (4 * sub + x)) & 1u) && t <= last;
+        sc[sub][x] = seen ? sc[sub][x] * a.scale_log2 : -INFINITY;
+      }
+    }
+    if constexpr (ADD) {
+      const float2 st = col_ok ? stats[done + int64_t(hkv) * cols + c] : float2{0.f, 0.f};
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float p = sc[sub][x] == -INFINITY ? 0.f : fast_exp2(sc[sub][x] - st.x) * st.y;
+          mass[sub][x] += col_ok ? p : 0.f;
+        }
+    } else {
+      float m = kNegBig;
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) m = fmaxf(m, sc[sub][x]);
+      m = across_groups_max(m);
+      float l = 0.f;
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) l += fast_exp2(sc[sub][x] - m);
+      l = across_groups_sum(l);
+      if (tg == 0) s_stat[turn][wave][j] = float2{m, l};
+      __syncthreads();   // the other half is written next: one barrier a turn
+      if (wave == 0 && tg == 0 && col_ok) {
+        float mx = kNegBig, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) mx = fmaxf(mx, s_stat[turn][i][j].x);
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i)
+          sum += s_stat[turn][i][j].y * fast_exp2(s_stat[turn][i][j].x - mx);
+        stats[int64_t(part0 / kPartTokens) * all + int64_t(hkv) * cols + c] = float2{mx, sum};
+      }
+    }
+  }
+  if constexpr (ADD) {
+    // Sums over the 16 columns of a lane row; lane j then takes result 4 sub
+    // + x = j: token t0 + 16 (j / 4) + 4 tg + j % 4.
+    float mine = 0.f;
+#pragma unroll
+    for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float s = row16_sum(mass[sub][x]);
+        mine = j == 4 * sub + x ? s : mine;
+      }
+    const int t = t0 + 16 * (j >> 2) + 4 * tg + (j & 3);
+    const int p = page_of(t);
+    if (p >= 0) {
+      float* w = a.w + int64_t(hkv) * a.w_head + int64_t(p) * a.w_page + (t & mask);
+      *w = (t >= n - q_len ? 0.f : *w) + mine;
+    }
+  }
+}
+
+// A column's maximum and 1 / sum over the row's partitions.
+__global__ __launch_bounds__(kThreads) void weights_combine_kernel(WeightsArgs a) {
+  const int32_t* rec = a.combines + 4 * blockIdx.x;
+  const int seq = rec[0], parts = rec[3];
+  const int q_len = a.q_indptr[seq + 1] - a.q_indptr[seq];
+  const int all = min(q_len, a.window) * a.num_qo_heads;
+  const int c = rec[1] + threadIdx.x;
+  if (c >= all) return;
+  float2* stats = a.stats + int64_t(rec[2]) + c;
+  float mx = kNegBig, sum = 0.f;
+  for (int i = 0; i < parts; ++i) {
+    const float2 s = stats[int64_t(i) * all];
+    const float m = fmaxf(mx, s.x);
+    sum = sum * fast_exp2(mx - m) + s.y * fast_exp2(s.x - m);
+    mx = m;
+  }
+  stats[int64_t(parts) * all] = float2{mx, sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum};
+}
+
+template <typename T, int D>
+int run_weights(const WeightsArgs& a, const kunserve_weights_plan_info& info, hipStream_t s) {
+  const dim3 grid(unsigned(info.num_items), unsigned(a.num_kv_heads));
+  weights_scores_kernel<T, D, false><<<grid, kThreads, 0, s>>>(a);
+  KSV_CHECK_LAUNCH();
+  weights_combine_kernel<<<dim3(unsigned(info.num_combines)), kThreads, 0, s>>>(a);
+  KSV_CHECK_LAUNCH();
+  weights_scores_kernel<T, D, true><<<grid, kThreads, 0, s>>>(a);
+  KSV_CHECK_LAUNCH();
+  return KUNSERVE_OK;
+}
+
+template <typename T>
+int run_weights_dim(int head_dim, const WeightsArgs& a, const kunserve_weights_plan_info& info,
+                    hipStream_t s) {
+  switch (head_dim) {
+    case 64: return run_weights<T, 64>(a, info, s);
+    case 128: return run_weights<T, 128>(a, info, s);
+    default: return run_weights<T, 256>(a, info, s);
+  }
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int weights_plan(const int32_t* q_indptr, const int32_t* kv_len, int32_t num_seqs,
+                 int32_t num_qo_heads, int32_t window, std::vector<int32_t>& plan,
+                 kunserve_weights_plan_info* info) {
+  std::vector<int32_t> items, combines;
+  int64_t columns = 0;
+  for (int32_t b = 0; b < num_seqs; ++b) {
+    const int64_t q_len = int64_t(q_indptr[b + 1]) - q_indptr[b];
+    KSV_CHECK_ARG(q_len >= 0 && kv_len[b] >= q_len, "row %d: kv_len %d for %lld new tokens", b,
+                  kv_len[b], (long long)q_len);
+    if (q_len == 0) continue;
+    const int64_t cols = std::min<int64_t>(q_len, window) * num_qo_heads;
+    const int64_t parts = ceil_div(kv_len[b], kPartTokens);
+    KSV_CHECK_ARG(columns + (parts + 1) * cols < (int64_t(1) << 31),
+                  "too many observed columns (%lld)", (long long)(columns + (parts + 1) * cols));
+    for (int64_t p = 0; p < parts; ++p)
+      items.insert(items.end(), {b, int32_t(p * kPartTokens), int32_t(columns), int32_t(parts)});
+    for (int64_t c = 0; c < cols; c += kThreads)
+      combines.insert(combines.end(), {b, int32_t(c), int32_t(columns), int32_t(parts)});
+    columns += (parts + 1) * cols;
+  }
+  plan = std::move(items);
+  info->num_items = int32_t(plan.size() / 4);
+  plan.insert(plan.end(), combines.begin(), combines.end());
+  info->num_combines = int32_t(combines.size() / 4);
+  info->window = window;
+  info->num_qo_heads = num_qo_heads;
+  info->plan_ints = int32_t(plan.size());
+  info->num_columns = columns;
+  return KUNSERVE_OK;
+}
+
+}  // namespace
+}  // namespace kunserve
+
+using namespace kunserve;
+
+extern "C" int64_t kunserve_weights_plan_bound(const int32_t* q_indptr_host,
+                                               const int32_t* kv_len_host, int32_t num_seqs,
+                                               int32_t num_qo_heads, int32_t window) {
+  if (num_seqs < 0 || num_qo_heads <= 0 || window <= 0 ||
+      (num_seqs > 0 && (!q_indptr_host || !kv_len_host)))
+    return -1;
+  int64_t records = 0;
+  for (int32_t b = 0; b < num_seqs; ++b) {
+    const int64_t q_len = std::max<int64_t>(0, int64_t(q_indptr_host[b + 1]) - q_indptr_host[b]);
+    records += ceil_div(std::max(kv_len_host[b], 0), kPartTokens) +
+               ceil_div(std::min<int64_t>(q_len, window) * num_qo_heads, kThreads);
+  }
+  return 4 * records;
+}
+
+extern "C" int kunserve_weights_plan(const int32_t* q_indptr_host, const int32_t* kv_len_host,
+                                     int32_t num_seqs, int32_t num_qo_heads, int32_t window,
+                                     int32_t* plan_host, int64_t plan_capacity,
+                                     kunserve_weights_plan_info* info) {
+  clear_error();
+  KSV_CHECK_ARG(info && plan_host, "null plan buffer or info");
+  KSV_CHECK_ARG(num_seqs >= 0 && (num_seqs == 0 || (q_indptr_host && kv_len_host)),
+                "bad q_indptr, kv_len or num_seqs");
+  KSV_CHECK_ARG(num_qo_heads > 0, "num_qo_heads %d", num_qo_heads);
+  KSV_CHECK_ARG(window > 0, "window %d must be positive", window);
+  return no_throw([&] {
+    std::vector<int32_t> plan;
+    const int rc = weights_plan(q_indptr_host, kv_len_host, num_seqs, num_qo_heads, window, plan,
+                                info);
+    if (rc) return rc;
+    if (int64_t(plan.size()) > plan_capacity) {
+      set_error("plan needs %lld ints, capacity %lld", (long long)plan.size(),
+                (long long)plan_capacity);
+      return int(KUNSERVE_ENOSPC);
+    }
+    std::copy(plan.begin(), plan.end(), plan_host);
+    return int(KUNSERVE_OK);
+  });
+}
+
+extern "C" int64_t kunserve_weights_workspace_bytes(const kunserve_weights_plan_info* info) {
+  if (!info) return -1;
+  return info->num_columns * int64_t(sizeof(float2));
+}
+
+extern "C" int kunserve_cache_weights(const kunserve_kv_pool* pool,
+                                      const kunserve_kv_weights* weights, int32_t layer,
+                                      const kunserve_page_table* table,
+                                      const int32_t* q_indptr_dev, const kunserve_tensor3* q,
+                                      int32_t num_qo_heads, float sm_scale,
+                                      const int32_t* plan_dev,
+                                      const kunserve_weights_plan_info* info, void* workspace_dev,
+                                      int64_t workspace_bytes, kunserve_stream_t stream) {
+  clear_error();
+  int rc = check_pool(pool, true);
+  if (rc) return rc;
+  rc = check_weights(weights, pool);
+  if (rc) return rc;
+  KSV_CHECK_ARG(table && q && info, "null argument");
+  KSV_CHECK_ARG(layer >= 0 && layer < pool->num_layers, "layer %d outside [0, %d)", layer,
+                pool->num_layers);
+  KSV_CHECK_ARG(std::isfinite(sm_scale) && sm_scale > 0.f,
+                "sm_scale %g must be finite and positive", double(sm_scale));
+  KSV_CHECK_ARG(num_qo_heads > 0 && num_qo_heads % pool->num_kv_heads == 0,
+                "num_qo_heads %d not a multiple of num_kv_heads %d", num_qo_heads,
+                pool->num_kv_heads);
+  KSV_CHECK_ARG(info->num_qo_heads == num_qo_heads, "plan made for %d query heads, not %d",
+                info->num_qo_heads, num_qo_heads);
+  if (info->num_items == 0) return KUNSERVE_OK;
+  KSV_CHECK_ARG(plan_dev && q_indptr_dev && table->indptr_dev && table->indices_dev &&
+                    table->kv_len_dev,
+                "null plan or table");
+  KSV_CHECK_ARG(q->data && aligned16(q->data) && q->token_stride % 8 == 0 &&
+                    q->head_stride % 8 == 0,
+                "q must be 16-byte aligned with strides that are multiples of 8");
+  KSV_CHECK_ARG(pool->num_kv_heads < 65536, "%d KV heads: at most 65535", pool->num_kv_heads);
+  const int64_t need = kunserve_weights_workspace_bytes(info);
+  if (!workspace_dev || workspace_bytes < need) {
+    set_error("weights workspace holds %lld bytes, %lld needed", (long long)workspace_bytes,
+              (long long)need);
+    return KUNSERVE_ENOSPC;
+  }
+  KSV_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace_dev) & 7u) == 0,
+                "workspace must be 8-byte aligned");
+  WeightsArgs a{};
+  a.q = static_cast<const f16*>(q->data);
+  a.q_tok = q->token_stride;
+  a.q_head = q->head_stride;
+  a.k = static_cast<const f16*>(pool->k) + int64_t(layer) * pool->layer_stride;
+  a.page_stride = pool->page_stride;
+  a.head_stride = pool->head_stride;
+  a.token_stride = pool->token_stride;
+  a.w = weights->w + int64_t(layer) * weights->layer_stride;
+  a.w_page = weights->page_stride;
+  a.w_head = weights->head_stride;
+  a.num_pages = int32_t(pool->num_pages);
+  a.page_shift = __builtin_ctz(pool->page_size);
+  a.indptr = table->indptr_dev;
+  a.indices = table->indices_dev;
+  a.kv_len = table->kv_len_dev;
+  a.q_indptr = q_indptr_dev;
+  a.items = plan_dev;
+  a.combines = plan_dev + 4 * int64_t(info->num_items);
+  a.stats = static_cast<float2*>(workspace_dev);
+  a.num_qo_heads = num_qo_heads;
+  a.num_kv_heads = pool->num_kv_heads;
+  a.ratio = num_qo_heads / pool->num_kv_heads;
+  a.window = info->window;
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (pool->dtype == KUNSERVE_DTYPE_BF16)
+    return run_weights_dim<bf16>(pool->head_dim, a, *info, s);
+  return run_weights_dim<f16>(pool->head_dim, a, *info, s);
+}

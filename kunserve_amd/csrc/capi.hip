@@ -46,6 +46,14 @@ int check_pool(const kunserve_kv_pool* p, bool need_vec_align) {
   return KUNSERVE_OK;
 }
 
+int check_weights(const kunserve_kv_weights* w, const kunserve_kv_pool* pool) {
+  KSV_CHECK_ARG(w && w->w, "null weights");
+  KSV_CHECK_ARG((reinterpret_cast<uintptr_t>(w->w) & 3u) == 0, "weights must be 4-byte aligned");
+  KSV_CHECK_ARG(w->page_stride >= pool->page_size && w->layer_stride >= 0 && w->head_stride >= 0,
+                "bad weight strides");
+  return KUNSERVE_OK;
+}
+
 }  // namespace kunserve
 
 extern "C" int32_t kunserve_version(void) { return 300; }

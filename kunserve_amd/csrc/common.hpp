@@ -9,6 +9,7 @@
 #include <cstdio>
 #include <new>
 #include <string>
+#include <vector>
 
 #include "../../include/kunserve_hip.h"
 
@@ -72,6 +73,8 @@ inline bool aligned16(const void* p) {
 // Validates the pool descriptor for kernels that issue 16-byte loads along
 // head_dim. Returns KUNSERVE_OK or an error code (message set).
 int check_pool(const kunserve_kv_pool* pool, bool need_vec_align);
+// The same for the weights of a pool's tokens.
+int check_weights(const kunserve_kv_weights* weights, const kunserve_kv_pool* pool);
 
 // What a decode or prefill launch can take on beside attention: the append of
 // its rows' new K/V (k_new and v_new; the caller has checked
@@ -88,6 +91,25 @@ int paged_decode(const kunserve_kv_pool* pool, int32_t layer, const kunserve_pag
                  int32_t num_qo_heads, float sm_scale, const int32_t* plan_dev,
                  const kunserve_decode_plan_info* info, void* workspace_dev,
                  int64_t workspace_bytes, const StepFusion& fusion, kunserve_stream_t stream);
+
+int shared_decode(const kunserve_kv_pool* pool, int32_t layer, const kunserve_page_table* table,
+                  const int32_t* q_token_dev, const kunserve_tensor3* q, kunserve_tensor3* out,
+                  int32_t num_qo_heads, float sm_scale, const int32_t* plan_dev,
+                  const kunserve_shared_plan_info* info, void* workspace_dev,
+                  int64_t workspace_bytes, const StepFusion& fusion, kunserve_stream_t stream);
+
+// Pieces of the decode plan for plans that add to it. An item: tokens [b, e) of
+// a sequence, its partial's slot (-1: the output itself). decode_records orders
+// the items and appends the plan's work records (returns how many);
+// decode_part_tokens is the partition length of a grouped plan for rows of these
+// lengths, decode_group its query heads of a workgroup.
+struct DecodeItem {
+  int32_t seq, b, e, slot;
+};
+int32_t decode_records(std::vector<DecodeItem>& items, std::vector<int32_t>& records);
+int32_t decode_part_tokens(const int32_t* lens, int32_t n, int32_t num_qo_heads, int group,
+                           int head_dim, int32_t num_cus);
+int decode_group(int32_t num_qo_heads, int32_t num_kv_heads);
 
 int paged_prefill(const kunserve_kv_pool* pool, int32_t layer, const kunserve_page_table* table,
                   const int32_t* q_indptr_dev, const int32_t* q_start_dev,

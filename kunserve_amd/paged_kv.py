@@ -19,12 +19,13 @@ import array
 import ctypes
 import math
 from dataclasses import dataclass
-from typing import Callable, Optional, Sequence
+from typing import Callable, Optional, Sequence, Union
 
 import numpy as np
 import torch
 
 from . import _lib
+from .rotary import Rotary
 
 FP16 = torch.float16
 
@@ -414,6 +415,51 @@ class DecodePlan:
             ctypes.byref(self.info), self.num_qo_heads, head_dim))
 
 
+class SharedDecodePlan:
+    """Plan of decode rows whose page lists begin alike (kunserve_shared_plan),
+    computed on the host once per step and shared by every layer. Runs of whole
+    pages that two or more rows hold at the same place are read once for them;
+    num_segments counts these runs."""
+
+    def __init__(self, table: "PageTable", num_qo_heads: int, num_kv_heads: int, page_size: int,
+                 device: torch.device, num_cus: Optional[int] = None, upload: bool = True,
+                 head_dim: int = 128):
+        n = table.num_seqs
+        kv, indices = table.kv_len_host, table.indices_host
+        if n and int(table.indptr_host[-1]) > indices.size:
+            raise ValueError("the table's indptr runs past its indices")
+        kv_ptr = kv.ctypes.data if n else None
+        cap = int(_lib.lib().kunserve_shared_plan_bound(kv_ptr, n))
+        buf = np.empty(max(cap, 4), dtype=np.int32)   # the plan writes what it uses
+        self.shared_info = _lib.SharedPlanInfo()
+        _lib.call("kunserve_shared_plan", table.indptr_host.ctypes.data, indices.ctypes.data,
+                  kv_ptr, n, num_qo_heads, num_kv_heads, page_size, head_dim,
+                  num_cus if num_cus is not None else _num_cus(device), buf.ctypes.data, buf.size,
+                  ctypes.byref(self.shared_info))
+        self.info = self.shared_info.decode
+        self.num_counters = 0
+        self.plan_host = buf[: self.shared_info.plan_ints].copy()
+        self.plan = None
+        if upload:
+            self.bind(_upload_packed(self.host_arrays(), device))
+        self.num_qo_heads = num_qo_heads
+        self.num_kv_heads = num_kv_heads
+
+    @property
+    def num_segments(self) -> int:
+        return self.shared_info.num_segments
+
+    def host_arrays(self) -> list:
+        return [self.plan_host]
+
+    def bind(self, dev: Sequence[torch.Tensor]) -> None:
+        self.plan = dev[0] if self.shared_info.plan_ints else None
+
+    def workspace_bytes(self, head_dim: int) -> int:
+        return int(_lib.lib().kunserve_decode_workspace_bytes(
+            ctypes.byref(self.info), self.num_qo_heads, head_dim))
+
+
 class PrefillPlan:
     """(row, q tile, KV head) work items of the prefill rows, XCD-ordered
     (kunserve_prefill_plan_packed). Steps with too few items to fill the device
@@ -584,6 +630,39 @@ def rope_append_kv(pool: KVPool, layer: int, table: PageTable, q_indptr: torch.T
     return q
 
 
+def rotary_append_kv(pool: KVPool, layer: int, table: PageTable, q_indptr: torch.Tensor,
+                     q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, rotary: Rotary,
+                     positions: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The attention prologue of one layer with a Rotary: q and k_new rotated, the
+    rotated k and v_new written into their pages. positions (device int32
+    [num_tokens]): the tokens' rotary positions, where they are not their places in
+    the cache. The rotated q goes to out (default: q, in place), which must be q
+    or lie apart from q, k_new and v_new. Returns out."""
+    if k_new.shape != v_new.shape or k_new.shape[1:] != (pool.num_kv_heads, pool.head_dim):
+        raise ValueError(f"k_new / v_new must be [tokens, {pool.num_kv_heads}, {pool.head_dim}]")
+    if q.shape[0] != k_new.shape[0] or q.shape[2] != pool.head_dim:
+        raise ValueError(f"q {tuple(q.shape)} does not match k_new {tuple(k_new.shape)}")
+    if q_indptr.numel() != table.num_seqs + 1:
+        raise ValueError("q_indptr must have num_seqs + 1 entries")
+    if out is None:
+        out = q
+    if out.shape != q.shape:
+        raise ValueError(f"out shape {tuple(out.shape)} differs from q's {tuple(q.shape)}")
+    for name, t in (("q", q), ("k_new", k_new), ("v_new", v_new), ("out", out)):
+        if t.device != pool.device:
+            raise ValueError(f"{name} is on {t.device}, the pool on {pool.device}")
+    rotary.check(pool.head_dim, pool.device)
+    _check_row_map(positions, k_new.shape[0], pool.device, "positions")
+    pool.check_dtype(q, k_new, v_new, out)
+    qd, od, kd, vd = _tensor3(q), _tensor3(out), _tensor3(k_new), _tensor3(v_new)
+    _lib.call("kunserve_rotary_append_kv", pool.desc(), layer, table.desc(), q_indptr.data_ptr(),
+              k_new.shape[0], ctypes.byref(qd), ctypes.byref(od), q.shape[1], ctypes.byref(kd),
+              ctypes.byref(vd), ctypes.byref(rotary._desc), _ptr(positions),
+              _stream_ptr(pool.device))
+    return out
+
+
 def _check_row_map(m: Optional[torch.Tensor], n: int, device: torch.device, what: str) -> None:
     if m is not None and (m.dtype != torch.int32 or m.shape != (n,) or m.device != device
                           or not m.is_contiguous()):
@@ -599,6 +678,22 @@ def paged_decode(pool: KVPool, layer: int, table: PageTable, q: torch.Tensor, pl
     With q_token (device int32 [num_seqs], each entry < q.shape[0]), row b's
     query and output are token q_token[b] of q and out ([num_tokens, Hq, D]):
     the decode rows of a mixed step, read and written in place."""
+    return _decode("kunserve_paged_decode", plan.info, pool, layer, table, q, plan, sm_scale, out,
+                   workspace, q_token)
+
+
+def shared_decode(pool: KVPool, layer: int, table: PageTable, q: torch.Tensor,
+                  plan: SharedDecodePlan, sm_scale: Optional[float] = None,
+                  out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                  q_token: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_decode of rows that share pages, on the plan made from their table."""
+    return _decode("kunserve_shared_decode", plan.shared_info, pool, layer, table, q, plan,
+                   sm_scale, out, workspace, q_token)
+
+
+def _decode(entry: str, info, pool: KVPool, layer: int, table: PageTable, q: torch.Tensor, plan,
+            sm_scale: Optional[float], out: Optional[torch.Tensor],
+            workspace: Optional[torch.Tensor], q_token: Optional[torch.Tensor]) -> torch.Tensor:
     hq = q.shape[1]
     if q_token is None and q.shape[0] != table.num_seqs:
         raise ValueError(f"q has {q.shape[0]} tokens for {table.num_seqs} rows")
@@ -615,9 +710,9 @@ def paged_decode(pool: KVPool, layer: int, table: PageTable, q: torch.Tensor, pl
     if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
         workspace = torch.empty(need, dtype=torch.uint8, device=pool.device)
     qd, od = _tensor3(q), _tensor3(out)
-    _lib.call("kunserve_paged_decode", pool.desc(), layer, table.desc(), _ptr(q_token),
+    _lib.call(entry, pool.desc(), layer, table.desc(), _ptr(q_token),
               ctypes.byref(qd), ctypes.byref(od), hq, ctypes.c_float(scale),
-              _ptr(plan.plan), ctypes.byref(plan.info), _ptr(workspace),
+              _ptr(plan.plan), ctypes.byref(info), _ptr(workspace),
               0 if workspace is None else workspace.numel() * workspace.element_size(),
               _stream_ptr(pool.device))
     return out
@@ -679,9 +774,26 @@ class AttentionStep:
     run(layer, ...) addresses pool layer layer - layer_offset, so a fused
     stage runs its global layer indices on its local layers.
 
+    share_prefixes: decode rows whose page lists begin alike read the pages they
+    share once (SharedDecodePlan); a step that shares nothing runs as without.
+
+    weights (a KVWeights of the pool): every layer adds the attention weight that
+    each cached token got to it, from a decode row's token and from the last
+    `window` tokens of a prefill row; new tokens start at 0. The step's pages must
+    then be in one place of its lists each (ValueError), and out may not overlap
+    q.
+
+    rope_positions: for each row the rotary position of its first new token, where
+    that is not its place in the cache (rows shortened by evict). Only a Rotary
+    takes them.
+
     All of the step's index arrays (tables, plans, row and token indices)
     reach the device in one copy on the current stream, with no host wait.
     """
+
+    weights = None
+    positions = None
+    _extras_ref = None
 
     def __init__(self, pool: KVPool, num_qo_heads: int, q_lens: Sequence[int],
                  first_token_indexes: Sequence[int], is_prefill_requests: Sequence[int],
@@ -689,7 +801,9 @@ class AttentionStep:
                  decode_part_tokens: int = 0, use_tensor_cores: bool = False,
                  is_context_stage: Optional[Sequence[int]] = None, layer_offset: int = 0,
                  id_map: Optional[Callable[[np.ndarray], np.ndarray]] = None,
-                 num_ids: Optional[int] = None):
+                 num_ids: Optional[int] = None, share_prefixes: bool = False,
+                 weights=None, window: int = 16,
+                 rope_positions: Optional[Sequence[int]] = None):
         self.pool = pool
         self.num_qo_heads = num_qo_heads
         self.layer_offset = layer_offset
@@ -714,6 +828,25 @@ class AttentionStep:
         if not (math.isfinite(self.scale) and self.scale > 0):
             raise ValueError(f"sm_scale {self.scale} must be finite and positive")
 
+        if weights is not None:
+            weights.check(pool)
+            if window < 1:
+                raise ValueError(f"window {window} must be positive")
+            ids = self.table.indices_host
+            if np.unique(ids).size != ids.size:
+                raise ValueError("attention weights need pages that are in one place of the "
+                                 "step's lists")
+            self.weights = weights
+        positions = None
+        if rope_positions is not None:
+            starts = np.asarray(rope_positions, dtype=np.int64)
+            if starts.shape != (n_rows,):
+                raise ValueError(f"{n_rows} rows but {starts.shape} rope_positions")
+            positions = np.repeat(starts - self.q_indptr_host[:-1], q_lens) + np.arange(
+                self.num_tokens)
+            if np.any(starts < 0) or (positions.size and positions.max() >= 2**31):
+                raise ValueError("rope_positions must lie in [0, 2^31)")
+
         # Host side of every device array of the step; uploaded together below.
         uploads = [[self.q_indptr_host], self.table]
         self.decode = self.prefill = None
@@ -732,9 +865,15 @@ class AttentionStep:
             whole = dec_rows.size == n_rows
             table = self.table if whole else sub_table(dec_rows)
             tokens = None if whole else self.q_indptr_host[dec_rows].astype(np.int32)
-            plan = DecodePlan(self.kv_len[dec_rows], num_qo_heads, pool.num_kv_heads, dev,
-                              part_tokens=decode_part_tokens, upload=False,
-                              head_dim=pool.head_dim)
+            plan = None
+            if share_prefixes and dec_rows.size > 1:
+                plan = SharedDecodePlan(table, num_qo_heads, pool.num_kv_heads, pool.page_size,
+                                        dev, upload=False, head_dim=pool.head_dim)
+                plan = plan if plan.num_segments else None
+            if plan is None:
+                plan = DecodePlan(self.kv_len[dec_rows], num_qo_heads, pool.num_kv_heads, dev,
+                                  part_tokens=decode_part_tokens, upload=False,
+                                  head_dim=pool.head_dim)
             self.decode = _Subset(dec_rows, tokens, table, None, plan)
             uploads += ([] if whole else [table, [tokens]]) + [plan]
         if pre_rows.size:
@@ -750,6 +889,13 @@ class AttentionStep:
                                upload=False, head_dim=pool.head_dim)
             self.prefill = _Subset(pre_rows, tokens, table, None, plan)
             uploads += ([] if whole else [table, [tokens], [qi]]) + [plan]
+
+        if positions is not None:
+            uploads.append([positions])
+        self._weights_plan = None
+        if weights is not None:
+            self._weights_plan = weights.plan(self.q_indptr_host, self.kv_len, num_qo_heads, window)
+            uploads.append(self._weights_plan)
 
         # Counters with which the launches combine their split rows (the
         # decode launch's, then the prefill launch's): zeroed once, each layer
@@ -791,10 +937,15 @@ class AttentionStep:
                 self.prefill.q_indptr = next(rest)[0]
             else:
                 self.prefill.q_indptr = self.q_indptr
+        if positions is not None:
+            self.positions = next(rest)[0]
         # Scratch shared by every layer of the step (launches are serialised on one stream).
         ws = max(self.decode.plan.workspace_bytes(pool.head_dim) if self.decode else 0,
                  self.prefill.plan.workspace_bytes() if self.prefill else 0)
         self.workspace = torch.empty(ws, dtype=torch.uint8, device=dev) if ws > 0 else None
+        if weights is not None:
+            self._weights_workspace = torch.empty(self._weights_plan.workspace_bytes(),
+                                                  dtype=torch.uint8, device=dev)
         self._describe(appends)
 
     def _describe(self, appends: int) -> None:
@@ -815,6 +966,20 @@ class AttentionStep:
             counters if n_dec else None, n_dec, appends,
             counters + 4 * n_dec if n_pre else None, n_pre)
         self._step_ref = ctypes.byref(self._step)
+        shared = d is not None and isinstance(d.plan, SharedDecodePlan)
+        if shared or self.weights is not None or self.positions is not None:
+            self._extras = _lib.StepExtras()
+            if shared:
+                self._extras.shared_plan_dev = _ptr(d.plan.plan)
+                self._extras.shared_info = d.plan.shared_info
+            if self.weights is not None:
+                self._extras.weights = self.weights._desc
+                self._extras.weights_plan_dev = _ptr(self._weights_plan.plan)
+                self._extras.weights_info = self._weights_plan.info
+                self._extras.weights_workspace_dev = self._weights_workspace.data_ptr()
+                self._extras.weights_workspace_bytes = self._weights_workspace.numel()
+            self._extras.positions_dev = _ptr(self.positions)
+            self._extras_ref = ctypes.byref(self._extras)
         self._device = self.pool.device
         self._device_index = self._device.index   # a device tensor's is never None
         self._q_shape = (self.num_tokens, self.num_qo_heads, self.pool.head_dim)
@@ -822,11 +987,11 @@ class AttentionStep:
 
     def run(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             out: Optional[torch.Tensor] = None,
-            rope: Optional[tuple] = None) -> torch.Tensor:
+            rope: Union[tuple, Rotary, None] = None) -> torch.Tensor:
         """q [num_tokens, Hq, D], k/v [num_tokens, Hkv, D] -> out [num_tokens, Hq, D].
 
-        With rope = (inv_freq, interleave), q and k are first rotated at their
-        positions (q in place) by the fused prologue kernel; without it they
+        With rope = (inv_freq, interleave) or a Rotary, q and k are first rotated at
+        their positions (q in place) by the fused prologue kernel; without it they
         are taken as already rotated. out may be q, or lie in k's or v's memory
         (the append is then a launch of its own)."""
         q_shape, k_shape = q.shape, k.shape
@@ -836,10 +1001,14 @@ class AttentionStep:
         if not 0 <= local < self.pool.num_layers:
             raise ValueError(f"layer {layer} outside this step's layers "
                              f"[{self.layer_offset}, {self.layer_offset + self.pool.num_layers})")
-        dtype, inv_freq, interleave = self.pool.dtype, None, 0
-        if rope is not None:
+        dtype, inv_freq, interleave, rotary = self.pool.dtype, None, 0, None
+        if isinstance(rope, Rotary):
+            rotary = rope
+        elif rope is not None:
             inv_freq, interleave = rope   # exactly two
             interleave = int(bool(interleave))
+            if self.positions is not None:
+                raise ValueError("rope_positions need a Rotary")
         if out is None:
             out = torch.empty_like(q)
         qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
@@ -848,25 +1017,39 @@ class AttentionStep:
                      == self._device_index)   # -1 on the host
                 and q.dtype == k.dtype == v.dtype == out.dtype == dtype
                 and qs[2] == ks[2] == vs[2] == os[2] == 1
-                and (rope is None
+                and (rope is None or rotary is not None
                      or (isinstance(inv_freq, torch.Tensor) and inv_freq.dtype == torch.float32 and inv_freq.device == q.device
                          and inv_freq.numel() == self.pool.head_dim // 2
                          and inv_freq.is_contiguous()))):
             # One native call for the layer.
             self.pool.desc()
+            if rotary is not None:
+                rotary.check(self.pool.head_dim, self._device)
             io = _lib.STEP_IO.pack(
                 q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
                 vs[1], out.data_ptr(), os[0], os[1],
                 0 if inv_freq is None else inv_freq.data_ptr(), interleave)
-            _lib.call("kunserve_attention_step", self._step_ref, local, io,
-                      _stream_ptr(self._device))
+            if rotary is None and self._extras_ref is None:
+                _lib.call("kunserve_attention_step", self._step_ref, local, io,
+                          _stream_ptr(self._device))
+            else:
+                _lib.call("kunserve_attention_step_with", self._step_ref, self._extras_ref, local,
+                          io, None if rotary is None else ctypes.byref(rotary._desc),
+                          _stream_ptr(self._device))
             return out
         # Tensors the step does not describe: op by op, each with its checks.
         for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
             # Kernels can read pinned host memory, and no other device's.
             if t.device != self._device and not (t.device.type == "cpu" and t.is_pinned()):
                 raise ValueError(f"{name} is on {t.device}, the step's pool on {self._device}")
-        if rope is not None:
+        if self.weights is not None and _lib.call(
+                "kunserve_tensors_overlap", ctypes.byref(_tensor3(out)), out.shape[1],
+                ctypes.byref(_tensor3(q)), q.shape[1], self.num_tokens, self.pool.head_dim):
+            raise ValueError("out overlaps q, which the attention weights are formed from")
+        if rotary is not None:
+            rotary_append_kv(self.pool, local, self.table, self.q_indptr, q, k, v, rotary,
+                             positions=self.positions)
+        elif rope is not None:
             rope_append_kv(self.pool, local, self.table, self.q_indptr, q, k, v, inv_freq,
                            interleave)
         else:
@@ -875,10 +1058,14 @@ class AttentionStep:
         # mixed step through the subset's row -> token map.
         if self.decode is not None:
             d = self.decode
-            paged_decode(self.pool, local, d.table, q, d.plan, self.scale, out=out,
-                         workspace=self.workspace, q_token=d.tokens)
+            decode = shared_decode if isinstance(d.plan, SharedDecodePlan) else paged_decode
+            decode(self.pool, local, d.table, q, d.plan, self.scale, out=out,
+                   workspace=self.workspace, q_token=d.tokens)
         if self.prefill is not None:
             p = self.prefill
             paged_prefill(self.pool, local, p.table, p.q_indptr, q, p.plan, self.scale,
                           out=out, workspace=self.workspace, q_start=p.tokens)
+        if self.weights is not None:
+            self.weights.add(self.pool, local, self.table, self.q_indptr, q, self._weights_plan,
+                             self.scale, self._weights_workspace)
         return out

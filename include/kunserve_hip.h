@@ -345,7 +345,7 @@ typedef struct {
   kunserve_decode_plan_info decode; /* what the rows hold for themselves, and
                                        the joining of all partials           */
   int32_t num_shared;    /* work records of shared pages (incl. padding)      */
-  int32_t tiles;         /* 16-column tiles of a workgroup                    */
+  int32_t wide;          /* whether some run in workgroups of 128 columns     */
   int32_t num_pairs;     /* (row, first partial) records                      */
   int32_t num_segments;  /* runs of pages that several rows share             */
   int32_t head_dim;      /* head_dim the plan was made for                    */
@@ -353,7 +353,8 @@ typedef struct {
 } kunserve_shared_plan_info;
 
 /* Upper bound of the plan buffer length (int32 entries) for these lengths. */
-int64_t kunserve_shared_plan_bound(const int32_t* kv_len_host, int32_t num_seqs);
+int64_t kunserve_shared_plan_bound(const int32_t* kv_len_host, int32_t num_seqs,
+                                   int32_t num_qo_heads);
 
 /* Host-side plan of decode rows whose page lists (CSR, host arrays) may begin
  * with the same ids: every run of at least 64 tokens of whole pages that two

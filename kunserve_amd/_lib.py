@@ -77,9 +77,9 @@ class Step(Structure):
 
 
 class SharedPlanInfo(Structure):
-    _fields_ = [("decode", DecodePlanInfo), ("num_shared", c_int32), ("tiles", c_int32),
-                ("num_pairs", c_int32), ("num_segments", c_int32), ("head_dim", c_int32),
-                ("plan_ints", c_int32)]
+    _fields_ = [("decode", DecodePlanInfo), ("num_shared", c_int32), ("wide", c_int32),
+                ("num_pairs", c_int32), ("num_segments", c_int32),
+                ("head_dim", c_int32), ("plan_ints", c_int32)]
 
 
 class KVWeights(Structure):
@@ -136,7 +136,7 @@ SIGNATURES = {
                                           c_int32, POINTER(Tensor3), POINTER(Tensor3), c_int32,
                                           POINTER(Tensor3), POINTER(Tensor3), POINTER(Rotary),
                                           c_void_p, c_void_p]),
-    "kunserve_shared_plan_bound": (c_int64, [c_void_p, c_int32]),
+    "kunserve_shared_plan_bound": (c_int64, [c_void_p, c_int32, c_int32]),
     "kunserve_shared_plan": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,
                                      c_int32, c_int32, c_int32, c_void_p, c_int64,
                                      POINTER(SharedPlanInfo)]),

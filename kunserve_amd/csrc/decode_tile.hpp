@@ -1,29 +1,12 @@
 // What the decode kernels share: the launch's arguments, the order of its
 // work, appending and combining rows, and the MFMA kernels' tile of K and V.
-// Everything is local to the source that includes this.
+// Kernels, their constants and device helpers are local to the source that includes
+// this.
 #pragma once
 
 #include "common.hpp"
 
 namespace kunserve {
-namespace {
-
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
-constexpr int kLoadsPerChunk = 4;        // 16-byte loads per lane per chunk (K and V each)
-constexpr int kMaxPartTokens = 4096;
-constexpr int kMinPageSize = 4;
-constexpr int kMaxPartPages = kMaxPartTokens / kMinPageSize + 2;
-constexpr int kMinPartTokens = 256;
-constexpr int kMinAutoPartTokens = 128;  // shortest the grouped plan chooses by itself: a step of every wave
-constexpr int kMaxCountedParts = 8;      // partitions a counting workgroup combines (one batch)
-constexpr int kMaxGroup = 16;            // query heads of one workgroup (MFMA columns)
-constexpr int kXcds = 8;                 // MI355X: workgroup b runs on XCD b % 8
-constexpr float kNegBig = -1.0e30f;      // finite "minus infinity" for running maxima
-
-// Source of the loads of lanes past a partition's end and of bad page ids:
-// one zero K/V row (head_dim <= 256), so loaded data is never masked.
-__device__ __attribute__((aligned(16))) f16 g_zero_row[256];
 
 struct DecodeArgs {
   const int32_t* q_token;   // null, or [num_seqs]: token of q and out of each sequence
@@ -62,6 +45,35 @@ struct DecodeArgs {
   int32_t ratio;            // num_qo_heads / num_kv_heads
   float scale_log2;         // sm_scale * log2(e)
 };
+
+// The launch's arguments, checked, for a plan of DecodeItems (paged_decode);
+// num_work 0: nothing to launch. And the launch that joins split rows.
+int decode_args(const kunserve_kv_pool* pool, int32_t layer, const kunserve_page_table* table,
+                const int32_t* q_token_dev, const kunserve_tensor3* q, kunserve_tensor3* out,
+                int32_t num_qo_heads, float sm_scale, const int32_t* plan_dev,
+                const kunserve_decode_plan_info* info, void* workspace_dev,
+                int64_t workspace_bytes, const StepFusion& fusion, DecodeArgs* args);
+int decode_merge(const kunserve_kv_pool* pool, const DecodeArgs& a,
+                 const kunserve_decode_plan_info* info, const int32_t* plan_dev, hipStream_t s);
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kLoadsPerChunk = 4;        // 16-byte loads per lane per chunk (K and V each)
+constexpr int kMaxPartTokens = 4096;
+constexpr int kMinPageSize = 4;
+constexpr int kMaxPartPages = kMaxPartTokens / kMinPageSize + 2;
+constexpr int kMinPartTokens = 256;
+constexpr int kMinAutoPartTokens = 128;  // shortest the grouped plan chooses by itself: a step of every wave
+constexpr int kMaxCountedParts = 8;      // partitions a counting workgroup combines (one batch)
+constexpr int kMaxGroup = 16;            // query heads of one workgroup (MFMA columns)
+constexpr int kXcds = 8;                 // MI355X: workgroup b runs on XCD b % 8
+constexpr float kNegBig = -1.0e30f;      // finite "minus infinity" for running maxima
+
+// Source of the loads of lanes past a partition's end and of bad page ids:
+// one zero K/V row (head_dim <= 256), so loaded data is never masked.
+__device__ __attribute__((aligned(16))) f16 g_zero_row[256];
 
 // Work record and head group of workgroup b. The hardware hands workgroup
 // b to XCD b % 8. The plan's records are 8 lanes interleaved (record
@@ -238,23 +250,24 @@ __device__ __forceinline__ float groups_max(float x) {
   return fmaxf(bits_to_f32(b[0]), bits_to_f32(b[1]));
 }
 
-// One head's attention over the tokens of a wave's steps, in fp32 on the vector
+// One head's attention over the tokens of a wave's steps (from t0 on, every
+// `stride`), in fp32 on the vector
 // units and a load at a time: what the MFMA kernel falls back to for values
 // that its products do not carry. Lane (row lane / CH, chunk lane % CH) holds
 // dims 8 chunk .. + 7 in acc, the same in every row after the merge; kb and vb
 // point at the lane's chunk.
-template <typename T, int D, int W>
+template <typename T, int D>
 __device__ __forceinline__ void wave_rows(const DecodeArgs& a, typename Vec<T>::v8 q, const f16* kb,
-                                          const f16* vb, int tb, int te, const int* s_pages,
-                                          const NewRow& nr, float& m, float& l, float (&acc)[8]) {
+                                          const f16* vb, int tb, int t0, int stride, int te,
+                                          const int* s_pages, const NewRow& nr, float& m, float& l,
+                                          float (&acc)[8]) {
   typedef DecodeTile<D> L;
   const int lane = threadIdx.x & (kWave - 1);
-  const int wave = threadIdx.x >> 6;
   m = kNegBig;
   l = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-  for (int t0 = tb + wave * L::STEP; t0 < te; t0 += W * L::STEP)
+  for (; t0 < te; t0 += stride)
 #pragma unroll 1
     for (int i = 0; i < L::LOADS; ++i) {
       const int t = t0 + L::TPL * i + lane / L::CH;

@@ -517,8 +517,8 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
 #pragma unroll 1
     for (int g = 0; g < G; ++g) {
       float m1, l1, acc[8];
-      wave_rows<T, D, W>(a, load_v8<T>(qp + int64_t(g) * a.q_head + 8 * lcol), kb, vb, tb, te,
-                         s_pages, nr, m1, l1, acc);
+      wave_rows<T, D>(a, load_v8<T>(qp + int64_t(g) * a.q_head + 8 * lcol), kb, vb, tb,
+                      tb + wave * STEP, W * STEP, te, s_pages, nr, m1, l1, acc);
       if (lrow == 0) {
         if (lcol == 0) {
           s_m[wave][g] = m1;
@@ -713,10 +713,27 @@ int launch_merge(const int32_t* merges, int num_merge, const int32_t* q_token, c
   return KUNSERVE_OK;
 }
 
+template <typename T>
+int run_merge(const DecodeArgs& a, const kunserve_decode_plan_info& info, const int32_t* plan_dev,
+              int head_dim, hipStream_t s) {
+  const int32_t* merges = plan_dev + 4 * int64_t(info.num_work);
+  switch (head_dim) {
+    case 64:
+      return launch_merge<T, 64>(merges, info.num_merge, a.q_token, a.part_o, a.part_lse, a.out, a.o_tok,
+                                 a.o_head, a.num_qo_heads, s);
+    case 128:
+      return launch_merge<T, 128>(merges, info.num_merge, a.q_token, a.part_o, a.part_lse, a.out, a.o_tok,
+                                  a.o_head, a.num_qo_heads, s);
+    default:
+      return launch_merge<T, 256>(merges, info.num_merge, a.q_token, a.part_o, a.part_lse, a.out, a.o_tok,
+                                  a.o_head, a.num_qo_heads, s);
+  }
+}
+
 // Partition kernel, then (for split rows) the merge, for element type T.
 template <typename T>
 int run_decode(const DecodeArgs& a, const kunserve_decode_plan_info& info, const int32_t* plan_dev,
-               int head_dim, int num_qo_heads, dim3 grid, hipStream_t s) {
+               int head_dim, dim3 grid, hipStream_t s) {
   int rc;
   switch (head_dim) {
     case 64: rc = launch_decode<T, 64>(a, grid, s); break;
@@ -725,18 +742,7 @@ int run_decode(const DecodeArgs& a, const kunserve_decode_plan_info& info, const
     default: set_error("head_dim %d not compiled", head_dim); return KUNSERVE_EUNSUPPORTED;
   }
   if (rc || info.num_merge == 0 || a.counters) return rc;
-  const int32_t* merges = plan_dev + 4 * int64_t(info.num_work);
-  switch (head_dim) {
-    case 64:
-      return launch_merge<T, 64>(merges, info.num_merge, a.q_token, a.part_o, a.part_lse, a.out, a.o_tok,
-                                 a.o_head, num_qo_heads, s);
-    case 128:
-      return launch_merge<T, 128>(merges, info.num_merge, a.q_token, a.part_o, a.part_lse, a.out, a.o_tok,
-                                  a.o_head, num_qo_heads, s);
-    default:
-      return launch_merge<T, 256>(merges, info.num_merge, a.q_token, a.part_o, a.part_lse, a.out, a.o_tok,
-                                  a.o_head, num_qo_heads, s);
-  }
+  return run_merge<T>(a, info, plan_dev, head_dim, s);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -808,6 +814,15 @@ static int32_t grouped_part_tokens(const int32_t* kv_len, int32_t n, int64_t hea
     }
   }
   return best;
+}
+
+int kunserve::decode_merge(const kunserve_kv_pool* pool, const DecodeArgs& a,
+                           const kunserve_decode_plan_info* info, const int32_t* plan_dev,
+                           hipStream_t s) {
+  if (info->num_merge == 0) return KUNSERVE_OK;
+  return pool->dtype == KUNSERVE_DTYPE_BF16
+             ? run_merge<bf16>(a, *info, plan_dev, pool->head_dim, s)
+             : run_merge<f16>(a, *info, plan_dev, pool->head_dim, s);
 }
 
 // Full partitions first, then tails by decreasing length, so the longest items
@@ -1006,13 +1021,12 @@ extern "C" int64_t kunserve_decode_workspace_bytes(const kunserve_decode_plan_in
   return slots * num_qo_heads * (int64_t(head_dim) + 1) * int64_t(sizeof(float));
 }
 
-int kunserve::paged_decode(const kunserve_kv_pool* pool, int32_t layer,
-                           const kunserve_page_table* table, const int32_t* q_token_dev,
-                           const kunserve_tensor3* q, kunserve_tensor3* out, int32_t num_qo_heads,
-                           float sm_scale, const int32_t* plan_dev,
-                           const kunserve_decode_plan_info* info, void* workspace_dev,
-                           int64_t workspace_bytes, const StepFusion& fusion,
-                           kunserve_stream_t stream) {
+int kunserve::decode_args(const kunserve_kv_pool* pool, int32_t layer,
+                          const kunserve_page_table* table, const int32_t* q_token_dev,
+                          const kunserve_tensor3* q, kunserve_tensor3* out, int32_t num_qo_heads,
+                          float sm_scale, const int32_t* plan_dev,
+                          const kunserve_decode_plan_info* info, void* workspace_dev,
+                          int64_t workspace_bytes, const StepFusion& fusion, DecodeArgs* args) {
   clear_error();
   int rc = check_pool(pool, true);
   if (rc) return rc;
@@ -1031,6 +1045,7 @@ int kunserve::paged_decode(const kunserve_kv_pool* pool, int32_t layer,
     set_error("unsupported group size %d", info->group_size);
     return KUNSERVE_EUNSUPPORTED;
   }
+  *args = DecodeArgs{};
   if (info->num_work == 0) return KUNSERVE_OK;
   KSV_CHECK_ARG(plan_dev && table->indptr_dev && table->indices_dev, "null plan or table");
   KSV_CHECK_ARG(q->data && out->data && aligned16(q->data) &&
@@ -1042,7 +1057,7 @@ int kunserve::paged_decode(const kunserve_kv_pool* pool, int32_t layer,
               (long long)ws_need);
     return KUNSERVE_ENOSPC;
   }
-  DecodeArgs a{};
+  DecodeArgs& a = *args;
   a.q_token = q_token_dev;
   a.q = static_cast<const f16*>(q->data);
   a.q_tok = q->token_stride;
@@ -1086,22 +1101,35 @@ int kunserve::paged_decode(const kunserve_kv_pool* pool, int32_t layer,
   a.num_qo_heads = num_qo_heads;
   a.ratio = ratio;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.group = info->group_size;
+  a.head_groups = num_qo_heads / info->group_size;
+  a.num_work = info->num_work;
+  return KUNSERVE_OK;
+}
 
+int kunserve::paged_decode(const kunserve_kv_pool* pool, int32_t layer,
+                           const kunserve_page_table* table, const int32_t* q_token_dev,
+                           const kunserve_tensor3* q, kunserve_tensor3* out, int32_t num_qo_heads,
+                           float sm_scale, const int32_t* plan_dev,
+                           const kunserve_decode_plan_info* info, void* workspace_dev,
+                           int64_t workspace_bytes, const StepFusion& fusion,
+                           kunserve_stream_t stream) {
+  DecodeArgs a;
+  const int rc = decode_args(pool, layer, table, q_token_dev, q, out, num_qo_heads, sm_scale,
+                             plan_dev, info, workspace_dev, workspace_bytes, fusion, &a);
+  if (rc || a.num_work == 0) return rc;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   // One dimension, mapped to (record, head group) by decode_work: on every
   // XCD the dispatch order is its lane's longest-first order (a launch ends
   // on short items), with an item's head groups, which read the same pages,
   // back to back.
-  a.group = info->group_size;
-  a.head_groups = num_qo_heads / info->group_size;
-  a.num_work = info->num_work;
   const int64_t nblocks = 8 * ceil_div(info->num_work, 8) * a.head_groups;
   KSV_CHECK_ARG(nblocks < (int64_t(1) << 31), "decode grid of %lld workgroups is too large",
                 (long long)nblocks);
   const dim3 grid(static_cast<unsigned>(nblocks));
   if (pool->dtype == KUNSERVE_DTYPE_BF16)
-    return run_decode<bf16>(a, *info, plan_dev, pool->head_dim, num_qo_heads, grid, s);
-  return run_decode<f16>(a, *info, plan_dev, pool->head_dim, num_qo_heads, grid, s);
+    return run_decode<bf16>(a, *info, plan_dev, pool->head_dim, grid, s);
+  return run_decode<f16>(a, *info, plan_dev, pool->head_dim, grid, s);
 }
 
 extern "C" int kunserve_paged_decode(const kunserve_kv_pool* pool, int32_t layer,

@@ -8,14 +8,14 @@
 // o_i and lse_i of disjoint token ranges,
 //   o = sum_i 2^(lse_i - lse) o_i,  lse = log2 sum_i 2^lse_i
 // so segments and tails are attended apart and joined as the partitions of a
-// split row are. The tails run in the decode kernels (paged_decode); this
-// file holds the plan and the kernel of the segments.
+// split row are.
 //
-// The kernel has the (row, query head of a KV head) pairs of a segment as the
-// columns of its products, up to 64 to a workgroup. K and V are read, parked
-// and transposed as in paged_decode_mfma_kernel; a step's operands serve every
-// 16-column tile, so a segment costs its bytes once and the matrix units
-// 16 columns at a time.
+// One launch for both: the matrix units' work on segments hides behind the
+// tails' bytes. The (row, query head of a KV head) pairs of a segment are the
+// columns of a workgroup's products, up to 64; a tail is a segment of one row.
+// K and V are read, parked and transposed as in paged_decode_mfma_kernel; a
+// step's operands serve every 16-column tile, so a segment costs its bytes once
+// and the matrix units 16 columns at a time.
 #include <algorithm>
 #include <cmath>
 #include <vector>
@@ -28,37 +28,164 @@ namespace {
 constexpr int kMinSegmentTokens = 64;   // shorter runs of shared pages stay with their rows
 constexpr int kRecord = 8;              // ints of a work record
 constexpr int kMinPieceTokens = 128;
+constexpr int kMinWideCols = 64;        // columns from which a segment's workgroups are wide
 
 struct SharedArgs {
-  DecodeArgs d;
+  DecodeArgs d;            // work: the tails'
   const int32_t* shared;   // [num_shared][kRecord]: rows (0: padding), their first pair,
-                           // token begin, end, place among a row's partials, a row of them
+                           // token begin, end, place among a row's partials, a row of them,
+                           // head group
   const int32_t* pairs;    // [...][2]: row, its first slot
   int32_t num_shared;
 };
 
-// Columns of a workgroup: 16-column tiles as the accumulators allow.
-constexpr int max_tiles(int head_dim) { return head_dim == 128 ? 4 : 2; }
+// Columns of a workgroup: 16, its waves taking the tokens in turn (narrow), or
+// kWideCols, every wave with columns of its own (wide, at head_dim 128).
+constexpr int kWideTiles = 2;                          // 16-column tiles of a wave
+constexpr int kWideCols = kWaves * kWideTiles * 16;    // 128
 
-template <typename T, int D, int CT>
-__global__ __launch_bounds__(kThreads, (CT == 4 || (CT == 2 && D == 256) ? 1 : 2)) void shared_decode_kernel(SharedArgs sa) {
+// Where a workgroup's columns are in q and out: pairs of rows and their first
+// partials, or one row (a tail: pairs null).
+struct Columns {
+  const int32_t* pairs;
+  int seq, group, hq0;
+  __device__ __forceinline__ int row(int c) const { return pairs ? pairs[2 * (c / group)] : seq; }
+  __device__ __forceinline__ int token(const DecodeArgs& a, int c) const {
+    return a.q_token ? a.q_token[row(c)] : row(c);
+  }
+  __device__ __forceinline__ int head(int c) const { return hq0 + c % group; }
+  __device__ __forceinline__ const f16* q(const DecodeArgs& a, int c) const {
+    return a.q + int64_t(token(a, c)) * a.q_tok + int64_t(head(c)) * a.q_head;
+  }
+};
+
+// Scores of a step's 16-token tiles (masked where `whole` is not set) to
+// probabilities of a column tile, in two 16-bit terms, with the lazy running
+// maximum of paged_decode_mfma_kernel; o: the column's accumulators.
+template <typename T, int D>
+__device__ __forceinline__ void tile_softmax(f32x4 (&sc)[DecodeTile<D>::PAIRS][2], float scale_log2,
+                                             float& m, float& lsum,
+                                             f32x4 (&o)[DecodeTile<D>::ACCS][8],
+                                             typename Vec<T>::v8 (&ph)[DecodeTile<D>::ACCS],
+                                             typename Vec<T>::v8 (&pl)[DecodeTile<D>::ACCS]) {
+  typedef DecodeTile<D> L;
+  typedef typename Vec<T>::v8 V8;
+  float mx = -INFINITY;
+#pragma unroll
+  for (int p = 0; p < L::PAIRS; ++p)
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) mx = fmaxf(mx, sc[p][sub][x]);
+  mx = groups_max(mx) * scale_log2;
+  if (__any(mx > m + 8.f)) {
+    const float m_new = mx > m + 8.f ? mx : m;
+    const float alpha = fast_exp2(m - m_new);
+    m = m_new;
+    lsum *= alpha;
+#pragma unroll
+    for (int x = 0; x < L::ACCS; ++x)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[x][e] *= alpha;
+  }
+#pragma unroll
+  for (int p = 0; p < L::PAIRS; ++p)
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float pr = fast_exp2(fmaf(sc[p][sub][x], scale_log2, -m));
+        lsum += pr;
+        const T hi = T(pr);
+        ph[p][4 * sub + x] = hi;
+        pl[p][4 * sub + x] = T(pr - float(hi));
+      }
+  if constexpr (D == 256) {   // set x takes the lane groups of its half of the row
+    const V8 zero = {};
+    const bool odd = (threadIdx.x >> 4) & 1;
+    ph[1] = odd ? ph[0] : zero;
+    pl[1] = odd ? pl[0] : zero;
+    ph[0] = odd ? zero : ph[0];
+    pl[0] = odd ? zero : pl[0];
+  }
+}
+
+// Step tokens past the partition, and those of page ids outside the pool.
+template <int D>
+__device__ __forceinline__ void mask_scores(f32x4 (&sc)[DecodeTile<D>::PAIRS][2], int t0, int te,
+                                            int tg, bool any_bad, const int* s_pages,
+                                            int page_shift, int pb) {
+  typedef DecodeTile<D> L;
+#pragma unroll
+  for (int p = 0; p < L::PAIRS; ++p)
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int t = t0 + L::token(4 * sub + x, tg, p);
+        bool drop = t >= te;
+        if (any_bad) drop |= s_pages[min((min(t, te - 1) >> page_shift) - pb, kMaxPartPages - 1)] < 0;
+        if (drop) sc[p][sub][x] = -INFINITY;
+      }
+}
+
+// vt[e]: dim 8 chunk + e of the lane's 8 tokens.
+template <typename V8>
+__device__ __forceinline__ void transpose8(const V8 (&v)[8], V8 (&vt)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    u32x4 d;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      d[x] = __builtin_amdgcn_perm(__builtin_bit_cast(u32x4, v[2 * x + 1])[e >> 1],
+                                   __builtin_bit_cast(u32x4, v[2 * x])[e >> 1],
+                                   (e & 1) ? 0x07060302u : 0x05040100u);
+    vt[e] = __builtin_bit_cast(V8, d);
+  }
+}
+
+// 0 x every sum: NaN where one is not finite (paged_decode_mfma_kernel).
+template <int D>
+__device__ __forceinline__ bool not_finite(const f32x4 (&o)[DecodeTile<D>::ACCS][8]) {
+  float z[4] = {};
+#pragma unroll
+  for (int x = 0; x < (D == 256 ? 2 : 1); ++x)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] = fmaf(o[x][e][i], 0.f, z[i]);
+  return __any(!(z[0] + z[1] + z[2] + z[3] == 0.f));
+}
+
+// A column's partial: its log-sum-exp, and its quotient of sums. A NaN score
+// makes the column's output NaN, at whatever weight.
+__device__ __forceinline__ float partial_lse(float m, float sum) {
+  return sum > 0.f ? m + __log2f(sum) : sum == 0.f ? -INFINITY : m;
+}
+
+template <typename T, int D, bool WIDE>
+__global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs sa) {
   typedef typename Vec<T>::v8 V8;
   typedef DecodeTile<D> L;
   constexpr int STEP = L::STEP, TPL = L::TPL, LOADS = L::LOADS, PAIRS = L::PAIRS;
   constexpr int BLK = STEP * D;
   constexpr int KS = D / 32;
   constexpr int W = kWaves;
-  constexpr int COLS = 16 * CT;
 
   const DecodeArgs& a = sa.d;
   __shared__ int s_pages[kMaxPartPages];
   __shared__ int s_bad[W];
-  // The waves' K blocks; after the loop, their O of 16 columns (fp32).
-  constexpr int kKBytes = W * BLK * int(sizeof(T)), kOBytes = W * 16 * D * int(sizeof(float));
+  // The waves' K blocks and, where they share columns, their V; after the loop of
+  // a narrow workgroup, the waves' O (fp32, 16 x D each).
+  constexpr int kKBytes = (WIDE ? 2 : 1) * W * BLK * int(sizeof(T));
+  constexpr int kOBytes = W * 16 * D * int(sizeof(float));
   __shared__ __attribute__((aligned(16))) char s_raw[kKBytes > kOBytes ? kKBytes : kOBytes];
   __shared__ float s_m[W][16];
   __shared__ float s_l[W][16];
-  __shared__ __attribute__((aligned(16))) T s_q[COLS * D];   // column g's chunk c at c ^ (g & 7)
+  // Q of a narrow workgroup at head_dim 256 (column g's chunk c at c ^ (g & 7)):
+  // in registers it would push the step's buffers out.
+  constexpr bool kQInLds = D == 256;
+  __shared__ __attribute__((aligned(16))) T s_q[kQInLds ? 16 * D : 8];
 
   const int tid = threadIdx.x;
   const int lane = tid & (kWave - 1);
@@ -67,32 +194,44 @@ __global__ __launch_bounds__(kThreads, (CT == 4 || (CT == 2 && D == 256) ? 1 : 2
   const int tg = lane >> 4;
   const int lrow = lane / L::CH;
   const int lcol = lane % L::CH;
-  const int G = a.group;
 
-  const int b = int(blockIdx.x);
-  const int local = (b >> 3) / a.head_groups;
-  const int hg = (b >> 3) - local * a.head_groups;
-  const int item = 8 * local + (b & 7);
-  if (item >= sa.num_shared) return;   // uniform, as the next
-  const int32_t* rec = sa.shared + kRecord * item;
-  const int nrows = rec[0];
-  if (nrows <= 0) return;
-  const int32_t* pairs = sa.pairs + 2 * rec[1];
-  const int tb = rec[2], te = rec[3], place = rec[4], rep = rec[5];
-  const int cols = nrows * G;
-  const int ntiles = (cols + 15) >> 4;
-  const int hq0 = hg * G;
+  // The segments' workgroups come first (a multiple of 8, so that those of the
+  // tails are on the XCDs their plan has them on).
+  int nrows = 1, hg, tb, te, place = 0, slot = -1;
+  Columns columns{nullptr, 0, a.group, 0};
+  const bool tail = int(blockIdx.x) >= sa.num_shared;   // uniform, as all of this
+  if (!tail) {
+    const int32_t* rec = sa.shared + kRecord * int(blockIdx.x);
+    nrows = rec[0];
+    if (nrows <= 0) return;
+    columns.pairs = sa.pairs + 2 * rec[1];
+    tb = rec[2];
+    te = rec[3];
+    place = rec[4];
+    columns.seq = rec[5];
+    hg = rec[6];
+  } else {
+    const int b = int(blockIdx.x) - sa.num_shared;
+    const int local = (b >> 3) / a.head_groups;
+    hg = (b >> 3) - local * a.head_groups;
+    const int item = 8 * local + (b & 7);
+    if (item >= a.num_work) return;
+    const int32_t* w = a.work + 4 * item;
+    columns.seq = w[0];
+    if (columns.seq < 0) return;
+    tb = w[1];
+    te = w[2];
+    slot = w[3];
+  }
+  const int cols = nrows * a.group;
+  const int hq0 = hg * a.group;
+  columns.hq0 = hq0;
   const int hkv = hq0 / a.ratio;
   const int page_mask = (1 << a.page_shift) - 1;
-  auto q_row = [&](int c) {   // q of column c
-    const int seq = pairs[2 * (c / G)];
-    const int tok = a.q_token ? a.q_token[seq] : seq;
-    return a.q + int64_t(tok) * a.q_tok + int64_t(hq0 + c % G) * a.q_head;
-  };
 
   const int pb = tb >> a.page_shift;
-  const int np = ((te - 1) >> a.page_shift) + 1 - pb;
-  const int32_t* seq_pages = a.indices + a.indptr[rep];
+  const int np = te > tb ? ((te - 1) >> a.page_shift) + 1 - pb : 0;
+  const int32_t* seq_pages = a.indices + a.indptr[columns.seq];
   bool bad_id = false;
   for (int i = tid; i < np; i += W * kWave) {
     const int p = seq_pages[pb + i];
@@ -102,21 +241,12 @@ __global__ __launch_bounds__(kThreads, (CT == 4 || (CT == 2 && D == 256) ? 1 : 2
   }
   const bool wave_bad = __any(bad_id);
   if (lane == 0) s_bad[wave] = wave_bad;
-  for (int i = tid; i < COLS * L::CH; i += W * kWave) {
-    const int g = i / L::CH, c = i % L::CH;
-    *reinterpret_cast<V8*>(&s_q[g * D + 8 * (c ^ (g & 7))]) =
-        g < cols ? load_v8<T>(q_row(g) + 8 * c) : V8{};
-  }
-  f32x4 o[CT][L::ACCS][8];
-  float m[CT], lsum[CT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    m[ct] = kNegBig;
-    lsum[ct] = 0.f;
-#pragma unroll
-    for (int x = 0; x < L::ACCS; ++x)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[ct][x][e] = f32x4{};
+  if constexpr (kQInLds) {
+    for (int i = tid; i < 16 * L::CH; i += W * kWave) {
+      const int g = i / L::CH, c = i % L::CH;
+      *reinterpret_cast<V8*>(&s_q[g * D + 8 * (c ^ (g & 7))]) =
+          g < cols ? load_v8<T>(columns.q(a, g) + 8 * c) : V8{};
+    }
   }
   __syncthreads();
   int bad_votes = 0;
@@ -124,10 +254,14 @@ __global__ __launch_bounds__(kThreads, (CT == 4 || (CT == 2 && D == 256) ? 1 : 2
   for (int wv = 0; wv < W; ++wv) bad_votes |= s_bad[wv];
   const bool any_bad = __builtin_amdgcn_readfirstlane(bad_votes) != 0;
 
+  const NewRow nr = tail ? new_row(a, columns.seq, columns.token(a, 0), hkv) : NewRow{-1, 0, 0};
+  if (nr.pos >= tb && nr.pos < te && hq0 % a.ratio == 0)
+    append_row<D>(a, nr, s_pages[(nr.pos >> a.page_shift) - pb], hkv);
   const f16* kb = a.k + int64_t(hkv) * a.head_stride + lcol * 8;
   const f16* vb = a.v + int64_t(hkv) * a.head_stride + lcol * 8;
   const int nsteps = (te - tb + STEP - 1) / STEP;
-  T* sk = reinterpret_cast<T*>(s_raw) + wave * BLK;
+  T* const blocks = reinterpret_cast<T*>(s_raw);
+  T* sk = blocks + wave * BLK;
 
   V8 k[LOADS], v[LOADS];
   auto load = [&](int c) {
@@ -137,226 +271,297 @@ __global__ __launch_bounds__(kThreads, (CT == 4 || (CT == 2 && D == 256) ? 1 : 2
       const int pi = min((t >> a.page_shift) - pb, kMaxPartPages - 1);
       const int p = (c < nsteps && t < te) ? s_pages[pi] : -1;
       const int64_t off = int64_t(max(p, 0)) * a.page_stride + int64_t(t & page_mask) * a.token_stride;
-      k[i] = load_v8<T>(p >= 0 ? kb + off : g_zero_row + lcol * 8);
-      v[i] = load_v8<T>(p >= 0 ? vb + off : g_zero_row + lcol * 8);
+      k[i] = load_v8<T>(p >= 0 ? kb + (t == nr.pos ? nr.k : off) : g_zero_row + lcol * 8);
+      v[i] = load_v8<T>(p >= 0 ? vb + (t == nr.pos ? nr.v : off) : g_zero_row + lcol * 8);
     }
   };
-  if (wave < nsteps) load(wave);
-  for (int c = wave; c < nsteps; c += W) {
+  auto park = [&] {   // K in the wave's block
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int t = TPL * i + lrow;
       *reinterpret_cast<V8*>(&sk[t * D + ((lcol ^ L::swz(t)) << 3)]) = k[i];
     }
-    V8 vt[8];   // vt[e]: dim 8 lcol + e of the lane's 8 tokens
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      u32x4 d;
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        d[x] = __builtin_amdgcn_perm(__builtin_bit_cast(u32x4, v[2 * x + 1])[e >> 1],
-                                     __builtin_bit_cast(u32x4, v[2 * x])[e >> 1],
-                                     (e & 1) ? 0x07060302u : 0x05040100u);
-      vt[e] = __builtin_bit_cast(V8, d);
-    }
-    load(c + W);
+  };
+  // Score tile row j of pair p, subtile sub: its token's chunks in a block.
+  auto k_row = [&](const T* block, int p, int sub, int s) {
+    const int t = L::token(4 * sub + (j & 3), j >> 2, p);
+    return *reinterpret_cast<const V8*>(&block[t * D + (((4 * s + tg) ^ L::swz(t)) << 3)]);
+  };
 
+  if constexpr (WIDE) {
+    if (cols > 16) {   // uniform
+      // Every wave has tiles of its own; a round of the loop is a step of each
+      // wave's tokens, which all waves take from LDS.
+      const int c0 = wave * kWideTiles * 16;
+      V8 q[kWideTiles][KS];
+#pragma unroll
+      for (int ct = 0; ct < kWideTiles; ++ct) {
+        const int c = c0 + 16 * ct + j;
+        const f16* qp = columns.q(a, min(c, cols - 1)) + 8 * tg;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[ct][s] = c < cols ? load_v8<T>(qp + 32 * s) : V8{};
+      }
+      f32x4 o[kWideTiles][L::ACCS][8];
+      float m[kWideTiles], lsum[kWideTiles];
+#pragma unroll
+      for (int ct = 0; ct < kWideTiles; ++ct) {
+        m[ct] = kNegBig;
+        lsum[ct] = 0.f;
+#pragma unroll
+        for (int x = 0; x < L::ACCS; ++x)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[ct][x][e] = f32x4{};
+      }
+      V8* const values = reinterpret_cast<V8*>(blocks + W * BLK);   // [wave][dim e][lane]
+      load(wave);
+      for (int c = 0; c < nsteps; c += W) {
+        park();
+        V8 vt[8];
+        transpose8(v, vt);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) values[(wave * 8 + e) * kWave + lane] = vt[e];
+        load(c + W + wave);
+        __syncthreads();
+        if (c0 < cols) {   // uniform
+          for (int blk = 0; blk < W && c + blk < nsteps; ++blk) {
+            const T* block = blocks + blk * BLK;
+            const int t0 = tb + (c + blk) * STEP;
+            f32x4 sc[kWideTiles][PAIRS][2];
+#pragma unroll
+            for (int p = 0; p < PAIRS; ++p)
+#pragma unroll
+              for (int sub = 0; sub < 2; ++sub) {
+#pragma unroll
+                for (int ct = 0; ct < kWideTiles; ++ct) sc[ct][p][sub] = f32x4{};
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                  const V8 ka = k_row(block, p, sub, s);
+#pragma unroll
+                  for (int ct = 0; ct < kWideTiles; ++ct)
+                    sc[ct][p][sub] = mfma16(ka, q[ct][s], sc[ct][p][sub]);
+                }
+              }
+            // Probabilities in one 16-bit term: at 64 columns and more the matrix
+            // units' work counts (128 rows behind 8192 tokens, 64 heads: 112 us a
+            // layer against 124 with the second term).
+            V8 ph[kWideTiles][L::ACCS], unused[L::ACCS];
+#pragma unroll
+            for (int ct = 0; ct < kWideTiles; ++ct) {
+              if (any_bad || t0 + STEP > te)
+                mask_scores<D>(sc[ct], t0, te, tg, any_bad, s_pages, a.page_shift, pb);
+              tile_softmax<T, D>(sc[ct], a.scale_log2, m[ct], lsum[ct], o[ct], ph[ct], unused);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const V8 ve = values[(blk * 8 + e) * kWave + lane];
+#pragma unroll
+              for (int x = 0; x < L::ACCS; ++x)
+#pragma unroll
+                for (int ct = 0; ct < kWideTiles; ++ct) {
+                  o[ct][x][e] = mfma16(ve, ph[ct][x], o[ct][x][e]);
+                }
+            }
+          }
+        }
+        __syncthreads();   // the round's blocks are done with
+      }
+#pragma unroll
+      for (int ct = 0; ct < kWideTiles; ++ct) {
+        const int first = c0 + 16 * ct;
+        if (first >= cols) break;   // uniform
+        float sum = lsum[ct];
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        auto partial = [&](int c) {
+          return int64_t(columns.pairs[2 * (c / a.group) + 1] + place) * a.num_qo_heads +
+                 columns.head(c);
+        };
+        if (not_finite<D>(o[ct])) {
+#pragma unroll 1
+          for (int c = first; c < min(first + 16, cols); ++c) {
+            float m1, l1, acc[8];
+            wave_rows<T, D>(a, load_v8<T>(columns.q(a, c) + 8 * lcol), kb, vb, tb, tb, STEP, te,
+                            s_pages, nr, m1, l1, acc);
+            const int64_t row = partial(c);
+            if (lrow == 0) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                a.part_o[row * D + 8 * lcol + e] = l1 == 0.f ? 0.f : acc[e] / l1;
+              if (lcol == 0) a.part_lse[row] = partial_lse(m1, l1);
+            }
+          }
+        } else if (first + j < cols) {
+          const int64_t row = partial(first + j);
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)   // dims 8 (4 tg + x) + 4 half ..
+              *reinterpret_cast<f32x4*>(a.part_o + row * D + 8 * (4 * tg + x) + 4 * half) =
+                  f32x4{o[ct][0][4 * half][x], o[ct][0][4 * half + 1][x],
+                        o[ct][0][4 * half + 2][x], o[ct][0][4 * half + 3][x]} * inv;
+          if (tg == 0) a.part_lse[row] = partial_lse(m[ct], sum);
+        }
+      }
+      return;
+    }
+  }
+
+  V8 qb[kQInLds ? 1 : KS];
+  if constexpr (!kQInLds) {
+    const f16* qp = columns.q(a, min(j, cols - 1)) + 8 * tg;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qb[s] = j < cols ? load_v8<T>(qp + 32 * s) : V8{};
+  }
+  f32x4 o[L::ACCS][8];
+#pragma unroll
+  for (int x = 0; x < L::ACCS; ++x)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[x][e] = f32x4{};
+  float m = kNegBig, lsum = 0.f;
+  if (wave < nsteps) load(wave);
+  for (int c = wave; c < nsteps; c += W) {
+    park();
+    V8 vt[8];
+    transpose8(v, vt);
+    load(c + W);
     // LDS runs a wave's accesses in order; keep the compiler from moving them.
+    f32x4 sc[PAIRS][2];
     __builtin_amdgcn_wave_barrier();
-    V8 ka[PAIRS][2][KS];
 #pragma unroll
     for (int p = 0; p < PAIRS; ++p)
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
-        const int t = L::token(4 * sub + (j & 3), j >> 2, p);   // tile row j
+        sc[p][sub] = f32x4{};
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
-          ka[p][sub][s] = *reinterpret_cast<const V8*>(&sk[t * D + (((4 * s + tg) ^ L::swz(t)) << 3)]);
+        for (int s = 0; s < KS; ++s) {
+          const V8 ka = k_row(sk, p, sub, s);
+          V8 qs;
+          if constexpr (kQInLds)
+            qs = *reinterpret_cast<const V8*>(&s_q[j * D + 8 * ((4 * s + tg) ^ (j & 7))]);
+          else
+            qs = qb[s];
+          sc[p][sub] = mfma16(ka, qs, sc[p][sub]);
+        }
       }
     __builtin_amdgcn_wave_barrier();
     const int t0 = tb + c * STEP;
-    const bool whole = !any_bad && t0 + STEP <= te;   // uniform: nothing to mask
+    if (any_bad || t0 + STEP > te)   // uniform
+      mask_scores<D>(sc, t0, te, tg, any_bad, s_pages, a.page_shift, pb);
+    V8 ph[L::ACCS], pl[L::ACCS];
+    tile_softmax<T, D>(sc, a.scale_log2, m, lsum, o, ph, pl);
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      if (ct >= ntiles) break;   // uniform
-      V8 qs[KS];
+    for (int e = 0; e < 8; ++e)
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
-        qs[s] = *reinterpret_cast<const V8*>(&s_q[(16 * ct + j) * D + 8 * ((4 * s + tg) ^ (j & 7))]);
-      f32x4 sc[PAIRS][2];
-      float mx = -INFINITY;
+      for (int x = 0; x < L::ACCS; ++x) o[x][e] = mfma16(vt[e], ph[x], o[x][e]);
 #pragma unroll
-      for (int p = 0; p < PAIRS; ++p)
+    for (int e = 0; e < 8; ++e)
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-          sc[p][sub] = f32x4{};
-#pragma unroll
-          for (int s = 0; s < KS; ++s) sc[p][sub] = mfma16(ka[p][sub][s], qs[s], sc[p][sub]);
-          if (!whole) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int t = t0 + L::token(4 * sub + x, tg, p);
-              bool drop = t >= te;
-              if (any_bad) drop |= s_pages[min((min(t, te - 1) >> a.page_shift) - pb, kMaxPartPages - 1)] < 0;
-              if (drop) sc[p][sub][x] = -INFINITY;
-            }
-          }
-#pragma unroll
-          for (int x = 0; x < 4; ++x) mx = fmaxf(mx, sc[p][sub][x]);
-        }
-      mx = groups_max(mx) * a.scale_log2;
-      if (__any(mx > m[ct] + 8.f)) {
-        const float m_new = mx > m[ct] + 8.f ? mx : m[ct];
-        const float alpha = fast_exp2(m[ct] - m_new);
-        m[ct] = m_new;
-        lsum[ct] *= alpha;
-#pragma unroll
-        for (int x = 0; x < L::ACCS; ++x)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[ct][x][e] *= alpha;
-      }
-      V8 ph[L::ACCS], pl[L::ACCS];   // probabilities: rounded, and what rounding left
-#pragma unroll
-      for (int p = 0; p < PAIRS; ++p)
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float pr = fast_exp2(fmaf(sc[p][sub][x], a.scale_log2, -m[ct]));
-            lsum[ct] += pr;
-            const T hi = T(pr);
-            ph[p][4 * sub + x] = hi;
-            pl[p][4 * sub + x] = T(pr - float(hi));
-          }
-      if constexpr (D == 256) {   // set x takes the lane groups of its half of the row
-        const V8 zero = {};
-        ph[1] = (tg & 1) ? ph[0] : zero;
-        pl[1] = (tg & 1) ? pl[0] : zero;
-        ph[0] = (tg & 1) ? zero : ph[0];
-        pl[0] = (tg & 1) ? zero : pl[0];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int x = 0; x < L::ACCS; ++x) {
-          o[ct][x][e] = mfma16(vt[e], ph[x], o[ct][x][e]);
-          o[ct][x][e] = mfma16(vt[e], pl[x], o[ct][x][e]);
-        }
-    }
+      for (int x = 0; x < L::ACCS; ++x) o[x][e] = mfma16(vt[e], pl[x], o[x][e]);
   }
 
-  // Tile by tile: the waves' sums joined, and the columns' partials written.
+  // The waves' sums joined, and the columns' outputs or partials written.
+  lsum += __shfl_xor(lsum, 16);
+  lsum += __shfl_xor(lsum, 32);
+  if constexpr (D == 256) lsum *= 0.5f;   // every token is in two of the groups
+  // At 64 a group's rows are chunks 4 (tg % 2) + row of set tg / 2's tokens: add
+  // the other set's, held by group tg ^ 2.
+  if constexpr (D == 64) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float own = tg >> 1 ? o[1][e][x] : o[0][e][x];
+        o[0][e][x] = own + __shfl_xor(own, 32);
+      }
+  }
+  const bool again = not_finite<D>(o);
+  __syncthreads();   // every wave is done with its K block
   float* s_o = reinterpret_cast<float*>(s_raw);
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    if (ct >= ntiles) break;   // uniform
-    float ls = lsum[ct];
-    ls += __shfl_xor(ls, 16);
-    ls += __shfl_xor(ls, 32);
-    if constexpr (D == 256) ls *= 0.5f;   // every token is in two of the groups
-    // At 64 a group's rows are chunks 4 (tg % 2) + row of set tg / 2's tokens:
-    // add the other set's, held by group tg ^ 2.
-    if constexpr (D == 64) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float own = tg >> 1 ? o[ct][1][e][x] : o[ct][0][e][x];
-          o[ct][0][e][x] = own + __shfl_xor(own, 32);
-        }
-    }
-    // Infinite and NaN values of V, as in paged_decode_mfma_kernel.
-    float z[4] = {};
-#pragma unroll
-    for (int x = 0; x < (D == 256 ? 2 : 1); ++x)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) z[i] = fmaf(o[ct][x][e][i], 0.f, z[i]);
-    const bool again = __any(!(z[0] + z[1] + z[2] + z[3] == 0.f));
-    const int here = min(16, cols - 16 * ct);   // columns of this tile
-    __syncthreads();   // the K blocks, or the tile before, are done with
-    auto unit_at = [&](int g, int unit) { return &s_o[(wave * 16 + g) * D + 4 * (unit ^ (g & 7))]; };
-    if (again) {
+  auto unit_at = [&](int g, int unit) { return &s_o[(wave * 16 + g) * D + 4 * (unit ^ (g & 7))]; };
+  if (again) {
 #pragma unroll 1
-      for (int g = 0; g < here; ++g) {
-        float m1, l1, acc[8];
-        wave_rows<T, D, W>(a, load_v8<T>(q_row(16 * ct + g) + 8 * lcol), kb, vb, tb, te, s_pages,
-                           NewRow{-1, 0, 0}, m1, l1, acc);
-        if (lrow == 0) {
-          if (lcol == 0) {
-            s_m[wave][g] = m1;
-            s_l[wave][g] = l1;
-          }
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-            *reinterpret_cast<f32x4*>(unit_at(g, 2 * lcol + half)) =
-                f32x4{acc[4 * half], acc[4 * half + 1], acc[4 * half + 2], acc[4 * half + 3]};
+    for (int g = 0; g < cols; ++g) {
+      float m1, l1, acc[8];
+      wave_rows<T, D>(a, load_v8<T>(columns.q(a, g) + 8 * lcol), kb, vb, tb, tb + wave * STEP,
+                      W * STEP, te, s_pages, nr, m1, l1, acc);
+      if (lrow == 0) {
+        if (lcol == 0) {
+          s_m[wave][g] = m1;
+          s_l[wave][g] = l1;
         }
-      }
-    } else if (j < here) {
-      if (tg == 0) {
-        s_m[wave][j] = m[ct];
-        s_l[wave][j] = ls;
-      }
-      if (D != 64 || tg < 2) {
 #pragma unroll
-        for (int x = 0; x < (D == 256 ? 2 : 1); ++x)
-#pragma unroll
-          for (int row = 0; row < 4; ++row)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              // dims 8 (4 tg + row + 16 x) + 4 half ..
-              const int unit = 2 * (4 * tg + row + 16 * x) + half;
-              *reinterpret_cast<f32x4*>(unit_at(j, unit)) =
-                  f32x4{o[ct][x][4 * half][row], o[ct][x][4 * half + 1][row],
-                        o[ct][x][4 * half + 2][row], o[ct][x][4 * half + 3][row]};
-            }
+        for (int half = 0; half < 2; ++half)
+          *reinterpret_cast<f32x4*>(unit_at(g, 2 * lcol + half)) =
+              f32x4{acc[4 * half], acc[4 * half + 1], acc[4 * half + 2], acc[4 * half + 3]};
       }
     }
-    __syncthreads();
-    for (int idx = tid; idx < here * (D / 4); idx += W * kWave) {
-      const int g = idx / (D / 4), unit = idx % (D / 4);
-      float mxw = kNegBig;
-#pragma unroll
-      for (int wv = 0; wv < W; ++wv) mxw = fmaxf(mxw, s_m[wv][g]);
-      float sum = 0.f;
-      f32x4 x = {};
-#pragma unroll
-      for (int wv = 0; wv < W; ++wv) {
-        const float f = fast_exp2(s_m[wv][g] - mxw);
-        sum += s_l[wv][g] * f;
-        x += *reinterpret_cast<const f32x4*>(&s_o[(wv * 16 + g) * D + 4 * (unit ^ (g & 7))]) * f;
-      }
-      const int c = 16 * ct + g;
-      const int64_t row = int64_t(pairs[2 * (c / G) + 1] + place) * a.num_qo_heads + hq0 + c % G;
-      // A NaN score makes the columns' outputs NaN, at whatever weight.
-      *reinterpret_cast<f32x4*>(a.part_o + row * D + 4 * unit) = sum == 0.f ? f32x4{} : x / sum;
-      if (unit == 0)
-        a.part_lse[row] = sum > 0.f ? mxw + __log2f(sum) : sum == 0.f ? -INFINITY : mxw;
+  } else if (j < cols) {
+    if (tg == 0) {
+      s_m[wave][j] = m;
+      s_l[wave][j] = lsum;
     }
+    if (D != 64 || tg < 2) {
+#pragma unroll
+      for (int x = 0; x < (D == 256 ? 2 : 1); ++x)
+#pragma unroll
+        for (int row = 0; row < 4; ++row)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            // dims 8 (4 tg + row + 16 x) + 4 half ..
+            const int unit = 2 * (4 * tg + row + 16 * x) + half;
+            *reinterpret_cast<f32x4*>(unit_at(j, unit)) =
+                f32x4{o[x][4 * half][row], o[x][4 * half + 1][row], o[x][4 * half + 2][row],
+                      o[x][4 * half + 3][row]};
+          }
+    }
+  }
+  __syncthreads();
+  for (int idx = tid; idx < cols * (D / 4); idx += W * kWave) {
+    const int g = idx / (D / 4), unit = idx % (D / 4);
+    float mxw = kNegBig;
+#pragma unroll
+    for (int wv = 0; wv < W; ++wv) mxw = fmaxf(mxw, s_m[wv][g]);
+    float sum = 0.f;
+    f32x4 x = {};
+#pragma unroll
+    for (int wv = 0; wv < W; ++wv) {
+      const float f = fast_exp2(s_m[wv][g] - mxw);
+      sum += s_l[wv][g] * f;
+      x += *reinterpret_cast<const f32x4*>(&s_o[(wv * 16 + g) * D + 4 * (unit ^ (g & 7))]) * f;
+    }
+    x = sum == 0.f ? f32x4{} : x / sum;
+    if (tail && slot < 0) {
+      T* op = reinterpret_cast<T*>(a.out) + int64_t(columns.token(a, g)) * a.o_tok +
+              int64_t(hq0 + g) * a.o_head + 4 * unit;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) op[i] = T(x[i]);
+      continue;
+    }
+    const int64_t row = int64_t(tail ? slot : columns.pairs[2 * (g / a.group) + 1] + place) *
+                            a.num_qo_heads + columns.head(g);
+    *reinterpret_cast<f32x4*>(a.part_o + row * D + 4 * unit) = x;
+    if (unit == 0) a.part_lse[row] = partial_lse(mxw, sum);
   }
 }
 
 template <typename T, int D>
-int launch_shared(const SharedArgs& a, int tiles, unsigned blocks, hipStream_t s) {
-  if (tiles == 1)
-    shared_decode_kernel<T, D, 1><<<blocks, kThreads, 0, s>>>(a);
-  else if (tiles == 2)
-    shared_decode_kernel<T, D, 2><<<blocks, kThreads, 0, s>>>(a);
+int launch_shared(const SharedArgs& a, bool wide, unsigned blocks, hipStream_t s) {
+  if (wide && D == 128)
+    shared_decode_kernel<T, D, D == 128><<<blocks, kThreads, 0, s>>>(a);
   else
-    shared_decode_kernel<T, D, max_tiles(D)><<<blocks, kThreads, 0, s>>>(a);
+    shared_decode_kernel<T, D, false><<<blocks, kThreads, 0, s>>>(a);
   KSV_CHECK_LAUNCH();
   return KUNSERVE_OK;
 }
 
 template <typename T>
-int launch_shared_dim(int head_dim, const SharedArgs& a, int tiles, unsigned blocks,
+int launch_shared_dim(int head_dim, const SharedArgs& a, bool wide, unsigned blocks,
                       hipStream_t s) {
   switch (head_dim) {
-    case 64: return launch_shared<T, 64>(a, tiles, blocks, s);
-    case 128: return launch_shared<T, 128>(a, tiles, blocks, s);
-    default: return launch_shared<T, 256>(a, tiles, blocks, s);
+    case 64: return launch_shared<T, 64>(a, wide, blocks, s);
+    case 128: return launch_shared<T, 128>(a, wide, blocks, s);
+    default: return launch_shared<T, 256>(a, wide, blocks, s);
   }
 }
 
@@ -430,19 +635,41 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
   std::vector<Segment> segments;
   find_segments(pages, count, page_size, order, segments);
 
-  // Segments in workgroups of whole rows; pieces of their tokens so that the
-  // device is filled once.
-  int32_t tiles = 1;
-  for (const Segment& s : segments)
-    tiles = std::max<int64_t>(tiles, std::min<int64_t>(max_tiles(head_dim),
-                                                       ceil_div(int64_t(s.hi - s.lo) * group, 16)));
-  if (tiles == 3) tiles = 4;
-  const int32_t tile_rows = 16 * tiles / group;   // group is 16 at most
-  int64_t work = 0;
-  for (const Segment& s : segments)
-    work += int64_t(s.end - s.begin) * ceil_div(s.hi - s.lo, tile_rows) * head_groups;
-  const int64_t piece = std::min<int64_t>(
-      kMaxPartTokens, std::max<int64_t>(kMinPieceTokens, 64 * ceil_div(work, 64 * cus)));
+  // Segments in workgroups of whole rows (group is 16 at most), wide ones where
+  // their columns are worth it; pieces of their tokens so that the device is
+  // filled.
+  auto is_wide = [&](const Segment& s) {
+    return head_dim == 128 && (s.hi - s.lo) * group >= kMinWideCols;
+  };
+  auto tile_rows = [&](const Segment& s) { return (is_wide(s) ? kWideCols : 16) / group; };
+  // us of a workgroup per token of its piece, and of the launch for the tails'
+  // bytes. A piece takes at most a CU's share of the segments' work (or 1.6 of it,
+  // for narrow ones, which run two and more to a CU), or what ends behind the
+  // tails: fewer pieces are fewer partials. 64 rows behind 2048 tokens, 32 heads on
+  // 8: 51.5 us in pieces of 512, 60 in pieces of 128; 128 rows behind 8192, 64 on 8:
+  // 112 in pieces of 2048, 125 in 1152, 154 in 4096.
+  auto token_us = [&](const Segment& s) {
+    return is_wide(s) ? 0.035 : 0.0115 * std::pow(head_dim / 128.0, 1.4);
+  };
+  double work = 0.0;   // of all segments' workgroups
+  int64_t tail_tokens = 0;
+  for (int32_t b = 0; b < num_seqs; ++b) tail_tokens += kv_len[b];
+  info->wide = 0;
+  for (const Segment& s : segments) {
+    work += token_us(s) * double(s.end - s.begin) *
+            double(ceil_div(s.hi - s.lo, tile_rows(s)) * head_groups);
+    tail_tokens -= int64_t(s.end - s.begin) * (s.hi - s.lo);
+    info->wide |= is_wide(s);
+  }
+  const double tails_us = double(tail_tokens) * num_kv_heads * head_dim * 4 / (6.6e6 * cus / 256);
+  const double share_us = work / double(cus);
+  auto pieces_of = [&](const Segment& s) {
+    const double most = std::min(double(kMaxPartTokens),
+                                 std::max(double(kMinPieceTokens),
+                                          std::max((is_wide(s) ? 1.0 : 1.6) * share_us,
+                                                   0.8 * tails_us) / token_us(s)));
+    return int64_t(std::ceil(double(s.end - s.begin) / most));
+  };
 
   // A row's partials: its segments' pieces, then its tail's partitions.
   std::vector<int32_t> partials(num_seqs, 0), covered(num_seqs, 0);
@@ -452,8 +679,7 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
   std::vector<Piece> pieces;
   for (size_t i = 0; i < segments.size(); ++i) {   // a parent comes before its children
     const Segment& s = segments[i];
-    const int32_t n = int32_t(ceil_div(s.end - s.begin, piece));
-    const int32_t len = int32_t(64 * ceil_div(s.end - s.begin, 64 * int64_t(n)));
+    const int32_t len = int32_t(64 * ceil_div(s.end - s.begin, 64 * pieces_of(s)));
     const int32_t first = partials[order[s.lo]];
     int32_t made = 0;
     for (int32_t t = s.begin; t < s.end; t += len, ++made)
@@ -492,8 +718,9 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
   info->decode.group_size = group;
   info->decode.plan_ints = int32_t(plan.size());
 
-  // Work records: a piece's row tiles on one XCD, one after the other (they
-  // read the same K and V), longest pieces first, to the XCD with least to do.
+  // Work records: the row tiles of a piece and head group, which read the same K
+  // and V, on one XCD, one after the other; longest pieces first, to the XCD with
+  // least to do.
   std::stable_sort(pieces.begin(), pieces.end(), [](const Piece& x, const Piece& y) {
     return x.end - x.begin > y.end - y.begin;
   });
@@ -508,13 +735,16 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
   size_t depth = 0;
   for (const Piece& p : pieces) {
     const Segment& s = segments[p.segment];
-    const int x = int(std::min_element(load, load + kXcds) - load);
-    for (int32_t r = s.lo; r < s.hi; r += tile_rows) {
-      lanes[x].insert(lanes[x].end(), {std::min(tile_rows, s.hi - r), pair_at[p.segment] + r - s.lo,
-                                       p.begin, p.end, p.place, order[s.lo], 0, 0});
-      load[x] += p.end - p.begin;
+    for (int32_t hg = 0; hg < head_groups; ++hg) {
+      const int x = int(std::min_element(load, load + kXcds) - load);
+      for (int32_t r = s.lo; r < s.hi; r += tile_rows(s)) {
+        lanes[x].insert(lanes[x].end(),
+                        {std::min(tile_rows(s), s.hi - r), pair_at[p.segment] + r - s.lo, p.begin,
+                         p.end, p.place, order[s.lo], hg, 0});
+        load[x] += p.end - p.begin;
+      }
+      depth = std::max(depth, lanes[x].size() / kRecord);
     }
-    depth = std::max(depth, lanes[x].size() / kRecord);
   }
   for (size_t r = 0; r < depth; ++r)
     for (int x = 0; x < kXcds; ++x)
@@ -522,7 +752,6 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
         plan.push_back(kRecord * r + i < lanes[x].size() ? lanes[x][kRecord * r + i] : 0);
   plan.insert(plan.end(), pairs.begin(), pairs.end());
   info->num_shared = int32_t(kXcds * depth);
-  info->tiles = tiles;
   info->num_pairs = int32_t(pairs.size() / 2);
   info->num_segments = int32_t(segments.size());
   info->head_dim = head_dim;
@@ -536,14 +765,16 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
 
 using namespace kunserve;
 
-extern "C" int64_t kunserve_shared_plan_bound(const int32_t* kv_len_host, int32_t num_seqs) {
-  if (num_seqs < 0 || (num_seqs > 0 && !kv_len_host)) return -1;
+extern "C" int64_t kunserve_shared_plan_bound(const int32_t* kv_len_host, int32_t num_seqs,
+                                              int32_t num_qo_heads) {
+  if (num_seqs < 0 || num_qo_heads <= 0 || (num_seqs > 0 && !kv_len_host)) return -1;
   // A row's partials: pieces and partitions of 64 tokens or more, but the last
   // of each of its segments, of which there is one to kMinSegmentTokens.
   int64_t partials = 0;
   for (int32_t b = 0; b < num_seqs; ++b)
     partials += 2 * ceil_div(std::max(kv_len_host[b], 0), kMinSegmentTokens) + 2;
-  return (4 * kXcds + kRecord * kXcds + 2) * partials + 4 * int64_t(num_seqs);
+  return (4 * kXcds + kRecord * kXcds * int64_t(num_qo_heads) + 2) * partials +
+         4 * int64_t(num_seqs);
 }
 
 extern "C" int kunserve_shared_plan(const int32_t* indptr_host, const int32_t* indices_host,
@@ -601,57 +832,28 @@ int kunserve::shared_decode(const kunserve_kv_pool* pool, int32_t layer,
   KSV_CHECK_ARG(info->decode.group_size == decode_group(num_qo_heads, pool->num_kv_heads),
                 "plan group size %d is not that of %d query heads on %d", info->decode.group_size,
                 num_qo_heads, pool->num_kv_heads);
-  if (info->num_shared > 0) {
-    KSV_CHECK_ARG(plan_dev && table->indptr_dev && table->indices_dev, "null plan or table");
-    KSV_CHECK_ARG(q->data && aligned16(q->data) && q->token_stride % 8 == 0 &&
-                      q->head_stride % 8 == 0,
-                  "q must be 16-byte aligned with strides that are multiples of 8");
-    const int64_t need =
-        kunserve_decode_workspace_bytes(&info->decode, num_qo_heads, pool->head_dim);
-    if (!workspace_dev || workspace_bytes < need) {
-      set_error("decode workspace holds %lld bytes, %lld needed", (long long)workspace_bytes,
-                (long long)need);
-      return KUNSERVE_ENOSPC;
-    }
-    KSV_CHECK_ARG(aligned16(workspace_dev), "workspace must be 16-byte aligned");
-    SharedArgs sa{};
-    DecodeArgs& a = sa.d;
-    a.q_token = q_token_dev;
-    a.q = static_cast<const f16*>(q->data);
-    a.q_tok = q->token_stride;
-    a.q_head = q->head_stride;
-    a.k = static_cast<const f16*>(pool->k) + int64_t(layer) * pool->layer_stride;
-    a.v = static_cast<const f16*>(pool->v) + int64_t(layer) * pool->layer_stride;
-    a.page_stride = pool->page_stride;
-    a.head_stride = pool->head_stride;
-    a.token_stride = pool->token_stride;
-    a.num_pages = int32_t(pool->num_pages);
-    a.page_shift = __builtin_ctz(pool->page_size);
-    a.indptr = table->indptr_dev;
-    a.indices = table->indices_dev;
-    a.part_o = static_cast<float*>(workspace_dev);
-    a.part_lse = a.part_o + int64_t(info->decode.num_slots) * num_qo_heads * pool->head_dim;
-    a.num_qo_heads = num_qo_heads;
-    a.group = info->decode.group_size;
-    a.head_groups = num_qo_heads / a.group;
-    a.ratio = num_qo_heads / pool->num_kv_heads;
-    a.scale_log2 = sm_scale * 1.4426950408889634f;
-    sa.shared = plan_dev + info->decode.plan_ints;
-    sa.pairs = sa.shared + kRecord * int64_t(info->num_shared);
-    sa.num_shared = info->num_shared;
-    const int64_t blocks = 8 * ceil_div(info->num_shared, 8) * a.head_groups;
-    KSV_CHECK_ARG(blocks < (int64_t(1) << 31), "grid of %lld workgroups is too large",
-                  (long long)blocks);
-    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    rc = pool->dtype == KUNSERVE_DTYPE_BF16
-             ? launch_shared_dim<bf16>(pool->head_dim, sa, info->tiles, unsigned(blocks), s)
-             : launch_shared_dim<f16>(pool->head_dim, sa, info->tiles, unsigned(blocks), s);
-    if (rc) return rc;
-  }
-  StepFusion tails = fusion;
-  tails.counters = nullptr;   // a row's partials are not its partitions alone
-  return paged_decode(pool, layer, table, q_token_dev, q, out, num_qo_heads, sm_scale, plan_dev,
-                      &info->decode, workspace_dev, workspace_bytes, tails, stream);
+  // Rows that share nothing run in the decode kernels.
+  if (info->num_segments == 0)
+    return paged_decode(pool, layer, table, q_token_dev, q, out, num_qo_heads, sm_scale, plan_dev,
+                        &info->decode, workspace_dev, workspace_bytes, fusion, stream);
+  SharedArgs sa{};
+  rc = decode_args(pool, layer, table, q_token_dev, q, out, num_qo_heads, sm_scale, plan_dev,
+                   &info->decode, workspace_dev, workspace_bytes, fusion, &sa.d);
+  if (rc) return rc;
+  KSV_CHECK_ARG(aligned16(workspace_dev), "workspace must be 16-byte aligned");
+  sa.shared = plan_dev + info->decode.plan_ints;
+  sa.pairs = sa.shared + kRecord * int64_t(info->num_shared);
+  sa.num_shared = info->num_shared;
+  const int64_t blocks = int64_t(info->num_shared) +
+                         8 * ceil_div(info->decode.num_work, 8) * sa.d.head_groups;
+  KSV_CHECK_ARG(blocks < (int64_t(1) << 31), "grid of %lld workgroups is too large",
+                (long long)blocks);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  rc = pool->dtype == KUNSERVE_DTYPE_BF16
+           ? launch_shared_dim<bf16>(pool->head_dim, sa, info->wide != 0, unsigned(blocks), s)
+           : launch_shared_dim<f16>(pool->head_dim, sa, info->wide != 0, unsigned(blocks), s);
+  if (rc) return rc;
+  return decode_merge(pool, sa.d, &info->decode, plan_dev, s);
 }
 
 extern "C" int kunserve_shared_decode(const kunserve_kv_pool* pool, int32_t layer,

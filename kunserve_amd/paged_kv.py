@@ -429,7 +429,7 @@ class SharedDecodePlan:
         if n and int(table.indptr_host[-1]) > indices.size:
             raise ValueError("the table's indptr runs past its indices")
         kv_ptr = kv.ctypes.data if n else None
-        cap = int(_lib.lib().kunserve_shared_plan_bound(kv_ptr, n))
+        cap = int(_lib.lib().kunserve_shared_plan_bound(kv_ptr, n, num_qo_heads))
         buf = np.empty(max(cap, 4), dtype=np.int32)   # the plan writes what it uses
         self.shared_info = _lib.SharedPlanInfo()
         _lib.call("kunserve_shared_plan", table.indptr_host.ctypes.data, indices.ctypes.data,
@@ -437,7 +437,7 @@ class SharedDecodePlan:
                   num_cus if num_cus is not None else _num_cus(device), buf.ctypes.data, buf.size,
                   ctypes.byref(self.shared_info))
         self.info = self.shared_info.decode
-        self.num_counters = 0
+        self.num_counters = 0   # a launch of its own joins the partials
         self.plan_host = buf[: self.shared_info.plan_ints].copy()
         self.plan = None
         if upload:

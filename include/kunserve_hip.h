@@ -360,13 +360,15 @@ int64_t kunserve_shared_plan_bound(const int32_t* kv_len_host, int32_t num_seqs,
  * with the same ids: every run of at least 64 tokens of whole pages that two
  * or more rows hold at the same place, before their new tokens' pages, is read
  * once for those rows (a prefix tree: rows may share a prefix of a prefix).
- * Rows that share nothing are planned as by kunserve_decode_plan_grouped. */
+ * Where that saves less than min_bytes of K and V in a layer (negative: what
+ * measured worth its cost), nothing is shared (num_segments 0). Rows that share
+ * nothing are planned as by kunserve_decode_plan_grouped. */
 int kunserve_shared_plan(const int32_t* indptr_host, const int32_t* indices_host,
                          const int32_t* kv_len_host, int32_t num_seqs,
                          int32_t num_qo_heads, int32_t num_kv_heads,
                          int32_t page_size, int32_t head_dim, int32_t num_cus,
-                         int32_t* plan_host, int64_t plan_capacity,
-                         kunserve_shared_plan_info* info);
+                         int64_t min_bytes, int32_t* plan_host,
+                         int64_t plan_capacity, kunserve_shared_plan_info* info);
 
 /* kunserve_paged_decode on such a plan, for the table it was made from (other
  * ids or lengths: not this plan). The workspace is 16-byte aligned and holds
@@ -479,9 +481,12 @@ typedef struct {
 } kunserve_kv_weights;
 
 typedef struct {
-  int64_t num_columns;   /* workspace entries (8 bytes each)                  */
+  int64_t num_columns;   /* observed (column, partition) entries              */
+  int64_t score_tokens;  /* cached tokens of the decode rows                  */
   int32_t num_items;     /* work records (row, partition)                     */
   int32_t num_combines;  /* records of the columns' combination               */
+  int32_t num_score_items; /* records of the decode rows' tokens              */
+  int32_t num_score_rows;  /* decode rows                                     */
   int32_t window;        /* observers of a row at most                        */
   int32_t num_qo_heads;  /* heads the plan was made for                       */
   int32_t plan_ints;     /* int32 entries of the plan buffer in use           */
@@ -492,15 +497,19 @@ int64_t kunserve_weights_plan_bound(const int32_t* q_indptr_host,
                                     const int32_t* kv_len_host, int32_t num_seqs,
                                     int32_t num_qo_heads, int32_t window);
 
-/* Host-side plan of kunserve_cache_weights, shared by every layer of a step. */
+/* Host-side plan of a step's attention weights, shared by its layers. Rows with a
+ * non-zero decodes_host[b] (NULL: none; they have one new token) are the decode
+ * rows of kunserve_attention_step_with, whose decode launch leaves its scores
+ * for the weights; the others are kunserve_cache_weights'. */
 int kunserve_weights_plan(const int32_t* q_indptr_host, const int32_t* kv_len_host,
                           int32_t num_seqs, int32_t num_qo_heads, int32_t window,
-                          int32_t* plan_host, int64_t plan_capacity,
-                          kunserve_weights_plan_info* info);
+                          const int32_t* decodes_host, int32_t* plan_host,
+                          int64_t plan_capacity, kunserve_weights_plan_info* info);
 
 int64_t kunserve_weights_workspace_bytes(const kunserve_weights_plan_info* info);
 
-/* What a step's attention says of the cache: for every row b with new tokens,
+/* What a step's attention says of the cache: for every row b with new tokens
+ * (but the plan's decode rows),
  * cached token t and KV head g,
  *   w := (t new ? 0 : w) + sum of softmax(q . K^T * sm_scale)[t]
  * over the last min(q_len[b], window) new tokens of the row that see t (their
@@ -611,8 +620,9 @@ int kunserve_attention_step(const kunserve_step* step, int32_t layer,
  * decode rows share pages, and run by this plan (shared_plan_dev) in place of
  * decode_plan_dev and without counters. weights.w not NULL: the attention
  * weights of the whole step's rows are added by this plan, after the attention,
- * in the workspace weights_workspace_dev; the step's pages are then private,
- * each in one place of the table. positions_dev (may be NULL): the tokens'
+ * in the workspace weights_workspace_dev (8-byte aligned); the plan's decode
+ * rows are then the step's, and the step's pages private, each in one place of
+ * the table. positions_dev (may be NULL): the tokens'
  * rotary positions (kunserve_rotary_append_kv). */
 typedef struct {
   const int32_t* shared_plan_dev;

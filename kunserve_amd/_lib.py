@@ -88,8 +88,9 @@ class KVWeights(Structure):
 
 
 class WeightsPlanInfo(Structure):
-    _fields_ = [("num_columns", c_int64), ("num_items", c_int32), ("num_combines", c_int32),
-                ("window", c_int32), ("num_qo_heads", c_int32), ("plan_ints", c_int32)]
+    _fields_ = [("num_columns", c_int64), ("score_tokens", c_int64), ("num_items", c_int32),
+                ("num_combines", c_int32), ("num_score_items", c_int32),
+                ("num_score_rows", c_int32), ("window", c_int32), ("num_qo_heads", c_int32), ("plan_ints", c_int32)]
 
 
 class Rotary(Structure):
@@ -138,7 +139,7 @@ SIGNATURES = {
                                           c_void_p, c_void_p]),
     "kunserve_shared_plan_bound": (c_int64, [c_void_p, c_int32, c_int32]),
     "kunserve_shared_plan": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,
-                                     c_int32, c_int32, c_int32, c_void_p, c_int64,
+                                     c_int32, c_int32, c_int32, c_int64, c_void_p, c_int64,
                                      POINTER(SharedPlanInfo)]),
     "kunserve_shared_decode": (c_int, [POINTER(KVPool), c_int32, POINTER(PageTable), c_void_p,
                                        POINTER(Tensor3), POINTER(Tensor3), c_int32, c_float,
@@ -146,7 +147,7 @@ SIGNATURES = {
                                        c_void_p]),
     "kunserve_weights_plan_bound": (c_int64, [c_void_p, c_void_p, c_int32, c_int32, c_int32]),
     "kunserve_weights_plan": (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p,
-                                      c_int64, POINTER(WeightsPlanInfo)]),
+                                      c_void_p, c_int64, POINTER(WeightsPlanInfo)]),
     "kunserve_weights_workspace_bytes": (c_int64, [POINTER(WeightsPlanInfo)]),
     "kunserve_cache_weights": (c_int, [POINTER(KVPool), POINTER(KVWeights), c_int32,
                                        POINTER(PageTable), c_void_p, POINTER(Tensor3), c_int32,

@@ -43,10 +43,11 @@ class KVWeights:
             raise ValueError(f"the weights {tuple(self.w.shape)} on {self.w.device} are not those "
                              f"of a pool {shape} on {pool.device}")
 
-    def plan(self, q_indptr_host, kv_len_host, num_qo_heads: int, window: int) -> "WeightsPlan":
+    def plan(self, q_indptr_host, kv_len_host, num_qo_heads: int, window: int,
+             decodes: Optional[Sequence[int]] = None) -> "WeightsPlan":
         """The plan of a step's rows, not yet on the device (WeightsPlan.bind)."""
         return WeightsPlan(q_indptr_host, kv_len_host, num_qo_heads, window, self.w.device,
-                           upload=False)
+                           upload=False, decodes=decodes)
 
     def add(self, pool: KVPool, layer: int, table: PageTable, q_indptr: torch.Tensor,
             q: torch.Tensor, plan: "WeightsPlan", sm_scale: Optional[float] = None,
@@ -57,10 +58,13 @@ class KVWeights:
 
 class WeightsPlan:
     """Work of add_weights for a step's rows, computed on the host once per step and
-    shared by every layer (kunserve_weights_plan)."""
+    shared by every layer (kunserve_weights_plan). decodes marks the rows whose
+    decode launch leaves its scores for the weights (AttentionStep's); add_weights
+    passes over them."""
 
     def __init__(self, q_indptr_host: Sequence[int], kv_len_host: Sequence[int],
-                 num_qo_heads: int, window: int, device: torch.device, upload: bool = True):
+                 num_qo_heads: int, window: int, device: torch.device, upload: bool = True,
+                 decodes: Optional[Sequence[int]] = None):
         qi, kv = _i32(q_indptr_host), _i32(kv_len_host)
         n = len(kv)
         if len(qi) != n + 1:
@@ -70,8 +74,11 @@ class WeightsPlan:
                                                          window))
         buf = np.empty(max(cap, 4), dtype=np.int32)   # the plan writes what it uses
         self.info = _lib.WeightsPlanInfo()
+        marks = None if decodes is None else _i32(decodes)
+        if marks is not None and marks.shape != (n,):
+            raise ValueError(f"{n} rows but {marks.shape} decode marks")
         _lib.call("kunserve_weights_plan", qi.ctypes.data, kv_ptr, n, num_qo_heads, window,
-                  buf.ctypes.data, buf.size, ctypes.byref(self.info))
+                  None if marks is None else marks.ctypes.data, buf.ctypes.data, buf.size, ctypes.byref(self.info))
         self.plan_host = buf[: self.info.plan_ints].copy()
         self.plan = None
         if upload:

@@ -76,10 +76,35 @@ extern "C" int kunserve_attention_step_with(const kunserve_step* step,
     return false;
   };
   int rc = KUNSERVE_OK;
-  if (weighted)   // they are formed from q after out is written
+  if (weighted) {   // they are formed from q after out is written
+    rc = check_weights(&extras->weights, &step->pool);
+    if (rc) return rc;
     KSV_CHECK_ARG(!kunserve_tensors_overlap(&out, step->num_qo_heads, &q, step->num_qo_heads,
                                             step->num_tokens, step->pool.head_dim),
                   "out overlaps q, which the attention weights are formed from");
+    const kunserve_weights_plan_info& info = extras->weights_info;
+    KSV_CHECK_ARG(info.num_qo_heads == step->num_qo_heads &&
+                      info.num_score_rows == step->decode_table.num_seqs,
+                  "the weights' plan is of another step");
+    KSV_CHECK_ARG(extras->shared_info.num_segments == 0, "rows that share pages have no weights");
+    const int64_t need = kunserve_weights_workspace_bytes(&info);
+    if (need > 0 && (!extras->weights_workspace_dev || extras->weights_workspace_bytes < need)) {
+      set_error("weights workspace holds %lld bytes, %lld needed",
+                (long long)extras->weights_workspace_bytes, (long long)need);
+      return KUNSERVE_ENOSPC;
+    }
+    KSV_CHECK_ARG((reinterpret_cast<uintptr_t>(extras->weights_workspace_dev) & 7u) == 0,
+                  "weights workspace must be 8-byte aligned");
+    KSV_CHECK_ARG(info.plan_ints == 0 || extras->weights_plan_dev, "null weights plan");
+    KSV_CHECK_ARG(step->pool.num_kv_heads < 65536, "%d KV heads: at most 65535",
+                  step->pool.num_kv_heads);
+    if (info.num_score_rows > 0) {
+      KSV_CHECK_ARG(step->decode_info.group_size ==
+                        decode_group(step->num_qo_heads, step->pool.num_kv_heads),
+                    "attention weights need a grouped decode plan");
+      weights_scores(&info, extras->weights_plan_dev, extras->weights_workspace_dev, &decode);
+    }
+  }
   if (rotary) {
     rc = kunserve_rotary_append_kv(&step->pool, layer, &step->table, step->q_indptr_dev,
                                    step->num_tokens, &q, &q, step->num_qo_heads, &io->k, &io->v,
@@ -116,12 +141,17 @@ extern "C" int kunserve_attention_step_with(const kunserve_step* step,
                        step->workspace_bytes, prefill, stream);
     if (rc) return rc;
   }
-  if (weighted)
+  if (weighted) {
+    rc = weights_from_scores(&step->pool, &extras->weights, layer, &step->decode_table,
+                             step->num_qo_heads, extras->weights_plan_dev, &extras->weights_info,
+                             extras->weights_workspace_dev, stream);
+    if (rc) return rc;
     return kunserve_cache_weights(&step->pool, &extras->weights, layer, &step->table,
                                   step->q_indptr_dev, &q, step->num_qo_heads, step->sm_scale,
                                   extras->weights_plan_dev, &extras->weights_info,
                                   extras->weights_workspace_dev, extras->weights_workspace_bytes,
                                   stream);
+  }
   return KUNSERVE_OK;
 }
 

@@ -11,7 +11,8 @@
 // launches: the maximum and sum of every column over each partition of
 // kPartTokens tokens; their combination; and the scores once more, this time
 // as probabilities summed over the columns. The sums run in one order, with no
-// atomics, so results do not depend on timing. A workgroup keeps its partition
+// atomics, so results do not depend on timing. A step's decode rows need no second
+// look at K: their decode launch leaves its scores. Of the three launches a workgroup keeps its partition
 // of K in registers (64 tokens a wave, as MFMA operands) and takes the columns
 // 16 at a time, so K is read once by each of the two launches.
 #include <algorithm>
@@ -197,6 +198,31 @@ __global__ __launch_bounds__(kThreads) void weights_combine_kernel(WeightsArgs a
   stats[int64_t(parts) * all] = float2{mx, sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum};
 }
 
+// Decode rows: the decode launch left their scores and log-sum-exps (DecodeArgs::
+// scores), so K is not read again: 4 bytes written and read per token and query
+// head beside the 4 head_dim bytes of K and V that a KV head's token has. A thread per
+// token and KV head.
+__global__ __launch_bounds__(kThreads) void weights_from_scores_kernel(
+    const int32_t* items, const float* scores, const float* lse, const int32_t* indptr,
+    const int32_t* indices, const int32_t* kv_len, int32_t num_pages, int32_t page_shift,
+    float* w, int64_t w_page, int64_t w_head, int32_t num_qo_heads, int32_t ratio, int32_t group) {
+  const int32_t* item = items + 4 * blockIdx.x;
+  const int seq = item[0], t = item[1] + threadIdx.x, hkv = blockIdx.y;
+  const int n = kv_len[seq];
+  if (t >= n) return;
+  const int p = indices[indptr[seq] + (t >> page_shift)];
+  if (p < 0 || p >= num_pages) return;
+  float sum = 0.f;
+  for (int h0 = hkv * ratio; h0 < (hkv + 1) * ratio; h0 += group) {   // a head group
+    const float* s = scores + int64_t(item[2]) * num_qo_heads +
+                     (int64_t(h0 / group) * n + t) * group;
+    const float* l = lse + int64_t(seq) * num_qo_heads + h0;
+    for (int g = 0; g < group; ++g) sum += fast_exp2(s[g] - l[g]);
+  }
+  float* at = w + int64_t(hkv) * w_head + int64_t(p) * w_page + (t & ((1 << page_shift) - 1));
+  *at = (t == n - 1 ? 0.f : *at) + sum;
+}
+
 template <typename T, int D>
 int run_weights(const WeightsArgs& a, const kunserve_weights_plan_info& info, hipStream_t s) {
   const dim3 grid(unsigned(info.num_items), unsigned(a.num_kv_heads));
@@ -222,14 +248,24 @@ int run_weights_dim(int head_dim, const WeightsArgs& a, const kunserve_weights_p
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int weights_plan(const int32_t* q_indptr, const int32_t* kv_len, int32_t num_seqs,
-                 int32_t num_qo_heads, int32_t window, std::vector<int32_t>& plan,
-                 kunserve_weights_plan_info* info) {
-  std::vector<int32_t> items, combines;
-  int64_t columns = 0;
+                 int32_t num_qo_heads, int32_t window, const int32_t* decodes,
+                 std::vector<int32_t>& plan, kunserve_weights_plan_info* info) {
+  std::vector<int32_t> items, combines, score_items, score_at;
+  int64_t columns = 0, score_tokens = 0;
   for (int32_t b = 0; b < num_seqs; ++b) {
     const int64_t q_len = int64_t(q_indptr[b + 1]) - q_indptr[b];
     KSV_CHECK_ARG(q_len >= 0 && kv_len[b] >= q_len, "row %d: kv_len %d for %lld new tokens", b,
                   kv_len[b], (long long)q_len);
+    if (decodes && decodes[b]) {
+      KSV_CHECK_ARG(q_len == 1, "row %d decodes %lld tokens", b, (long long)q_len);
+      const int32_t row = int32_t(score_at.size());
+      for (int32_t t = 0; t < kv_len[b]; t += kThreads)
+        score_items.insert(score_items.end(), {row, t, int32_t(score_tokens), 0});
+      score_at.push_back(int32_t(score_tokens));
+      score_tokens += kv_len[b];
+      KSV_CHECK_ARG(score_tokens < (int64_t(1) << 31), "too many cached tokens");
+      continue;
+    }
     if (q_len == 0) continue;
     const int64_t cols = std::min<int64_t>(q_len, window) * num_qo_heads;
     const int64_t parts = ceil_div(kv_len[b], kPartTokens);
@@ -245,6 +281,11 @@ int weights_plan(const int32_t* q_indptr, const int32_t* kv_len, int32_t num_seq
   info->num_items = int32_t(plan.size() / 4);
   plan.insert(plan.end(), combines.begin(), combines.end());
   info->num_combines = int32_t(combines.size() / 4);
+  plan.insert(plan.end(), score_items.begin(), score_items.end());
+  info->num_score_items = int32_t(score_items.size() / 4);
+  plan.insert(plan.end(), score_at.begin(), score_at.end());
+  info->num_score_rows = int32_t(score_at.size());
+  info->score_tokens = score_tokens;
   info->window = window;
   info->num_qo_heads = num_qo_heads;
   info->plan_ints = int32_t(plan.size());
@@ -267,14 +308,14 @@ extern "C" int64_t kunserve_weights_plan_bound(const int32_t* q_indptr_host,
   for (int32_t b = 0; b < num_seqs; ++b) {
     const int64_t q_len = std::max<int64_t>(0, int64_t(q_indptr_host[b + 1]) - q_indptr_host[b]);
     records += ceil_div(std::max(kv_len_host[b], 0), kPartTokens) +
-               ceil_div(std::min<int64_t>(q_len, window) * num_qo_heads, kThreads);
+               ceil_div(std::min<int64_t>(q_len, window) * num_qo_heads, kThreads) + 1;
   }
   return 4 * records;
 }
 
 extern "C" int kunserve_weights_plan(const int32_t* q_indptr_host, const int32_t* kv_len_host,
                                      int32_t num_seqs, int32_t num_qo_heads, int32_t window,
-                                     int32_t* plan_host, int64_t plan_capacity,
+                                     const int32_t* decodes_host, int32_t* plan_host, int64_t plan_capacity,
                                      kunserve_weights_plan_info* info) {
   clear_error();
   KSV_CHECK_ARG(info && plan_host, "null plan buffer or info");
@@ -284,8 +325,8 @@ extern "C" int kunserve_weights_plan(const int32_t* q_indptr_host, const int32_t
   KSV_CHECK_ARG(window > 0, "window %d must be positive", window);
   return no_throw([&] {
     std::vector<int32_t> plan;
-    const int rc = weights_plan(q_indptr_host, kv_len_host, num_seqs, num_qo_heads, window, plan,
-                                info);
+    const int rc = weights_plan(q_indptr_host, kv_len_host, num_seqs, num_qo_heads, window,
+                                decodes_host, plan, info);
     if (rc) return rc;
     if (int64_t(plan.size()) > plan_capacity) {
       set_error("plan needs %lld ints, capacity %lld", (long long)plan.size(),
@@ -299,7 +340,37 @@ extern "C" int kunserve_weights_plan(const int32_t* q_indptr_host, const int32_t
 
 extern "C" int64_t kunserve_weights_workspace_bytes(const kunserve_weights_plan_info* info) {
   if (!info) return -1;
-  return info->num_columns * int64_t(sizeof(float2));
+  return info->num_columns * int64_t(sizeof(float2)) +
+         (info->score_tokens + info->num_score_rows) * info->num_qo_heads * int64_t(sizeof(float));
+}
+
+void kunserve::weights_scores(const kunserve_weights_plan_info* info, const int32_t* plan_dev,
+                              void* workspace_dev, StepFusion* fusion) {
+  float* at = reinterpret_cast<float*>(static_cast<float2*>(workspace_dev) + info->num_columns);
+  fusion->scores = at;
+  fusion->lse = at + info->score_tokens * info->num_qo_heads;
+  fusion->score_at = plan_dev + 4 * (int64_t(info->num_items) + info->num_combines +
+                                     info->num_score_items);
+}
+
+int kunserve::weights_from_scores(const kunserve_kv_pool* pool, const kunserve_kv_weights* weights,
+                                  int32_t layer, const kunserve_page_table* decode_table,
+                                  int32_t num_qo_heads, const int32_t* plan_dev,
+                                  const kunserve_weights_plan_info* info, void* workspace_dev,
+                                  kunserve_stream_t stream) {
+  if (info->num_score_items == 0) return KUNSERVE_OK;
+  StepFusion f;
+  weights_scores(info, plan_dev, workspace_dev, &f);
+  const int group = decode_group(num_qo_heads, pool->num_kv_heads);
+  weights_from_scores_kernel<<<dim3(unsigned(info->num_score_items), unsigned(pool->num_kv_heads)),
+                               kThreads, 0, reinterpret_cast<hipStream_t>(stream)>>>(
+      plan_dev + 4 * (int64_t(info->num_items) + info->num_combines), f.scores, f.lse,
+      decode_table->indptr_dev, decode_table->indices_dev, decode_table->kv_len_dev,
+      int32_t(pool->num_pages), __builtin_ctz(pool->page_size),
+      weights->w + int64_t(layer) * weights->layer_stride, weights->page_stride,
+      weights->head_stride, num_qo_heads, num_qo_heads / pool->num_kv_heads, group);
+  KSV_CHECK_LAUNCH();
+  return KUNSERVE_OK;
 }
 
 extern "C" int kunserve_cache_weights(const kunserve_kv_pool* pool,

@@ -78,13 +78,17 @@ int check_weights(const kunserve_kv_weights* weights, const kunserve_kv_pool* po
 
 // What a decode or prefill launch can take on beside attention: the append of
 // its rows' new K/V (k_new and v_new; the caller has checked
-// kunserve_new_pages_private), and combining split rows (zeroed counters, as
-// many as kunserve_decode_counters or kunserve_prefill_counters says).
+// kunserve_new_pages_private), combining split rows (zeroed counters, as many as
+// kunserve_decode_counters or kunserve_prefill_counters says), and, of a decode
+// launch, its scores (DecodeArgs::scores).
 struct StepFusion {
   const kunserve_tensor3* k_new = nullptr;
   const kunserve_tensor3* v_new = nullptr;
   int32_t* counters = nullptr;
   int64_t num_counters = 0;
+  float* scores = nullptr;
+  float* lse = nullptr;
+  const int32_t* score_at = nullptr;
 };
 int paged_decode(const kunserve_kv_pool* pool, int32_t layer, const kunserve_page_table* table,
                  const int32_t* q_token_dev, const kunserve_tensor3* q, kunserve_tensor3* out,
@@ -97,6 +101,16 @@ int shared_decode(const kunserve_kv_pool* pool, int32_t layer, const kunserve_pa
                   int32_t num_qo_heads, float sm_scale, const int32_t* plan_dev,
                   const kunserve_shared_plan_info* info, void* workspace_dev,
                   int64_t workspace_bytes, const StepFusion& fusion, kunserve_stream_t stream);
+
+// The attention weights of a step's decode rows from the scores that their decode
+// launch left in the plan's workspace (weights_scores says where).
+void weights_scores(const kunserve_weights_plan_info* info, const int32_t* plan_dev,
+                    void* workspace_dev, StepFusion* fusion);
+int weights_from_scores(const kunserve_kv_pool* pool, const kunserve_kv_weights* weights,
+                        int32_t layer, const kunserve_page_table* decode_table,
+                        int32_t num_qo_heads, const int32_t* plan_dev,
+                        const kunserve_weights_plan_info* info, void* workspace_dev,
+                        kunserve_stream_t stream);
 
 // Pieces of the decode plan for plans that add to it. An item: tokens [b, e) of
 // a sequence, its partial's slot (-1: the output itself). decode_records orders

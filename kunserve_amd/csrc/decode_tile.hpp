@@ -34,6 +34,13 @@ struct DecodeArgs {
   // null, or one zeroed counter per (first slot of a split row, head group):
   // the last of the row's workgroups to finish combines the partials.
   int32_t* counters;
+  // null, or where the launch leaves its scores (in log2 units) and every row's
+  // log-sum-exp: of row b, head group hg, token t and head g of the group at
+  // scores[score_at[b] * num_qo_heads + (hg * kv_len[b] + t) * group + g], and
+  // lse[b * num_qo_heads + head]. A NaN score makes a log-sum-exp NaN.
+  float* scores;
+  float* lse;
+  const int32_t* score_at;
   int32_t part_tokens;
   const int32_t* work;      // [num_work][4]: seq (-1: padding), tok_begin, tok_end, slot (-1: direct)
   float* part_o;            // [slots][num_qo_heads][D]
@@ -155,6 +162,7 @@ __device__ __forceinline__ void decode_finish(const DecodeArgs& a, int seq, int 
     result(g, d, x, y, lse);
     if (slot < 0) {
       write_out(g, d, x, y);
+      if (d == 0 && a.lse) a.lse[int64_t(seq) * a.num_qo_heads + hq0 + g] = lse;
       continue;
     }
     const int64_t row = int64_t(slot) * a.num_qo_heads + hq0 + g;
@@ -218,6 +226,8 @@ __device__ __forceinline__ void decode_finish(const DecodeArgs& a, int seq, int 
     }
     const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
     write_out(g, d, x * inv, y * inv);
+    if (d == 0 && a.lse)
+      a.lse[int64_t(seq) * a.num_qo_heads + hq0 + g] = wsum == 0.f ? -INFINITY : mx + __log2f(wsum);
   }
 }
 
@@ -241,6 +251,12 @@ struct DecodeTile {
     return D == 64 ? ((t >> 3) & 3) | ((t & 2) << 1) : D == 128 ? t & 15 : t & 7;
   }
 };
+
+// A row's log-sum-exp from its maximum and sum; for a launch that leaves its
+// scores, NaN where a score is.
+__device__ __forceinline__ float row_lse(const DecodeArgs& a, float m, float sum) {
+  return sum > 0.f ? m + __log2f(sum) : a.lse && sum != sum ? sum : -INFINITY;
+}
 
 // Maximum and sum over the four 16-lane groups.
 __device__ __forceinline__ float groups_max(float x) {

@@ -40,7 +40,8 @@ namespace {
 template <typename T, int G>
 constexpr int valu_waves() { return G == 1 ? (__is_same(T, f16) ? 5 : 4) : G == 2 ? 4 : 3; }
 
-template <typename T, int D, int G>
+// SCORES: the launch leaves its scores (DecodeArgs::scores).
+template <typename T, int D, int G, bool SCORES = false>
 __global__ __launch_bounds__(kThreads, (valu_waves<T, G>())) void paged_decode_kernel(DecodeArgs a) {
   typedef typename Vec<T>::v8 V8;
   constexpr int LPT = D / 8;            // lanes per token row (16 for D = 128)
@@ -123,7 +124,10 @@ __global__ __launch_bounds__(kThreads, (valu_waves<T, G>())) void paged_decode_k
       ch.v[i] = load_v8_nt<T>(ch.ok[i] ? vb + (t == nr.pos ? nr.v : off) : g_zero_row + col * 8);
     }
   };
-  auto consume = [&](const Chunk& ch) {
+  float* scores = nullptr;   // of the row and head group
+  if constexpr (SCORES)
+    scores = a.scores + int64_t(a.score_at[seq]) * a.num_qo_heads + int64_t(hg) * a.kv_len[seq] * G;
+  auto consume = [&](const Chunk& ch, int chunk) {
     float vf[kLoadsPerChunk][8];
 #pragma unroll
     for (int i = 0; i < kLoadsPerChunk; ++i)
@@ -138,6 +142,11 @@ __global__ __launch_bounds__(kThreads, (valu_waves<T, G>())) void paged_decode_k
         s[i] = group_sum<LPT>(dot8(qv[g], ch.k[i], 0.f)) * a.scale_log2;
         s[i] = ch.ok[i] ? s[i] : -INFINITY;
         mx = fmaxf(mx, s[i]);
+      }
+      if constexpr (SCORES) {   // a row's lane i has token i of its four
+        const float mine = col == 0 ? s[0] : col == 1 ? s[1] : col == 2 ? s[2] : s[3];
+        const int t = tb + chunk * CHUNK + col * TPL + row;
+        if (col < kLoadsPerChunk && t < te) scores[int64_t(t) * G + g] = mine;
       }
       const float alpha = fast_exp2(m[g] - mx);
       m[g] = mx;
@@ -167,11 +176,11 @@ __global__ __launch_bounds__(kThreads, (valu_waves<T, G>())) void paged_decode_k
     load_chunk(c, c0);
     while (true) {
       load_chunk(c + kWaves, c1);
-      consume(c0);
+      consume(c0, c);
       c += kWaves;
       if (c >= nchunks) break;
       load_chunk(c + kWaves, c0);
-      consume(c1);
+      consume(c1, c);
       c += kWaves;
       if (c >= nchunks) break;
     }
@@ -225,7 +234,7 @@ __global__ __launch_bounds__(kThreads, (valu_waves<T, G>())) void paged_decode_k
     }
     x = lsum > 0.f ? x / lsum : 0.f;
     y = lsum > 0.f ? y / lsum : 0.f;
-    lse = lsum > 0.f ? mx + __log2f(lsum) : -INFINITY;
+    lse = SCORES ? row_lse(a, mx, lsum) : lsum > 0.f ? mx + __log2f(lsum) : -INFINITY;
   });
 }
 
@@ -269,7 +278,7 @@ __global__ __launch_bounds__(kThreads, (valu_waves<T, G>())) void paged_decode_k
 //    meets one does its tokens again (wave_rows).
 //  * Online softmax per head column in fp32 with a lazy running max, merged
 //    across waves through LDS; partial results as in the VALU kernel.
-template <typename T, int D, int W>
+template <typename T, int D, int W, bool SCORES = false>
 __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(2)))
 void paged_decode_mfma_kernel(DecodeArgs a) {
   typedef typename Vec<T>::v8 V8;
@@ -358,6 +367,9 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
   const f16* vb = a.v + int64_t(hkv) * a.head_stride + lcol * 8;
   const int nsteps = (te - tb + STEP - 1) / STEP;
   T* sk = reinterpret_cast<T*>(s_raw) + wave * BLK;
+  float* scores = nullptr;   // of the row and head group
+  if constexpr (SCORES)
+    scores = a.scores + int64_t(a.score_at[seq]) * a.num_qo_heads + int64_t(hg) * a.kv_len[seq] * G;
 
   // Unconditional loads (see the VALU kernel): past-the-end lanes and bad
   // page ids read the zero row.
@@ -440,6 +452,19 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
           if (drop) sc[p][sub][x] = -INFINITY;
           mx = fmaxf(mx, sc[p][sub][x]);
         }
+    if constexpr (SCORES) {   // at 256 lane groups 2 g and 2 g + 1 have the same ones
+      if (j < G && !(D == 256 && (tg & 1))) {
+#pragma unroll
+        for (int p = 0; p < PAIRS; ++p)
+#pragma unroll
+          for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int t = t0 + L::token(4 * sub + x, tg, p);
+              if (t < te) scores[int64_t(t) * G + j] = sc[p][sub][x] * a.scale_log2;
+            }
+      }
+    }
     mx = groups_max(mx) * a.scale_log2;
     if (__any(mx > m + 8.f)) {
       const float m_new = mx > m + 8.f ? mx : m;
@@ -568,7 +593,7 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
     }
     x = ls > 0.f ? x / ls : 0.f;
     y = ls > 0.f ? y / ls : 0.f;
-    lse = ls > 0.f ? mxw + __log2f(ls) : -INFINITY;
+    lse = SCORES ? row_lse(a, mxw, ls) : ls > 0.f ? mxw + __log2f(ls) : -INFINITY;
   });
 }
 
@@ -582,7 +607,7 @@ __global__ __launch_bounds__(kWave) void decode_merge_kernel(const int32_t* merg
                                                              const float* part_o,
                                                              const float* part_lse, T* out,
                                                              int64_t o_tok, int64_t o_head,
-                                                             int32_t num_qo_heads) {
+                                                             int32_t num_qo_heads, float* lse_out) {
   constexpr int DPL = D / kWave;
   typedef float PartVec __attribute__((ext_vector_type(DPL)));
   const int32_t* mg = merges + 4 * blockIdx.x;
@@ -637,6 +662,8 @@ __global__ __launch_bounds__(kWave) void decode_merge_kernel(const int32_t* merg
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) wsum += __shfl_xor(wsum, off);
   const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+  if (lse_out && lane == 0)
+    lse_out[int64_t(seq) * num_qo_heads + hq] = wsum == 0.f ? -INFINITY : mx + __log2f(wsum);
   const int tok = q_token ? q_token[seq] : seq;
   T* dst = out + int64_t(tok) * o_tok + int64_t(hq) * o_head + lane * DPL;
 #pragma unroll
@@ -688,27 +715,26 @@ int64_t max_counted_workgroups(int group, int head_dim, int64_t cus) {
   return cus * (head_dim == 256 ? 1 : std::min(3, resident_workgroups(group, head_dim)));
 }
 
-template <typename T, int D>
+template <typename T, int D, bool SCORES>
 int launch_decode(const DecodeArgs& a, dim3 grid, hipStream_t s) {
   if (uses_mfma(a.group, D))
-    paged_decode_mfma_kernel<T, D, 4><<<grid, kThreads, 0, s>>>(a);
+    paged_decode_mfma_kernel<T, D, 4, SCORES><<<grid, kThreads, 0, s>>>(a);
   else if (a.group == 2)
-    paged_decode_kernel<T, D, 2><<<grid, kThreads, 0, s>>>(a);
+    paged_decode_kernel<T, D, 2, SCORES><<<grid, kThreads, 0, s>>>(a);
   else if (D == 64 && a.group == 4)
-    paged_decode_kernel<T, D == 64 ? D : 64, 4><<<grid, kThreads, 0, s>>>(a);
+    paged_decode_kernel<T, D == 64 ? D : 64, 4, SCORES><<<grid, kThreads, 0, s>>>(a);
   else
-    paged_decode_kernel<T, D, 1><<<grid, kThreads, 0, s>>>(a);
+    paged_decode_kernel<T, D, 1, SCORES><<<grid, kThreads, 0, s>>>(a);
   KSV_CHECK_LAUNCH();
   return KUNSERVE_OK;
 }
 
 template <typename T, int D>
-int launch_merge(const int32_t* merges, int num_merge, const int32_t* q_token, const float* po,
-                 const float* pl, f16* out, int64_t o_tok, int64_t o_head, int hq, hipStream_t s) {
-  dim3 grid(num_merge, hq);
-  decode_merge_kernel<T, D><<<grid, kWave, 0, s>>>(merges, q_token, po, pl,
-                                                   reinterpret_cast<T*>(out),
-                                                   o_tok, o_head, hq);
+int launch_merge(const DecodeArgs& a, const int32_t* merges, int num_merge, hipStream_t s) {
+  dim3 grid(num_merge, a.num_qo_heads);
+  decode_merge_kernel<T, D><<<grid, kWave, 0, s>>>(merges, a.q_token, a.part_o, a.part_lse,
+                                                   reinterpret_cast<T*>(a.out), a.o_tok, a.o_head,
+                                                   a.num_qo_heads, a.lse);
   KSV_CHECK_LAUNCH();
   return KUNSERVE_OK;
 }
@@ -718,15 +744,9 @@ int run_merge(const DecodeArgs& a, const kunserve_decode_plan_info& info, const 
               int head_dim, hipStream_t s) {
   const int32_t* merges = plan_dev + 4 * int64_t(info.num_work);
   switch (head_dim) {
-    case 64:
-      return launch_merge<T, 64>(merges, info.num_merge, a.q_token, a.part_o, a.part_lse, a.out, a.o_tok,
-                                 a.o_head, a.num_qo_heads, s);
-    case 128:
-      return launch_merge<T, 128>(merges, info.num_merge, a.q_token, a.part_o, a.part_lse, a.out, a.o_tok,
-                                  a.o_head, a.num_qo_heads, s);
-    default:
-      return launch_merge<T, 256>(merges, info.num_merge, a.q_token, a.part_o, a.part_lse, a.out, a.o_tok,
-                                  a.o_head, a.num_qo_heads, s);
+    case 64: return launch_merge<T, 64>(a, merges, info.num_merge, s);
+    case 128: return launch_merge<T, 128>(a, merges, info.num_merge, s);
+    default: return launch_merge<T, 256>(a, merges, info.num_merge, s);
   }
 }
 
@@ -736,9 +756,9 @@ int run_decode(const DecodeArgs& a, const kunserve_decode_plan_info& info, const
                int head_dim, dim3 grid, hipStream_t s) {
   int rc;
   switch (head_dim) {
-    case 64: rc = launch_decode<T, 64>(a, grid, s); break;
-    case 128: rc = launch_decode<T, 128>(a, grid, s); break;
-    case 256: rc = launch_decode<T, 256>(a, grid, s); break;
+    case 64: rc = a.scores ? launch_decode<T, 64, true>(a, grid, s) : launch_decode<T, 64, false>(a, grid, s); break;
+    case 128: rc = a.scores ? launch_decode<T, 128, true>(a, grid, s) : launch_decode<T, 128, false>(a, grid, s); break;
+    case 256: rc = a.scores ? launch_decode<T, 256, true>(a, grid, s) : launch_decode<T, 256, false>(a, grid, s); break;
     default: set_error("head_dim %d not compiled", head_dim); return KUNSERVE_EUNSUPPORTED;
   }
   if (rc || info.num_merge == 0 || a.counters) return rc;
@@ -1096,7 +1116,13 @@ int kunserve::decode_args(const kunserve_kv_pool* pool, int32_t layer,
       fusion.num_counters >= int64_t(info->num_slots) * (num_qo_heads / info->group_size) &&
       (reinterpret_cast<uintptr_t>(ws) & 7) == 0)
     a.counters = fusion.counters;
-  a.kv_len = a.k_new || a.counters ? table->kv_len_dev : nullptr;
+  if (fusion.scores) {
+    KSV_CHECK_ARG(fusion.lse && fusion.score_at && table->kv_len_dev, "null lse, score_at or kv_len");
+    a.scores = fusion.scores;
+    a.lse = fusion.lse;
+    a.score_at = fusion.score_at;
+  }
+  a.kv_len = a.k_new || a.counters || a.scores ? table->kv_len_dev : nullptr;
   a.part_tokens = info->part_tokens;
   a.num_qo_heads = num_qo_heads;
   a.ratio = ratio;

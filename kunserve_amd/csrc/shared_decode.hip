@@ -26,6 +26,12 @@ namespace kunserve {
 namespace {
 
 constexpr int kMinSegmentTokens = 64;   // shorter runs of shared pages stay with their rows
+// Bytes of K and V that sharing has to save in a layer: joining the partials in a
+// launch of their own takes about 4 us. Per layer, shared against not: 3 rows
+// behind 6917 tokens (4 KV heads of 64, 14 MB saved) 14.2 against 18.5 us, 7 behind
+// 851 (8 of 128, 19 MB) 11.6 against 13.0; 5 behind 672 (11 MB) 11.5 against 9.9, 12
+// behind 100 (4 MB) 11.6 against 8.7.
+constexpr int64_t kMinSavedBytes = 13 << 20;
 constexpr int kRecord = 8;              // ints of a work record
 constexpr int kMinPieceTokens = 128;
 constexpr int kMinWideCols = 64;        // columns from which a segment's workgroups are wide
@@ -616,7 +622,7 @@ void find_segments(const std::vector<const int32_t*>& pages, const std::vector<i
 
 int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv_len,
                 int32_t num_seqs, int32_t num_qo_heads, int32_t num_kv_heads, int32_t page_size,
-                int32_t head_dim, int32_t num_cus, std::vector<int32_t>& plan,
+                int32_t head_dim, int32_t num_cus, int64_t min_bytes, std::vector<int32_t>& plan,
                 kunserve_shared_plan_info* info) {
   const int group = decode_group(num_qo_heads, num_kv_heads);
   const int64_t head_groups = num_qo_heads / group;
@@ -634,6 +640,10 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
   std::vector<int32_t> order;
   std::vector<Segment> segments;
   find_segments(pages, count, page_size, order, segments);
+  int64_t saved = 0;   // K and V tokens that are not read again
+  for (const Segment& s : segments) saved += int64_t(s.end - s.begin) * (s.hi - s.lo - 1);
+  if (saved * num_kv_heads * head_dim * 4 < (min_bytes < 0 ? kMinSavedBytes * cus / 256 : min_bytes))
+    segments.clear();
 
   // Segments in workgroups of whole rows (group is 16 at most), wide ones where
   // their columns are worth it; pieces of their tokens so that the device is
@@ -780,8 +790,9 @@ extern "C" int64_t kunserve_shared_plan_bound(const int32_t* kv_len_host, int32_
 extern "C" int kunserve_shared_plan(const int32_t* indptr_host, const int32_t* indices_host,
                                     const int32_t* kv_len_host, int32_t num_seqs,
                                     int32_t num_qo_heads, int32_t num_kv_heads, int32_t page_size,
-                                    int32_t head_dim, int32_t num_cus, int32_t* plan_host,
-                                    int64_t plan_capacity, kunserve_shared_plan_info* info) {
+                                    int32_t head_dim, int32_t num_cus, int64_t min_bytes,
+                                    int32_t* plan_host, int64_t plan_capacity,
+                                    kunserve_shared_plan_info* info) {
   clear_error();
   KSV_CHECK_ARG(info && plan_host, "null plan buffer or info");
   KSV_CHECK_ARG(num_seqs >= 0 && (num_seqs == 0 || (indptr_host && indices_host && kv_len_host)),
@@ -797,7 +808,7 @@ extern "C" int kunserve_shared_plan(const int32_t* indptr_host, const int32_t* i
   return no_throw([&] {
     std::vector<int32_t> plan;
     const int rc = shared_plan(indptr_host, indices_host, kv_len_host, num_seqs, num_qo_heads,
-                               num_kv_heads, page_size, head_dim, num_cus, plan, info);
+                               num_kv_heads, page_size, head_dim, num_cus, min_bytes, plan, info);
     if (rc) return rc;
     if (int64_t(plan.size()) > plan_capacity) {
       set_error("plan needs %lld ints, capacity %lld", (long long)plan.size(),

@@ -419,11 +419,12 @@ class SharedDecodePlan:
     """Plan of decode rows whose page lists begin alike (kunserve_shared_plan),
     computed on the host once per step and shared by every layer. Runs of whole
     pages that two or more rows hold at the same place are read once for them;
-    num_segments counts these runs."""
+    num_segments counts these runs, none if they save less than min_bytes of K and V
+    in a layer (None: what measured worth its cost)."""
 
     def __init__(self, table: "PageTable", num_qo_heads: int, num_kv_heads: int, page_size: int,
                  device: torch.device, num_cus: Optional[int] = None, upload: bool = True,
-                 head_dim: int = 128):
+                 head_dim: int = 128, min_bytes: Optional[int] = None):
         n = table.num_seqs
         kv, indices = table.kv_len_host, table.indices_host
         if n and int(table.indptr_host[-1]) > indices.size:
@@ -434,7 +435,8 @@ class SharedDecodePlan:
         self.shared_info = _lib.SharedPlanInfo()
         _lib.call("kunserve_shared_plan", table.indptr_host.ctypes.data, indices.ctypes.data,
                   kv_ptr, n, num_qo_heads, num_kv_heads, page_size, head_dim,
-                  num_cus if num_cus is not None else _num_cus(device), buf.ctypes.data, buf.size,
+                  num_cus if num_cus is not None else _num_cus(device),
+                  -1 if min_bytes is None else min_bytes, buf.ctypes.data, buf.size,
                   ctypes.byref(self.shared_info))
         self.info = self.shared_info.decode
         self.num_counters = 0   # a launch of its own joins the partials
@@ -775,7 +777,8 @@ class AttentionStep:
     stage runs its global layer indices on its local layers.
 
     share_prefixes: decode rows whose page lists begin alike read the pages they
-    share once (SharedDecodePlan); a step that shares nothing runs as without.
+    share once (SharedDecodePlan), where that saves share_min_bytes of K and V in a
+    layer (None: what measured worth its cost); other steps run as without.
 
     weights (a KVWeights of the pool): every layer adds the attention weight that
     each cached token got to it, from a decode row's token and from the last
@@ -802,7 +805,7 @@ class AttentionStep:
                  is_context_stage: Optional[Sequence[int]] = None, layer_offset: int = 0,
                  id_map: Optional[Callable[[np.ndarray], np.ndarray]] = None,
                  num_ids: Optional[int] = None, share_prefixes: bool = False,
-                 weights=None, window: int = 16,
+                 share_min_bytes: Optional[int] = None, weights=None, window: int = 16,
                  rope_positions: Optional[Sequence[int]] = None):
         self.pool = pool
         self.num_qo_heads = num_qo_heads
@@ -868,7 +871,8 @@ class AttentionStep:
             plan = None
             if share_prefixes and dec_rows.size > 1:
                 plan = SharedDecodePlan(table, num_qo_heads, pool.num_kv_heads, pool.page_size,
-                                        dev, upload=False, head_dim=pool.head_dim)
+                                        dev, upload=False, head_dim=pool.head_dim,
+                                        min_bytes=share_min_bytes)
                 plan = plan if plan.num_segments else None
             if plan is None:
                 plan = DecodePlan(self.kv_len[dec_rows], num_qo_heads, pool.num_kv_heads, dev,
@@ -894,7 +898,8 @@ class AttentionStep:
             uploads.append([positions])
         self._weights_plan = None
         if weights is not None:
-            self._weights_plan = weights.plan(self.q_indptr_host, self.kv_len, num_qo_heads, window)
+            self._weights_plan = weights.plan(self.q_indptr_host, self.kv_len, num_qo_heads, window,
+                                              is_decode)
             uploads.append(self._weights_plan)
 
         # Counters with which the launches combine their split rows (the
@@ -1066,6 +1071,9 @@ class AttentionStep:
             paged_prefill(self.pool, local, p.table, p.q_indptr, q, p.plan, self.scale,
                           out=out, workspace=self.workspace, q_start=p.tokens)
         if self.weights is not None:
-            self.weights.add(self.pool, local, self.table, self.q_indptr, q, self._weights_plan,
-                             self.scale, self._weights_workspace)
+            # Every row through add_weights: these launches left no scores.
+            plan = self.weights.plan(self.q_indptr_host, self.kv_len, self.num_qo_heads,
+                                     self._weights_plan.info.window)
+            plan.bind(_upload_packed(plan.host_arrays(), self._device))
+            self.weights.add(self.pool, local, self.table, self.q_indptr, q, plan, self.scale)
         return out

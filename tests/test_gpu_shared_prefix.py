@@ -45,7 +45,8 @@ def run(device, specs, hq, hkv, ps, d, dtype, seed=0, layers=2, layer=1, poke=No
     if poke:
         poke(pool, tables)
     before = [pool.k.clone(), pool.v.clone()]
-    step = AttentionStep(pool, hq, [1] * n, kvs, [0] * n, tables, share_prefixes=True, **kw)
+    step = AttentionStep(pool, hq, [1] * n, kvs, [0] * n, tables, share_prefixes=True,
+                         share_min_bytes=0, **kw)
     out = step.run(layer, q, k, v)
     torch.cuda.synchronize()
     # the new tokens are appended, nothing else changes
@@ -136,7 +137,8 @@ def test_within_a_mixed_step(device):
     q_lens, first, flag = [1, 1, 30, 1], [161, 200, 20, 170], [0, 0, 1, 0]
     q, k, v = (random_tensor((33, h, 128), device, 9 + h) for h in (8, 2, 2))
     twin = KVPool(pool.k.clone(), pool.v.clone())
-    out = AttentionStep(pool, 8, q_lens, first, flag, tables, share_prefixes=True).run(0, q, k, v)
+    out = AttentionStep(pool, 8, q_lens, first, flag, tables, share_prefixes=True,
+                        share_min_bytes=0).run(0, q, k, v)
     want = AttentionStep(twin, 8, q_lens, first, flag, tables).run(0, q, k, v)
     assert torch.equal(pool.k.view(torch.int16), twin.k.view(torch.int16))
     assert torch.equal(out[2:32].view(torch.int16), want[2:32].view(torch.int16))
@@ -195,7 +197,7 @@ def test_page_ids_outside_the_pool_drop_out(device):
     kvs = [160, 200]
     indptr = np.r_[0, np.cumsum([len(t) for t in bad])]
     table = PageTable(indptr, np.concatenate(bad), kvs, device)
-    plan = SharedDecodePlan(table, 8, 2, 16, device)
+    plan = SharedDecodePlan(table, 8, 2, 16, device, min_bytes=0)
     assert plan.num_segments == 1
     q = random_tensor((2, 8, 128), device, 12, 2.0)
     out = shared_decode(pool, 0, table, q, plan)
@@ -214,7 +216,8 @@ def test_captured_layer_replays(device):
     tables, pages = tree(rng, 16, [([("r", 20)], n) for n in kvs])
     pool = random_pool(pages, 1, 2, 16, 128, device, 13)
     q, k, v = (random_tensor((3, h, 128), device, 14 + h) for h in (8, 2, 2))
-    step = AttentionStep(pool, 8, [1] * 3, kvs, [0] * 3, tables, share_prefixes=True)
+    step = AttentionStep(pool, 8, [1] * 3, kvs, [0] * 3, tables, share_prefixes=True,
+                         share_min_bytes=0)
     out = torch.empty_like(q)
     eager = step.run(0, q, k, v).clone()
     graph = torch.cuda.CUDAGraph()
@@ -256,13 +259,13 @@ def test_refusals(device):
     pool = random_pool(pages, 1, 2, 16, 128, device, 15)
     table = PageTable.from_lists(tables, [160, 200], pool)
     q = random_tensor((2, 8, 128), device, 16)
-    plan = SharedDecodePlan(table, 16, 2, 16, device)
+    plan = SharedDecodePlan(table, 16, 2, 16, device, min_bytes=0)
     with pytest.raises(RuntimeError, match="group size"):
         shared_decode(pool, 0, table, q, plan)
-    plan = SharedDecodePlan(table, 8, 2, 16, device, head_dim=64)
+    plan = SharedDecodePlan(table, 8, 2, 16, device, head_dim=64, min_bytes=0)
     with pytest.raises(RuntimeError, match="head_dim"):
         shared_decode(pool, 0, table, q, plan)
-    plan = SharedDecodePlan(table, 8, 2, 16, device)
+    plan = SharedDecodePlan(table, 8, 2, 16, device, min_bytes=0)
     with pytest.raises(ValueError, match="rows"):
         shared_decode(pool, 0, table, q[:1], plan)
     with pytest.raises(RuntimeError, match="sm_scale"):

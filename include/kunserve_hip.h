@@ -515,7 +515,8 @@ int64_t kunserve_weights_workspace_bytes(const kunserve_weights_plan_info* info)
  * over the last min(q_len[b], window) new tokens of the row that see t (their
  * positions are t or later) and the query heads of g. The step's K is in its
  * pages already and q rotated. No page may be in two places of the table. Slots
- * past a row's end and pages outside the pool are left as they are. */
+ * past a row's end and pages outside the pool are left as they are. The
+ * workspace is 16-byte aligned. */
 int kunserve_cache_weights(const kunserve_kv_pool* pool,
                            const kunserve_kv_weights* weights, int32_t layer,
                            const kunserve_page_table* table,
@@ -620,7 +621,7 @@ int kunserve_attention_step(const kunserve_step* step, int32_t layer,
  * decode rows share pages, and run by this plan (shared_plan_dev) in place of
  * decode_plan_dev and without counters. weights.w not NULL: the attention
  * weights of the whole step's rows are added by this plan, after the attention,
- * in the workspace weights_workspace_dev (8-byte aligned); the plan's decode
+ * in the workspace weights_workspace_dev (16-byte aligned); the plan's decode
  * rows are then the step's, and the step's pages private, each in one place of
  * the table. positions_dev (may be NULL): the tokens'
  * rotary positions (kunserve_rotary_append_kv). */

@@ -93,8 +93,8 @@ extern "C" int kunserve_attention_step_with(const kunserve_step* step,
                 (long long)extras->weights_workspace_bytes, (long long)need);
       return KUNSERVE_ENOSPC;
     }
-    KSV_CHECK_ARG((reinterpret_cast<uintptr_t>(extras->weights_workspace_dev) & 7u) == 0,
-                  "weights workspace must be 8-byte aligned");
+    KSV_CHECK_ARG(aligned16(extras->weights_workspace_dev),
+                  "weights workspace must be 16-byte aligned");
     KSV_CHECK_ARG(info.plan_ints == 0 || extras->weights_plan_dev, "null weights plan");
     KSV_CHECK_ARG(step->pool.num_kv_heads < 65536, "%d KV heads: at most 65535",
                   step->pool.num_kv_heads);

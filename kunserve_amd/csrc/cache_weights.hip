@@ -28,6 +28,9 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kSubs = 4;                            // 16-token tiles of a wave
 constexpr int kPartTokens = kWaves * kSubs * 16;    // 256
+constexpr int kCols = 64;                           // columns in LDS at a time
+// Partitions up to which the last launch combines the columns itself.
+constexpr int kMaxOwnParts = 64;
 constexpr float kNegBig = -1.0e30f;                 // finite "minus infinity" for running maxima
 
 struct WeightsArgs {
@@ -51,24 +54,44 @@ struct WeightsArgs {
 
 // Maximum and sum over the four 16-lane groups.
 __device__ __forceinline__ float across_groups_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  const auto a = __builtin_amdgcn_permlane16_swap(f32_to_bits(x), f32_to_bits(x), false, false);
+  x = fmaxf(bits_to_f32(a[0]), bits_to_f32(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(f32_to_bits(x), f32_to_bits(x), false, false);
+  return fmaxf(bits_to_f32(b[0]), bits_to_f32(b[1]));
 }
 __device__ __forceinline__ float across_groups_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+  const auto a = __builtin_amdgcn_permlane16_swap(f32_to_bits(x), f32_to_bits(x), false, false);
+  x = bits_to_f32(a[0]) + bits_to_f32(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(f32_to_bits(x), f32_to_bits(x), false, false);
+  return bits_to_f32(b[0]) + bits_to_f32(b[1]);
 }
 
-// ADD false: the partition's maxima and sums; true: its tokens' weights.
-template <typename T, int D, bool ADD>
+// m and l of two disjoint sets of scores.
+__device__ __forceinline__ float2 join(float2 x, float2 y) {
+  const float m = fmaxf(x.x, y.x);
+  return {m, x.y * fast_exp2(x.x - m) + y.y * fast_exp2(y.x - m)};
+}
+// What a probability is formed with: the maximum, and 1 / sum (a NaN sum stays).
+__device__ __forceinline__ float2 normaliser(float2 s) {
+  return {s.x, s.y > 0.f ? 1.f / s.y : s.y};
+}
+
+// ADD false: the partition's maxima and sums; true: its tokens' weights. COMBINE
+// (with ADD): it combines the partitions' maxima and sums itself.
+// Columns come kCols at a time: their q through LDS, the next ones' on the way
+// meanwhile.
+template <typename T, int D, bool ADD, bool COMBINE>
 __global__ __launch_bounds__(kThreads) void weights_scores_kernel(WeightsArgs a) {
   typedef typename Vec<T>::v8 V8;
   constexpr int KS = D / 32;   // MFMAs of a 16-token tile
-  __shared__ float2 s_stat[2][kWaves][16];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  constexpr int CH = D / 8;    // 16-byte chunks of a row
+  constexpr int QL = kCols * CH / kThreads;
+  __shared__ __attribute__((aligned(16))) T s_q[kCols * D];   // column g's chunk c at c ^ (g & 7)
+  __shared__ float2 s_stat[kWaves][kCols];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6;
   const int j = lane & 15, tg = lane >> 4;
   const int32_t* item = a.items + 4 * blockIdx.x;
-  const int seq = item[0], part0 = item[1], hkv = blockIdx.y;
+  const int seq = item[0], part0 = item[1], hkv = blockIdx.y, parts = item[3];
   const int64_t offset = item[2];
   const int n = a.kv_len[seq], q0 = a.q_indptr[seq], q_len = a.q_indptr[seq + 1] - q0;
   const int obs = min(q_len, a.window);       // observers
@@ -82,6 +105,18 @@ __global__ __launch_bounds__(kThreads) void weights_scores_kernel(WeightsArgs a)
     const int p = pages[t >> a.page_shift];
     return p >= 0 && p < a.num_pages ? p : -1;
   };
+  // Column c: observer c / ratio, query head c % ratio of the KV head's.
+  V8 qn[QL];
+  auto fetch = [&](int c0) {
+#pragma unroll
+    for (int i = 0; i < QL; ++i) {
+      const int c = c0 + (tid + i * kThreads) / CH, chunk = (tid + i * kThreads) % CH;
+      const int o = min(c, cols - 1) / a.ratio, h = hkv * a.ratio + min(c, cols - 1) % a.ratio;
+      qn[i] = load_v8<T>(a.q + int64_t(q0 + q_len - obs + o) * a.q_tok + int64_t(h) * a.q_head +
+                         8 * chunk);
+    }
+  };
+  fetch(0);
 
   // K as the A operand: row j of tile `sub` is token t0 + 16 sub + j.
   V8 k[kSubs][KS];
@@ -99,63 +134,104 @@ __global__ __launch_bounds__(kThreads) void weights_scores_kernel(WeightsArgs a)
   }
   float mass[kSubs][4] = {};
   float2* stats = a.stats + offset;
-  const int64_t done = int64_t(item[3]) * all;   // the combined columns
-  int turn = 0;
-  for (int c0 = 0; c0 < cols; c0 += 16, turn ^= 1) {
-    const int c = c0 + j;
-    const int o = c / a.ratio, h = hkv * a.ratio + c % a.ratio;
-    const bool col_ok = c < cols;
-    const f16* qp = a.q + int64_t(q0 + q_len - obs + min(o, obs - 1)) * a.q_tok +
-                    int64_t(h) * a.q_head + 8 * tg;
-    V8 q[KS];
+  // Every token of the wave is there, and seen by every observer.
+  const bool whole = __all(ok == 0xffffu) && t0 + kSubs * 16 <= n - obs + 1;
+  for (int c0 = 0; c0 < cols; c0 += kCols) {
+    __syncthreads();   // the columns before are done with
 #pragma unroll
-    for (int s = 0; s < KS; ++s) q[s] = col_ok ? load_v8<T>(qp + 32 * s) : V8{};
-    const int last = n - obs + o;   // the last token that the observer sees
-    f32x4 sc[kSubs];
+    for (int i = 0; i < QL; ++i) {
+      const int g = (tid + i * kThreads) / CH, chunk = (tid + i * kThreads) % CH;
+      *reinterpret_cast<V8*>(&s_q[g * D + 8 * (chunk ^ (g & 7))]) = qn[i];
+    }
+    const int here = min(kCols, cols - c0);
+    if constexpr (ADD) {
+      // The columns' normalisers (columns past the last one: none gets anything).
+      // A quarter of the partitions to each wave.
+      float2 st = {kNegBig, 0.f};
+      const float2* src = stats + int64_t(hkv) * cols + c0 + min(lane, here - 1);
+      if constexpr (COMBINE) {
+        for (int i0 = 0; i0 < parts; i0 += 4 * kWaves) {
+          float2 x[4];
 #pragma unroll
-    for (int sub = 0; sub < kSubs; ++sub) {
-      sc[sub] = f32x4{};
+          for (int u = 0; u < 4; ++u)
+            x[u] = src[int64_t(min(i0 + u * kWaves + wave, parts - 1)) * all];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) sc[sub] = mfma16(k[sub][s], q[s], sc[sub]);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int t = t0 + 16 * sub + 4 * tg + x;
-        const bool seen = ((ok >> (4 * sub + x)) & 1u) && t <= last;
-        sc[sub][x] = seen ? sc[sub][x] * a.scale_log2 : -INFINITY;
+          for (int u = 0; u < 4; ++u)
+            if (i0 + u * kWaves + wave < parts) st = join(st, x[u]);
+        }
+        s_stat[wave][lane] = st;
+      } else if (wave == 0) {
+        s_stat[0][lane] = lane < here ? src[int64_t(parts) * all] : float2{-kNegBig, 0.f};
       }
     }
-    if constexpr (ADD) {
-      const float2 st = col_ok ? stats[done + int64_t(hkv) * cols + c] : float2{0.f, 0.f};
+    __syncthreads();
+    if (c0 + kCols < cols) fetch(c0 + kCols);
+    if constexpr (ADD && COMBINE) {
+      if (wave == 0) {
+        float2 st = s_stat[0][lane];
 #pragma unroll
-      for (int sub = 0; sub < kSubs; ++sub)
+        for (int i = 1; i < kWaves; ++i) st = join(st, s_stat[i][lane]);
+        s_stat[0][lane] = lane < here ? normaliser(st) : float2{-kNegBig, 0.f};
+      }
+      __syncthreads();
+    }
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float p = sc[sub][x] == -INFINITY ? 0.f : fast_exp2(sc[sub][x] - st.x) * st.y;
-          mass[sub][x] += col_ok ? p : 0.f;
-        }
-    } else {
-      float m = kNegBig;
+    for (int ct = 0; ct < kCols / 16; ++ct) {
+      if (16 * ct >= here) break;   // uniform
+      const int c = 16 * ct + j;
+      const int last = n - obs + (c0 + c) / a.ratio;   // the last token that the observer sees
+      V8 q[KS];
 #pragma unroll
-      for (int sub = 0; sub < kSubs; ++sub)
+      for (int s = 0; s < KS; ++s)
+        q[s] = *reinterpret_cast<const V8*>(&s_q[c * D + 8 * ((4 * s + tg) ^ (c & 7))]);
+      f32x4 sc[kSubs];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) m = fmaxf(m, sc[sub][x]);
-      m = across_groups_max(m);
-      float l = 0.f;
+      for (int sub = 0; sub < kSubs; ++sub) {
+        sc[sub] = f32x4{};
 #pragma unroll
-      for (int sub = 0; sub < kSubs; ++sub)
+        for (int s = 0; s < KS; ++s) sc[sub] = mfma16(k[sub][s], q[s], sc[sub]);
+      }
+      if (!whole) {   // uniform; the scale is positive
 #pragma unroll
-        for (int x = 0; x < 4; ++x) l += fast_exp2(sc[sub][x] - m);
-      l = across_groups_sum(l);
-      if (tg == 0) s_stat[turn][wave][j] = float2{m, l};
-      __syncthreads();   // the other half is written next: one barrier a turn
-      if (wave == 0 && tg == 0 && col_ok) {
-        float mx = kNegBig, sum = 0.f;
+        for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) mx = fmaxf(mx, s_stat[turn][i][j].x);
+          for (int x = 0; x < 4; ++x) {
+            const int t = t0 + 16 * sub + 4 * tg + x;
+            const bool seen = ((ok >> (4 * sub + x)) & 1u) && t <= last;
+            sc[sub][x] = seen ? sc[sub][x] : -INFINITY;
+          }
+      }
+      if constexpr (ADD) {
+        const float2 st = s_stat[0][c];
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i)
-          sum += s_stat[turn][i][j].y * fast_exp2(s_stat[turn][i][j].x - mx);
-        stats[int64_t(part0 / kPartTokens) * all + int64_t(hkv) * cols + c] = float2{mx, sum};
+        for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            mass[sub][x] = fmaf(fast_exp2(fmaf(sc[sub][x], a.scale_log2, -st.x)), st.y,
+                                mass[sub][x]);
+      } else {
+        float m = -INFINITY;
+#pragma unroll
+        for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) m = fmaxf(m, sc[sub][x]);
+        m = fmaxf(across_groups_max(m) * a.scale_log2, kNegBig);
+        float l = 0.f;
+#pragma unroll
+        for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) l += fast_exp2(fmaf(sc[sub][x], a.scale_log2, -m));
+        l = across_groups_sum(l);
+        if (tg == 0) s_stat[wave][c] = float2{m, l};
+      }
+    }
+    if constexpr (!ADD) {
+      __syncthreads();
+      if (tid < here) {
+        float2 st = s_stat[0][tid];
+#pragma unroll
+        for (int i = 1; i < kWaves; ++i) st = join(st, s_stat[i][tid]);
+        stats[int64_t(part0 / kPartTokens) * all + int64_t(hkv) * cols + c0 + tid] = st;
       }
     }
   }
@@ -188,49 +264,84 @@ __global__ __launch_bounds__(kThreads) void weights_combine_kernel(WeightsArgs a
   const int c = rec[1] + threadIdx.x;
   if (c >= all) return;
   float2* stats = a.stats + int64_t(rec[2]) + c;
-  float mx = kNegBig, sum = 0.f;
-  for (int i = 0; i < parts; ++i) {
-    const float2 s = stats[int64_t(i) * all];
-    const float m = fmaxf(mx, s.x);
-    sum = sum * fast_exp2(mx - m) + s.y * fast_exp2(s.x - m);
-    mx = m;
+  float2 st = {kNegBig, 0.f};
+  int i = 0;
+  for (; i + 8 <= parts; i += 8) {   // loads together, one order of joining
+    float2 x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[u] = stats[int64_t(i + u) * all];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) st = join(st, x[u]);
   }
-  stats[int64_t(parts) * all] = float2{mx, sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum};
+  for (; i < parts; ++i) st = join(st, stats[int64_t(i) * all]);
+  stats[int64_t(parts) * all] = normaliser(st);
 }
 
 // Decode rows: the decode launch left their scores and log-sum-exps (DecodeArgs::
 // scores), so K is not read again: 4 bytes written and read per token and query
-// head beside the 4 head_dim bytes of K and V that a KV head's token has. A thread per
-// token and KV head.
-__global__ __launch_bounds__(kThreads) void weights_from_scores_kernel(
-    const int32_t* items, const float* scores, const float* lse, const int32_t* indptr,
-    const int32_t* indices, const int32_t* kv_len, int32_t num_pages, int32_t page_shift,
-    float* w, int64_t w_page, int64_t w_head, int32_t num_qo_heads, int32_t ratio, int32_t group) {
-  const int32_t* item = items + 4 * blockIdx.x;
-  const int seq = item[0], t = item[1] + threadIdx.x, hkv = blockIdx.y;
-  const int n = kv_len[seq];
+// head beside the 4 head_dim bytes of K and V that a KV head's token has. A thread
+// per token, which looks its page up once for kScoreHeads KV heads; V scores to a
+// load (V 4 where the group allows: lanes apart by more than their loads cost a line
+// each).
+constexpr int kScoreHeads = 4;
+
+struct ScoreArgs {
+  const int32_t* items;   // [..][4]: row, first token, the row's score_at
+  const float* scores;
+  const float* lse;
+  const int32_t* indptr;
+  const int32_t* indices;
+  const int32_t* kv_len;
+  float* w;
+  int64_t w_page, w_head;
+  int32_t num_pages, page_shift, num_qo_heads, num_kv_heads, ratio, group;
+};
+
+template <int V>
+__global__ __launch_bounds__(kThreads) void weights_from_scores_kernel(ScoreArgs a) {
+  typedef float VecF __attribute__((ext_vector_type(V)));
+  const int32_t* item = a.items + 4 * blockIdx.x;
+  const int seq = item[0], t = item[1] + threadIdx.x, h0 = int(blockIdx.y) * kScoreHeads;
+  const int n = a.kv_len[seq];
   if (t >= n) return;
-  const int p = indices[indptr[seq] + (t >> page_shift)];
-  if (p < 0 || p >= num_pages) return;
-  float sum = 0.f;
-  for (int h0 = hkv * ratio; h0 < (hkv + 1) * ratio; h0 += group) {   // a head group
-    const float* s = scores + int64_t(item[2]) * num_qo_heads +
-                     (int64_t(h0 / group) * n + t) * group;
-    const float* l = lse + int64_t(seq) * num_qo_heads + h0;
-    for (int g = 0; g < group; ++g) sum += fast_exp2(s[g] - l[g]);
+  const int p = a.indices[a.indptr[seq] + (t >> a.page_shift)];
+  const bool ok = p >= 0 && p < a.num_pages;
+  float* w = a.w + int64_t(ok ? p : 0) * a.w_page + (t & ((1 << a.page_shift) - 1));
+  const float* lse = a.lse + int64_t(seq) * a.num_qo_heads;
+  // of KV head h: its head groups one after the other, [token][head of the group]
+  const float* scores = a.scores + int64_t(item[2]) * a.num_qo_heads;
+  float sum[kScoreHeads], old[kScoreHeads];
+#pragma unroll
+  for (int i = 0; i < kScoreHeads; ++i) {
+    const int h = min(h0 + i, a.num_kv_heads - 1);
+    old[i] = t < n - 1 ? w[int64_t(h) * a.w_head] : 0.f;   // the new token starts at 0
+    sum[i] = 0.f;
+    for (int q0 = h * a.ratio; q0 < (h + 1) * a.ratio; q0 += a.group) {
+      const float* s = scores + (int64_t(q0 / a.group) * n + t) * a.group;
+      for (int g = 0; g < a.group; g += V) {
+        const VecF x = *reinterpret_cast<const VecF*>(s + g);
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[i] += fast_exp2(x[e] - lse[q0 + g + e]);
+      }
+    }
   }
-  float* at = w + int64_t(hkv) * w_head + int64_t(p) * w_page + (t & ((1 << page_shift) - 1));
-  *at = (t == n - 1 ? 0.f : *at) + sum;
+#pragma unroll
+  for (int i = 0; i < kScoreHeads; ++i)
+    if (ok && h0 + i < a.num_kv_heads) w[int64_t(h0 + i) * a.w_head] = old[i] + sum[i];
 }
 
 template <typename T, int D>
 int run_weights(const WeightsArgs& a, const kunserve_weights_plan_info& info, hipStream_t s) {
   const dim3 grid(unsigned(info.num_items), unsigned(a.num_kv_heads));
-  weights_scores_kernel<T, D, false><<<grid, kThreads, 0, s>>>(a);
+  weights_scores_kernel<T, D, false, false><<<grid, kThreads, 0, s>>>(a);
   KSV_CHECK_LAUNCH();
-  weights_combine_kernel<<<dim3(unsigned(info.num_combines)), kThreads, 0, s>>>(a);
-  KSV_CHECK_LAUNCH();
-  weights_scores_kernel<T, D, true><<<grid, kThreads, 0, s>>>(a);
+  if (info.num_combines > 0) {
+    weights_combine_kernel<<<dim3(unsigned(info.num_combines)), kThreads, 0, s>>>(a);
+    KSV_CHECK_LAUNCH();
+    weights_scores_kernel<T, D, true, false><<<grid, kThreads, 0, s>>>(a);
+  } else {
+    weights_scores_kernel<T, D, true, true><<<grid, kThreads, 0, s>>>(a);
+  }
   KSV_CHECK_LAUNCH();
   return KUNSERVE_OK;
 }
@@ -251,7 +362,7 @@ int weights_plan(const int32_t* q_indptr, const int32_t* kv_len, int32_t num_seq
                  int32_t num_qo_heads, int32_t window, const int32_t* decodes,
                  std::vector<int32_t>& plan, kunserve_weights_plan_info* info) {
   std::vector<int32_t> items, combines, score_items, score_at;
-  int64_t columns = 0, score_tokens = 0;
+  int64_t columns = 0, score_tokens = 0, most_parts = 0;
   for (int32_t b = 0; b < num_seqs; ++b) {
     const int64_t q_len = int64_t(q_indptr[b + 1]) - q_indptr[b];
     KSV_CHECK_ARG(q_len >= 0 && kv_len[b] >= q_len, "row %d: kv_len %d for %lld new tokens", b,
@@ -269,6 +380,7 @@ int weights_plan(const int32_t* q_indptr, const int32_t* kv_len, int32_t num_seq
     if (q_len == 0) continue;
     const int64_t cols = std::min<int64_t>(q_len, window) * num_qo_heads;
     const int64_t parts = ceil_div(kv_len[b], kPartTokens);
+    most_parts = std::max(most_parts, parts);
     KSV_CHECK_ARG(columns + (parts + 1) * cols < (int64_t(1) << 31),
                   "too many observed columns (%lld)", (long long)(columns + (parts + 1) * cols));
     for (int64_t p = 0; p < parts; ++p)
@@ -277,6 +389,7 @@ int weights_plan(const int32_t* q_indptr, const int32_t* kv_len, int32_t num_seq
       combines.insert(combines.end(), {b, int32_t(c), int32_t(columns), int32_t(parts)});
     columns += (parts + 1) * cols;
   }
+  if (most_parts <= kMaxOwnParts) combines.clear();
   plan = std::move(items);
   info->num_items = int32_t(plan.size() / 4);
   plan.insert(plan.end(), combines.begin(), combines.end());
@@ -340,13 +453,16 @@ extern "C" int kunserve_weights_plan(const int32_t* q_indptr_host, const int32_t
 
 extern "C" int64_t kunserve_weights_workspace_bytes(const kunserve_weights_plan_info* info) {
   if (!info) return -1;
-  return info->num_columns * int64_t(sizeof(float2)) +
+  if (info->num_columns == 0 && info->num_score_rows == 0) return 0;
+  return 16 + info->num_columns * int64_t(sizeof(float2)) +
          (info->score_tokens + info->num_score_rows) * info->num_qo_heads * int64_t(sizeof(float));
 }
 
 void kunserve::weights_scores(const kunserve_weights_plan_info* info, const int32_t* plan_dev,
                               void* workspace_dev, StepFusion* fusion) {
-  float* at = reinterpret_cast<float*>(static_cast<float2*>(workspace_dev) + info->num_columns);
+  // 16-byte aligned, as the workspace is (an even number of columns)
+  float* at = reinterpret_cast<float*>(static_cast<float2*>(workspace_dev) +
+                                       (info->num_columns + 1) / 2 * 2);
   fusion->scores = at;
   fusion->lse = at + info->score_tokens * info->num_qo_heads;
   fusion->score_at = plan_dev + 4 * (int64_t(info->num_items) + info->num_combines +
@@ -361,14 +477,29 @@ int kunserve::weights_from_scores(const kunserve_kv_pool* pool, const kunserve_k
   if (info->num_score_items == 0) return KUNSERVE_OK;
   StepFusion f;
   weights_scores(info, plan_dev, workspace_dev, &f);
-  const int group = decode_group(num_qo_heads, pool->num_kv_heads);
-  weights_from_scores_kernel<<<dim3(unsigned(info->num_score_items), unsigned(pool->num_kv_heads)),
-                               kThreads, 0, reinterpret_cast<hipStream_t>(stream)>>>(
-      plan_dev + 4 * (int64_t(info->num_items) + info->num_combines), f.scores, f.lse,
-      decode_table->indptr_dev, decode_table->indices_dev, decode_table->kv_len_dev,
-      int32_t(pool->num_pages), __builtin_ctz(pool->page_size),
-      weights->w + int64_t(layer) * weights->layer_stride, weights->page_stride,
-      weights->head_stride, num_qo_heads, num_qo_heads / pool->num_kv_heads, group);
+  ScoreArgs a{};
+  a.items = plan_dev + 4 * (int64_t(info->num_items) + info->num_combines);
+  a.scores = f.scores;
+  a.lse = f.lse;
+  a.indptr = decode_table->indptr_dev;
+  a.indices = decode_table->indices_dev;
+  a.kv_len = decode_table->kv_len_dev;
+  a.w = weights->w + int64_t(layer) * weights->layer_stride;
+  a.w_page = weights->page_stride;
+  a.w_head = weights->head_stride;
+  a.num_pages = int32_t(pool->num_pages);
+  a.page_shift = __builtin_ctz(pool->page_size);
+  a.num_qo_heads = num_qo_heads;
+  a.num_kv_heads = pool->num_kv_heads;
+  a.ratio = num_qo_heads / pool->num_kv_heads;
+  a.group = decode_group(num_qo_heads, pool->num_kv_heads);
+  const dim3 grid(unsigned(info->num_score_items),
+                  unsigned(ceil_div(pool->num_kv_heads, kScoreHeads)));
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (a.group % 4 == 0)
+    weights_from_scores_kernel<4><<<grid, kThreads, 0, s>>>(a);
+  else
+    weights_from_scores_kernel<1><<<grid, kThreads, 0, s>>>(a);
   KSV_CHECK_LAUNCH();
   return KUNSERVE_OK;
 }
@@ -410,8 +541,7 @@ extern "C" int kunserve_cache_weights(const kunserve_kv_pool* pool,
               (long long)need);
     return KUNSERVE_ENOSPC;
   }
-  KSV_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace_dev) & 7u) == 0,
-                "workspace must be 8-byte aligned");
+  KSV_CHECK_ARG(aligned16(workspace_dev), "workspace must be 16-byte aligned");
   WeightsArgs a{};
   a.q = static_cast<const f16*>(q->data);
   a.q_tok = q->token_stride;

@@ -298,6 +298,11 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
   // would push the step's buffers out.
   constexpr bool kQInLds = D == 256;
   __shared__ __attribute__((aligned(16))) T s_q[kQInLds ? kMaxGroup * D : 8];
+  // A step's scores, in whole lines; at 256 they leave straight from registers (the
+  // block would leave one workgroup to a CU: 16 rows of 1250-2500 tokens, 32 heads
+  // on 8, 62 us a layer against 54).
+  constexpr bool kScoresInLds = SCORES && D != 256;
+  __shared__ float s_scores[kScoresInLds ? W * STEP * kMaxGroup : 1];
 
   const int tid = threadIdx.x;
   const int lane = tid & (kWave - 1);
@@ -368,6 +373,7 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
   const int nsteps = (te - tb + STEP - 1) / STEP;
   T* sk = reinterpret_cast<T*>(s_raw) + wave * BLK;
   float* scores = nullptr;   // of the row and head group
+  float* step_scores = s_scores + (kScoresInLds ? wave * STEP * kMaxGroup : 0);
   if constexpr (SCORES)
     scores = a.scores + int64_t(a.score_at[seq]) * a.num_qo_heads + int64_t(hg) * a.kv_len[seq] * G;
 
@@ -399,6 +405,16 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
     }
   };
 
+  // A step's scores wait in LDS ([token][head], so that they leave in whole lines)
+  // until the next step's loads are on their way.
+  auto flush_scores = [&](int c) {
+    if constexpr (kScoresInLds) {
+      const int first = (tb + c * STEP) * G, count = min(STEP, te - tb - c * STEP) * G;
+      __builtin_amdgcn_wave_barrier();
+      for (int i = lane; i < count; i += kWave) scores[first + i] = step_scores[i];
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
   if (wave < nsteps) load(wave);
   for (int c = wave; c < nsteps; c += W) {
     // Park K in LDS and transpose V in registers, which frees both for the
@@ -411,6 +427,7 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
     V8 vt[8];
     transpose(vt);
     load(c + W);
+    if (c > wave) flush_scores(c - W);
 
     // Scores. LDS runs a wave's accesses in order; keep the compiler from
     // moving them.
@@ -460,8 +477,12 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
           for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              const int t = t0 + L::token(4 * sub + x, tg, p);
-              if (t < te) scores[int64_t(t) * G + j] = sc[p][sub][x] * a.scale_log2;
+              const int t = L::token(4 * sub + x, tg, p);
+              const float score = sc[p][sub][x] * a.scale_log2;
+              if constexpr (kScoresInLds)
+                step_scores[t * G + j] = score;
+              else if (t0 + t < te)
+                scores[int64_t(t0 + t) * G + j] = score;
             }
       }
     }
@@ -505,6 +526,8 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
 #pragma unroll
       for (int x = 0; x < L::ACCS; ++x) o[x][e] = mfma16(vt[e], pl[x], o[x][e]);
   }
+
+  if (wave < nsteps) flush_scores(wave + (nsteps - 1 - wave) / W * W);
 
   // Head j's sum over the 4 row groups of this wave (at 256 every token is
   // in two of them).

@@ -531,7 +531,7 @@ int kunserve_cache_weights(const kunserve_kv_pool* pool,
  * tokens, the last `recent` ones and the heaviest of those between stay, keep[b]
  * in all (device int32; kv_len[b] and max_keep at most; below sinks + recent
  * the first ones come first; equal weights: the lowest index; NaN: below every
- * number). Their K, V and weights are copied in their order to the pages
+ * number). max_len bounds every kv_len[b]. Their K, V and weights are copied in their order to the pages
  * out_indices[out_indptr[b]..], slots 0, 1, .., which must not be pages of the
  * table nor twice in the list; slots behind the last kept one are left as they
  * are. kept (int32 [num_seqs][num_layers][num_kv_heads][kept_stride]) receives
@@ -540,8 +540,8 @@ int kunserve_cache_weights(const kunserve_kv_pool* pool,
 int kunserve_evict(const kunserve_kv_pool* pool, const kunserve_kv_weights* weights,
                    const kunserve_page_table* table, const int32_t* out_indptr_dev,
                    const int32_t* out_indices_dev, const int32_t* keep_dev,
-                   int32_t max_keep, int32_t sinks, int32_t recent,
-                   int32_t* kept_dev, int64_t kept_stride,
+                   int32_t max_keep, int32_t max_len, int32_t sinks,
+                   int32_t recent, int32_t* kept_dev, int64_t kept_stride,
                    kunserve_stream_t stream);
 
 /* ------------------------------------------------ a step's layers */

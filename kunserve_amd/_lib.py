@@ -154,8 +154,8 @@ SIGNATURES = {
                                        c_float, c_void_p, POINTER(WeightsPlanInfo), c_void_p,
                                        c_int64, c_void_p]),
     "kunserve_evict": (c_int, [POINTER(KVPool), POINTER(KVWeights), POINTER(PageTable), c_void_p,
-                               c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_int64,
-                               c_void_p]),
+                               c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p,
+                               c_int64, c_void_p]),
     "kunserve_decode_plan_bound": (c_int64, [c_void_p, c_int32]),
     "kunserve_decode_plan": (c_int, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
                                      c_void_p, c_int64, POINTER(DecodePlanInfo)]),

@@ -135,37 +135,43 @@ def evict(pool: KVPool, weights: KVWeights, pages_of_reqs: Sequence[Sequence[int
     indices kept, int32 [requests, layers, kv_heads, most kept], -1 behind a
     request's last."""
     weights.check(pool)
-    kv = np.asarray(kv_lens, dtype=np.int64).reshape(-1)
-    n = len(kv)
+    n = len(kv_lens)
     if len(pages_of_reqs) != n or len(pages_out) != n:
         raise ValueError(f"{n} kv lengths but {len(pages_of_reqs)} and {len(pages_out)} page lists")
+    lens = np.empty(2 * n, dtype=np.int64)   # of the requests, then what stays of them
+    kv, keep = lens[:n], lens[n:]
+    kv[:] = kv_lens
     budget = np.asarray(budget, dtype=np.int64)
-    if budget.ndim > 1 or (budget.ndim == 1 and len(budget) != n):
+    if budget.shape not in ((), (n,)):
         raise ValueError(f"budget must be one number or one per request ({n})")
-    if np.any(budget < 0) or np.any(kv < 0) or sinks < 0 or recent < 0:
+    np.minimum(budget, kv, out=keep)
+    # a negative length or budget is the least of a request's
+    if sinks < 0 or recent < 0 or (n and keep.min() < 0):
         raise ValueError("budget, kv_lens, sinks and recent must not be negative")
+    longest, most = (int(kv.max()), int(keep.max())) if n else (0, 0)
     limit = 2**31 - 1   # tokens of a request are counted in int32
-    if np.any(kv > limit):
+    if longest > limit:
         raise ValueError(f"a request of over {limit} tokens")
-    keep = np.minimum(np.broadcast_to(budget, kv.shape), kv)
-    indptr, indices = csr_from_lists(pages_of_reqs, kv, pool.page_size, pool.num_pages)
-    out_indptr, out_indices = csr_from_lists(pages_out, keep, pool.page_size, pool.num_pages)
-    taken = np.zeros(pool.num_pages, dtype=bool)
-    taken[indices] = True
-    if taken[out_indices].any():
-        raise ValueError(f"page {int(out_indices[taken[out_indices]][0])} of pages_out holds "
-                         "tokens of the requests")
-    if np.unique(out_indices).size != out_indices.size:
-        raise ValueError("a page is twice in pages_out")
-    most = int(keep.max()) if n else 0
     kept = torch.empty((n, pool.num_layers, pool.num_kv_heads, most), dtype=torch.int32,
                        device=pool.device)
     if most == 0:
         return kept
-    table = PageTable(indptr, indices, kv, pool.device, upload=False)
-    dev = _upload_packed(table.host_arrays() + [out_indptr, out_indices, _i32(keep)], pool.device)
-    table.bind(dev[:3])
-    _lib.call("kunserve_evict", pool.desc(), ctypes.byref(weights._desc), table.desc(),
-              dev[3].data_ptr(), dev[4].data_ptr(), dev[5].data_ptr(), most, min(sinks, limit),
-              min(recent, limit), kept.data_ptr(), most, _stream_ptr(pool.device))
+    # one table: the requests' pages, then those that are filled
+    indptr, indices = csr_from_lists([*pages_of_reqs, *pages_out], lens, pool.page_size,
+                                     pool.num_pages)
+    out = indices[indptr[n]:]
+    use = np.zeros(pool.num_pages, dtype=np.int8)
+    use[indices[:indptr[n]]] = 1
+    if use[out].any():
+        raise ValueError(f"page {int(out[use[out] != 0][0])} of pages_out holds tokens of the "
+                         "requests")
+    use[out] = 2
+    if np.count_nonzero(use == 2) != out.size:
+        raise ValueError("a page is twice in pages_out")
+    at, lengths, ids = _upload_packed([indptr, lens, indices], pool.device)
+    table = _lib.PageTable(at.data_ptr(), ids.data_ptr(), lengths.data_ptr(), n)
+    _lib.call("kunserve_evict", pool.desc(), ctypes.byref(weights._desc), ctypes.byref(table),
+              at.data_ptr() + 4 * n, ids.data_ptr(), lengths.data_ptr() + 4 * n, most, longest,
+              min(sinks, limit), min(recent, limit), kept.data_ptr(), most,
+              _stream_ptr(pool.device))
     return kept

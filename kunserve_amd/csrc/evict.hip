@@ -4,23 +4,25 @@
 //
 // The heaviest are found by radix selection on the weights' bits (an order on
 // unsigned integers that agrees with the order of fp32): the key of the last
-// one that stays is built from the top, 8 bits at a time, from histograms of
-// the tokens that agree with it so far. Tokens above it stay, and of those
-// that equal it the first ones (the lowest indices).
+// one that stays is built from the top, 11, 11 and 10 bits at a time, from
+// histograms of the tokens that agree with it so far. Tokens above it stay, and
+// of those that equal it the first ones (the lowest indices).
 //
 // HBM-bound: 4 bytes per cached token and head are read to choose, and the K,
 // V and weight of what stays are read and written once. Two launches: a
 // workgroup per (row, layer, head) chooses; then workgroups of kMoveTokens
 // kept tokens move them, so that a single row's move is spread over the device
-// too.
+// too. The choice reads its weights once, into registers: the tokens of a wave are
+// consecutive, 64 at a time, so a ballot gives a token's place among those that
+// stay and only the waves' totals meet in LDS.
 #include "common.hpp"
 
 namespace kunserve {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
+constexpr int kMoveThreads = 256;
 constexpr int kMoveTokens = 64;
+constexpr int kBins = 2048;   // of 11 bits
 
 struct EvictArgs {
   f16* k;
@@ -47,7 +49,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// Exclusive prefix sum of x over the workgroup; total: the sum.
+// Exclusive prefix sum of x over the workgroup of W waves; total: the sum.
+template <int W>
 __device__ __forceinline__ int block_scan(int x, int* s_sums, int& total) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   int incl = x;
@@ -62,89 +65,151 @@ __device__ __forceinline__ int block_scan(int x, int* s_sums, int& total) {
   int before = 0;
   total = 0;
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
-    if (i < wave) before += s_sums[i];
-    total += s_sums[i];
+  for (int i = 0; i < W; ++i) {
+    const int y = s_sums[i];
+    if (i < wave) before += y;
+    total += y;
   }
   return before + incl - x;
 }
 
-__global__ __launch_bounds__(kThreads) void evict_choose_kernel(EvictArgs a) {
-  __shared__ int s_hist[256];
-  __shared__ int s_sums[kWaves];
+// KPT: keys a thread holds in registers (0: they are read again where they are
+// needed; for middles longer than W * 64 * 32).
+template <int W, int KPT>
+__global__ __launch_bounds__(W * kWave) void evict_choose_kernel(EvictArgs a) {
+  constexpr int THREADS = W * kWave, BPT = kBins / THREADS;
+  __shared__ int s_hist[kBins];
+  __shared__ int s_sums[W];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6;
   const int head = blockIdx.x, layer = blockIdx.y, seq = blockIdx.z;
   const int n = a.kv_len[seq];
   const int keep = min(min(a.keep[seq], a.max_keep), n);
   int32_t* kept = a.kept + ((int64_t(seq) * a.num_layers + layer) * a.num_kv_heads + head) *
                                a.kept_stride;
-  for (int64_t j = max(keep, 0) + tid; j < a.kept_stride; j += kThreads) kept[j] = -1;
+  for (int64_t j = max(keep, 0) + tid; j < a.kept_stride; j += THREADS) kept[j] = -1;
   if (keep <= 0) return;   // uniform
   if (keep == n) {
-    for (int j = tid; j < n; j += kThreads) kept[j] = j;
+    for (int j = tid; j < n; j += THREADS) kept[j] = j;
     return;
   }
   // The first ones come before the last ones where both are more than stay.
   // The middle [lo, hi) is longer than the tokens it keeps (n > keep).
   const int lo = min(a.sinks, keep), recent = min(a.recent, keep - lo), hi = n - recent;
   int need = keep - lo - recent;
+  for (int j = tid; j < lo; j += THREADS) kept[j] = j;
+  for (int j = tid; j < recent; j += THREADS) kept[keep - recent + j] = hi + j;
+  if (need == 0) return;   // uniform
   const int32_t* pages = a.indices + a.indptr[seq];
   const float* w = a.w + int64_t(layer) * a.w_layer + int64_t(head) * a.w_head;
   const int mask = (1 << a.page_shift) - 1;
-  auto key_at = [&](int t) -> uint32_t {
+  // Round r of a wave: tokens lo + (wave * rounds + r) * 64 + lane.
+  const int rounds = (hi - lo + THREADS - 1) / THREADS;
+  const int first = lo + wave * rounds * kWave + lane;
+  auto read_key = [&](int t) -> uint32_t {
     const int p = pages[t >> a.page_shift];
     return p >= 0 && p < a.num_pages ? weight_key(w[int64_t(p) * a.w_page + (t & mask)]) : 0u;
   };
-  uint32_t prefix = 0;   // the key's bits so far
-  if (need > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      s_hist[tid] = 0;
-      __syncthreads();
-      const uint32_t high = shift == 24 ? 0u : ~0u << (shift + 8);
-      for (int t = lo + tid; t < hi; t += kThreads) {
-        const uint32_t key = key_at(t);
-        if ((key & high) == prefix) atomicAdd(&s_hist[(key >> shift) & 255], 1);
-      }
-      __syncthreads();
-      // Bin 255 - tid counted from above: the one in which the need-th falls.
-      int total;
-      const int mine = s_hist[255 - tid];
-      const int above = block_scan(mine, s_sums, total);
-      if (above < need && need <= above + mine) {
-        s_prefix = prefix | uint32_t(255 - tid) << shift;
-        s_need = need - above;
-      }
-      __syncthreads();
-      prefix = s_prefix;
-      need = s_need;   // tokens wanted among those that agree with prefix
+  uint32_t keys[KPT > 0 ? KPT : 1];
+  if constexpr (KPT > 0) {
+#pragma unroll
+    for (int r = 0; r < KPT; ++r) {
+      const int t = first + r * kWave;
+      keys[r] = r < rounds && t < hi ? read_key(t) : 0u;
     }
   }
-  // In index order: the first ones, the middle's choice, the last ones.
-  for (int j = tid; j < lo; j += kThreads) kept[j] = j;
-  for (int j = tid; j < recent; j += kThreads) kept[keep - recent + j] = hi + j;
-  if (keep == lo + recent) return;   // uniform
-  int at = lo, equal = 0;
-  for (int t0 = lo; t0 < hi; t0 += kThreads) {
-    const int t = t0 + tid;
-    const uint32_t key = t < hi ? key_at(t) : 0u;
-    const bool tie = t < hi && key == prefix;
-    int ties, chosen;
-    const int rank = equal + block_scan(tie, s_sums, ties);
-    const bool stays = t < hi && (key > prefix || (tie && rank < need));
-    const int pos = at + block_scan(stays, s_sums, chosen);
-    if (stays) kept[pos] = t;
-    equal += ties;
-    at += chosen;
+  // f(token, key) for the thread's tokens, by whole waves (token >= hi: none).
+  auto each = [&](auto f) {
+    if constexpr (KPT > 0) {
+#pragma unroll
+      for (int r = 0; r < KPT; ++r)
+        if (r < rounds) f(first + r * kWave, keys[r]);   // uniform
+    } else {
+      for (int r = 0; r < rounds; ++r) {
+        const int t = first + r * kWave;
+        f(t, t < hi ? read_key(t) : 0u);
+      }
+    }
+  };
+
+  uint32_t prefix = 0;   // the key's bits so far
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t high = pass == 0 ? 0u : ~0u << (pass == 1 ? 21 : 10);
+    const uint32_t digits = pass == 2 ? 1023u : 2047u;
+#pragma unroll
+    for (int i = 0; i < BPT; ++i) s_hist[tid + i * THREADS] = 0;
+    __syncthreads();
+    each([&](int t, uint32_t key) {
+      const bool in = t < hi && (key & high) == prefix;
+      const int bin = int((key >> shift) & digits);
+      if (in) {
+        // Tokens of equal weight are many where weights are few (zeros): one add.
+        const int bin0 = __builtin_amdgcn_readfirstlane(bin);
+        const uint64_t who = __ballot(true);
+        if (__ballot(bin != bin0) != 0)
+          atomicAdd(&s_hist[bin], 1);
+        else if (lane == __builtin_ctzll(who))
+          atomicAdd(&s_hist[bin0], __popcll(who));
+      }
+    });
+    __syncthreads();
+    // Bins from above, BPT to a thread: the one in which the need-th falls.
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < BPT; ++i) mine += s_hist[kBins - 1 - tid * BPT - i];
+    int total;
+    int above = block_scan<W>(mine, s_sums, total);
+    if (above < need && need <= above + mine) {
+#pragma unroll
+      for (int i = 0; i < BPT; ++i) {
+        const int bin = kBins - 1 - tid * BPT - i, count = s_hist[bin];
+        if (above < need && need <= above + count) {
+          s_prefix = prefix | uint32_t(bin) << shift;
+          s_need = need - above;
+        }
+        above += count;
+      }
+    }
+    __syncthreads();
+    prefix = s_prefix;
+    need = s_need;   // tokens wanted among those that agree with prefix
   }
+
+  // The wave's tokens above the key, and its ties; then both before the wave.
+  int over = 0, ties = 0, total;
+  each([&](int t, uint32_t key) {
+    over += __popcll(__ballot(t < hi && key > prefix));
+    ties += __popcll(__ballot(t < hi && key == prefix));
+  });
+  int seen = block_scan<W>(lane == 0 ? ties : 0, s_sums, total);
+  seen = __shfl(seen, 0);   // ties before
+  const int staying = over + min(max(need - seen, 0), ties);
+  int at = block_scan<W>(lane == 0 ? staying : 0, s_sums, total);
+  at = lo + __shfl(at, 0);
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  each([&](int t, uint32_t key) {
+    const uint64_t tie = __ballot(t < hi && key == prefix);
+    const bool stays = t < hi && (key > prefix || (key == prefix && seen + __popcll(tie & below) < need));
+    seen += __popcll(tie);
+    const uint64_t who = __ballot(stays);
+    if (stays) kept[at + __popcll(who & below)] = t;
+    at += __popcll(who);
+  });
 }
 
-// Moves kept tokens: a 16-byte chunk of K and of V per thread and step.
+// Moves kept tokens: 16-byte chunks of K and of V, a thread's loads of all its
+// tokens before their stores. Non-temporal both ways: 8 rows halved, 32 layers of 8
+// heads of 128 (3.4 GB) 666 us against 688 with plain stores: 5.2 TB/s, what a
+// large copy reaches.
 template <int D>
-__global__ __launch_bounds__(kThreads) void evict_move_kernel(EvictArgs a) {
-  constexpr int CH = D / 8;                   // 16-byte chunks per row
-  constexpr int ROWS = kThreads / CH;         // tokens per step
+__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
+  constexpr int CH = D / 8;                       // 16-byte chunks per row
+  constexpr int ROWS = kMoveThreads / CH;         // tokens per step
+  constexpr int STEPS = kMoveTokens / ROWS;
+  constexpr int BATCH = STEPS < 4 ? STEPS : 4;
   __shared__ int64_t s_src[kMoveTokens], s_dst[kMoveTokens];
   const int seq = blockIdx.z;
   const int head = int(blockIdx.y) % a.num_kv_heads, layer = int(blockIdx.y) / a.num_kv_heads;
@@ -153,37 +218,71 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(EvictArgs a) {
   if (j0 >= n) return;   // uniform
   const int cnt = min(kMoveTokens, n - j0);
   const int mask = (1 << a.page_shift) - 1;
-  if (int(threadIdx.x) < cnt) {
-    const int j = j0 + threadIdx.x;
-    const int t = a.kept[((int64_t(seq) * a.num_layers + layer) * a.num_kv_heads + head) *
-                             a.kept_stride + j];
-    const int p = a.indices[a.indptr[seq] + (t >> a.page_shift)];
-    const int d = a.out_indices[a.out_indptr[seq] + (j >> a.page_shift)];
-    const bool src_ok = p >= 0 && p < a.num_pages, dst_ok = d >= 0 && d < a.num_pages;
-    s_src[threadIdx.x] = src_ok ? int64_t(p) * a.page_stride + int64_t(t & mask) * a.token_stride : -1;
-    s_dst[threadIdx.x] = dst_ok ? int64_t(d) * a.page_stride + int64_t(j & mask) * a.token_stride : -1;
-    float* w = a.w + int64_t(layer) * a.w_layer + int64_t(head) * a.w_head;
-    if (dst_ok)
-      w[int64_t(d) * a.w_page + (j & mask)] = src_ok ? w[int64_t(p) * a.w_page + (t & mask)] : 0.f;
+  if (int(threadIdx.x) < kMoveTokens) {
+    int64_t from = -1, to = -1;
+    if (int(threadIdx.x) < cnt) {
+      const int j = j0 + threadIdx.x;
+      const int t = a.kept[((int64_t(seq) * a.num_layers + layer) * a.num_kv_heads + head) *
+                               a.kept_stride + j];
+      const int p = a.indices[a.indptr[seq] + (t >> a.page_shift)];
+      const int d = a.out_indices[a.out_indptr[seq] + (j >> a.page_shift)];
+      const bool src_ok = p >= 0 && p < a.num_pages, dst_ok = d >= 0 && d < a.num_pages;
+      if (src_ok) from = int64_t(p) * a.page_stride + int64_t(t & mask) * a.token_stride;
+      if (dst_ok) to = int64_t(d) * a.page_stride + int64_t(j & mask) * a.token_stride;
+      float* w = a.w + int64_t(layer) * a.w_layer + int64_t(head) * a.w_head;
+      if (dst_ok)
+        w[int64_t(d) * a.w_page + (j & mask)] = src_ok ? w[int64_t(p) * a.w_page + (t & mask)] : 0.f;
+    }
+    s_src[threadIdx.x] = from;
+    s_dst[threadIdx.x] = to;
   }
   __syncthreads();
   const int64_t base = int64_t(layer) * a.layer_stride + int64_t(head) * a.head_stride +
                        8 * (threadIdx.x % CH);
-  for (int i = threadIdx.x / CH; i < cnt; i += ROWS) {
-    if (s_dst[i] < 0) continue;
-    f16x8 x = {}, y = {};   // a token of no page of the pool: zeros
-    if (s_src[i] >= 0) {
-      x = load_f16x8_nt(a.k + base + s_src[i]);
-      y = load_f16x8_nt(a.v + base + s_src[i]);
+  const int row = threadIdx.x / CH;
+#pragma unroll
+  for (int i0 = 0; i0 < STEPS; i0 += BATCH) {
+    f16x8 x[BATCH], y[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int64_t from = s_src[row + (i0 + i) * ROWS];
+      x[i] = y[i] = f16x8{};   // a token of no page of the pool: zeros
+      if (from >= 0) {
+        x[i] = load_f16x8_nt(a.k + base + from);
+        y[i] = load_f16x8_nt(a.v + base + from);
+      }
     }
-    store_f16x8(a.k + base + s_dst[i], x);
-    store_f16x8(a.v + base + s_dst[i], y);
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int64_t to = s_dst[row + (i0 + i) * ROWS];
+      if (to < 0) continue;
+      __builtin_nontemporal_store(x[i], reinterpret_cast<f16x8*>(a.k + base + to));
+      __builtin_nontemporal_store(y[i], reinterpret_cast<f16x8*>(a.v + base + to));
+    }
   }
+}
+
+// How many waves choose, and what they hold. A workgroup waits at barriers most of
+// its time: few of them take 16 waves each, many take 4 so that a CU holds more of
+// them (2048 of up to 5000 tokens: 63 us against 96 with 16 waves; 56 and, for 64 of
+// 5000 with 16 waves, 13 since ties and what is above them are counted in one pass).
+void launch_choose(const EvictArgs& a, dim3 grid, int32_t max_len, hipStream_t s) {
+  const int64_t workgroups = int64_t(grid.x) * grid.y * grid.z;
+  if (max_len <= 4 * kWave * 16)
+    evict_choose_kernel<4, 16><<<grid, 4 * kWave, 0, s>>>(a);
+  else if (max_len <= 4 * kWave * 32 && workgroups >= 512)
+    evict_choose_kernel<4, 32><<<grid, 4 * kWave, 0, s>>>(a);
+  else if (max_len <= 16 * kWave * 16)
+    evict_choose_kernel<16, 16><<<grid, 16 * kWave, 0, s>>>(a);
+  else if (max_len <= 16 * kWave * 32)
+    evict_choose_kernel<16, 32><<<grid, 16 * kWave, 0, s>>>(a);
+  else
+    evict_choose_kernel<16, 0><<<grid, 16 * kWave, 0, s>>>(a);
 }
 
 template <int D>
 int launch_move(const EvictArgs& a, dim3 grid, hipStream_t s) {
-  evict_move_kernel<D><<<grid, kThreads, 0, s>>>(a);
+  evict_move_kernel<D><<<grid, kMoveThreads, 0, s>>>(a);
   KSV_CHECK_LAUNCH();
   return KUNSERVE_OK;
 }
@@ -197,8 +296,9 @@ using namespace kunserve;
 extern "C" int kunserve_evict(const kunserve_kv_pool* pool, const kunserve_kv_weights* weights,
                               const kunserve_page_table* table, const int32_t* out_indptr_dev,
                               const int32_t* out_indices_dev, const int32_t* keep_dev,
-                              int32_t max_keep, int32_t sinks, int32_t recent, int32_t* kept_dev,
-                              int64_t kept_stride, kunserve_stream_t stream) {
+                              int32_t max_keep, int32_t max_len, int32_t sinks, int32_t recent,
+                              int32_t* kept_dev, int64_t kept_stride,
+                              kunserve_stream_t stream) {
   clear_error();
   int rc = check_pool(pool, true);
   if (rc) return rc;
@@ -206,6 +306,7 @@ extern "C" int kunserve_evict(const kunserve_kv_pool* pool, const kunserve_kv_we
   if (rc) return rc;
   KSV_CHECK_ARG(table && table->num_seqs >= 0, "null table or num_seqs < 0");
   KSV_CHECK_ARG(sinks >= 0 && recent >= 0, "sinks %d or recent %d < 0", sinks, recent);
+  KSV_CHECK_ARG(max_len >= 0, "max_len %d < 0", max_len);
   KSV_CHECK_ARG(max_keep >= 0 && kept_stride >= max_keep, "kept_stride %lld below max_keep %d",
                 (long long)kept_stride, max_keep);
   if (table->num_seqs == 0 || max_keep == 0) return KUNSERVE_OK;
@@ -244,9 +345,8 @@ extern "C" int kunserve_evict(const kunserve_kv_pool* pool, const kunserve_kv_we
   a.kept = kept_dev;
   a.kept_stride = kept_stride;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  evict_choose_kernel<<<dim3(unsigned(a.num_kv_heads), unsigned(a.num_layers),
-                             unsigned(table->num_seqs)),
-                        kThreads, 0, s>>>(a);
+  launch_choose(a, dim3(unsigned(a.num_kv_heads), unsigned(a.num_layers),
+                        unsigned(table->num_seqs)), max_len, s);
   KSV_CHECK_LAUNCH();
   const dim3 grid(unsigned((max_keep + kMoveTokens - 1) / kMoveTokens),
                   unsigned(a.num_layers * a.num_kv_heads), unsigned(table->num_seqs));

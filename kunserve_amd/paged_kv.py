@@ -641,27 +641,33 @@ def rotary_append_kv(pool: KVPool, layer: int, table: PageTable, q_indptr: torch
     [num_tokens]): the tokens' rotary positions, where they are not their places in
     the cache. The rotated q goes to out (default: q, in place), which must be q
     or lie apart from q, k_new and v_new. Returns out."""
-    if k_new.shape != v_new.shape or k_new.shape[1:] != (pool.num_kv_heads, pool.head_dim):
-        raise ValueError(f"k_new / v_new must be [tokens, {pool.num_kv_heads}, {pool.head_dim}]")
-    if q.shape[0] != k_new.shape[0] or q.shape[2] != pool.head_dim:
-        raise ValueError(f"q {tuple(q.shape)} does not match k_new {tuple(k_new.shape)}")
+    q_shape, k_shape, device = q.shape, k_new.shape, pool.device
+    tokens, dim, dtype = k_shape[0], pool.head_dim, pool.dtype
+    if k_shape != v_new.shape or k_shape[1:] != (pool.num_kv_heads, dim):
+        raise ValueError(f"k_new / v_new must be [tokens, {pool.num_kv_heads}, {dim}]")
+    if q_shape[0] != tokens or q_shape[2] != dim:
+        raise ValueError(f"q {tuple(q_shape)} does not match k_new {tuple(k_shape)}")
     if q_indptr.numel() != table.num_seqs + 1:
         raise ValueError("q_indptr must have num_seqs + 1 entries")
     if out is None:
         out = q
-    if out.shape != q.shape:
-        raise ValueError(f"out shape {tuple(out.shape)} differs from q's {tuple(q.shape)}")
-    for name, t in (("q", q), ("k_new", k_new), ("v_new", v_new), ("out", out)):
-        if t.device != pool.device:
-            raise ValueError(f"{name} is on {t.device}, the pool on {pool.device}")
-    rotary.check(pool.head_dim, pool.device)
-    _check_row_map(positions, k_new.shape[0], pool.device, "positions")
-    pool.check_dtype(q, k_new, v_new, out)
-    qd, od, kd, vd = _tensor3(q), _tensor3(out), _tensor3(k_new), _tensor3(v_new)
+    elif out.shape != q_shape:
+        raise ValueError(f"out shape {tuple(out.shape)} differs from q's {tuple(q_shape)}")
+    index = device.index   # a device tensor's is never None
+    if not (q.get_device() == k_new.get_device() == v_new.get_device() == out.get_device()
+            == index):   # -1 on the host
+        bad = next(t for t in (q, k_new, v_new, out) if t.get_device() != index)
+        raise ValueError(f"q, k_new, v_new or out is on {bad.device}, the pool on {device}")
+    rotary.check(dim, device)
+    _check_row_map(positions, tokens, device, "positions")
+    if not q.dtype == k_new.dtype == v_new.dtype == out.dtype == dtype:
+        pool.check_dtype(q, k_new, v_new, out)
+    qd = _tensor3(q)
+    od, kd, vd = qd if out is q else _tensor3(out), _tensor3(k_new), _tensor3(v_new)
+    ref = ctypes.byref
     _lib.call("kunserve_rotary_append_kv", pool.desc(), layer, table.desc(), q_indptr.data_ptr(),
-              k_new.shape[0], ctypes.byref(qd), ctypes.byref(od), q.shape[1], ctypes.byref(kd),
-              ctypes.byref(vd), ctypes.byref(rotary._desc), _ptr(positions),
-              _stream_ptr(pool.device))
+              tokens, ref(qd), ref(od), q_shape[1], ref(kd), ref(vd), rotary.desc,
+              None if positions is None else positions.data_ptr(), _stream_ptr(device))
     return out
 
 
@@ -1039,7 +1045,7 @@ class AttentionStep:
                           _stream_ptr(self._device))
             else:
                 _lib.call("kunserve_attention_step_with", self._step_ref, self._extras_ref, local,
-                          io, None if rotary is None else ctypes.byref(rotary._desc),
+                          io, None if rotary is None else rotary.desc,
                           _stream_ptr(self._device))
             return out
         # Tensors the step does not describe: op by op, each with its checks.

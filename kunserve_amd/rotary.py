@@ -5,6 +5,7 @@ it does not ship; the position of a step's tokens is kunserve/request.py:447-462
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Mapping, Optional
 
@@ -115,6 +116,7 @@ class Rotary:
         self.device = self.frequencies.device
         self._desc = _lib.Rotary(self.frequencies.data_ptr(), rotary_dim, int(self.interleave),
                                  self.scale)
+        self.desc = ctypes.byref(self._desc)   # as the C entries take it
 
     def check(self, head_dim: int, device: torch.device) -> None:
         if self.rotary_dim > head_dim:

@@ -487,6 +487,7 @@ typedef struct {
   int32_t num_combines;  /* records of the columns' combination               */
   int32_t num_score_items; /* records of the decode rows' tokens              */
   int32_t num_score_rows;  /* decode rows                                     */
+  int32_t num_seqs;      /* rows the plan was made for                        */
   int32_t window;        /* observers of a row at most                        */
   int32_t num_qo_heads;  /* heads the plan was made for                       */
   int32_t plan_ints;     /* int32 entries of the plan buffer in use           */

@@ -90,7 +90,8 @@ class KVWeights(Structure):
 class WeightsPlanInfo(Structure):
     _fields_ = [("num_columns", c_int64), ("score_tokens", c_int64), ("num_items", c_int32),
                 ("num_combines", c_int32), ("num_score_items", c_int32),
-                ("num_score_rows", c_int32), ("window", c_int32), ("num_qo_heads", c_int32), ("plan_ints", c_int32)]
+                ("num_score_rows", c_int32), ("num_seqs", c_int32), ("window", c_int32),
+                ("num_qo_heads", c_int32), ("plan_ints", c_int32)]
 
 
 class Rotary(Structure):

@@ -24,12 +24,20 @@ class KVWeights:
     """Accumulated attention weights of a pool's tokens: w [num_pages, num_layers,
     num_kv_heads, page_size], float32 with the slots contiguous. A new token's
     weight starts at 0 in the step that appends it, so nothing has to be cleared
-    when pages are used again."""
+    when pages are used again. The weights are those of one pool: of its fused
+    views, or of the pool after a pmm drop or restore, they are others."""
 
     def __init__(self, pool: KVPool, w: Optional[torch.Tensor] = None):
         shape = (pool.num_pages, pool.num_layers, pool.num_kv_heads, pool.page_size)
         if w is None:
             w = torch.zeros(shape, dtype=torch.float32, device=pool.device)
+        # Every element in a place of its own: by stride, each dim past the ones below.
+        reach, apart = 1, True
+        for step, size in sorted(zip(w.stride(), w.shape)):
+            apart &= size <= 1 or step >= reach
+            reach = max(reach, step * (size - 1) + reach)
+        if not apart:
+            raise ValueError("weights must not share memory among themselves")
         if (tuple(w.shape) != shape or w.dtype != torch.float32 or w.stride(-1) != 1
                 or w.device != pool.device):
             raise ValueError(f"weights must be float32 {shape} on {pool.device} with the slots "
@@ -74,6 +82,7 @@ class WeightsPlan:
                                                          window))
         buf = np.empty(max(cap, 4), dtype=np.int32)   # the plan writes what it uses
         self.info = _lib.WeightsPlanInfo()
+        self.kv_len_host = kv
         marks = None if decodes is None else _i32(decodes)
         if marks is not None and marks.shape != (n,):
             raise ValueError(f"{n} rows but {marks.shape} decode marks")
@@ -100,8 +109,14 @@ def add_weights(pool: KVPool, weights: KVWeights, layer: int, table: PageTable,
                 workspace: Optional[torch.Tensor] = None) -> None:
     """Adds to `weights` what the last new tokens of every row attend to
     (kunserve_cache_weights): q [num_tokens, Hq, D] after its rotation, the step's
-    K in its pages. No page may be in two places of the table."""
+    K in its pages. No page may be in two places of the table (ValueError)."""
     weights.check(pool)
+    if q.device != pool.device:
+        raise ValueError(f"q is on {q.device}, the pool on {pool.device}")
+    if not np.array_equal(plan.kv_len_host, table.kv_len_host):
+        raise ValueError("the plan was made for other rows than the table's")
+    if not table.pages_private:
+        raise ValueError("attention weights need pages that are in one place of the table")
     if q.shape[2] != pool.head_dim:
         raise ValueError(f"q shape {tuple(q.shape)} does not match head_dim {pool.head_dim}")
     if q_indptr.numel() != table.num_seqs + 1:
@@ -133,8 +148,10 @@ def evict(pool: KVPool, weights: KVWeights, pages_of_reqs: Sequence[Sequence[int
     The shortened request goes on with min(budget, kv_len) cached tokens, its
     positions where they were (AttentionStep(rope_positions=...)). Returns the
     indices kept, int32 [requests, layers, kv_heads, most kept], -1 behind a
-    request's last."""
+    request's last. The tables are built on the host: not for a graph capture."""
     weights.check(pool)
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("evict cannot be captured: its tables are built on the host")
     n = len(kv_lens)
     if len(pages_of_reqs) != n or len(pages_out) != n:
         raise ValueError(f"{n} kv lengths but {len(pages_of_reqs)} and {len(pages_out)} page lists")

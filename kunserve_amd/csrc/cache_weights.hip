@@ -399,6 +399,7 @@ int weights_plan(const int32_t* q_indptr, const int32_t* kv_len, int32_t num_seq
   plan.insert(plan.end(), score_at.begin(), score_at.end());
   info->num_score_rows = int32_t(score_at.size());
   info->score_tokens = score_tokens;
+  info->num_seqs = num_seqs;
   info->window = window;
   info->num_qo_heads = num_qo_heads;
   info->plan_ints = int32_t(plan.size());
@@ -527,6 +528,8 @@ extern "C" int kunserve_cache_weights(const kunserve_kv_pool* pool,
                 pool->num_kv_heads);
   KSV_CHECK_ARG(info->num_qo_heads == num_qo_heads, "plan made for %d query heads, not %d",
                 info->num_qo_heads, num_qo_heads);
+  KSV_CHECK_ARG(info->num_seqs == table->num_seqs, "plan made for %d rows, not %d", info->num_seqs,
+                table->num_seqs);
   if (info->num_items == 0) return KUNSERVE_OK;
   KSV_CHECK_ARG(plan_dev && q_indptr_dev && table->indptr_dev && table->indices_dev &&
                     table->kv_len_dev,

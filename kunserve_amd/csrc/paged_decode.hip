@@ -409,9 +409,10 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
   // until the next step's loads are on their way.
   auto flush_scores = [&](int c) {
     if constexpr (kScoresInLds) {
-      const int first = (tb + c * STEP) * G, count = min(STEP, te - tb - c * STEP) * G;
+      float* to = scores + int64_t(tb + c * STEP) * G;
+      const int count = min(STEP, te - tb - c * STEP) * G;
       __builtin_amdgcn_wave_barrier();
-      for (int i = lane; i < count; i += kWave) scores[first + i] = step_scores[i];
+      for (int i = lane; i < count; i += kWave) to[i] = step_scores[i];
       __builtin_amdgcn_wave_barrier();
     }
   };

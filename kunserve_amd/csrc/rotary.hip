@@ -186,6 +186,13 @@ extern "C" int kunserve_rotary_append_kv(const kunserve_kv_pool* pool, int32_t l
   const bool in_place = q_out->data == q->data && q_out->token_stride == q->token_stride &&
                         q_out->head_stride == q->head_stride;
   const int heads = pool->num_kv_heads, dim = pool->head_dim;
+  const int64_t by_head = num_qo_heads > 1 ? q_out->head_stride : dim;
+  const int64_t by_token = num_tokens > 1 ? q_out->token_stride : dim;
+  KSV_CHECK_ARG(by_head >= dim && by_token >= dim &&
+                    (num_qo_heads == 1 || num_tokens == 1 ||
+                     by_token >= int64_t(num_qo_heads - 1) * by_head + dim ||
+                     by_head >= int64_t(num_tokens - 1) * by_token + dim),
+                "q_out's rows share memory");
   KSV_CHECK_ARG(in_place || !kunserve_tensors_overlap(q_out, num_qo_heads, q, num_qo_heads,
                                                       num_tokens, dim),
                 "q_out overlaps q without being q");

@@ -31,6 +31,7 @@ from typing import Dict, List, Optional, Sequence
 import numpy as np
 import torch
 
+from .cache_weights import KVWeights
 from .paged_kv import (AttentionStep, KVPool, copy_blocks, fused_page_ids, kv_pack,
                        kv_scatter)
 from .pmm import PmmPool
@@ -100,7 +101,10 @@ class LlamaOp:
                  is_prefill_requests: List[int], pages_of_reqs: List[List[int]],
                  num_restore_requests: int = 0, pages_of_pp: Optional[List[List[int]]] = None,
                  pages_of_dp: Optional[List[List[int]]] = None, receiver_rank: int = 0,
-                 is_context_stage: Optional[List[int]] = None) -> AttentionStep:
+                 is_context_stage: Optional[List[int]] = None, *,
+                 share_prefixes: bool = False, weights: Optional[KVWeights] = None,
+                 window: int = 16,
+                 rope_positions: Optional[List[int]] = None) -> AttentionStep:
         """Prepares the attention stage of one step (kunserve/worker.py:270-312).
 
         Argument meanings follow kunserve/flash_backend.py:2448-2469. A layer
@@ -113,6 +117,8 @@ class LlamaOp:
         num_restore_requests = 0 (kunserve/flash_backend.py:2465).
         is_context_stage (not in the reference signature) gives the rows'
         real stages when use_tensor_cores hides them (kv_lens_for_step).
+        share_prefixes, weights, window and rope_positions (not in it either)
+        are AttentionStep's.
         """
         if len(input_tokens_batched) != num_requests or len(pages_of_reqs) != num_requests:
             raise ValueError("num_requests does not match the per-row argument lists")
@@ -145,7 +151,9 @@ class LlamaOp:
                              is_prefill_requests, pages_of_reqs,
                              use_tensor_cores=self.use_tensor_cores,
                              is_context_stage=is_context_stage, layer_offset=offset,
-                             id_map=id_map, num_ids=min(max_num_pages, num_ids))
+                             id_map=id_map, num_ids=min(max_num_pages, num_ids),
+                             share_prefixes=share_prefixes, weights=weights, window=window,
+                             rope_positions=rope_positions)
         step.layer_range = (local_layer_start, local_layer_end)
         return step
 

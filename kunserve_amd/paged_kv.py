@@ -332,6 +332,7 @@ class PageTable:
         if len(self.indptr_host) != self.num_seqs + 1:
             raise ValueError("indptr must have num_seqs + 1 entries")
         self._desc = None
+        self._private: Optional[bool] = None
         if upload:
             self.bind(_upload_packed(self.host_arrays(), device))
 
@@ -358,6 +359,14 @@ class PageTable:
         if self._desc is None:
             raise RuntimeError("page table used before its device arrays were bound")
         return ctypes.byref(self._desc)
+
+    @property
+    def pages_private(self) -> bool:
+        """Whether no page is in two places of the table (looked at once)."""
+        if self._private is None:
+            ids = self.indices_host
+            self._private = np.unique(ids).size == ids.size
+        return self._private
 
 
 def _tensor3(t: torch.Tensor) -> _lib.Tensor3:
@@ -446,6 +455,8 @@ class SharedDecodePlan:
             self.bind(_upload_packed(self.host_arrays(), device))
         self.num_qo_heads = num_qo_heads
         self.num_kv_heads = num_kv_heads
+        self.page_size = page_size
+        self.table = table
 
     @property
     def num_segments(self) -> int:
@@ -695,6 +706,11 @@ def shared_decode(pool: KVPool, layer: int, table: PageTable, q: torch.Tensor,
                   out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
                   q_token: Optional[torch.Tensor] = None) -> torch.Tensor:
     """paged_decode of rows that share pages, on the plan made from their table."""
+    if plan.table is not table or plan.page_size != pool.page_size:
+        raise ValueError("the plan was made from another table or page size")
+    for t in (q, out):
+        if t is not None and t.device != pool.device:
+            raise ValueError(f"q or out is on {t.device}, the pool on {pool.device}")
     return _decode("kunserve_shared_decode", plan.shared_info, pool, layer, table, q, plan,
                    sm_scale, out, workspace, q_token)
 
@@ -841,8 +857,7 @@ class AttentionStep:
             weights.check(pool)
             if window < 1:
                 raise ValueError(f"window {window} must be positive")
-            ids = self.table.indices_host
-            if np.unique(ids).size != ids.size:
+            if not self.table.pages_private:
                 raise ValueError("attention weights need pages that are in one place of the "
                                  "step's lists")
             self.weights = weights

@@ -161,6 +161,10 @@ def test_refusals(device):
     with pytest.raises(RuntimeError, match="overlaps k_new"):
         kv4 = torch.zeros((3, 4, 64), dtype=torch.float16, device=device)
         rotary_append_kv(pool, 0, table, indptr, q, kv4[:, :2], v, rot, out=kv4)
+    with pytest.raises(RuntimeError, match="share memory"):
+        rotary_append_kv(pool, 0, table, indptr, q, k, v, rot,
+                         out=torch.zeros((1, 4, 64), dtype=torch.float16,
+                                         device=device).expand(3, 4, 64))
     with pytest.raises(ValueError, match="does not match the pool"):
         rotary_append_kv(pool, 0, table, indptr, q.bfloat16(), k, v, rot)
     with pytest.raises(ValueError, match="on cpu"):

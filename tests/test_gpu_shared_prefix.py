@@ -58,10 +58,10 @@ def run(device, specs, hq, hkv, ps, d, dtype, seed=0, layers=2, layer=1, poke=No
     return step, pool, tables, kvs, q, out
 
 
-def check(pool, tables, kvs, q, out, layer=1, step=None):
+def check(pool, tables, kvs, q, out, layer=1, step=None, plan=None):
     """A workgroup of many columns rounds its probabilities once to the element type
     for the matrix units, u of each, so of sum p |v| (others: in two terms, u^2)."""
-    plan = step.decode.plan if step is not None else None
+    plan = step.decode.plan if step is not None else plan
     wide = isinstance(plan, SharedDecodePlan) and plan.shared_info.wide
     p_err = ref.half_step(pool.dtype) if wide else None
     kh, vh = pool.k.cpu(), pool.v.cpu()
@@ -210,6 +210,54 @@ def test_page_ids_outside_the_pool_drop_out(device):
         assert np.all(np.abs(out[b].cpu().double().numpy() - want[0]) <= tol[0])
 
 
+def test_rows_of_no_and_of_one_token(device):
+    """Through the op: a row with an empty cache gives zeros beside rows that
+    share, a row of one token its value."""
+    rng = np.random.default_rng(17)
+    kvs = [0, 160, 1, 200]
+    tables, pages = tree(rng, 16, [([], 0), ([("r", 9)], 160), ([], 1), ([("r", 9)], 200)])
+    pool = random_pool(pages, 1, 2, 16, 128, device, 17, dtype=torch.bfloat16)
+    table = PageTable.from_lists(tables, kvs, pool)
+    plan = SharedDecodePlan(table, 8, 2, 16, device, min_bytes=0)
+    assert plan.num_segments == 1
+    q = random_tensor((4, 8, 128), device, 18, 2.0, torch.bfloat16)
+    out = shared_decode(pool, 0, table, q, plan)
+    assert not out[0].any()
+    one = pool.v[tables[2][0], 0, :, 0].repeat_interleave(4, dim=0)
+    assert torch.equal(out[2].view(torch.int16), one.view(torch.int16))
+    rows = [1, 3]
+    check(pool, [tables[b] for b in rows], [kvs[b] for b in rows], q[rows], out[rows], layer=0)
+    none = PageTable.from_lists([], [], pool)
+    empty = SharedDecodePlan(none, 8, 2, 16, device)
+    assert shared_decode(pool, 0, none, q[:0], empty).shape == (0, 8, 128)
+
+
+def test_strided_tensors_and_a_row_map(device):
+    """q and out as slices of wider tensors, rows anywhere among the tokens, what
+    is of no row left as it was; pools with gaps."""
+    from kunserve_amd import KVPool
+    rng = np.random.default_rng(19)
+    kvs = [150 + 11 * i for i in range(20)]
+    tables, pages = tree(rng, 16, [([("r", 9)], n) for n in kvs])
+    dense = random_pool(pages, 2, 2, 16, 128, device, 19, dtype=torch.bfloat16)
+    k, v = (torch.zeros((pages, 2, 3, 16, 136), dtype=torch.bfloat16,
+                        device=device)[:, :, :2, :, :128] for _ in range(2))
+    k.copy_(dense.k)
+    v.copy_(dense.v)
+    pool = KVPool(k, v)
+    table = PageTable.from_lists(tables, kvs, pool)
+    plan = SharedDecodePlan(table, 8, 2, 16, device, min_bytes=0)
+    wide = random_tensor((40, 12, 128), device, 20, 2.0, torch.bfloat16)
+    q = wide[:, 2:10]
+    where = torch.tensor(rng.permutation(40)[:20], dtype=torch.int32, device=device)
+    outs = torch.full((40, 10, 128), 7.0, dtype=torch.bfloat16, device=device)
+    out = shared_decode(pool, 1, table, q, plan, out=outs[:, 1:9], q_token=where)
+    check(dense, tables, kvs, q[where.long()], out[where.long()], plan=plan)
+    rest = torch.ones(40, dtype=torch.bool, device=device)
+    rest[where.long()] = False
+    assert (outs[rest] == 7).all() and (outs[:, 0] == 7).all() and (outs[:, 9] == 7).all()
+
+
 def test_captured_layer_replays(device):
     rng = np.random.default_rng(13)
     kvs = [330, 400, 321]
@@ -268,6 +316,10 @@ def test_refusals(device):
     plan = SharedDecodePlan(table, 8, 2, 16, device, min_bytes=0)
     with pytest.raises(ValueError, match="rows"):
         shared_decode(pool, 0, table, q[:1], plan)
+    with pytest.raises(ValueError, match="another table"):
+        shared_decode(pool, 0, PageTable.from_lists(tables, [160, 200], pool), q, plan)
+    with pytest.raises(ValueError, match="on cpu"):
+        shared_decode(pool, 0, table, q.cpu(), plan)
     with pytest.raises(RuntimeError, match="sm_scale"):
         shared_decode(pool, 0, table, q, plan, sm_scale=0.0)
     with pytest.raises(RuntimeError):

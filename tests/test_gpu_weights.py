@@ -173,6 +173,47 @@ def _with(before, weights, table):
     return w
 
 
+def test_strides_and_another_stream(device):
+    """Weights with gaps, q as a slice, pools whose heads lie apart, on a stream of
+    its own."""
+    from kunserve_amd import KVPool
+    q_lens, kvs = [1, 30, 1], [300, 90, 17]
+    pool, tables, q, k, v, weights = build(device, q_lens, kvs, 8, 2, 16, 128, torch.float16)
+    kk, vv = (torch.zeros((pool.num_pages, 2, 1, 16, 136), dtype=torch.float16,
+                          device=device).transpose(1, 2)[..., :128] for _ in range(2))
+    kk.copy_(pool.k)
+    vv.copy_(pool.v)
+    other = KVPool(kk, vv)
+    wide = torch.full((pool.num_pages, 2, 2, 24), 5.0, device=device)
+    w = KVWeights(other, wide[:, 1:, :, 4:20])
+    w.w.copy_(weights.w)
+    before = w.w.clone()
+    big = random_tensor((32, 12, 128), device, 77, 2.0)
+    big[:, 3:11] = q
+    s = torch.cuda.Stream(device)
+    s.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(s):
+        step = AttentionStep(other, 8, q_lens, [300, 60, 17], [0, 1, 0], tables, weights=w,
+                             window=7)
+        out = step.run(0, big[:, 3:11], k, v)
+    s.synchronize()
+    check(other, tables, q, w, before, out, q_lens, kvs, 0, 7)
+    wide[:, 1:, :, 4:20] = 5.0
+    assert (wide == 5.0).all()
+
+
+def test_rows_over_many_partitions(device):
+    """A chunk on a prefix of more partitions than the last launch combines."""
+    q_lens, kvs = [20, 40], [64 * 256 + 300, 50]
+    pool, tables, q, k, v, weights = build(device, q_lens, kvs, 4, 2, 256, 64, torch.bfloat16)
+    before = weights.w.clone()
+    first = [n - t for t, n in zip(q_lens, kvs)]
+    step = AttentionStep(pool, 4, q_lens, first, [1, 1], tables, weights=weights, window=5)
+    assert step._weights_plan.info.num_combines > 0
+    out = step.run(0, q, k, v)
+    check(pool, tables, q, weights, before, out, q_lens, kvs, 0, 5)
+
+
 def test_captured_step_replays(device):
     """A captured layer, replayed with eager work between, adds each time what
     the eager one adds."""
@@ -218,6 +259,14 @@ def test_refusals(device):
     qi = torch.tensor([0, 1, 2], dtype=torch.int32, device=device)
     with pytest.raises(RuntimeError, match="plan made for 8"):
         add_weights(pool, weights, 0, table, qi, q, plan)
+    plan = WeightsPlan([0, 1, 2], [40, 21], 4, 4, device)
+    with pytest.raises(ValueError, match="other rows"):
+        add_weights(pool, weights, 0, table, qi, q, plan)
     plan = WeightsPlan([0, 1, 2], kvs, 4, 4, device)
+    with pytest.raises(ValueError, match="on cpu"):
+        add_weights(pool, weights, 0, table, qi, q.cpu(), plan)
+    twice = PageTable.from_lists([tables[0], tables[0]], kvs, pool)
+    with pytest.raises(ValueError, match="in one place"):
+        add_weights(pool, weights, 0, twice, qi, q, plan)
     with pytest.raises(RuntimeError, match="sm_scale"):
         add_weights(pool, weights, 0, table, qi, q, plan, sm_scale=float("nan"))

@@ -122,6 +122,7 @@ __device__ __forceinline__ void mask_scores(f32x4 (&sc)[DecodeTile<D>::PAIRS][2]
                                             int tg, bool any_bad, const int* s_pages,
                                             int page_shift, int pb) {
   typedef DecodeTile<D> L;
+  asm volatile("" : "+v"(tg));   // keeps the indexes' arithmetic within the branch
 #pragma unroll
   for (int p = 0; p < L::PAIRS; ++p)
 #pragma unroll
@@ -319,34 +320,76 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
           for (int e = 0; e < 8; ++e) o[ct][x][e] = f32x4{};
       }
       V8* const values = reinterpret_cast<V8*>(blocks + W * BLK);   // [wave][dim e][lane]
-      load(wave);
+      // A load's TPL token rows lie in one page (a segment's pieces start and end
+      // at multiples of 4): its address is a lane's pointer and a scalar offset.
+      // Rows past the piece and of page ids outside the pool are read from page 0
+      // and dropped: their scores masked, their V cleared.
+      const f16* kl = kb + int64_t(lrow) * a.token_stride;
+      const f16* vl = vb + int64_t(lrow) * a.token_stride;
+      int dropped = 0;   // loads (bits) of the step on its way
+      auto load_step = [&](int c) {
+        dropped = 0;
+        int page[LOADS];
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+          page[i] = s_pages[min(max(((tb + c * STEP + TPL * i) >> a.page_shift) - pb, 0), np - 1)];
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int t = tb + c * STEP + TPL * i;
+          const int p = t < te ? __builtin_amdgcn_readfirstlane(page[i]) : -1;
+          dropped |= int(p < 0) << i;
+          const int64_t off = int64_t(max(p, 0)) * a.page_stride +
+                              (p >= 0 ? int64_t(t & page_mask) * a.token_stride : 0);
+          k[i] = load_v8<T>(kl + off);
+          v[i] = load_v8<T>(vl + off);
+        }
+      };
+      const int wave_s = __builtin_amdgcn_readfirstlane(wave);
+      load_step(wave_s);
       for (int c = 0; c < nsteps; c += W) {
         park();
+        if (dropped) {   // uniform
+#pragma unroll
+          for (int i = 0; i < LOADS; ++i)
+            if (dropped >> i & 1) v[i] = V8{};
+        }
         V8 vt[8];
         transpose8(v, vt);
 #pragma unroll
         for (int e = 0; e < 8; ++e) values[(wave * 8 + e) * kWave + lane] = vt[e];
-        load(c + W + wave);
+        load_step(c + W + wave_s);
         __syncthreads();
         if (c0 < cols) {   // uniform
           for (int blk = 0; blk < W && c + blk < nsteps; ++blk) {
             const T* block = blocks + blk * BLK;
             const int t0 = tb + (c + blk) * STEP;
+            // A tile's operands are read together, V's before the softmax: a read
+            // right before its use would be waited for each time.
+            V8 ka[PAIRS][2][KS];
+#pragma unroll
+            for (int p = 0; p < PAIRS; ++p)
+#pragma unroll
+              for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                for (int s = 0; s < KS; ++s) ka[p][sub][s] = k_row(block, p, sub, s);
+            __builtin_amdgcn_sched_barrier(0);
             f32x4 sc[kWideTiles][PAIRS][2];
 #pragma unroll
             for (int p = 0; p < PAIRS; ++p)
 #pragma unroll
-              for (int sub = 0; sub < 2; ++sub) {
+              for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-                for (int ct = 0; ct < kWideTiles; ++ct) sc[ct][p][sub] = f32x4{};
+                for (int ct = 0; ct < kWideTiles; ++ct) {
+                  sc[ct][p][sub] = f32x4{};
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                  const V8 ka = k_row(block, p, sub, s);
-#pragma unroll
-                  for (int ct = 0; ct < kWideTiles; ++ct)
-                    sc[ct][p][sub] = mfma16(ka, q[ct][s], sc[ct][p][sub]);
+                  for (int s = 0; s < KS; ++s)
+                    sc[ct][p][sub] = mfma16(ka[p][sub][s], q[ct][s], sc[ct][p][sub]);
                 }
-              }
+            __builtin_amdgcn_sched_barrier(0);
+            V8 ve[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ve[e] = values[(blk * 8 + e) * kWave + lane];
+            __builtin_amdgcn_sched_barrier(0);
             // Probabilities in one 16-bit term: at 64 columns and more the matrix
             // units' work counts (128 rows behind 8192 tokens, 64 heads: 112 us a
             // layer against 124 with the second term).
@@ -358,15 +401,12 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
               tile_softmax<T, D>(sc[ct], a.scale_log2, m[ct], lsum[ct], o[ct], ph[ct], unused);
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const V8 ve = values[(blk * 8 + e) * kWave + lane];
+            for (int e = 0; e < 8; ++e)
 #pragma unroll
               for (int x = 0; x < L::ACCS; ++x)
 #pragma unroll
-                for (int ct = 0; ct < kWideTiles; ++ct) {
-                  o[ct][x][e] = mfma16(ve, ph[ct][x], o[ct][x][e]);
-                }
-            }
+                for (int ct = 0; ct < kWideTiles; ++ct)
+                  o[ct][x][e] = mfma16(ve[e], ph[ct][x], o[ct][x][e]);
           }
         }
         __syncthreads();   // the round's blocks are done with

@@ -122,7 +122,6 @@ __device__ __forceinline__ void mask_scores(f32x4 (&sc)[DecodeTile<D>::PAIRS][2]
                                             int tg, bool any_bad, const int* s_pages,
                                             int page_shift, int pb) {
   typedef DecodeTile<D> L;
-  asm volatile("" : "+v"(tg));   // keeps the indexes' arithmetic within the branch
 #pragma unroll
   for (int p = 0; p < L::PAIRS; ++p)
 #pragma unroll
@@ -396,8 +395,11 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
             V8 ph[kWideTiles][L::ACCS], unused[L::ACCS];
 #pragma unroll
             for (int ct = 0; ct < kWideTiles; ++ct) {
-              if (any_bad || t0 + STEP > te)
-                mask_scores<D>(sc[ct], t0, te, tg, any_bad, s_pages, a.page_shift, pb);
+              if (any_bad || t0 + STEP > te) {
+                int g = tg;
+                asm volatile("" : "+v"(g));   // keeps the indexes' arithmetic in here
+                mask_scores<D>(sc[ct], t0, te, g, any_bad, s_pages, a.page_shift, pb);
+              }
               tile_softmax<T, D>(sc[ct], a.scale_log2, m[ct], lsum[ct], o[ct], ph[ct], unused);
             }
 #pragma unroll

@@ -12,7 +12,7 @@
 //
 // One launch for both: the matrix units' work on segments hides behind the
 // tails' bytes. The (row, query head of a KV head) pairs of a segment are the
-// columns of a workgroup's products, up to 64; a tail is a segment of one row.
+// columns of a workgroup's products, up to 128; a tail is a segment of one row.
 // K and V are read, parked and transposed as in paged_decode_mfma_kernel; a
 // step's operands serve every 16-column tile, so a segment costs its bytes once
 // and the matrix units 16 columns at a time.

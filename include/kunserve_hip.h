@@ -532,7 +532,8 @@ int kunserve_cache_weights(const kunserve_kv_pool* pool,
  * tokens, the last `recent` ones and the heaviest of those between stay, keep[b]
  * in all (device int32; kv_len[b] and max_keep at most; below sinks + recent
  * the first ones come first; equal weights: the lowest index; NaN: below every
- * number). max_len bounds every kv_len[b]. Their K, V and weights are copied in their order to the pages
+ * number). Of a row longer than
+ * max_len only the first max_len tokens count. Their K, V and weights are copied in their order to the pages
  * out_indices[out_indptr[b]..], slots 0, 1, .., which must not be pages of the
  * table nor twice in the list; slots behind the last kept one are left as they
  * are. kept (int32 [num_seqs][num_layers][num_kv_heads][kept_stride]) receives

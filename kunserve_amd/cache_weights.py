@@ -158,7 +158,9 @@ def evict(pool: KVPool, weights: KVWeights, pages_of_reqs: Sequence[Sequence[int
     lens = np.empty(2 * n, dtype=np.int64)   # of the requests, then what stays of them
     kv, keep = lens[:n], lens[n:]
     kv[:] = kv_lens
-    budget = np.asarray(budget, dtype=np.int64)
+    budget = np.asarray(budget) if n else np.zeros((), dtype=np.int64)
+    if budget.dtype.kind not in "iu":
+        raise ValueError("budget counts tokens: whole numbers")
     if budget.shape not in ((), (n,)):
         raise ValueError(f"budget must be one number or one per request ({n})")
     np.minimum(budget, kv, out=keep)

@@ -84,6 +84,7 @@ extern "C" int kunserve_attention_step_with(const kunserve_step* step,
                   "out overlaps q, which the attention weights are formed from");
     const kunserve_weights_plan_info& info = extras->weights_info;
     KSV_CHECK_ARG(info.num_qo_heads == step->num_qo_heads &&
+                      info.num_seqs == step->table.num_seqs &&
                       info.num_score_rows == step->decode_table.num_seqs,
                   "the weights' plan is of another step");
     KSV_CHECK_ARG(extras->shared_info.num_segments == 0, "rows that share pages have no weights");

@@ -37,7 +37,7 @@ struct EvictArgs {
   const int32_t* out_indptr;   // the pages that are filled
   const int32_t* out_indices;
   const int32_t* keep;         // [num_seqs] tokens that stay (kv_len and max_keep at most)
-  int32_t max_keep, sinks, recent;
+  int32_t max_keep, max_len, sinks, recent;
   int32_t* kept;               // [num_seqs][layers][heads][kept_stride]
   int64_t kept_stride;
 };
@@ -84,7 +84,7 @@ __global__ __launch_bounds__(W * kWave) void evict_choose_kernel(EvictArgs a) {
   __shared__ int s_need;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6;
   const int head = blockIdx.x, layer = blockIdx.y, seq = blockIdx.z;
-  const int n = a.kv_len[seq];
+  const int n = min(a.kv_len[seq], a.max_len);
   const int keep = min(min(a.keep[seq], a.max_keep), n);
   int32_t* kept = a.kept + ((int64_t(seq) * a.num_layers + layer) * a.num_kv_heads + head) *
                                a.kept_stride;
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
   __shared__ int64_t s_src[kMoveTokens], s_dst[kMoveTokens];
   const int seq = blockIdx.z;
   const int head = int(blockIdx.y) % a.num_kv_heads, layer = int(blockIdx.y) / a.num_kv_heads;
-  const int n = min(min(a.keep[seq], a.max_keep), a.kv_len[seq]);
+  const int n = min(min(a.keep[seq], a.max_keep), min(a.kv_len[seq], a.max_len));
   const int j0 = int(blockIdx.x) * kMoveTokens;
   if (j0 >= n) return;   // uniform
   const int cnt = min(kMoveTokens, n - j0);
@@ -340,6 +340,7 @@ extern "C" int kunserve_evict(const kunserve_kv_pool* pool, const kunserve_kv_we
   a.out_indices = out_indices_dev;
   a.keep = keep_dev;
   a.max_keep = max_keep;
+  a.max_len = max_len;
   a.sinks = sinks;
   a.recent = recent;
   a.kept = kept_dev;

@@ -424,6 +424,9 @@ class DecodePlan:
             ctypes.byref(self.info), self.num_qo_heads, head_dim))
 
 
+_SHARED_PLAN_INTS = 1 << 20   # 4 MiB
+
+
 class SharedDecodePlan:
     """Plan of decode rows whose page lists begin alike (kunserve_shared_plan),
     computed on the host once per step and shared by every layer. Runs of whole
@@ -440,13 +443,20 @@ class SharedDecodePlan:
             raise ValueError("the table's indptr runs past its indices")
         kv_ptr = kv.ctypes.data if n else None
         cap = int(_lib.lib().kunserve_shared_plan_bound(kv_ptr, n, num_qo_heads))
-        buf = np.empty(max(cap, 4), dtype=np.int32)   # the plan writes what it uses
         self.shared_info = _lib.SharedPlanInfo()
-        _lib.call("kunserve_shared_plan", table.indptr_host.ctypes.data, indices.ctypes.data,
-                  kv_ptr, n, num_qo_heads, num_kv_heads, page_size, head_dim,
-                  num_cus if num_cus is not None else _num_cus(device),
-                  -1 if min_bytes is None else min_bytes, buf.ctypes.data, buf.size,
-                  ctypes.byref(self.shared_info))
+        # The bound holds for any tree of pages and is far above what plans use.
+        for size in (min(cap, _SHARED_PLAN_INTS), cap):
+            buf = np.empty(max(size, 4), dtype=np.int32)   # the plan writes what it uses
+            try:
+                _lib.call("kunserve_shared_plan", table.indptr_host.ctypes.data,
+                          indices.ctypes.data, kv_ptr, n, num_qo_heads, num_kv_heads, page_size,
+                          head_dim, num_cus if num_cus is not None else _num_cus(device),
+                          -1 if min_bytes is None else min_bytes, buf.ctypes.data, buf.size,
+                          ctypes.byref(self.shared_info))
+                break
+            except _lib.KunserveError as e:
+                if e.code != _lib.ENOSPC or size >= cap:
+                    raise
         self.info = self.shared_info.decode
         self.num_counters = 0   # a launch of its own joins the partials
         self.plan_host = buf[: self.shared_info.plan_ints].copy()

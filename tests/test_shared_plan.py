@@ -146,6 +146,26 @@ def test_sharing_has_to_pay():
     assert plan_of(t, kv, 32, 8, 16, 128, min_bytes=-1)[0].num_segments == 1   # 29 MB
 
 
+def test_plans_beyond_the_first_buffer(monkeypatch):
+    """SharedDecodePlan tries a small buffer before the bound's; a plan that does
+    not fit is made again."""
+    import torch
+    from kunserve_amd import PageTable, SharedDecodePlan, paged_kv
+
+    t = rows(20, [1] * 40)
+    kv = [len(x) * 16 - 5 for x in t]
+    indptr = np.r_[0, np.cumsum([len(x) for x in t])]
+    table = PageTable(indptr, np.concatenate(t), kv, torch.device("cpu"), upload=False)
+    make = lambda: SharedDecodePlan(table, 8, 2, 16, torch.device("cpu"), num_cus=256,   # noqa: E731
+                                    upload=False, min_bytes=0)
+    want = make().plan_host
+    monkeypatch.setattr(paged_kv, "_SHARED_PLAN_INTS", 16)
+    assert len(want) > 16
+    np.testing.assert_array_equal(make().plan_host, want)
+    with pytest.raises(_lib.KunserveError, match="power of two"):
+        SharedDecodePlan(table, 8, 2, 12, torch.device("cpu"), num_cus=256, upload=False)
+
+
 def test_refusals():
     with pytest.raises(_lib.KunserveError, match="multiple"):
         plan_of([[0]], [3], 5, 2, 16, 128)

@@ -106,6 +106,7 @@ def test_evict_refusals(pool, monkeypatch):
     assert evict(pool, w, [], [], [], 9).shape == (0, 2, 2, 0)
     for kw, what in ((dict(budget=[20, 10, 3]), "one per request"), (dict(budget=-1), "negative"),
                      (dict(budget=[[20, 10]]), "one per request"),
+                     (dict(budget=0.2), "whole numbers"), (dict(budget=[1.0, 2.0]), "whole"),
                      (dict(ok, sinks=-1), "negative"), (dict(ok, recent=-2), "negative")):
         with pytest.raises(ValueError, match=what):
             evict(pool, w, tables, kv, out, **kw)

@@ -348,7 +348,8 @@ typedef struct {
   int32_t wide;          /* whether some run in workgroups of 128 columns     */
   int32_t num_pairs;     /* (row, first partial) records                      */
   int32_t num_segments;  /* runs of pages that several rows share             */
-  int32_t head_dim;      /* head_dim the plan was made for                    */
+  int32_t head_dim;      /* head_dim and page_size the plan was made for      */
+  int32_t page_size;
   int32_t plan_ints;     /* int32 entries of the plan buffer in use           */
 } kunserve_shared_plan_info;
 

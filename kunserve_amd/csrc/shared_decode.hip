@@ -18,6 +18,7 @@
 // and the matrix units 16 columns at a time.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 #include "decode_tile.hpp"
@@ -65,17 +66,15 @@ struct Columns {
   }
 };
 
-// Scores of a step's 16-token tiles (masked where `whole` is not set) to
-// probabilities of a column tile, in two 16-bit terms, with the lazy running
-// maximum of paged_decode_mfma_kernel; o: the column's accumulators.
-template <typename T, int D>
-__device__ __forceinline__ void tile_softmax(f32x4 (&sc)[DecodeTile<D>::PAIRS][2], float scale_log2,
-                                             float& m, float& lsum,
-                                             f32x4 (&o)[DecodeTile<D>::ACCS][8],
-                                             typename Vec<T>::v8 (&ph)[DecodeTile<D>::ACCS],
-                                             typename Vec<T>::v8 (&pl)[DecodeTile<D>::ACCS]) {
+// Scores of a step's 16-token tiles (masked where the step is not whole) to
+// probabilities of a column tile, with the lazy running maximum of
+// paged_decode_mfma_kernel (o: the column's accumulators): first its update, seldom
+// made, for which alone the lanes' maxima are joined.
+template <int D>
+__device__ __forceinline__ void tile_max(const f32x4 (&sc)[DecodeTile<D>::PAIRS][2],
+                                         float scale_log2, float& m, float& lsum,
+                                         f32x4 (&o)[DecodeTile<D>::ACCS][8]) {
   typedef DecodeTile<D> L;
-  typedef typename Vec<T>::v8 V8;
   float mx = -INFINITY;
 #pragma unroll
   for (int p = 0; p < L::PAIRS; ++p)
@@ -83,8 +82,8 @@ __device__ __forceinline__ void tile_softmax(f32x4 (&sc)[DecodeTile<D>::PAIRS][2
     for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
       for (int x = 0; x < 4; ++x) mx = fmaxf(mx, sc[p][sub][x]);
-  mx = groups_max(mx) * scale_log2;
-  if (__any(mx > m + 8.f)) {
+  if (__any(mx * scale_log2 > m + 8.f)) {
+    mx = groups_max(mx) * scale_log2;
     const float m_new = mx > m + 8.f ? mx : m;
     const float alpha = fast_exp2(m - m_new);
     m = m_new;
@@ -94,6 +93,15 @@ __device__ __forceinline__ void tile_softmax(f32x4 (&sc)[DecodeTile<D>::PAIRS][2
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[x][e] *= alpha;
   }
+}
+// The probabilities, in two 16-bit terms (pl is left out by callers of one).
+template <typename T, int D>
+__device__ __forceinline__ void tile_exp(const f32x4 (&sc)[DecodeTile<D>::PAIRS][2],
+                                         float scale_log2, float m, float& lsum,
+                                         typename Vec<T>::v8 (&ph)[DecodeTile<D>::ACCS],
+                                         typename Vec<T>::v8 (&pl)[DecodeTile<D>::ACCS]) {
+  typedef DecodeTile<D> L;
+  typedef typename Vec<T>::v8 V8;
 #pragma unroll
   for (int p = 0; p < L::PAIRS; ++p)
 #pragma unroll
@@ -186,6 +194,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
   constexpr int kKBytes = (WIDE ? 2 : 1) * W * BLK * int(sizeof(T));
   constexpr int kOBytes = W * 16 * D * int(sizeof(float));
   __shared__ __attribute__((aligned(16))) char s_raw[kKBytes > kOBytes ? kKBytes : kOBytes];
+  __shared__ __attribute__((aligned(16))) T s_new[2 * D];   // the new token's K and V row
   __shared__ float s_m[W][16];
   __shared__ float s_l[W][16];
   // Q of a narrow workgroup at head_dim 256 (column g's chunk c at c ^ (g & 7)):
@@ -245,6 +254,15 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
     s_pages[i] = ok ? p : -1;
     bad_id |= !ok;
   }
+  const NewRow nr = tail ? new_row(a, columns.seq, columns.token(a, 0), hkv) : NewRow{-1, 0, 0};
+  const bool has_new = nr.pos >= tb && nr.pos < te;   // uniform
+  const bool new_v = tid >= L::CH;
+  V8 fresh;   // of the first 2 CH threads
+  if (has_new && tid < 2 * L::CH) {
+    const f16* base = (new_v ? a.v : a.k) + int64_t(hkv) * a.head_stride + 8 * (tid % L::CH);
+    fresh = load_v8<T>(base + (new_v ? nr.v : nr.k));
+    *reinterpret_cast<V8*>(&s_new[8 * tid]) = fresh;
+  }
   const bool wave_bad = __any(bad_id);
   if (lane == 0) s_bad[wave] = wave_bad;
   if constexpr (kQInLds) {
@@ -260,17 +278,76 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
   for (int wv = 0; wv < W; ++wv) bad_votes |= s_bad[wv];
   const bool any_bad = __builtin_amdgcn_readfirstlane(bad_votes) != 0;
 
-  const NewRow nr = tail ? new_row(a, columns.seq, columns.token(a, 0), hkv) : NewRow{-1, 0, 0};
-  if (nr.pos >= tb && nr.pos < te && hq0 % a.ratio == 0)
-    append_row<D>(a, nr, s_pages[(nr.pos >> a.page_shift) - pb], hkv);
+  if (has_new && hq0 % a.ratio == 0 && tid < 2 * L::CH) {   // as append_row
+    const int page = s_pages[(nr.pos >> a.page_shift) - pb];
+    f16* base = const_cast<f16*>(new_v ? a.v : a.k) + int64_t(hkv) * a.head_stride +
+                8 * (tid % L::CH);
+    if (page >= 0)
+      *reinterpret_cast<V8*>(base + int64_t(page) * a.page_stride +
+                             int64_t(nr.pos & page_mask) * a.token_stride) = fresh;
+  }
   const f16* kb = a.k + int64_t(hkv) * a.head_stride + lcol * 8;
   const f16* vb = a.v + int64_t(hkv) * a.head_stride + lcol * 8;
   const int nsteps = (te - tb + STEP - 1) / STEP;
   T* const blocks = reinterpret_cast<T*>(s_raw);
   T* sk = blocks + wave * BLK;
 
+  // Pages that hold a load's TPL token rows whole: the load's address is a scalar
+  // and the lane's 32-bit offset (pieces begin at multiples of a page and of 64,
+  // partitions of 128). Looked up for each lane's row instead, addresses were half
+  // of a tail's instructions.
+  const bool scalar = (1 << a.page_shift) >= TPL;   // uniform; of D 64 not with 4-token pages
+  const char* const ks = reinterpret_cast<const char*>(a.k + int64_t(hkv) * a.head_stride);
+  const char* const vs = reinterpret_cast<const char*>(a.v + int64_t(hkv) * a.head_stride);
+  const uint32_t lane_at = 2 * (uint32_t(lrow) * uint32_t(a.token_stride) + 8 * uint32_t(lcol));
+  const int wave_s = __builtin_amdgcn_readfirstlane(wave);   // branches on it are scalar
+  int64_t at[LOADS];   // bytes, of the loads of the step on its way
+  int dropped = 0;     // those (bits) that lie past `te` or in a page outside the pool: from page 0
+  auto find_step = [&](int c) {
+    const int ts = tb + c * STEP;
+    auto find = [&](auto loads_per_page) {
+      constexpr int P = decltype(loads_per_page)::value;
+      int page[LOADS / P];
+#pragma unroll
+      for (int h = 0; h < LOADS / P; ++h)
+        page[h] = s_pages[min(max(((ts + h * P * TPL) >> a.page_shift) - pb, 0), np - 1)];
+      dropped = 0;
+#pragma unroll
+      for (int h = 0; h < LOADS / P; ++h) {
+        const int t = ts + h * P * TPL;
+        const int id = __builtin_amdgcn_readfirstlane(page[h]);
+        const bool drop = t >= te || id < 0;
+        dropped |= drop ? ((1 << P) - 1) << (h * P) : 0;
+        const int64_t off = drop ? 0 : 2 * (int64_t(id) * a.page_stride +
+                                            int64_t(t & page_mask) * a.token_stride);
+#pragma unroll
+        for (int i = 0; i < P; ++i) at[h * P + i] = off + i * (2 * TPL * a.token_stride);
+      }
+    };
+    if (a.page_shift >= 4)   // uniform
+      find(std::integral_constant<int, 16 / TPL>{});
+    else
+      find(std::integral_constant<int, 1>{});
+  };
+
   V8 k[LOADS], v[LOADS];
+  auto load_rows = [&](int i) {
+    k[i] = load_v8<T>(ks + at[i] + lane_at);
+    v[i] = load_v8<T>(vs + at[i] + lane_at);
+  };
+  auto drop_rows = [&] {   // their scores are masked; 0 x V has to be 0
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+      if (dropped >> i & 1) v[i] = V8{};
+  };
   auto load = [&](int c) {
+    if (scalar) {
+      if (c >= nsteps) return;
+      find_step(c);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) load_rows(i);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int t = tb + c * STEP + TPL * i + lrow;
@@ -295,10 +372,11 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
   };
 
   if constexpr (WIDE) {
+    static_assert(PAIRS == 1 && L::ACCS == 1 && kWideTiles == 2 && 2 * KS == 8);
     if (cols > 16) {   // uniform
       // Every wave has tiles of its own; a round of the loop is a step of each
       // wave's tokens, which all waves take from LDS.
-      const int c0 = wave * kWideTiles * 16;
+      const int c0 = wave_s * kWideTiles * 16;
       V8 q[kWideTiles][KS];
 #pragma unroll
       for (int ct = 0; ct < kWideTiles; ++ct) {
@@ -319,96 +397,114 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
           for (int e = 0; e < 8; ++e) o[ct][x][e] = f32x4{};
       }
       V8* const values = reinterpret_cast<V8*>(blocks + W * BLK);   // [wave][dim e][lane]
-      // A load's TPL token rows lie in one page (a segment's pieces start and end
-      // at multiples of 4): its address is a lane's pointer and a scalar offset.
-      // Rows past the piece and of page ids outside the pool are read from page 0
-      // and dropped: their scores masked, their V cleared.
-      const f16* kl = kb + int64_t(lrow) * a.token_stride;
-      const f16* vl = vb + int64_t(lrow) * a.token_stride;
-      int dropped = 0;   // loads (bits) of the step on its way
-      auto load_step = [&](int c) {
-        dropped = 0;
-        int page[LOADS];
+      // The blocks' places (k_row, park) differ by an XOR of bits 6 and 7 and by
+      // constants: one register, and the XOR made at each use, so that none is kept.
+      auto moved = [&](int base, int x) {
+        asm volatile("v_xor_b32 %0, %1, %2" : "=v"(base) : "n"(x << 6), "v"(base));
+        return base;
+      };
+      const int read_at = L::token(j & 3, j >> 2, 0) * D * 2 + ((tg ^ L::swz(L::token(j & 3, j >> 2, 0))) << 4);
+      const int park_at = (wave * BLK + lrow * D) * 2 + ((lcol ^ lrow) << 4);
+      find_step(wave_s);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) load_rows(i);
+      for (int c = 0; c < nsteps; c += W) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
-          page[i] = s_pages[min(max(((tb + c * STEP + TPL * i) >> a.page_shift) - pb, 0), np - 1)];
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-          const int t = tb + c * STEP + TPL * i;
-          const int p = t < te ? __builtin_amdgcn_readfirstlane(page[i]) : -1;
-          dropped |= int(p < 0) << i;
-          const int64_t off = int64_t(max(p, 0)) * a.page_stride +
-                              (p >= 0 ? int64_t(t & page_mask) * a.token_stride : 0);
-          k[i] = load_v8<T>(kl + off);
-          v[i] = load_v8<T>(vl + off);
-        }
-      };
-      const int wave_s = __builtin_amdgcn_readfirstlane(wave);
-      load_step(wave_s);
-      for (int c = 0; c < nsteps; c += W) {
-        park();
-        if (dropped) {   // uniform
-#pragma unroll
-          for (int i = 0; i < LOADS; ++i)
-            if (dropped >> i & 1) v[i] = V8{};
-        }
+          *reinterpret_cast<V8*>(s_raw + moved(park_at, i & 3) + i * TPL * D * 2) = k[i];
+        if (dropped) drop_rows();   // uniform
         V8 vt[8];
         transpose8(v, vt);
 #pragma unroll
         for (int e = 0; e < 8; ++e) values[(wave * 8 + e) * kWave + lane] = vt[e];
-        load_step(c + W + wave_s);
+        find_step(c + W + wave_s);
         __syncthreads();
-        if (c0 < cols) {   // uniform
-          for (int blk = 0; blk < W && c + blk < nsteps; ++blk) {
-            const T* block = blocks + blk * BLK;
+        // The next step's loads a few at a time between the products: together
+        // they would wait for the CU's one path to the caches.
+        auto load_some = [&](int blk) {
+#pragma unroll
+          for (int i = 0; i < LOADS / W; ++i) load_rows(blk * (LOADS / W) + i);
+        };
+        if (c0 >= cols) {   // uniform
+#pragma unroll
+          for (int blk = 0; blk < W; ++blk) load_some(blk);
+        } else {
+          // One wave to a SIMD: what overlaps does so within its instructions. A
+          // tile's exponentials stand between the products of the other tile (scores of the
+          // second, then P V of the first), and V and the next K are read into
+          // the registers that the products are done with. Probabilities in one
+          // 16-bit term: at 64 columns and more the matrix units' work counts.
+          // Steps past the piece are masked ones.
+          V8 ka[2][KS], ve[8];
+          auto read_k = [&](int blk, int i) {
+            ka[i & 1][i >> 1] = *reinterpret_cast<const V8*>(
+                s_raw + moved(read_at, i >> 1) + (blk * BLK + (i & 1) * 16 * D) * 2);
+          };
+#pragma unroll
+          for (int i = 0; i < 2 * KS; ++i) read_k(0, i);
+#pragma unroll
+          for (int blk = 0; blk < W; ++blk) {
+            load_some(blk);
             const int t0 = tb + (c + blk) * STEP;
-            // A tile's operands are read together, V's before the softmax: a read
-            // right before its use would be waited for each time.
-            V8 ka[PAIRS][2][KS];
-#pragma unroll
-            for (int p = 0; p < PAIRS; ++p)
-#pragma unroll
-              for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-                for (int s = 0; s < KS; ++s) ka[p][sub][s] = k_row(block, p, sub, s);
-            __builtin_amdgcn_sched_barrier(0);
+            const bool edge = any_bad || t0 + STEP > te;   // uniform
             f32x4 sc[kWideTiles][PAIRS][2];
-#pragma unroll
-            for (int p = 0; p < PAIRS; ++p)
+            V8 ph[kWideTiles][L::ACCS], unused[L::ACCS];
+            auto scores = [&](int ct, int s) {
 #pragma unroll
               for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-                for (int ct = 0; ct < kWideTiles; ++ct) {
-                  sc[ct][p][sub] = f32x4{};
-#pragma unroll
-                  for (int s = 0; s < KS; ++s)
-                    sc[ct][p][sub] = mfma16(ka[p][sub][s], q[ct][s], sc[ct][p][sub]);
-                }
-            __builtin_amdgcn_sched_barrier(0);
-            V8 ve[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ve[e] = values[(blk * 8 + e) * kWave + lane];
-            __builtin_amdgcn_sched_barrier(0);
-            // Probabilities in one 16-bit term: at 64 columns and more the matrix
-            // units' work counts (128 rows behind 8192 tokens, 64 heads: 112 us a
-            // layer against 124 with the second term).
-            V8 ph[kWideTiles][L::ACCS], unused[L::ACCS];
-#pragma unroll
-            for (int ct = 0; ct < kWideTiles; ++ct) {
-              if (any_bad || t0 + STEP > te) {
+                sc[ct][0][sub] = mfma16(ka[sub][s], q[ct][s], s == 0 ? f32x4{} : sc[ct][0][sub]);
+            };
+            auto maximum = [&](int ct) {
+              if (edge) {
                 int g = tg;
                 asm volatile("" : "+v"(g));   // keeps the indexes' arithmetic in here
                 mask_scores<D>(sc[ct], t0, te, g, any_bad, s_pages, a.page_shift, pb);
               }
-              tile_softmax<T, D>(sc[ct], a.scale_log2, m[ct], lsum[ct], o[ct], ph[ct], unused);
+              tile_max<D>(sc[ct], a.scale_log2, m[ct], lsum[ct], o[ct]);
+            };
+#pragma unroll
+            for (int s = 0; s < KS; ++s) scores(0, s);
+            __builtin_amdgcn_sched_barrier(0);
+            maximum(0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+              scores(1, s);
+              ve[2 * s] = values[(blk * 8 + 2 * s) * kWave + lane];
+              ve[2 * s + 1] = values[(blk * 8 + 2 * s + 1) * kWave + lane];
+            }
+            tile_exp<T, D>(sc[0], a.scale_log2, m[0], lsum[0], ph[0], unused);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // a product
+              __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);   // vector operations
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // reads
+              __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            maximum(1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[0][0][e] = mfma16(ve[e], ph[0][0], o[0][0][e]);
+            tile_exp<T, D>(sc[1], a.scale_log2, m[1], lsum[1], ph[1], unused);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              o[1][0][e] = mfma16(ve[e], ph[1][0], o[1][0][e]);
+              if (blk + 1 < W) read_k(blk + 1, e);
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-#pragma unroll
-              for (int x = 0; x < L::ACCS; ++x)
-#pragma unroll
-                for (int ct = 0; ct < kWideTiles; ++ct)
-                  o[ct][x][e] = mfma16(ve[e], ph[ct][x], o[ct][x][e]);
+            for (int e = 0; e < 8; ++e) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
         __syncthreads();   // the round's blocks are done with
@@ -455,6 +551,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
     }
   }
 
+  if constexpr (WIDE) __builtin_amdgcn_s_setprio(3);
   V8 qb[kQInLds ? 1 : KS];
   if constexpr (!kQInLds) {
     const f16* qp = columns.q(a, min(j, cols - 1)) + 8 * tg;
@@ -467,8 +564,22 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[x][e] = f32x4{};
   float m = kNegBig, lsum = 0.f;
-  if (wave < nsteps) load(wave);
-  for (int c = wave; c < nsteps; c += W) {
+  if (wave_s < nsteps) load(wave_s);
+  for (int c = wave_s; c < nsteps; c += W) {
+    if (scalar) {
+      if (tb + c * STEP + STEP >= te) {   // uniform: rows past the end, and the new one
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int t = tb + c * STEP + TPL * i + lrow;
+          if (t >= te) v[i] = V8{};
+          if (has_new && t == nr.pos) {
+            k[i] = *reinterpret_cast<const V8*>(&s_new[8 * lcol]);
+            v[i] = *reinterpret_cast<const V8*>(&s_new[D + 8 * lcol]);
+          }
+        }
+      }
+      if (dropped) drop_rows();   // uniform
+    }
     park();
     V8 vt[8];
     transpose8(v, vt);
@@ -497,7 +608,8 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
     if (any_bad || t0 + STEP > te)   // uniform
       mask_scores<D>(sc, t0, te, tg, any_bad, s_pages, a.page_shift, pb);
     V8 ph[L::ACCS], pl[L::ACCS];
-    tile_softmax<T, D>(sc, a.scale_log2, m, lsum, o, ph, pl);
+    tile_max<D>(sc, a.scale_log2, m, lsum, o);
+    tile_exp<T, D>(sc, a.scale_log2, m, lsum, ph, pl);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
 #pragma unroll
@@ -807,6 +919,7 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
   info->num_pairs = int32_t(pairs.size() / 2);
   info->num_segments = int32_t(segments.size());
   info->head_dim = head_dim;
+  info->page_size = page_size;
   KSV_CHECK_ARG(plan.size() < (size_t(1) << 31), "the plan is too long");
   info->plan_ints = int32_t(plan.size());
   return KUNSERVE_OK;
@@ -882,6 +995,10 @@ int kunserve::shared_decode(const kunserve_kv_pool* pool, int32_t layer,
                 pool->num_kv_heads);
   KSV_CHECK_ARG(info->head_dim == pool->head_dim, "plan made for head_dim %d, pool has %d",
                 info->head_dim, pool->head_dim);
+  KSV_CHECK_ARG(info->page_size == pool->page_size, "plan made for pages of %d, pool has %d",
+                info->page_size, pool->page_size);
+  KSV_CHECK_ARG(pool->token_stride < (int64_t(1) << 28),
+                "tokens %lld elements apart: less than 2^28 here", (long long)pool->token_stride);
   KSV_CHECK_ARG(info->decode.group_size == decode_group(num_qo_heads, pool->num_kv_heads),
                 "plan group size %d is not that of %d query heads on %d", info->decode.group_size,
                 num_qo_heads, pool->num_kv_heads);

@@ -185,3 +185,27 @@ def test_refusals():
                   np.array([7], np.int32).ctypes.data, 1, 4, 2, 16, 128, 256, 0, buf.ctypes.data,
                   4, ctypes.byref(info))
     assert e.value.code == _lib.ENOSPC
+
+
+def test_a_plan_and_its_pool():
+    """Checks of the launch that come before it: the pool's page size is the plan's,
+    and a token's stride fits the kernel's 32-bit offsets."""
+    info, _ = plan_of(rows(4, [1] * 3), [70, 70, 70], 4, 2, 16, 128)
+    buf = np.zeros(64, np.uint8)
+    at = -(-buf.ctypes.data // 16) * 16
+    three = _lib.Tensor3(at, 512, 128)
+
+    def decode(page_size=16, token_stride=128, **kw):
+        pool = _lib.KVPool(k=at, v=at, num_pages=1, page_stride=1 << 40, layer_stride=1 << 39,
+                           head_stride=1 << 38, token_stride=token_stride, num_layers=1,
+                           num_kv_heads=2, page_size=page_size, head_dim=128, dtype=0)
+        table = _lib.PageTable(at, at, at, 3)
+        _lib.call("kunserve_shared_decode", ctypes.byref(pool), 0, ctypes.byref(table), None,
+                  ctypes.byref(three), ctypes.byref(three), 4, 1.0, at, ctypes.byref(info), None,
+                  0, None)
+
+    assert info.num_segments == 1
+    with pytest.raises(_lib.KunserveError, match="pages of 16"):
+        decode(page_size=32)
+    with pytest.raises(_lib.KunserveError, match="2\\^28"):
+        decode(token_stride=1 << 28)

@@ -41,9 +41,14 @@ struct SharedArgs {
   DecodeArgs d;            // work: the tails'
   const int32_t* shared;   // [num_shared][kRecord]: rows (0: padding), their first pair,
                            // token begin, end, place among a row's partials, a row of them,
-                           // head group
+                           // head group, where that row's pages start in the table
   const int32_t* pairs;    // [...][2]: row, its first slot
+  const int32_t* tail_pages;   // [work]: where its row's pages start
+  const int32_t* first_ids;    // [work][waves][step_ids]: the pages of the waves' first steps
+  int32_t step_ids;
   int32_t num_shared;
+  uint32_t inv_group;          // 2^16 / group and 2^32 / head_groups, rounded up
+  uint32_t inv_head_groups;
 };
 
 // Columns of a workgroup: 16, its waves taking the tokens in turn (narrow), or
@@ -56,11 +61,13 @@ constexpr int kWideCols = kWaves * kWideTiles * 16;    // 128
 struct Columns {
   const int32_t* pairs;
   int seq, group, hq0;
-  __device__ __forceinline__ int row(int c) const { return pairs ? pairs[2 * (c / group)] : seq; }
+  uint32_t inv_group;
+  __device__ __forceinline__ int pair(int c) const { return int(uint32_t(c) * inv_group >> 16); }
+  __device__ __forceinline__ int row(int c) const { return pairs ? pairs[2 * pair(c)] : seq; }
   __device__ __forceinline__ int token(const DecodeArgs& a, int c) const {
     return a.q_token ? a.q_token[row(c)] : row(c);
   }
-  __device__ __forceinline__ int head(int c) const { return hq0 + c % group; }
+  __device__ __forceinline__ int head(int c) const { return hq0 + c - pair(c) * group; }
   __device__ __forceinline__ const f16* q(const DecodeArgs& a, int c) const {
     return a.q + int64_t(token(a, c)) * a.q_tok + int64_t(head(c)) * a.q_head;
   }
@@ -143,6 +150,22 @@ __device__ __forceinline__ void mask_scores(f32x4 (&sc)[DecodeTile<D>::PAIRS][2]
       }
 }
 
+// The same where whole loads are dropped.
+template <int D>
+__device__ __forceinline__ void mask_loads(f32x4 (&sc)[DecodeTile<D>::PAIRS][2], int t0, int te,
+                                           int tg, int dropped) {
+  typedef DecodeTile<D> L;
+#pragma unroll
+  for (int p = 0; p < L::PAIRS; ++p)
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int t = L::token(4 * sub + x, tg, p);
+        if (t0 + t >= te || (dropped >> (t / L::TPL) & 1)) sc[p][sub][x] = -INFINITY;
+      }
+}
+
 // vt[e]: dim 8 chunk + e of the lane's 8 tokens.
 template <typename V8>
 __device__ __forceinline__ void transpose8(const V8 (&v)[8], V8 (&vt)[8]) {
@@ -213,7 +236,8 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
   // The segments' workgroups come first (a multiple of 8, so that those of the
   // tails are on the XCDs their plan has them on).
   int nrows = 1, hg, tb, te, place = 0, slot = -1;
-  Columns columns{nullptr, 0, a.group, 0};
+  Columns columns{nullptr, 0, a.group, 0, sa.inv_group};
+  int page_at, item = 0;
   const bool tail = int(blockIdx.x) >= sa.num_shared;   // uniform, as all of this
   if (!tail) {
     const int32_t* rec = sa.shared + kRecord * int(blockIdx.x);
@@ -225,13 +249,15 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
     place = rec[4];
     columns.seq = rec[5];
     hg = rec[6];
+    page_at = rec[7];
   } else {
     const int b = int(blockIdx.x) - sa.num_shared;
-    const int local = (b >> 3) / a.head_groups;
+    const int local = a.head_groups == 1 ? b >> 3 : int(__umulhi(uint32_t(b >> 3), sa.inv_head_groups));
     hg = (b >> 3) - local * a.head_groups;
-    const int item = 8 * local + (b & 7);
+    item = 8 * local + (b & 7);
     if (item >= a.num_work) return;
     const int32_t* w = a.work + 4 * item;
+    page_at = sa.tail_pages[item];
     columns.seq = w[0];
     if (columns.seq < 0) return;
     tb = w[1];
@@ -241,51 +267,32 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
   const int cols = nrows * a.group;
   const int hq0 = hg * a.group;
   columns.hq0 = hq0;
-  const int hkv = hq0 / a.ratio;
+  const int hkv = a.group == a.ratio ? hg : hq0 / a.ratio;
   const int page_mask = (1 << a.page_shift) - 1;
 
   const int pb = tb >> a.page_shift;
   const int np = te > tb ? ((te - 1) >> a.page_shift) + 1 - pb : 0;
-  const int32_t* seq_pages = a.indices + a.indptr[columns.seq];
-  bool bad_id = false;
-  for (int i = tid; i < np; i += W * kWave) {
+  const int32_t* seq_pages = a.indices + page_at;
+  auto page_id = [&](int i) {   // -1: outside the pool
     const int p = seq_pages[pb + i];
-    const bool ok = p >= 0 && p < a.num_pages;
-    s_pages[i] = ok ? p : -1;
-    bad_id |= !ok;
-  }
-  const NewRow nr = tail ? new_row(a, columns.seq, columns.token(a, 0), hkv) : NewRow{-1, 0, 0};
-  const bool has_new = nr.pos >= tb && nr.pos < te;   // uniform
-  const bool new_v = tid >= L::CH;
-  V8 fresh;   // of the first 2 CH threads
-  if (has_new && tid < 2 * L::CH) {
-    const f16* base = (new_v ? a.v : a.k) + int64_t(hkv) * a.head_stride + 8 * (tid % L::CH);
-    fresh = load_v8<T>(base + (new_v ? nr.v : nr.k));
-    *reinterpret_cast<V8*>(&s_new[8 * tid]) = fresh;
-  }
-  const bool wave_bad = __any(bad_id);
-  if (lane == 0) s_bad[wave] = wave_bad;
-  if constexpr (kQInLds) {
-    for (int i = tid; i < 16 * L::CH; i += W * kWave) {
-      const int g = i / L::CH, c = i % L::CH;
-      *reinterpret_cast<V8*>(&s_q[g * D + 8 * (c ^ (g & 7))]) =
-          g < cols ? load_v8<T>(columns.q(a, g) + 8 * c) : V8{};
+    return p >= 0 && p < a.num_pages ? p : -1;
+  };
+  auto stage_pages = [&] {   // for all waves; whether one of the ids is bad
+    bool bad_id = false;
+    for (int i = tid; i < np; i += W * kWave) {
+      const int p = page_id(i);
+      s_pages[i] = p;
+      bad_id |= p < 0;
     }
-  }
-  __syncthreads();
-  int bad_votes = 0;
+    const bool wave_bad = __any(bad_id);
+    if (lane == 0) s_bad[wave] = wave_bad;
+    __syncthreads();
+    int bad_votes = 0;
 #pragma unroll
-  for (int wv = 0; wv < W; ++wv) bad_votes |= s_bad[wv];
-  const bool any_bad = __builtin_amdgcn_readfirstlane(bad_votes) != 0;
-
-  if (has_new && hq0 % a.ratio == 0 && tid < 2 * L::CH) {   // as append_row
-    const int page = s_pages[(nr.pos >> a.page_shift) - pb];
-    f16* base = const_cast<f16*>(new_v ? a.v : a.k) + int64_t(hkv) * a.head_stride +
-                8 * (tid % L::CH);
-    if (page >= 0)
-      *reinterpret_cast<V8*>(base + int64_t(page) * a.page_stride +
-                             int64_t(nr.pos & page_mask) * a.token_stride) = fresh;
-  }
+    for (int wv = 0; wv < W; ++wv) bad_votes |= s_bad[wv];
+    return __builtin_amdgcn_readfirstlane(bad_votes) != 0;
+  };
+  const bool wide = WIDE && cols > 16;   // uniform
   const f16* kb = a.k + int64_t(hkv) * a.head_stride + lcol * 8;
   const f16* vb = a.v + int64_t(hkv) * a.head_stride + lcol * 8;
   const int nsteps = (te - tb + STEP - 1) / STEP;
@@ -294,40 +301,61 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
 
   // Pages that hold a load's TPL token rows whole: the load's address is a scalar
   // and the lane's 32-bit offset (pieces begin at multiples of a page and of 64,
-  // partitions of 128). Looked up for each lane's row instead, addresses were half
-  // of a tail's instructions.
-  const bool scalar = (1 << a.page_shift) >= TPL;   // uniform; of D 64 not with 4-token pages
+  // partitions of 128): all but pages of 4 tokens at head_dim 64. Looked up for each
+  // lane's row instead, addresses were half of a tail's instructions.
+  const bool scalar = TPL <= kMinPageSize || (1 << a.page_shift) >= TPL;   // uniform
   const char* const ks = reinterpret_cast<const char*>(a.k + int64_t(hkv) * a.head_stride);
   const char* const vs = reinterpret_cast<const char*>(a.v + int64_t(hkv) * a.head_stride);
   const uint32_t lane_at = 2 * (uint32_t(lrow) * uint32_t(a.token_stride) + 8 * uint32_t(lcol));
   const int wave_s = __builtin_amdgcn_readfirstlane(wave);   // branches on it are scalar
   int64_t at[LOADS];   // bytes, of the loads of the step on its way
   int dropped = 0;     // those (bits) that lie past `te` or in a page outside the pool: from page 0
-  auto find_step = [&](int c) {
+  // A step's pages: id(h) of its tokens from h * granule on.
+  const int granule = a.page_shift >= 4 ? 16 : TPL;   // uniform
+  auto find = [&](int c, auto loads_per_page, auto id) {
+    constexpr int P = decltype(loads_per_page)::value;
     const int ts = tb + c * STEP;
-    auto find = [&](auto loads_per_page) {
+    dropped = 0;
+#pragma unroll
+    for (int h = 0; h < LOADS / P; ++h) {
+      const int t = ts + h * P * TPL;
+      const int p = id(h);
+      const bool drop = t >= te || p < 0;
+      dropped |= drop ? ((1 << P) - 1) << (h * P) : 0;
+      const int64_t off = drop ? 0 : 2 * (int64_t(p) * a.page_stride +
+                                          int64_t(t & page_mask) * a.token_stride);
+#pragma unroll
+      for (int i = 0; i < P; ++i) at[h * P + i] = off + i * (2 * TPL * a.token_stride);
+    }
+  };
+  typedef std::integral_constant<int, 16 / TPL> Granule16;
+  typedef std::integral_constant<int, 1> Granule1;
+  auto place_of = [&](int t) { return min(max((t >> a.page_shift) - pb, 0), np - 1); };
+  // From LDS.
+  auto find_step = [&](int c) {
+    auto look = [&](auto loads_per_page) {
       constexpr int P = decltype(loads_per_page)::value;
       int page[LOADS / P];
 #pragma unroll
-      for (int h = 0; h < LOADS / P; ++h)
-        page[h] = s_pages[min(max(((ts + h * P * TPL) >> a.page_shift) - pb, 0), np - 1)];
-      dropped = 0;
-#pragma unroll
-      for (int h = 0; h < LOADS / P; ++h) {
-        const int t = ts + h * P * TPL;
-        const int id = __builtin_amdgcn_readfirstlane(page[h]);
-        const bool drop = t >= te || id < 0;
-        dropped |= drop ? ((1 << P) - 1) << (h * P) : 0;
-        const int64_t off = drop ? 0 : 2 * (int64_t(id) * a.page_stride +
-                                            int64_t(t & page_mask) * a.token_stride);
-#pragma unroll
-        for (int i = 0; i < P; ++i) at[h * P + i] = off + i * (2 * TPL * a.token_stride);
-      }
+      for (int h = 0; h < LOADS / P; ++h) page[h] = s_pages[place_of(tb + c * STEP + h * P * TPL)];
+      find(c, loads_per_page, [&](int h) { return __builtin_amdgcn_readfirstlane(page[h]); });
     };
     if (a.page_shift >= 4)   // uniform
-      find(std::integral_constant<int, 16 / TPL>{});
+      look(Granule16{});
     else
-      find(std::integral_constant<int, 1>{});
+      look(Granule1{});
+  };
+  // From the lanes of a register: lane h has id(h).
+  auto ids_of = [&](int c) { return seq_pages[pb + place_of(tb + c * STEP + lane * granule)]; };
+  auto find_ids = [&](int c, int ids) {
+    auto id = [&](int h) {
+      const int p = __builtin_amdgcn_readlane(ids, h);
+      return p < a.num_pages ? p : -1;
+    };
+    if (a.page_shift >= 4)
+      find(c, Granule16{}, id);
+    else
+      find(c, Granule1{}, id);
   };
 
   V8 k[LOADS], v[LOADS];
@@ -340,14 +368,8 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
     for (int i = 0; i < LOADS; ++i)
       if (dropped >> i & 1) v[i] = V8{};
   };
-  auto load = [&](int c) {
-    if (scalar) {
-      if (c >= nsteps) return;
-      find_step(c);
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) load_rows(i);
-      return;
-    }
+  NewRow nr{-1, 0, 0};
+  auto load_lanes = [&](int c) {   // each lane's row looked up in LDS
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int t = tb + c * STEP + TPL * i + lrow;
@@ -373,7 +395,8 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
 
   if constexpr (WIDE) {
     static_assert(PAIRS == 1 && L::ACCS == 1 && kWideTiles == 2 && 2 * KS == 8);
-    if (cols > 16) {   // uniform
+    if (wide) {
+      const bool any_bad = stage_pages();
       // Every wave has tiles of its own; a round of the loop is a step of each
       // wave's tokens, which all waves take from LDS.
       const int c0 = wave_s * kWideTiles * 16;
@@ -517,7 +540,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
         auto partial = [&](int c) {
-          return int64_t(columns.pairs[2 * (c / a.group) + 1] + place) * a.num_qo_heads +
+          return int64_t(columns.pairs[2 * columns.pair(c) + 1] + place) * a.num_qo_heads +
                  columns.head(c);
         };
         if (not_finite<D>(o[ct])) {
@@ -551,26 +574,82 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
     }
   }
 
-  if constexpr (WIDE) __builtin_amdgcn_s_setprio(3);
+  // What stands between a workgroup's start and its first K and V is all that
+  // short tails wait for (2 us for each read that depends on another, while others
+  // stream): the first steps' page ids come with the plan, later ones into a register,
+  // a step ahead; q and the new row behind K and V; no barrier.
+  bool any_bad = false;
+  int ids = 0, ids_next = 0;   // lane h: the step's id(h)
+  constexpr bool kIds = D != 256;   // there the registers are short, and q waits at a barrier
+  if (!scalar || !kIds) {
+    any_bad = stage_pages();
+  } else if (wave_s < nsteps) {
+    ids = tail ? sa.first_ids[(item * W + wave_s) * sa.step_ids + min(lane, sa.step_ids - 1)]
+               : ids_of(wave_s);
+    ids_next = ids_of(wave_s + W);
+  }
+  int token;
+  if (tail) {   // uniform
+    token = a.q_token ? a.q_token[columns.seq] : columns.seq;
+    nr = new_row(a, columns.seq, token, hkv);
+  } else {
+    token = columns.token(a, min(j, cols - 1));
+  }
+  const bool has_new = nr.pos >= tb && nr.pos < te;   // uniform; then te - 1
+  if (scalar && wave_s < nsteps) {
+    if constexpr (kIds)
+      find_ids(wave_s, ids);
+    else
+      find_step(wave_s);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load_rows(i);
+  }
   V8 qb[kQInLds ? 1 : KS];
-  if constexpr (!kQInLds) {
-    const f16* qp = columns.q(a, min(j, cols - 1)) + 8 * tg;
+  if constexpr (kQInLds) {
+    for (int i = tid; i < 16 * L::CH; i += W * kWave) {
+      const int g = i / L::CH, c = i % L::CH;
+      *reinterpret_cast<V8*>(&s_q[g * D + 8 * (c ^ (g & 7))]) =
+          g < cols ? load_v8<T>(columns.q(a, g) + 8 * c) : V8{};
+    }
+    __syncthreads();
+  } else {
+    const f16* qp = a.q + int64_t(token) * a.q_tok +
+                    int64_t(columns.head(min(j, cols - 1))) * a.q_head + 8 * tg;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qb[s] = j < cols ? load_v8<T>(qp + 32 * s) : V8{};
   }
+  // The new row: to LDS and into its page by the wave that has the last step; lane
+  // c chunk c, K's first.
+  if (scalar && has_new && wave_s == (nsteps - 1) % W && lane < 2 * L::CH) {
+    const bool of_v = lane >= L::CH;
+    f16* base = const_cast<f16*>(of_v ? a.v : a.k) + int64_t(hkv) * a.head_stride + 8 * lcol;
+    const V8 row = load_v8<T>(base + (of_v ? nr.v : nr.k));
+    *reinterpret_cast<V8*>(&s_new[8 * lane]) = row;
+    const int p = page_id(np - 1);
+    if (p >= 0 && hq0 % a.ratio == 0)
+      *reinterpret_cast<V8*>(base + int64_t(p) * a.page_stride +
+                             int64_t(nr.pos & page_mask) * a.token_stride) = row;
+  }
+  __builtin_amdgcn_wave_barrier();
   f32x4 o[L::ACCS][8];
 #pragma unroll
   for (int x = 0; x < L::ACCS; ++x)
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[x][e] = f32x4{};
   float m = kNegBig, lsum = 0.f;
-  if (wave_s < nsteps) load(wave_s);
+  if (!scalar) {
+    if (has_new && hq0 % a.ratio == 0)
+      append_row<D>(a, nr, s_pages[(nr.pos >> a.page_shift) - pb], hkv);
+    if (wave_s < nsteps) load_lanes(wave_s);
+  }
   for (int c = wave_s; c < nsteps; c += W) {
+    const int t0 = tb + c * STEP;
+    const int gone = dropped;   // of this step
     if (scalar) {
-      if (tb + c * STEP + STEP >= te) {   // uniform: rows past the end, and the new one
+      if (t0 + STEP >= te) {   // uniform, the last step: rows past the end, and the new one
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-          const int t = tb + c * STEP + TPL * i + lrow;
+          const int t = t0 + TPL * i + lrow;
           if (t >= te) v[i] = V8{};
           if (has_new && t == nr.pos) {
             k[i] = *reinterpret_cast<const V8*>(&s_new[8 * lcol]);
@@ -578,12 +657,24 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
           }
         }
       }
-      if (dropped) drop_rows();   // uniform
+      if (gone) drop_rows();   // uniform
     }
     park();
     V8 vt[8];
     transpose8(v, vt);
-    load(c + W);
+    if (!scalar) {
+      load_lanes(c + W);
+    } else if (c + W < nsteps) {
+      if constexpr (kIds) {
+        ids = ids_next;
+        ids_next = ids_of(c + 2 * W);
+        find_ids(c + W, ids);
+      } else {
+        find_step(c + W);
+      }
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) load_rows(i);
+    }
     // LDS runs a wave's accesses in order; keep the compiler from moving them.
     f32x4 sc[PAIRS][2];
     __builtin_amdgcn_wave_barrier();
@@ -604,9 +695,12 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
         }
       }
     __builtin_amdgcn_wave_barrier();
-    const int t0 = tb + c * STEP;
-    if (any_bad || t0 + STEP > te)   // uniform
-      mask_scores<D>(sc, t0, te, tg, any_bad, s_pages, a.page_shift, pb);
+    if (any_bad || (scalar && gone) || t0 + STEP > te) {   // uniform
+      if (scalar)
+        mask_loads<D>(sc, t0, te, tg, gone);
+      else
+        mask_scores<D>(sc, t0, te, tg, any_bad, s_pages, a.page_shift, pb);
+    }
     V8 ph[L::ACCS], pl[L::ACCS];
     tile_max<D>(sc, a.scale_log2, m, lsum, o);
     tile_exp<T, D>(sc, a.scale_log2, m, lsum, ph, pl);
@@ -640,6 +734,8 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
   float* s_o = reinterpret_cast<float*>(s_raw);
   auto unit_at = [&](int g, int unit) { return &s_o[(wave * 16 + g) * D + 4 * (unit ^ (g & 7))]; };
   if (again) {
+    if (scalar)   // every wave that comes here the same
+      for (int i = lane; i < np; i += kWave) s_pages[i] = page_id(i);
 #pragma unroll 1
     for (int g = 0; g < cols; ++g) {
       float m1, l1, acc[8];
@@ -698,7 +794,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
       for (int i = 0; i < 4; ++i) op[i] = T(x[i]);
       continue;
     }
-    const int64_t row = int64_t(tail ? slot : columns.pairs[2 * (g / a.group) + 1] + place) *
+    const int64_t row = int64_t(tail ? slot : columns.pairs[2 * columns.pair(g) + 1] + place) *
                             a.num_qo_heads + columns.head(g);
     *reinterpret_cast<f32x4*>(a.part_o + row * D + 4 * unit) = x;
     if (unit == 0) a.part_lse[row] = partial_lse(mxw, sum);
@@ -726,6 +822,20 @@ int launch_shared_dim(int head_dim, const SharedArgs& a, bool wide, unsigned blo
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Page ids that a step of a wave's tokens needs (shared_decode_kernel's `granule`); none
+// where the kernel looks each row up.
+struct StepIds {
+  int32_t step, granule, count;
+};
+StepIds step_ids(int head_dim, int page_size) {
+  const int32_t step = head_dim == 64 ? DecodeTile<64>::STEP
+                       : head_dim == 128 ? DecodeTile<128>::STEP : DecodeTile<256>::STEP;
+  const int32_t load = step / DecodeTile<64>::LOADS;
+  if (page_size < load) return {step, 1, 0};
+  const int32_t granule = page_size >= 16 ? 16 : load;
+  return {step, granule, step / granule};
+}
 
 // Tokens [begin, end) that rows order[lo, hi) hold in the same pages.
 struct Segment {
@@ -904,7 +1014,7 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
       for (int32_t r = s.lo; r < s.hi; r += tile_rows(s)) {
         lanes[x].insert(lanes[x].end(),
                         {std::min(tile_rows(s), s.hi - r), pair_at[p.segment] + r - s.lo, p.begin,
-                         p.end, p.place, order[s.lo], hg, 0});
+                         p.end, p.place, order[s.lo], hg, indptr[order[s.lo]]});
         load[x] += p.end - p.begin;
       }
       depth = std::max(depth, lanes[x].size() / kRecord);
@@ -915,6 +1025,17 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
       for (int i = 0; i < kRecord; ++i)
         plan.push_back(kRecord * r + i < lanes[x].size() ? lanes[x][kRecord * r + i] : 0);
   plan.insert(plan.end(), pairs.begin(), pairs.end());
+  for (int32_t i = 0; i < info->decode.num_work; ++i)
+    plan.push_back(plan[4 * i] < 0 ? 0 : indptr[plan[4 * i]]);
+  const StepIds ids = step_ids(head_dim, page_size);
+  for (int32_t i = 0; i < info->decode.num_work; ++i)
+    for (int32_t x = 0; x < kWaves * ids.count; ++x) {
+      const int32_t b = plan[4 * i];
+      const int32_t t = plan[4 * i + 1] + x / ids.count * ids.step + x % ids.count * ids.granule;
+      plan.push_back(b < 0 || kv_len[b] == 0
+                         ? -1
+                         : pages[b][std::min(t, plan[4 * i + 2] - 1) / page_size]);
+    }
   info->num_shared = int32_t(kXcds * depth);
   info->num_pairs = int32_t(pairs.size() / 2);
   info->num_segments = int32_t(segments.size());
@@ -938,7 +1059,7 @@ extern "C" int64_t kunserve_shared_plan_bound(const int32_t* kv_len_host, int32_
   int64_t partials = 0;
   for (int32_t b = 0; b < num_seqs; ++b)
     partials += 2 * ceil_div(std::max(kv_len_host[b], 0), kMinSegmentTokens) + 2;
-  return (4 * kXcds + kRecord * kXcds * int64_t(num_qo_heads) + 2) * partials +
+  return ((5 + 8 * kWaves) * kXcds + kRecord * kXcds * int64_t(num_qo_heads) + 2) * partials +
          4 * int64_t(num_seqs);
 }
 
@@ -1013,11 +1134,16 @@ int kunserve::shared_decode(const kunserve_kv_pool* pool, int32_t layer,
   KSV_CHECK_ARG(aligned16(workspace_dev), "workspace must be 16-byte aligned");
   sa.shared = plan_dev + info->decode.plan_ints;
   sa.pairs = sa.shared + kRecord * int64_t(info->num_shared);
+  sa.tail_pages = sa.pairs + 2 * int64_t(info->num_pairs);
+  sa.first_ids = sa.tail_pages + info->decode.num_work;
+  sa.step_ids = step_ids(pool->head_dim, pool->page_size).count;
   sa.num_shared = info->num_shared;
+  sa.inv_group = (65536u + sa.d.group - 1) / sa.d.group;
+  sa.inv_head_groups = uint32_t((int64_t(1) << 32) / sa.d.head_groups + 1);
   const int64_t blocks = int64_t(info->num_shared) +
                          8 * ceil_div(info->decode.num_work, 8) * sa.d.head_groups;
-  KSV_CHECK_ARG(blocks < (int64_t(1) << 31), "grid of %lld workgroups is too large",
-                (long long)blocks);
+  KSV_CHECK_ARG(blocks < (int64_t(1) << 31) && blocks / 8 * sa.d.head_groups < (int64_t(1) << 32),
+                "grid of %lld workgroups is too large", (long long)blocks);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   rc = pool->dtype == KUNSERVE_DTYPE_BF16
            ? launch_shared_dim<bf16>(pool->head_dim, sa, info->wide != 0, unsigned(blocks), s)

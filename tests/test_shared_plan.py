@@ -33,8 +33,20 @@ def check(tables, kv, hq, hkv, ps, d, cus=256):
     work = plan[:4 * dec.num_work].reshape(-1, 4)
     merges = plan[4 * dec.num_work:dec.plan_ints].reshape(-1, 4)
     shared = plan[dec.plan_ints:dec.plan_ints + 8 * info.num_shared].reshape(-1, 8)
-    pairs = plan[dec.plan_ints + 8 * info.num_shared:].reshape(-1, 2)
-    assert len(pairs) == info.num_pairs
+    at = dec.plan_ints + 8 * info.num_shared
+    pairs = plan[at:at + 2 * info.num_pairs].reshape(-1, 2)
+    starts = np.r_[0, np.cumsum([len(t) for t in tables])]
+    at += 2 * info.num_pairs
+    np.testing.assert_array_equal(plan[at:at + dec.num_work],
+                                  np.where(work[:, 0] < 0, 0, starts[work[:, 0]]))
+    # the pages of four waves' first steps (4096 elements each), a granule at a time
+    step, load = 4096 // d, 512 // d
+    granule = 16 if ps >= 16 else load
+    ids = plan[at + dec.num_work:].reshape(dec.num_work, 0 if ps < load else 4 * step // granule)
+    for (b, lo, hi, _), got_ids in zip(work.tolist(), ids.tolist()):
+        if b >= 0 and kv[b]:
+            assert got_ids == [tables[b][min(lo + i * granule, hi - 1) // ps]
+                               for i in range(len(got_ids))]
     assert dec.num_work % 8 == 0 and info.num_shared % 8 == 0
     first = {int(b): (int(s0), int(m)) for b, s0, m, _ in merges}
     # (row, head group) -> [(begin, end, slot)]
@@ -43,13 +55,13 @@ def check(tables, kv, hq, hkv, ps, d, cus=256):
         assert hi - lo <= dec.part_tokens
         for h in range(heads):
             got[b, h].append((lo, hi, slot))
-    for nrows, at, lo, hi, place, rep, h, _ in shared[shared[:, 0] > 0].tolist():
+    for nrows, at, lo, hi, place, rep, h, pages_at in shared[shared[:, 0] > 0].tolist():
         cols = nrows * group
         wide = info.wide and d == 128
         assert 0 < cols <= (128 if wide else 16) and 0 <= h < heads and lo < hi
         assert lo % 4 == 0 and hi - lo <= 4096
         rows = pairs[at:at + nrows]
-        assert rep in pairs[:, 0]
+        assert rep in pairs[:, 0] and pages_at == starts[rep]
         want = tables[rep][lo // ps:-(-hi // ps)]
         for b, s0 in rows.tolist():
             assert tables[b][lo // ps:-(-hi // ps)] == want

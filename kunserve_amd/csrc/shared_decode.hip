@@ -35,7 +35,9 @@ constexpr int kMinSegmentTokens = 64;   // shorter runs of shared pages stay wit
 constexpr int64_t kMinSavedBytes = 13 << 20;
 constexpr int kRecord = 8;              // ints of a work record
 constexpr int kMinPieceTokens = 128;
-constexpr int kMinWideCols = 64;        // columns from which a segment's workgroups are wide
+// Columns, and us of the segments' work for each CU, from which workgroups are wide.
+constexpr int kMinWideCols = 64;
+constexpr double kMinWideShareUs = 20.0;
 
 struct SharedArgs {
   DecodeArgs d;            // work: the tails'
@@ -909,39 +911,46 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
   if (saved * num_kv_heads * head_dim * 4 < (min_bytes < 0 ? kMinSavedBytes * cus / 256 : min_bytes))
     segments.clear();
 
-  // Segments in workgroups of whole rows (group is 16 at most), wide ones where
-  // their columns are worth it; pieces of their tokens so that the device is
-  // filled.
-  auto is_wide = [&](const Segment& s) {
-    return head_dim == 128 && (s.hi - s.lo) * group >= kMinWideCols;
-  };
-  auto tile_rows = [&](const Segment& s) { return (is_wide(s) ? kWideCols : 16) / group; };
-  // us of a workgroup per token of its piece, and of the launch for the tails'
-  // bytes. A piece takes at most a CU's share of the segments' work (or 1.6 of it,
-  // for narrow ones, which run two and more to a CU), or what ends behind the
-  // tails: fewer pieces are fewer partials. 64 rows behind 2048 tokens, 32 heads on
-  // 8: 51.5 us in pieces of 512, 60 in pieces of 128; 128 rows behind 8192, 64 on 8:
-  // 112 in pieces of 2048, 125 in 1152, 154 in 4096.
-  auto token_us = [&](const Segment& s) {
-    return is_wide(s) ? 0.035 : 0.0115 * std::pow(head_dim / 128.0, 1.4);
-  };
-  double work = 0.0;   // of all segments' workgroups
+  // Segments in workgroups of whole rows (group is 16 at most). Wide ones where
+  // narrow ones would keep the CUs busy for long: they read K and V once for
+  // eight times as many columns, but take about 10 us to begin and end, and their
+  // number is an eighth. Per layer, 8 KV heads of 128, narrow against wide: 64 columns
+  // of 4000 tokens (a CU's share 6 us) 15.7 against 21, 160 of 3000 (11 us) 20 against
+  // 24, 320 of 3000 (22 us) 27.6 against 27, 256 of 8000 (46 us) 40 against 32.
+  double narrow_work = 0.0;
+  const double narrow_us = 0.0115 * std::pow(head_dim / 128.0, 1.4);   // a token, of a workgroup
   int64_t tail_tokens = 0;
   for (int32_t b = 0; b < num_seqs; ++b) tail_tokens += kv_len[b];
+  for (const Segment& s : segments) {
+    narrow_work += narrow_us * double(s.end - s.begin) *
+                   double(ceil_div(s.hi - s.lo, 16 / group) * head_groups);
+    tail_tokens -= int64_t(s.end - s.begin) * (s.hi - s.lo);
+  }
+  auto is_wide = [&](const Segment& s) {
+    return head_dim == 128 && (s.hi - s.lo) * group >= kMinWideCols &&
+           narrow_work >= kMinWideShareUs * double(cus);
+  };
+  auto tile_rows = [&](const Segment& s) { return (is_wide(s) ? kWideCols : 16) / group; };
+  auto token_us = [&](const Segment& s) { return is_wide(s) ? 0.035 : narrow_us; };
+  double work = 0.0;   // of all segments' workgroups
   info->wide = 0;
   for (const Segment& s : segments) {
     work += token_us(s) * double(s.end - s.begin) *
             double(ceil_div(s.hi - s.lo, tile_rows(s)) * head_groups);
-    tail_tokens -= int64_t(s.end - s.begin) * (s.hi - s.lo);
     info->wide |= is_wide(s);
   }
+  // A piece takes at most a CU's share of the segments' work (of a long one of narrow
+  // workgroups, which run two to a CU, 0.7 at head_dim 128: 24 rows behind 6000 tokens,
+  // 32 heads on 8, 21.2 us against 21.8 and, at 1.6, 24.4), or what ends behind the
+  // tails' bytes: fewer pieces are fewer partials. Wide, 128 rows behind 8192 tokens, 64 heads on 8: 102 us
+  // in pieces of 2048, 110 in 1600, 125 in 1024.
   const double tails_us = double(tail_tokens) * num_kv_heads * head_dim * 4 / (6.6e6 * cus / 256);
   const double share_us = work / double(cus);
   auto pieces_of = [&](const Segment& s) {
+    const double share = (is_wide(s) || head_dim != 128 || share_us < 12.0 ? 1.0 : 0.7) * share_us;
     const double most = std::min(double(kMaxPartTokens),
                                  std::max(double(kMinPieceTokens),
-                                          std::max((is_wide(s) ? 1.0 : 1.6) * share_us,
-                                                   0.8 * tails_us) / token_us(s)));
+                                          std::max(share, 0.8 * tails_us) / token_us(s)));
     return int64_t(std::ceil(double(s.end - s.begin) / most));
   };
 

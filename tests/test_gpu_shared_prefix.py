@@ -8,7 +8,7 @@ import torch
 
 import operators_ref as ref
 from helpers import random_pool, random_tensor
-from kunserve_amd import AttentionStep, PageTable, SharedDecodePlan, shared_decode
+from kunserve_amd import AttentionStep, PageTable, SharedDecodePlan, paged_kv, shared_decode
 
 pytestmark = pytest.mark.gpu
 
@@ -92,6 +92,32 @@ def test_numbers_of_rows(device, rows, d):
     root = [("r", 20)]
     specs = [(root, 320 + 1 + (7 * i) % 40) for i in range(rows)]
     step, *rest = run(device, specs, 8, 2, 16, d, torch.bfloat16, seed=rows)
+    assert step.decode.plan.num_segments == 1
+    check(*rest, step=step)
+
+
+@pytest.mark.parametrize("rows", [16, 17, 33, 70, 150])
+@pytest.mark.parametrize("ps,pages", [(4, 80), (8, 37), (16, 20), (64, 5), (256, 2)])
+def test_wide_workgroups(device, monkeypatch, rows, ps, pages):
+    """Planned for one CU, so that segments of 64 columns and more are work enough for
+    workgroups of 128."""
+    monkeypatch.setattr(paged_kv, "_num_cus", lambda device: 1)
+    root = [("r", pages)]
+    specs = [(root, pages * ps + 1 + (7 * i) % 40) for i in range(rows)]
+    step, *rest = run(device, specs, 8, 2, ps, 128, [torch.float16, torch.bfloat16][rows % 2],
+                      seed=rows + ps)
+    assert step.decode.plan.num_segments == 1 and step.decode.plan.shared_info.wide == 1
+    check(*rest, step=step)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("ps", [4, 8, 32])
+def test_other_pages(device, ps, d):
+    """Pages smaller than what a wave loads at a time, tails that end inside one, at
+    one, one token behind it, and longer than the waves' first steps."""
+    root = [("r", 96 // ps)]
+    specs = [(root, 96 + m) for m in (1, ps - 1, ps, ps + 1, 31, 64, 65, 255, 257, 600)]
+    step, *rest = run(device, specs, 4, 2, ps, d, torch.float16, seed=ps + d)
     assert step.decode.plan.num_segments == 1
     check(*rest, step=step)
 
@@ -185,6 +211,19 @@ def test_infinite_values_at_other_head_sizes(device, d):
     assert (out[bad] == -float("inf")).all() and torch.isfinite(out[~bad]).all()
 
 
+def test_infinite_values_in_wide_workgroups(device, monkeypatch):
+    monkeypatch.setattr(paged_kv, "_num_cus", lambda device: 1)
+
+    def poke(pool, tables):
+        pool.v[tables[0][2], 1, 0, 5, 40] = float("inf")
+    specs = [([("r", 20)], 330 + i) for i in range(21)]
+    step, _, _, _, _, out = run(device, specs, 8, 2, 16, 128, torch.bfloat16, poke=poke)
+    assert step.decode.plan.shared_info.wide == 1
+    bad = torch.zeros((21, 8, 128), dtype=torch.bool, device=device)
+    bad[:, :4, 40] = True
+    assert (out[bad] == float("inf")).all() and torch.isfinite(out[~bad]).all()
+
+
 def test_page_ids_outside_the_pool_drop_out(device):
     """Through the op itself, with a table the shim did not check: a shared id
     outside the pool drops its tokens for every row."""
@@ -208,6 +247,44 @@ def test_page_ids_outside_the_pool_drop_out(device):
         valid[48:64] = False
         want, tol, _, _ = ref.attend(qh[b:b + 1], k, v, 1 / math.sqrt(128), pool.dtype, valid=valid)
         assert np.all(np.abs(out[b].cpu().double().numpy() - want[0]) <= tol[0])
+
+
+@pytest.mark.parametrize("d,ps,cus", [(64, 4, 256), (64, 8, 256), (128, 4, 256), (128, 16, 1),
+                                      (128, 8, 1), (256, 16, 256), (256, 4, 256)])
+def test_page_ids_outside_the_pool_in_segments_and_tails(device, d, ps, cus):
+    """Bad ids in the shared pages and in each row's own, in first and later steps, NaN
+    in page 0, which is read in their place: 18 rows, narrow workgroups and wide ones."""
+    rng = np.random.default_rng(13)
+    kvs = [480 + 37 * i for i in range(18)]
+    tables, pages = tree(rng, ps, [([("r", 400 // ps)], n) for n in kvs])
+    pool = random_pool(pages + 1, 1, 2, ps, d, device, 13)
+    tables = [[p + 1 for p in t] for t in tables]
+    pool.k[0] = float("nan")
+    pool.v[0] = float("nan")
+    bad = [list(t) for t in tables]
+    drops = [[] for _ in kvs]
+    for b, t in enumerate(bad):
+        for at in (16 // ps, 200 // ps, 400 // ps + b % 3, (kvs[b] - 1) // ps - 1):
+            t[at] = [pages + 7, -1][at < 400 // ps and at > 20]
+            drops[b].append(at)
+    shared = bad[0][:400 // ps]
+    assert all(t[:400 // ps] == shared for t in bad)
+    indptr = np.r_[0, np.cumsum([len(t) for t in bad])]
+    table = PageTable(indptr, np.concatenate(bad), kvs, device)
+    plan = SharedDecodePlan(table, 8, 2, ps, device, head_dim=d, min_bytes=0, num_cus=cus)
+    assert plan.num_segments == 1 and plan.shared_info.wide == (cus == 1)
+    q = random_tensor((len(kvs), 8, d), device, 14, 2.0)
+    out = shared_decode(pool, 0, table, q, plan)
+    p_err = ref.half_step(pool.dtype) if cus == 1 else None
+    kh, vh, qh = pool.k.cpu(), pool.v.cpu(), q.cpu().double().numpy()
+    for b in range(len(kvs)):
+        k, v = (ref.row_cache(x, 0, tables[b], kvs[b]) for x in (kh, vh))
+        valid = np.ones(kvs[b], dtype=bool)
+        for at in drops[b]:
+            valid[at * ps:(at + 1) * ps] = False
+        want, tol, _, _ = ref.attend(qh[b:b + 1], k, v, 1 / math.sqrt(d), pool.dtype, p_err,
+                                     valid=valid)
+        assert np.all(np.abs(out[b].cpu().double().numpy() - want[0]) <= tol[0]), b
 
 
 def test_rows_of_no_and_of_one_token(device):

@@ -143,9 +143,13 @@ def test_segments_follow_the_tree():
 def test_wide_workgroups_take_many_columns():
     t = rows(20, [1] * 40)
     kv = [len(x) * 16 - 5 for x in t]
-    assert check(t, kv, 8, 2, 16, 128).wide == 1
-    assert check(t, kv, 8, 2, 16, 64).wide == 0
-    assert check(t[:15], kv[:15], 8, 2, 16, 128).wide == 0    # 60 columns
+    assert check(t, kv, 8, 2, 16, 128, cus=1).wide == 1
+    assert check(t, kv, 8, 2, 16, 64, cus=1).wide == 0
+    assert check(t[:15], kv[:15], 8, 2, 16, 128, cus=1).wide == 0    # 60 columns
+    # narrow ones would have 0.0115 us a token, 320 tokens, 10 tiles of columns and 2 KV
+    # heads of work: 73.6 us, 20 for each CU up to 3
+    assert check(t, kv, 8, 2, 16, 128, cus=3).wide == 1
+    assert check(t, kv, 8, 2, 16, 128, cus=4).wide == 0
 
 
 def test_sharing_has_to_pay():

@@ -372,8 +372,9 @@ int kunserve_shared_plan(const int32_t* indptr_host, const int32_t* indices_host
                          int64_t plan_capacity, kunserve_shared_plan_info* info);
 
 /* kunserve_paged_decode on such a plan, for the table it was made from (other
- * ids or lengths: not this plan). The workspace is 16-byte aligned and holds
- * kunserve_decode_workspace_bytes of info->decode. */
+ * ids or lengths: not this plan) and a pool of its page size and head_dim whose
+ * tokens are less than 2^28 elements apart. The workspace is 16-byte aligned and
+ * holds kunserve_decode_workspace_bytes of info->decode. */
 int kunserve_shared_decode(const kunserve_kv_pool* pool, int32_t layer,
                            const kunserve_page_table* table,
                            const int32_t* q_token_dev,

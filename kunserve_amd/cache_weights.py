@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from .paged_kv import (KVPool, PageTable, _i32, _ptr, _stream_ptr, _tensor3,
-                       _upload_packed, csr_from_lists)
+                       _upload, _upload_packed, csr_from_lists)
 
 
 class KVWeights:
@@ -155,19 +155,18 @@ def evict(pool: KVPool, weights: KVWeights, pages_of_reqs: Sequence[Sequence[int
     n = len(kv_lens)
     if len(pages_of_reqs) != n or len(pages_out) != n:
         raise ValueError(f"{n} kv lengths but {len(pages_of_reqs)} and {len(pages_out)} page lists")
-    lens = np.empty(2 * n, dtype=np.int64)   # of the requests, then what stays of them
-    kv, keep = lens[:n], lens[n:]
-    kv[:] = kv_lens
+    kv = [int(x) for x in kv_lens]
     budget = np.asarray(budget) if n else np.zeros((), dtype=np.int64)
     if budget.dtype.kind not in "iu":
         raise ValueError("budget counts tokens: whole numbers")
     if budget.shape not in ((), (n,)):
         raise ValueError(f"budget must be one number or one per request ({n})")
-    np.minimum(budget, kv, out=keep)
+    budgets = budget.tolist() if budget.shape else [int(budget)] * n
+    keep = list(map(min, budgets, kv))   # what stays of the requests
     # a negative length or budget is the least of a request's
-    if sinks < 0 or recent < 0 or (n and keep.min() < 0):
+    if sinks < 0 or recent < 0 or min(keep, default=0) < 0:
         raise ValueError("budget, kv_lens, sinks and recent must not be negative")
-    longest, most = (int(kv.max()), int(keep.max())) if n else (0, 0)
+    longest, most = max(kv, default=0), max(keep, default=0)
     limit = 2**31 - 1   # tokens of a request are counted in int32
     if longest > limit:
         raise ValueError(f"a request of over {limit} tokens")
@@ -176,6 +175,7 @@ def evict(pool: KVPool, weights: KVWeights, pages_of_reqs: Sequence[Sequence[int
     if most == 0:
         return kept
     # one table: the requests' pages, then those that are filled
+    lens = np.array(kv + keep, dtype=np.int64)
     indptr, indices = csr_from_lists([*pages_of_reqs, *pages_out], lens, pool.page_size,
                                      pool.num_pages)
     out = indices[indptr[n]:]
@@ -187,10 +187,14 @@ def evict(pool: KVPool, weights: KVWeights, pages_of_reqs: Sequence[Sequence[int
     use[out] = 2
     if np.count_nonzero(use == 2) != out.size:
         raise ValueError("a page is twice in pages_out")
-    at, lengths, ids = _upload_packed([indptr, lens, indices], pool.device)
-    table = _lib.PageTable(at.data_ptr(), ids.data_ptr(), lengths.data_ptr(), n)
+    tables = _upload(np.concatenate((indptr, lens, indices), dtype=np.int32, casting="unsafe"),
+                     pool.device)
+    at = tables.data_ptr()
+    lengths = at + 4 * (2 * n + 1)
+    ids = lengths + 4 * 2 * n
+    table = _lib.PageTable(at, ids, lengths, n)
     _lib.call("kunserve_evict", pool.desc(), ctypes.byref(weights._desc), ctypes.byref(table),
-              at.data_ptr() + 4 * n, ids.data_ptr(), lengths.data_ptr() + 4 * n, most, longest,
+              at + 4 * n, ids, lengths + 4 * n, most, longest,
               min(sinks, limit), min(recent, limit), kept.data_ptr(), most,
               _stream_ptr(pool.device))
     return kept

@@ -459,7 +459,9 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
           // second, then P V of the first), and V and the next K are read into
           // the registers that the products are done with. Probabilities in one
           // 16-bit term: at 64 columns and more the matrix units' work counts.
-          // Steps past the piece are masked ones.
+          // Steps past the piece are masked ones. 128 rows behind 8192 tokens, 64
+          // heads on 8: 65 us a layer without tails against 78 with one operation after
+          // the other, whose products alone are 33 at the rate of a large matrix product.
           V8 ka[2][KS], ve[8];
           auto read_k = [&](int blk, int i) {
             ka[i & 1][i >> 1] = *reinterpret_cast<const V8*>(
@@ -579,7 +581,8 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
   // What stands between a workgroup's start and its first K and V is all that
   // short tails wait for (2 us for each read that depends on another, while others
   // stream): the first steps' page ids come with the plan, later ones into a register,
-  // a step ahead; q and the new row behind K and V; no barrier.
+  // a step ahead; q and the new row behind K and V; no barrier. 64 rows behind 2048
+  // tokens with tails of 16 to 1500, 32 heads on 8: 47.5 us a layer against 50.
   bool any_bad = false;
   int ids = 0, ids_next = 0;   // lane h: the step's id(h)
   constexpr bool kIds = D != 256;   // there the registers are short, and q waits at a barrier

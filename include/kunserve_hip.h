@@ -351,6 +351,9 @@ typedef struct {
   int32_t head_dim;      /* head_dim and page_size the plan was made for      */
   int32_t page_size;
   int32_t plan_ints;     /* int32 entries of the plan buffer in use           */
+  int32_t num_seqs;      /* rows and heads the plan was made for              */
+  int32_t num_qo_heads;
+  int32_t num_kv_heads;
 } kunserve_shared_plan_info;
 
 /* Upper bound of the plan buffer length (int32 entries) for these lengths. */
@@ -372,8 +375,8 @@ int kunserve_shared_plan(const int32_t* indptr_host, const int32_t* indices_host
                          int64_t plan_capacity, kunserve_shared_plan_info* info);
 
 /* kunserve_paged_decode on such a plan, for the table it was made from (other
- * ids or lengths: not this plan) and a pool of its page size and head_dim whose
- * tokens are less than 2^28 elements apart. The workspace is 16-byte aligned and
+ * ids or lengths: not this plan), its head counts, and a pool of its page size and
+ * head_dim whose tokens are less than 2^28 elements apart. The workspace is 16-byte aligned and
  * holds kunserve_decode_workspace_bytes of info->decode. */
 int kunserve_shared_decode(const kunserve_kv_pool* pool, int32_t layer,
                            const kunserve_page_table* table,

@@ -79,7 +79,8 @@ class Step(Structure):
 class SharedPlanInfo(Structure):
     _fields_ = [("decode", DecodePlanInfo), ("num_shared", c_int32), ("wide", c_int32),
                 ("num_pairs", c_int32), ("num_segments", c_int32),
-                ("head_dim", c_int32), ("page_size", c_int32), ("plan_ints", c_int32)]
+                ("head_dim", c_int32), ("page_size", c_int32), ("plan_ints", c_int32),
+                ("num_seqs", c_int32), ("num_qo_heads", c_int32), ("num_kv_heads", c_int32)]
 
 
 class KVWeights(Structure):

@@ -1053,6 +1053,9 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
   info->num_segments = int32_t(segments.size());
   info->head_dim = head_dim;
   info->page_size = page_size;
+  info->num_seqs = num_seqs;
+  info->num_qo_heads = num_qo_heads;
+  info->num_kv_heads = num_kv_heads;
   KSV_CHECK_ARG(plan.size() < (size_t(1) << 31), "the plan is too long");
   info->plan_ints = int32_t(plan.size());
   return KUNSERVE_OK;
@@ -1135,6 +1138,12 @@ int kunserve::shared_decode(const kunserve_kv_pool* pool, int32_t layer,
   KSV_CHECK_ARG(info->decode.group_size == decode_group(num_qo_heads, pool->num_kv_heads),
                 "plan group size %d is not that of %d query heads on %d", info->decode.group_size,
                 num_qo_heads, pool->num_kv_heads);
+  // The segments' records hold rows and head groups.
+  KSV_CHECK_ARG(info->num_qo_heads == num_qo_heads && info->num_kv_heads == pool->num_kv_heads,
+                "plan made for %d query heads on %d, not %d on %d", info->num_qo_heads,
+                info->num_kv_heads, num_qo_heads, pool->num_kv_heads);
+  KSV_CHECK_ARG(info->num_seqs == table->num_seqs, "plan made for %d rows, not %d", info->num_seqs,
+                table->num_seqs);
   // Rows that share nothing run in the decode kernels.
   if (info->num_segments == 0)
     return paged_decode(pool, layer, table, q_token_dev, q, out, num_qo_heads, sm_scale, plan_dev,

@@ -503,7 +503,9 @@ int64_t kunserve_weights_plan_bound(const int32_t* q_indptr_host,
                                     const int32_t* kv_len_host, int32_t num_seqs,
                                     int32_t num_qo_heads, int32_t window);
 
-/* Host-side plan of a step's attention weights, shared by its layers. Rows with a
+/* Host-side plan of a step's attention weights, shared by its layers, for the
+ * launches of these rows alone: their q_indptr_dev and kv_len_dev are copies of
+ * q_indptr and kv_len as given here (the workspace is laid out by them). Rows with a
  * non-zero decodes_host[b] (NULL: none; they have one new token) are the decode
  * rows of kunserve_attention_step_with, whose decode launch leaves its scores
  * for the weights; the others are kunserve_cache_weights'. */

@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .paged_kv import (KVPool, PageTable, _i32, _ptr, _stream_ptr, _tensor3,
+from .paged_kv import (KVPool, PageTable, _check_row_map, _i32, _ptr, _stream_ptr, _tensor3,
                        _upload, _upload_packed, csr_from_lists)
 
 
@@ -68,7 +68,8 @@ class WeightsPlan:
     """Work of add_weights for a step's rows, computed on the host once per step and
     shared by every layer (kunserve_weights_plan). decodes marks the rows whose
     decode launch leaves its scores for the weights (AttentionStep's); add_weights
-    passes over them."""
+    passes over them. The workspace is laid out by q_indptr, so the kernels read the
+    plan's copy of it."""
 
     def __init__(self, q_indptr_host: Sequence[int], kv_len_host: Sequence[int],
                  num_qo_heads: int, window: int, device: torch.device, upload: bool = True,
@@ -82,22 +83,23 @@ class WeightsPlan:
                                                          window))
         buf = np.empty(max(cap, 4), dtype=np.int32)   # the plan writes what it uses
         self.info = _lib.WeightsPlanInfo()
-        self.kv_len_host = kv
+        self.kv_len_host, self.q_indptr_host = kv, qi.copy()
         marks = None if decodes is None else _i32(decodes)
         if marks is not None and marks.shape != (n,):
             raise ValueError(f"{n} rows but {marks.shape} decode marks")
         _lib.call("kunserve_weights_plan", qi.ctypes.data, kv_ptr, n, num_qo_heads, window,
                   None if marks is None else marks.ctypes.data, buf.ctypes.data, buf.size, ctypes.byref(self.info))
         self.plan_host = buf[: self.info.plan_ints].copy()
-        self.plan = None
+        self.plan = self.q_indptr = None
         if upload:
             self.bind(_upload_packed(self.host_arrays(), device))
 
     def host_arrays(self) -> list:
-        return [self.plan_host]
+        return [self.plan_host, self.q_indptr_host]
 
     def bind(self, dev: Sequence[torch.Tensor]) -> None:
         self.plan = dev[0] if self.info.plan_ints else None
+        self.q_indptr = dev[1]
 
     def workspace_bytes(self) -> int:
         return int(_lib.lib().kunserve_weights_workspace_bytes(ctypes.byref(self.info)))
@@ -109,7 +111,9 @@ def add_weights(pool: KVPool, weights: KVWeights, layer: int, table: PageTable,
                 workspace: Optional[torch.Tensor] = None) -> None:
     """Adds to `weights` what the last new tokens of every row attend to
     (kunserve_cache_weights): q [num_tokens, Hq, D] after its rotation, the step's
-    K in its pages. No page may be in two places of the table (ValueError)."""
+    K in its pages. q_indptr (device int32 [num_seqs + 1]) is that of the plan, whose
+    own copy is what the launches read. No page may be in two places of the table
+    (ValueError)."""
     weights.check(pool)
     if q.device != pool.device:
         raise ValueError(f"q is on {q.device}, the pool on {pool.device}")
@@ -119,8 +123,12 @@ def add_weights(pool: KVPool, weights: KVWeights, layer: int, table: PageTable,
         raise ValueError("attention weights need pages that are in one place of the table")
     if q.shape[2] != pool.head_dim:
         raise ValueError(f"q shape {tuple(q.shape)} does not match head_dim {pool.head_dim}")
-    if q_indptr.numel() != table.num_seqs + 1:
-        raise ValueError("q_indptr must have num_seqs + 1 entries")
+    _check_row_map(q_indptr, table.num_seqs + 1, pool.device, "q_indptr")
+    if q.shape[0] < plan.q_indptr_host[-1]:
+        raise ValueError(f"q has {q.shape[0]} tokens, the plan's rows end at "
+                         f"{plan.q_indptr_host[-1]}")
+    if plan.q_indptr is None:
+        raise RuntimeError("weights plan used before its device arrays were bound")
     pool.check_dtype(q)
     scale = sm_scale if sm_scale is not None else 1.0 / math.sqrt(pool.head_dim)
     need = plan.workspace_bytes()
@@ -128,7 +136,7 @@ def add_weights(pool: KVPool, weights: KVWeights, layer: int, table: PageTable,
         workspace = torch.empty(need, dtype=torch.uint8, device=pool.device)
     qd = _tensor3(q)
     _lib.call("kunserve_cache_weights", pool.desc(), ctypes.byref(weights._desc), layer,
-              table.desc(), q_indptr.data_ptr(), ctypes.byref(qd), q.shape[1],
+              table.desc(), plan.q_indptr.data_ptr(), ctypes.byref(qd), q.shape[1],
               ctypes.c_float(scale), _ptr(plan.plan), ctypes.byref(plan.info), _ptr(workspace),
               0 if workspace is None else workspace.numel() * workspace.element_size(),
               _stream_ptr(pool.device))

@@ -48,6 +48,7 @@ struct WeightsArgs {
   const int32_t* items;      // [num_items][4]: row, first token, column offset, partitions
   const int32_t* combines;   // [num_combines][4]: row, first column, column offset, partitions
   float2* stats;             // per row: [partitions + 1][columns]; the last: combined
+  int64_t num_columns;       // entries of stats
   int32_t num_qo_heads, num_kv_heads, ratio, window;
   float scale_log2;
 };
@@ -97,6 +98,8 @@ __global__ __launch_bounds__(kThreads) void weights_scores_kernel(WeightsArgs a)
   const int obs = min(q_len, a.window);       // observers
   const int cols = obs * a.ratio;             // columns of this KV head
   const int all = cols * a.num_kv_heads;
+  // A q_indptr that is not the plan's must not leave the workspace.
+  if (offset + int64_t(parts + 1) * all > a.num_columns) return;   // uniform
   const int t0 = part0 + wave * kSubs * 16;   // first token of the wave
   const int mask = (1 << a.page_shift) - 1;
   const int32_t* pages = a.indices + a.indptr[seq];
@@ -262,7 +265,7 @@ __global__ __launch_bounds__(kThreads) void weights_combine_kernel(WeightsArgs a
   const int q_len = a.q_indptr[seq + 1] - a.q_indptr[seq];
   const int all = min(q_len, a.window) * a.num_qo_heads;
   const int c = rec[1] + threadIdx.x;
-  if (c >= all) return;
+  if (c >= all || rec[2] + int64_t(parts + 1) * all > a.num_columns) return;
   float2* stats = a.stats + int64_t(rec[2]) + c;
   float2 st = {kNegBig, 0.f};
   int i = 0;
@@ -363,6 +366,7 @@ int weights_plan(const int32_t* q_indptr, const int32_t* kv_len, int32_t num_seq
                  std::vector<int32_t>& plan, kunserve_weights_plan_info* info) {
   std::vector<int32_t> items, combines, score_items, score_at;
   int64_t columns = 0, score_tokens = 0, most_parts = 0;
+  KSV_CHECK_ARG(num_seqs == 0 || q_indptr[0] >= 0, "q_indptr begins at %d", q_indptr[0]);
   for (int32_t b = 0; b < num_seqs; ++b) {
     const int64_t q_len = int64_t(q_indptr[b + 1]) - q_indptr[b];
     KSV_CHECK_ARG(q_len >= 0 && kv_len[b] >= q_len, "row %d: kv_len %d for %lld new tokens", b,
@@ -565,6 +569,7 @@ extern "C" int kunserve_cache_weights(const kunserve_kv_pool* pool,
   a.items = plan_dev;
   a.combines = plan_dev + 4 * int64_t(info->num_items);
   a.stats = static_cast<float2*>(workspace_dev);
+  a.num_columns = info->num_columns;
   a.num_qo_heads = num_qo_heads;
   a.num_kv_heads = pool->num_kv_heads;
   a.ratio = num_qo_heads / pool->num_kv_heads;

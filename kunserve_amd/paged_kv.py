@@ -668,8 +668,6 @@ def rotary_append_kv(pool: KVPool, layer: int, table: PageTable, q_indptr: torch
         raise ValueError(f"k_new / v_new must be [tokens, {pool.num_kv_heads}, {dim}]")
     if q_shape[0] != tokens or q_shape[2] != dim:
         raise ValueError(f"q {tuple(q_shape)} does not match k_new {tuple(k_shape)}")
-    if q_indptr.numel() != table.num_seqs + 1:
-        raise ValueError("q_indptr must have num_seqs + 1 entries")
     if out is None:
         out = q
     elif out.shape != q_shape:
@@ -680,6 +678,7 @@ def rotary_append_kv(pool: KVPool, layer: int, table: PageTable, q_indptr: torch
         bad = next(t for t in (q, k_new, v_new, out) if t.get_device() != index)
         raise ValueError(f"q, k_new, v_new or out is on {bad.device}, the pool on {device}")
     rotary.check(dim, device)
+    _check_row_map(q_indptr, table.num_seqs + 1, device, "q_indptr")
     _check_row_map(positions, tokens, device, "positions")
     if not q.dtype == k_new.dtype == v_new.dtype == out.dtype == dtype:
         pool.check_dtype(q, k_new, v_new, out)

@@ -15,6 +15,12 @@ import torch
 from . import _lib
 
 SCALINGS = ("linear", "ntk", "yarn", "llama3")
+# Keys of a scaling: those of every kind (original_max_position_embeddings has no
+# part in linear and ntk), and those of one.
+_KEYS = ("rope_type", "type", "factor", "rope_theta", "original_max_position_embeddings")
+_KEYS_OF = dict(yarn=("beta_fast", "beta_slow", "truncate", "attention_factor", "mscale",
+                      "mscale_all_dim"),
+                llama3=("low_freq_factor", "high_freq_factor"))
 
 
 def rotary_frequencies(rotary_dim: int, theta: float = 10000.0,
@@ -23,15 +29,20 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0,
     the rotated dims).
 
     f_j = theta^(-2j / rotary_dim). scaling, for contexts `factor` times as long
-    as those trained on, with the keys of a model configuration's rope_scaling:
+    as those trained on, with the keys of a model configuration's rope_scaling (a
+    value of None is a key left out; any other key raises, as does a rope_theta that
+    is not theta):
       linear  f / factor: positions are compressed
       ntk     theta * factor^(rotary_dim / (rotary_dim - 2)): the slowest pair
               is slowed by factor, the fastest not at all
       yarn    pairs that turn more than beta_fast times within
               original_max_position_embeddings keep f, those that turn less
               than beta_slow times get f / factor, with a linear ramp over the
-              pairs between; the factor on the rotated dims is
-              attention_factor, by default 0.1 ln(factor) + 1
+              pairs between, whose ends are rounded to whole pairs unless
+              truncate is false; the factor on the rotated dims is
+              attention_factor, by default m(mscale) / m(mscale_all_dim) where
+              both are given and m(1) where neither is, m(x) = 0.1 x ln(factor) + 1
+              (a softmax scale that such a model changes too is the caller's)
       llama3  the same with a ramp over the turns themselves, from
               low_freq_factor to high_freq_factor
     """
@@ -39,14 +50,24 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0,
         raise ValueError(f"rotary_dim {rotary_dim} must be positive and even")
     if not (math.isfinite(theta) and theta > 0):
         raise ValueError(f"theta {theta} must be finite and positive")
-    kind, get = None, {}.get
+    kind, factor = None, 1.0
     if scaling is not None:
-        kind, get = scaling.get("rope_type", scaling.get("type")), scaling.get
-        if kind == "default":
-            kind = None
-        elif kind not in SCALINGS:
+        scaling = {key: x for key, x in scaling.items() if x is not None}
+        kind = scaling.get("rope_type", scaling.get("type"))
+        if kind != "default" and kind not in SCALINGS:
             raise ValueError(f"rope_type {kind!r} is not one of {SCALINGS}")
-    factor = float(get("factor", 1.0)) if kind else 1.0
+        if scaling.get("type", kind) != kind:
+            raise ValueError(f"rope_type {kind!r} and type {scaling['type']!r} differ")
+        unknown = sorted(set(scaling) - set(_KEYS) - set(_KEYS_OF.get(kind, ())))
+        if unknown:
+            raise ValueError(f"{kind} scaling has no {', '.join(map(repr, unknown))}")
+        if float(scaling.get("rope_theta", theta)) != theta:
+            raise ValueError(f"scaling has rope_theta {scaling['rope_theta']}, not {theta}")
+        kind = None if kind == "default" else kind
+        if kind and "factor" not in scaling:
+            raise ValueError(f"{kind} scaling needs a factor")
+        factor = float(scaling["factor"]) if kind else 1.0
+    get = (scaling or {}).get
     if not (math.isfinite(factor) and factor >= 1):
         raise ValueError(f"scaling factor {factor} must be at least 1")
     half = rotary_dim // 2
@@ -78,11 +99,23 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0,
     def pair_of(turns):   # the (fractional) pair that turns so often within length
         return half * math.log(length / (turns * 2 * math.pi)) / math.log(theta)
 
-    first = max(math.floor(pair_of(fast)), 0)
-    last = min(math.ceil(pair_of(slow)), rotary_dim - 1)
+    truncate = get("truncate", True)
+    if truncate not in (True, False):
+        raise ValueError(f"truncate {truncate!r} is neither true nor false")
+    first, last = pair_of(fast), pair_of(slow)
+    if truncate:
+        first, last = math.floor(first), math.ceil(last)
+    first, last = max(first, 0), min(last, rotary_dim - 1)
     slowed = np.clip((np.arange(half) - first) / max(last - first, 1e-3), 0.0, 1.0)
-    given = get("attention_factor")
-    scale = 0.1 * math.log(factor) + 1.0 if given is None else float(given)
+    m = [float(get(key, 1.0)) for key in ("mscale", "mscale_all_dim")]
+    if ("mscale" in scaling) != ("mscale_all_dim" in scaling) or not all(0 < x < math.inf for x in m):
+        raise ValueError("mscale and mscale_all_dim are positive numbers given together")
+    scale = 0.1 * m[0] * math.log(factor) + 1.0
+    if "mscale" in scaling:
+        scale /= 0.1 * m[1] * math.log(factor) + 1.0
+    scale = float(get("attention_factor", scale))
+    if not math.isfinite(scale):
+        raise ValueError(f"attention_factor {scale} is not finite")
     return f * (1.0 - slowed) + f / factor * slowed, scale
 
 

@@ -195,7 +195,9 @@ __device__ __forceinline__ void decode_finish(const DecodeArgs& a, int seq, int 
     const int g = idx / (D / 2), d = 2 * (idx % (D / 2));
     const int64_t row0 = int64_t(s0) * a.num_qo_heads + hq0 + g;
     constexpr int kBatch = 8;   // partials read together, so their latencies overlap
-    float mx = -INFINITY, wsum = 0.f, x = 0.f, y = 0.f;
+    // The maximum from a number on: a row whose log-sum-exps are all NaN gets NaN
+    // weights, one of no tokens (all -infinity) none.
+    float mx = kNegBig, wsum = 0.f, x = 0.f, y = 0.f;
     for (int j = 0; j < n; j += kBatch) {
       float lse[kBatch];
       uint64_t po[kBatch];
@@ -209,7 +211,6 @@ __device__ __forceinline__ void decode_finish(const DecodeArgs& a, int seq, int 
       float m2 = mx;
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) m2 = j + u < n ? fmaxf(m2, lse[u]) : m2;
-      if (m2 == -INFINITY) continue;
       const float keep = fast_exp2(mx - m2);
       mx = m2;
       wsum *= keep;

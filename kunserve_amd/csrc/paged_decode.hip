@@ -655,7 +655,8 @@ __global__ __launch_bounds__(kWave) void decode_merge_kernel(const int32_t* merg
   };
   float lse = lane < n ? part_lse[int64_t(s0 + lane) * num_qo_heads + hq] : -INFINITY;
   load_batch(0, n);
-  float mx = lse;
+  // A number at least: where all are NaN the weights are, where all are -infinity 0.
+  float mx = fmaxf(lse, kNegBig);
   for (int j = lane + kWave; j < n; j += kWave)
     mx = fmaxf(mx, part_lse[int64_t(s0 + j) * num_qo_heads + hq]);
 #pragma unroll
@@ -663,22 +664,20 @@ __global__ __launch_bounds__(kWave) void decode_merge_kernel(const int32_t* merg
 
   float o[DPL] = {};
   float wsum = 0.f;
-  if (mx > -INFINITY) {
-    for (int base = 0; base < n; base += kWave) {
-      const int j = base + lane;
-      if (base > 0) lse = j < n ? part_lse[int64_t(s0 + j) * num_qo_heads + hq] : -INFINITY;
-      const float w = j < n ? fast_exp2(lse - mx) : 0.f;
-      wsum += w;
-      const int cnt = min(kWave, n - base);   // uniform
-      for (int t0 = 0; t0 < cnt; t0 += kBatch) {
-        if (base + t0 > 0) load_batch(base + t0, cnt - t0);
+  for (int base = 0; base < n; base += kWave) {
+    const int j = base + lane;
+    if (base > 0) lse = j < n ? part_lse[int64_t(s0 + j) * num_qo_heads + hq] : -INFINITY;
+    const float w = j < n ? fast_exp2(lse - mx) : 0.f;
+    wsum += w;
+    const int cnt = min(kWave, n - base);   // uniform
+    for (int t0 = 0; t0 < cnt; t0 += kBatch) {
+      if (base + t0 > 0) load_batch(base + t0, cnt - t0);
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const float wt = __shfl(w, t0 + u);   // every lane: t0 + u < kWave
-          if (t0 + u < cnt) {
+      for (int u = 0; u < kBatch; ++u) {
+        const float wt = __shfl(w, t0 + u);   // every lane: t0 + u < kWave
+        if (t0 + u < cnt) {
 #pragma unroll
-            for (int e = 0; e < DPL; ++e) o[e] = fmaf(wt, x[u][e], o[e]);
-          }
+          for (int e = 0; e < DPL; ++e) o[e] = fmaf(wt, x[u][e], o[e]);
         }
       }
     }

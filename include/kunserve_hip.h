@@ -308,7 +308,9 @@ int64_t kunserve_decode_workspace_bytes(const kunserve_decode_plan_info* info,
  * head_dim] of the pool dtype (fp16 or bf16); fp32 accumulation. q_token
  * (device int32 [num_seqs]) lets the decode rows of a mixed step
  * (kunserve/flash_backend.py:1870-1950, rows of request.py:654-670) read q
- * and write out in place, among the step's prefill tokens. */
+ * and write out in place, among the step's prefill tokens. A row of no tokens
+ * gives zeros; a NaN score, or one of +infinity, makes its row and head NaN,
+ * here, in kunserve_shared_decode and in a step. */
 int kunserve_paged_decode(const kunserve_kv_pool* pool, int32_t layer,
                           const kunserve_page_table* table,
                           const int32_t* q_token_dev,

@@ -225,7 +225,7 @@ __device__ __forceinline__ void decode_finish(const DecodeArgs& a, int seq, int 
         y = fmaf(w, bits_to_f32(int(uint32_t(po[u] >> 32))), y);
       }
     }
-    const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+    const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
     write_out(g, d, x * inv, y * inv);
     if (d == 0 && a.lse)
       a.lse[int64_t(seq) * a.num_qo_heads + hq0 + g] = wsum == 0.f ? -INFINITY : mx + __log2f(wsum);
@@ -253,8 +253,13 @@ struct DecodeTile {
   }
 };
 
-// A row's log-sum-exp from its maximum and sum; for a launch that leaves its
-// scores, NaN where a score is.
+// A partial's log-sum-exp from its maximum and sum. A NaN score makes the quotient of
+// sums NaN, and with a weight that is a number, 0 at least, the row's output.
+__device__ __forceinline__ float partial_lse(float m, float sum) {
+  return sum > 0.f ? m + __log2f(sum) : sum == 0.f ? -INFINITY : m;
+}
+
+// A row's; for a launch that leaves its scores, NaN where a score is.
 __device__ __forceinline__ float row_lse(const DecodeArgs& a, float m, float sum) {
   return sum > 0.f ? m + __log2f(sum) : a.lse && sum != sum ? sum : -INFINITY;
 }

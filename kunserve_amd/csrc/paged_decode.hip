@@ -232,9 +232,9 @@ __global__ __launch_bounds__(kThreads, (valu_waves<T, G>())) void paged_decode_k
       x += s_acc[wv][g][d] * f;
       y += s_acc[wv][g][d + 1] * f;
     }
-    x = lsum > 0.f ? x / lsum : 0.f;
-    y = lsum > 0.f ? y / lsum : 0.f;
-    lse = SCORES ? row_lse(a, mx, lsum) : lsum > 0.f ? mx + __log2f(lsum) : -INFINITY;
+    x = lsum == 0.f ? 0.f : x / lsum;
+    y = lsum == 0.f ? 0.f : y / lsum;
+    lse = SCORES ? row_lse(a, mx, lsum) : partial_lse(mx, lsum);
   });
 }
 
@@ -615,9 +615,9 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
       x += oc[0] * f;
       y += oc[1] * f;
     }
-    x = ls > 0.f ? x / ls : 0.f;
-    y = ls > 0.f ? y / ls : 0.f;
-    lse = SCORES ? row_lse(a, mxw, ls) : ls > 0.f ? mxw + __log2f(ls) : -INFINITY;
+    x = ls == 0.f ? 0.f : x / ls;
+    y = ls == 0.f ? 0.f : y / ls;
+    lse = SCORES ? row_lse(a, mxw, ls) : partial_lse(mxw, ls);
   });
 }
 
@@ -684,7 +684,7 @@ __global__ __launch_bounds__(kWave) void decode_merge_kernel(const int32_t* merg
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) wsum += __shfl_xor(wsum, off);
-  const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+  const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
   if (lse_out && lane == 0)
     lse_out[int64_t(seq) * num_qo_heads + hq] = wsum == 0.f ? -INFINITY : mx + __log2f(wsum);
   const int tok = q_token ? q_token[seq] : seq;

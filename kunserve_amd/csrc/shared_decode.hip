@@ -196,12 +196,6 @@ __device__ __forceinline__ bool not_finite(const f32x4 (&o)[DecodeTile<D>::ACCS]
   return __any(!(z[0] + z[1] + z[2] + z[3] == 0.f));
 }
 
-// A column's partial: its log-sum-exp, and its quotient of sums. A NaN score
-// makes the column's output NaN, at whatever weight.
-__device__ __forceinline__ float partial_lse(float m, float sum) {
-  return sum > 0.f ? m + __log2f(sum) : sum == 0.f ? -INFINITY : m;
-}
-
 template <typename T, int D, bool WIDE>
 __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs sa) {
   typedef typename Vec<T>::v8 V8;

@@ -37,7 +37,7 @@ constexpr int kRecord = 8;              // ints of a work record
 constexpr int kMinPieceTokens = 128;
 // Columns, and us of the segments' work for each CU, from which workgroups are wide.
 constexpr int kMinWideCols = 64;
-constexpr double kMinWideShareUs = 20.0;
+constexpr double kMinWideShareUs = 24.0;
 
 struct SharedArgs {
   DecodeArgs d;            // work: the tails'
@@ -451,11 +451,13 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
           // One wave to a SIMD: what overlaps does so within its instructions. A
           // tile's exponentials stand between the products of the other tile (scores of the
           // second, then P V of the first), and V and the next K are read into
-          // the registers that the products are done with. Probabilities in one
-          // 16-bit term: at 64 columns and more the matrix units' work counts.
-          // Steps past the piece are masked ones. 128 rows behind 8192 tokens, 64
-          // heads on 8: 65 us a layer without tails against 78 with one operation after
-          // the other, whose products alone are 33 at the rate of a large matrix product.
+          // the registers that the products are done with. Probabilities in two 16-bit terms, as in
+          // every decode launch (bf16: 1.7e-3 off 64 bits, 2.1e-3 in one), though the
+          // matrix units' work counts here. Steps past the piece are masked ones.
+          // 128 rows behind 8192 tokens with tails of 20-100, 64 heads on 8: 79 us a layer
+          // (65 with one term), whose products alone are 50 at the rate of a large
+          // matrix product. The second term's products behind the first's, those of
+          // the second tile unordered but for the reads: all in pairs 8 % more.
           V8 ka[2][KS], ve[8];
           auto read_k = [&](int blk, int i) {
             ka[i & 1][i >> 1] = *reinterpret_cast<const V8*>(
@@ -469,7 +471,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
             const int t0 = tb + (c + blk) * STEP;
             const bool edge = any_bad || t0 + STEP > te;   // uniform
             f32x4 sc[kWideTiles][PAIRS][2];
-            V8 ph[kWideTiles][L::ACCS], unused[L::ACCS];
+            V8 ph[kWideTiles][L::ACCS], pl[kWideTiles][L::ACCS];
             auto scores = [&](int ct, int s) {
 #pragma unroll
               for (int sub = 0; sub < 2; ++sub)
@@ -494,7 +496,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
               ve[2 * s] = values[(blk * 8 + 2 * s) * kWave + lane];
               ve[2 * s + 1] = values[(blk * 8 + 2 * s + 1) * kWave + lane];
             }
-            tile_exp<T, D>(sc[0], a.scale_log2, m[0], lsum[0], ph[0], unused);
+            tile_exp<T, D>(sc[0], a.scale_log2, m[0], lsum[0], ph[0], pl[0]);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
               __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // a product
@@ -508,16 +510,20 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(SharedArgs s
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[0][0][e] = mfma16(ve[e], ph[0][0], o[0][0][e]);
-            tile_exp<T, D>(sc[1], a.scale_log2, m[1], lsum[1], ph[1], unused);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 8; ++e) o[0][0][e] = mfma16(ve[e], pl[0][0], o[0][0][e]);
+            tile_exp<T, D>(sc[1], a.scale_log2, m[1], lsum[1], ph[1], pl[1]);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
               __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
               __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
+            for (int e = 0; e < 8; ++e) o[1][0][e] = mfma16(ve[e], ph[1][0], o[1][0][e]);
+#pragma unroll
             for (int e = 0; e < 8; ++e) {
-              o[1][0][e] = mfma16(ve[e], ph[1][0], o[1][0][e]);
+              o[1][0][e] = mfma16(ve[e], pl[1][0], o[1][0][e]);
               if (blk + 1 < W) read_k(blk + 1, e);
             }
 #pragma unroll
@@ -911,9 +917,10 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
   // Segments in workgroups of whole rows (group is 16 at most). Wide ones where
   // narrow ones would keep the CUs busy for long: they read K and V once for
   // eight times as many columns, but take about 10 us to begin and end, and their
-  // number is an eighth. Per layer, 8 KV heads of 128, narrow against wide: 64 columns
-  // of 4000 tokens (a CU's share 6 us) 15.7 against 21, 160 of 3000 (11 us) 20 against
-  // 24, 320 of 3000 (22 us) 27.6 against 27, 256 of 8000 (46 us) 40 against 32.
+  // number is an eighth. Per layer, 8 KV heads of 128, tails of 20-100, narrow against
+  // wide: 64 columns of 4000 tokens (a CU's share 6 us) 16.4 against 22.4, 160 of 3000
+  // (11 us) 21.1 against 26.8, 320 of 3000 (22 us) 31.4 against 32.1, 256 of 8000 (46 us)
+  // 41.6 against 34.8.
   double narrow_work = 0.0;
   const double narrow_us = 0.0115 * std::pow(head_dim / 128.0, 1.4);   // a token, of a workgroup
   int64_t tail_tokens = 0;
@@ -939,8 +946,9 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
   // A piece takes at most a CU's share of the segments' work (of a long one of narrow
   // workgroups, which run two to a CU, 0.7 at head_dim 128: 24 rows behind 6000 tokens,
   // 32 heads on 8, 21.2 us against 21.8 and, at 1.6, 24.4), or what ends behind the
-  // tails' bytes: fewer pieces are fewer partials. Wide, 128 rows behind 8192 tokens, 64 heads on 8: 102 us
-  // in pieces of 2048, 110 in 1600, 125 in 1024.
+  // tails' bytes: fewer pieces are fewer partials. Wide, 128 rows behind 8192 tokens with
+  // tails of up to 2000, 64 heads on 8: 110 us in pieces of 2048, 119 in 2752, 124 in 1600,
+  // 137 in 1024.
   const double tails_us = double(tail_tokens) * num_kv_heads * head_dim * 4 / (6.6e6 * cus / 256);
   const double share_us = work / double(cus);
   auto pieces_of = [&](const Segment& s) {

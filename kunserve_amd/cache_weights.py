@@ -16,8 +16,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from .paged_kv import (KVPool, PageTable, _check_row_map, _i32, _ptr, _stream_ptr, _tensor3,
-                       _upload, _upload_packed, csr_from_lists)
+from .paged_kv import (KVPool, PageTable, _check_reach, _check_row_map, _i32, _ptr, _stream_ptr,
+                       _tensor3, _upload, _upload_packed, csr_from_lists)
 
 
 class KVWeights:
@@ -115,8 +115,7 @@ def add_weights(pool: KVPool, weights: KVWeights, layer: int, table: PageTable,
     own copy is what the launches read. No page may be in two places of the table
     (ValueError)."""
     weights.check(pool)
-    if q.device != pool.device:
-        raise ValueError(f"q is on {q.device}, the pool on {pool.device}")
+    _check_reach(pool.device, q=q)
     if not np.array_equal(plan.kv_len_host, table.kv_len_host):
         raise ValueError("the plan was made for other rows than the table's")
     if not table.pages_private:

@@ -377,6 +377,13 @@ def _tensor3(t: torch.Tensor) -> _lib.Tensor3:
     return _lib.Tensor3(t.data_ptr(), t.stride(0), t.stride(1))
 
 
+def _check_reach(device: torch.device, **tensors: Optional[torch.Tensor]) -> None:
+    """Kernels reach their device's memory and pinned host memory."""
+    for name, t in tensors.items():
+        if t is not None and t.device != device and not (t.device.type == "cpu" and t.is_pinned()):
+            raise ValueError(f"{name} is on {t.device}, the pool on {device}")
+
+
 def _num_cus(device: torch.device) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count
 
@@ -675,8 +682,7 @@ def rotary_append_kv(pool: KVPool, layer: int, table: PageTable, q_indptr: torch
     index = device.index   # a device tensor's is never None
     if not (q.get_device() == k_new.get_device() == v_new.get_device() == out.get_device()
             == index):   # -1 on the host
-        bad = next(t for t in (q, k_new, v_new, out) if t.get_device() != index)
-        raise ValueError(f"q, k_new, v_new or out is on {bad.device}, the pool on {device}")
+        _check_reach(device, q=q, k_new=k_new, v_new=v_new, out=out)
     rotary.check(dim, device)
     _check_row_map(q_indptr, table.num_seqs + 1, device, "q_indptr")
     _check_row_map(positions, tokens, device, "positions")
@@ -717,9 +723,9 @@ def shared_decode(pool: KVPool, layer: int, table: PageTable, q: torch.Tensor,
     """paged_decode of rows that share pages, on the plan made from their table."""
     if plan.table is not table or plan.page_size != pool.page_size:
         raise ValueError("the plan was made from another table or page size")
-    for t in (q, out):
-        if t is not None and t.device != pool.device:
-            raise ValueError(f"q or out is on {t.device}, the pool on {pool.device}")
+    _check_reach(pool.device, q=q, out=out)
+    if out is None and q.device != pool.device:
+        out = torch.empty(q.shape, dtype=q.dtype, device=pool.device)
     return _decode("kunserve_shared_decode", plan.shared_info, pool, layer, table, q, plan,
                    sm_scale, out, workspace, q_token)
 

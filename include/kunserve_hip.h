@@ -510,7 +510,9 @@ int64_t kunserve_weights_plan_bound(const int32_t* q_indptr_host,
  * q_indptr and kv_len as given here (the workspace is laid out by them). Rows with a
  * non-zero decodes_host[b] (NULL: none; they have one new token) are the decode
  * rows of kunserve_attention_step_with, whose decode launch leaves its scores
- * for the weights; the others are kunserve_cache_weights'. */
+ * for the weights (4 bytes of workspace per cached token and query head), but for
+ * those marked 2; these and the others are kunserve_cache_weights', which reads
+ * their K again. */
 int kunserve_weights_plan(const int32_t* q_indptr_host, const int32_t* kv_len_host,
                           int32_t num_seqs, int32_t num_qo_heads, int32_t window,
                           const int32_t* decodes_host, int32_t* plan_host,

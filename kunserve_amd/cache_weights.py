@@ -25,9 +25,14 @@ class KVWeights:
     num_kv_heads, page_size], float32 with the slots contiguous. A new token's
     weight starts at 0 in the step that appends it, so nothing has to be cleared
     when pages are used again. The weights are those of one pool: of its fused
-    views, or of the pool after a pmm drop or restore, they are others."""
+    views, or of the pool after a pmm drop or restore, they are others.
 
-    def __init__(self, pool: KVPool, w: Optional[torch.Tensor] = None):
+    score_bytes: what a step may hold in scores that its decode launch leaves for the
+    weights, 4 bytes per cached token and query head; rows beyond it have their K
+    read twice more (at 1 / 128 of the bytes)."""
+
+    def __init__(self, pool: KVPool, w: Optional[torch.Tensor] = None,
+                 score_bytes: int = 256 << 20):
         shape = (pool.num_pages, pool.num_layers, pool.num_kv_heads, pool.page_size)
         if w is None:
             w = torch.zeros(shape, dtype=torch.float32, device=pool.device)
@@ -43,6 +48,7 @@ class KVWeights:
             raise ValueError(f"weights must be float32 {shape} on {pool.device} with the slots "
                              "contiguous")
         self.w = w
+        self.score_bytes = score_bytes
         self._desc = _lib.KVWeights(w.data_ptr(), w.stride(0), w.stride(1), w.stride(2))
 
     def check(self, pool: KVPool) -> None:
@@ -54,6 +60,10 @@ class KVWeights:
     def plan(self, q_indptr_host, kv_len_host, num_qo_heads: int, window: int,
              decodes: Optional[Sequence[int]] = None) -> "WeightsPlan":
         """The plan of a step's rows, not yet on the device (WeightsPlan.bind)."""
+        if decodes is not None:
+            marks = np.asarray(decodes, dtype=bool)
+            held = np.cumsum(np.where(marks, np.asarray(kv_len_host, dtype=np.int64), 0))
+            decodes = marks.astype(np.int32) + (marks & (4 * num_qo_heads * held > self.score_bytes))
         return WeightsPlan(q_indptr_host, kv_len_host, num_qo_heads, window, self.w.device,
                            upload=False, decodes=decodes)
 
@@ -67,8 +77,8 @@ class KVWeights:
 class WeightsPlan:
     """Work of add_weights for a step's rows, computed on the host once per step and
     shared by every layer (kunserve_weights_plan). decodes marks the rows whose
-    decode launch leaves its scores for the weights (AttentionStep's); add_weights
-    passes over them. The workspace is laid out by q_indptr, so the kernels read the
+    decode launch leaves its scores for the weights (AttentionStep's) with 1;
+    add_weights passes over them, not over other decode rows, marked 2. The workspace is laid out by q_indptr, so the kernels read the
     plan's copy of it."""
 
     def __init__(self, q_indptr_host: Sequence[int], kv_len_host: Sequence[int],

@@ -371,8 +371,11 @@ int weights_plan(const int32_t* q_indptr, const int32_t* kv_len, int32_t num_seq
     const int64_t q_len = int64_t(q_indptr[b + 1]) - q_indptr[b];
     KSV_CHECK_ARG(q_len >= 0 && kv_len[b] >= q_len, "row %d: kv_len %d for %lld new tokens", b,
                   kv_len[b], (long long)q_len);
-    if (decodes && decodes[b]) {
-      KSV_CHECK_ARG(q_len == 1, "row %d decodes %lld tokens", b, (long long)q_len);
+    KSV_CHECK_ARG(!decodes || !decodes[b] || q_len == 1, "row %d decodes %lld tokens", b,
+                  (long long)q_len);
+    if (decodes && decodes[b] == 2) {   // leaves no scores: its K is read again
+      score_at.push_back(-1);
+    } else if (decodes && decodes[b]) {
       const int32_t row = int32_t(score_at.size());
       for (int32_t t = 0; t < kv_len[b]; t += kThreads)
         score_items.insert(score_items.end(), {row, t, int32_t(score_tokens), 0});

@@ -37,7 +37,8 @@ struct DecodeArgs {
   // null, or where the launch leaves its scores (in log2 units) and every row's
   // log-sum-exp: of row b, head group hg, token t and head g of the group at
   // scores[score_at[b] * num_qo_heads + (hg * kv_len[b] + t) * group + g], and
-  // lse[b * num_qo_heads + head]. A NaN score makes a log-sum-exp NaN.
+  // lse[b * num_qo_heads + head]. A NaN score makes a log-sum-exp NaN. score_at -1: the
+  // row leaves no scores.
   float* scores;
   float* lse;
   const int32_t* score_at;

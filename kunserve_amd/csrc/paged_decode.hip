@@ -125,8 +125,11 @@ __global__ __launch_bounds__(kThreads, (valu_waves<T, G>())) void paged_decode_k
     }
   };
   float* scores = nullptr;   // of the row and head group
-  if constexpr (SCORES)
-    scores = a.scores + int64_t(a.score_at[seq]) * a.num_qo_heads + int64_t(hg) * a.kv_len[seq] * G;
+  if constexpr (SCORES) {
+    const int at = a.score_at[seq];
+    if (at >= 0)
+      scores = a.scores + int64_t(at) * a.num_qo_heads + int64_t(hg) * a.kv_len[seq] * G;
+  }
   auto consume = [&](const Chunk& ch, int chunk) {
     float vf[kLoadsPerChunk][8];
 #pragma unroll
@@ -146,7 +149,7 @@ __global__ __launch_bounds__(kThreads, (valu_waves<T, G>())) void paged_decode_k
       if constexpr (SCORES) {   // a row's lane i has token i of its four
         const float mine = col == 0 ? s[0] : col == 1 ? s[1] : col == 2 ? s[2] : s[3];
         const int t = tb + chunk * CHUNK + col * TPL + row;
-        if (col < kLoadsPerChunk && t < te) scores[int64_t(t) * G + g] = mine;
+        if (scores && col < kLoadsPerChunk && t < te) scores[int64_t(t) * G + g] = mine;
       }
       const float alpha = fast_exp2(m[g] - mx);
       m[g] = mx;
@@ -374,8 +377,11 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
   T* sk = reinterpret_cast<T*>(s_raw) + wave * BLK;
   float* scores = nullptr;   // of the row and head group
   float* step_scores = s_scores + (kScoresInLds ? wave * STEP * kMaxGroup : 0);
-  if constexpr (SCORES)
-    scores = a.scores + int64_t(a.score_at[seq]) * a.num_qo_heads + int64_t(hg) * a.kv_len[seq] * G;
+  if constexpr (SCORES) {
+    const int at = a.score_at[seq];
+    if (at >= 0)
+      scores = a.scores + int64_t(at) * a.num_qo_heads + int64_t(hg) * a.kv_len[seq] * G;
+  }
 
   // Unconditional loads (see the VALU kernel): past-the-end lanes and bad
   // page ids read the zero row.
@@ -408,7 +414,7 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
   // A step's scores wait in LDS ([token][head], so that they leave in whole lines)
   // until the next step's loads are on their way.
   auto flush_scores = [&](int c) {
-    if constexpr (kScoresInLds) {
+    if (kScoresInLds && scores) {   // uniform
       float* to = scores + int64_t(tb + c * STEP) * G;
       const int count = min(STEP, te - tb - c * STEP) * G;
       __builtin_amdgcn_wave_barrier();
@@ -482,7 +488,7 @@ void paged_decode_mfma_kernel(DecodeArgs a) {
               const float score = sc[p][sub][x] * a.scale_log2;
               if constexpr (kScoresInLds)
                 step_scores[t * G + j] = score;
-              else if (t0 + t < te)
+              else if (scores && t0 + t < te)
                 scores[int64_t(t0 + t) * G + j] = score;
             }
       }

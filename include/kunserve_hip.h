@@ -539,6 +539,14 @@ int kunserve_cache_weights(const kunserve_kv_pool* pool,
                            void* workspace_dev, int64_t workspace_bytes,
                            kunserve_stream_t stream);
 
+/* The weights of a step's new tokens (num_tokens of q_indptr's rows) become 0 in every
+ * layer: for tokens appended by steps that add no weights, whose slots otherwise
+ * keep what their pages' last user left. Tokens of no row and pages outside the pool
+ * are left out. */
+int kunserve_clear_weights(const kunserve_kv_pool* pool, const kunserve_kv_weights* weights,
+                           const kunserve_page_table* table, const int32_t* q_indptr_dev,
+                           int32_t num_tokens, kunserve_stream_t stream);
+
 /* Eviction: of row b, in every layer and KV head, the first `sinks` cached
  * tokens, the last `recent` ones and the heaviest of those between stay, keep[b]
  * in all (device int32; kv_len[b] and max_keep at most; below sinks + recent

@@ -155,6 +155,8 @@ SIGNATURES = {
                                        POINTER(PageTable), c_void_p, POINTER(Tensor3), c_int32,
                                        c_float, c_void_p, POINTER(WeightsPlanInfo), c_void_p,
                                        c_int64, c_void_p]),
+    "kunserve_clear_weights": (c_int, [POINTER(KVPool), POINTER(KVWeights), POINTER(PageTable),
+                                       c_void_p, c_int32, c_void_p]),
     "kunserve_evict": (c_int, [POINTER(KVPool), POINTER(KVWeights), POINTER(PageTable), c_void_p,
                                c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p,
                                c_int64, c_void_p]),

@@ -23,9 +23,12 @@ from .paged_kv import (KVPool, PageTable, _check_reach, _check_row_map, _i32, _p
 class KVWeights:
     """Accumulated attention weights of a pool's tokens: w [num_pages, num_layers,
     num_kv_heads, page_size], float32 with the slots contiguous. A new token's
-    weight starts at 0 in the step that appends it, so nothing has to be cleared
-    when pages are used again. The weights are those of one pool: of its fused
-    views, or of the pool after a pmm drop or restore, they are others.
+    weight starts at 0 in the step that appends it, if the step was given these
+    weights (learn=False where it is to learn nothing, as where its rows share
+    pages); what other steps and ops append keeps the weights that the page's last
+    user left until clear. The weights are those of one pool: of its fused views, or of
+    the pool after a pmm drop or restore, they are others; copies of pages leave
+    them behind.
 
     score_bytes: what a step may hold in scores that its decode launch leaves for the
     weights, 4 bytes per cached token and query head; rows beyond it have their K
@@ -66,6 +69,16 @@ class KVWeights:
             decodes = marks.astype(np.int32) + (marks & (4 * num_qo_heads * held > self.score_bytes))
         return WeightsPlan(q_indptr_host, kv_len_host, num_qo_heads, window, self.w.device,
                            upload=False, decodes=decodes)
+
+    def clear(self, pool: KVPool, table: PageTable, q_indptr: torch.Tensor,
+              num_tokens: int) -> None:
+        """The weights of a step's new tokens become 0 in every layer
+        (kunserve_clear_weights): num_tokens of q_indptr's (device int32 [num_seqs +
+        1]) rows, the last of the table's."""
+        self.check(pool)
+        _check_row_map(q_indptr, table.num_seqs + 1, pool.device, "q_indptr")
+        _lib.call("kunserve_clear_weights", pool.desc(), ctypes.byref(self._desc), table.desc(),
+                  q_indptr.data_ptr(), num_tokens, _stream_ptr(pool.device))
 
     def add(self, pool: KVPool, layer: int, table: PageTable, q_indptr: torch.Tensor,
             q: torch.Tensor, plan: "WeightsPlan", sm_scale: Optional[float] = None,
@@ -161,6 +174,9 @@ def evict(pool: KVPool, weights: KVWeights, pages_of_reqs: Sequence[Sequence[int
     are copied to pages_out, ceil(tokens / page_size) pages per request that are
     no pages of the requests; the old pages are the caller's to free once the
     stream has passed this call.
+
+    Every cached token's weight counts: those appended by steps without the weights
+    have to be cleared first (KVWeights).
 
     The shortened request goes on with min(budget, kv_len) cached tokens, its
     positions where they were (AttentionStep(rope_positions=...)). Returns the

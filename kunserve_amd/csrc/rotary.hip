@@ -52,19 +52,6 @@ struct RotaryArgs {
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 128;   // head_dim <= 256
 
-// Row of the table that owns token `tok`, -1 if none does. A step of decode
-// rows, one token each, is met by the first guess.
-__device__ __forceinline__ int row_of_token(const int32_t* q_indptr, int num_seqs, int tok) {
-  if (tok < num_seqs && q_indptr[tok] == tok && q_indptr[tok + 1] == tok + 1) return tok;
-  if (tok < q_indptr[0] || tok >= q_indptr[num_seqs]) return -1;
-  int lo = 0, hi = num_seqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (q_indptr[mid] <= tok) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
-
 template <typename T>
 __global__ __launch_bounds__(kThreads) void rotary_append_kernel(RotaryArgs a) {
   typedef typename Vec<T>::v8 V8;

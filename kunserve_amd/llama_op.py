@@ -104,7 +104,8 @@ class LlamaOp:
                  is_context_stage: Optional[List[int]] = None, *,
                  share_prefixes: bool = False, weights: Optional[KVWeights] = None,
                  window: int = 16,
-                 rope_positions: Optional[List[int]] = None) -> AttentionStep:
+                 rope_positions: Optional[List[int]] = None,
+                 learn: bool = True) -> AttentionStep:
         """Prepares the attention stage of one step (kunserve/worker.py:270-312).
 
         Argument meanings follow kunserve/flash_backend.py:2448-2469. A layer
@@ -117,7 +118,7 @@ class LlamaOp:
         num_restore_requests = 0 (kunserve/flash_backend.py:2465).
         is_context_stage (not in the reference signature) gives the rows'
         real stages when use_tensor_cores hides them (kv_lens_for_step).
-        share_prefixes, weights, window and rope_positions (not in it either)
+        share_prefixes, weights, window, rope_positions and learn (not in it either)
         are AttentionStep's.
         """
         if len(input_tokens_batched) != num_requests or len(pages_of_reqs) != num_requests:
@@ -153,7 +154,7 @@ class LlamaOp:
                              is_context_stage=is_context_stage, layer_offset=offset,
                              id_map=id_map, num_ids=min(max_num_pages, num_ids),
                              share_prefixes=share_prefixes, weights=weights, window=window,
-                             rope_positions=rope_positions)
+                             rope_positions=rope_positions, learn=learn)
         step.layer_range = (local_layer_start, local_layer_end)
         return step
 

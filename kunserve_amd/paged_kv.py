@@ -821,7 +821,9 @@ class AttentionStep:
     each cached token got to it, from a decode row's token and from the last
     `window` tokens of a prefill row; new tokens start at 0. The step's pages must
     then be in one place of its lists each (ValueError), and out may not overlap
-    q.
+    q. With learn=False nothing is added and neither is asked: the new tokens'
+    weights become 0 in every layer when the step is made, on the current stream
+    (rows that share pages, in a pool whose weights others learn).
 
     rope_positions: for each row the rotary position of its first new token, where
     that is not its place in the cache (rows shortened by evict). Only a Rotary
@@ -843,7 +845,7 @@ class AttentionStep:
                  id_map: Optional[Callable[[np.ndarray], np.ndarray]] = None,
                  num_ids: Optional[int] = None, share_prefixes: bool = False,
                  share_min_bytes: Optional[int] = None, weights=None, window: int = 16,
-                 rope_positions: Optional[Sequence[int]] = None):
+                 rope_positions: Optional[Sequence[int]] = None, learn: bool = True):
         self.pool = pool
         self.num_qo_heads = num_qo_heads
         self.layer_offset = layer_offset
@@ -868,8 +870,14 @@ class AttentionStep:
         if not (math.isfinite(self.scale) and self.scale > 0):
             raise ValueError(f"sm_scale {self.scale} must be finite and positive")
 
+        cleared = None
         if weights is not None:
             weights.check(pool)
+        if not learn:
+            if weights is None:
+                raise ValueError("learn=False is for a step with weights")
+            weights, cleared = None, weights
+        if weights is not None:
             if window < 1:
                 raise ValueError(f"window {window} must be positive")
             if not self.table.pages_private:
@@ -987,6 +995,8 @@ class AttentionStep:
         if weights is not None:
             self._weights_workspace = torch.empty(self._weights_plan.workspace_bytes(),
                                                   dtype=torch.uint8, device=dev)
+        if cleared is not None:
+            cleared.clear(pool, self.table, self.q_indptr, self.num_tokens)
         self._describe(appends)
 
     def _describe(self, appends: int) -> None:

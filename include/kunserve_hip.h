@@ -645,7 +645,8 @@ int kunserve_attention_step(const kunserve_step* step, int32_t layer,
  * in the workspace weights_workspace_dev (16-byte aligned); the plan's decode
  * rows are then the step's, and the step's pages private, each in one place of
  * the table. positions_dev (may be NULL): the tokens'
- * rotary positions (kunserve_rotary_append_kv). */
+ * rotary positions (kunserve_rotary_append_kv); io's frequencies, which rotate at
+ * the places in the cache, are refused beside them. */
 typedef struct {
   const int32_t* shared_plan_dev;
   kunserve_shared_plan_info shared_info;

@@ -58,6 +58,8 @@ extern "C" int kunserve_attention_step_with(const kunserve_step* step,
                                             kunserve_stream_t stream) {
   clear_error();
   KSV_CHECK_ARG(step && io, "null step or tensors");
+  KSV_CHECK_ARG(rotary || !io->inv_freq_dev || !extras || !extras->positions_dev,
+                "positions need a rotary: io's frequencies rotate at the tokens' places in the cache");
   const bool weighted = extras && extras->weights.w;
   kunserve_tensor3 q = io->q, out = io->out;
   StepFusion decode, prefill;

@@ -194,25 +194,31 @@ __global__ __launch_bounds__(kThreads) void weights_scores_kernel(WeightsArgs a)
 #pragma unroll
         for (int s = 0; s < KS; ++s) sc[sub] = mfma16(k[sub][s], q[s], sc[sub]);
       }
-      if (!whole) {   // uniform; the scale is positive
-#pragma unroll
-        for (int sub = 0; sub < kSubs; ++sub)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int t = t0 + 16 * sub + 4 * tg + x;
-            const bool seen = ((ok >> (4 * sub + x)) & 1u) && t <= last;
-            sc[sub][x] = seen ? sc[sub][x] : -INFINITY;
-          }
-      }
+      auto seen = [&](int sub, int x) {
+        return ((ok >> (4 * sub + x)) & 1u) && t0 + 16 * sub + 4 * tg + x <= last;
+      };
       if constexpr (ADD) {
         const float2 st = s_stat[0][c];
+        auto add = [&](bool all_seen) {   // a NaN column gives nothing to what it does not see
 #pragma unroll
-        for (int sub = 0; sub < kSubs; ++sub)
+          for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            mass[sub][x] = fmaf(fast_exp2(fmaf(sc[sub][x], a.scale_log2, -st.x)), st.y,
-                                mass[sub][x]);
+            for (int x = 0; x < 4; ++x) {
+              const float p = fast_exp2(fmaf(sc[sub][x], a.scale_log2, -st.x)) * st.y;
+              mass[sub][x] += all_seen || seen(sub, x) ? p : 0.f;
+            }
+        };
+        if (whole)   // uniform
+          add(true);
+        else
+          add(false);
       } else {
+        if (!whole) {   // uniform; the scale is positive
+#pragma unroll
+          for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sc[sub][x] = seen(sub, x) ? sc[sub][x] : -INFINITY;
+        }
         float m = -INFINITY;
 #pragma unroll
         for (int sub = 0; sub < kSubs; ++sub)

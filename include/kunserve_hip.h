@@ -310,7 +310,7 @@ int64_t kunserve_decode_workspace_bytes(const kunserve_decode_plan_info* info,
  * (kunserve/flash_backend.py:1870-1950, rows of request.py:654-670) read q
  * and write out in place, among the step's prefill tokens. A row of no tokens
  * gives zeros; a NaN score, or one of +infinity, makes its row and head NaN,
- * here, in kunserve_shared_decode and in a step. */
+ * here, in kunserve_shared_decode and in a step's decode launch. */
 int kunserve_paged_decode(const kunserve_kv_pool* pool, int32_t layer,
                           const kunserve_page_table* table,
                           const int32_t* q_token_dev,

@@ -65,6 +65,8 @@ class KVWeights:
         """The plan of a step's rows, not yet on the device (WeightsPlan.bind)."""
         if decodes is not None:
             marks = np.asarray(decodes, dtype=bool)
+            if marks.shape != (len(kv_len_host),):
+                raise ValueError(f"{len(kv_len_host)} rows but {marks.shape} decode marks")
             held = np.cumsum(np.where(marks, np.asarray(kv_len_host, dtype=np.int64), 0))
             decodes = marks.astype(np.int32) + (marks & (4 * num_qo_heads * held > self.score_bytes))
         return WeightsPlan(q_indptr_host, kv_len_host, num_qo_heads, window, self.w.device,

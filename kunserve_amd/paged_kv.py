@@ -886,9 +886,12 @@ class AttentionStep:
             self.weights = weights
         positions = None
         if rope_positions is not None:
-            starts = np.asarray(rope_positions, dtype=np.int64)
+            starts = np.asarray(rope_positions)
             if starts.shape != (n_rows,):
                 raise ValueError(f"{n_rows} rows but {starts.shape} rope_positions")
+            if n_rows and starts.dtype.kind not in "iu":
+                raise ValueError("rope_positions must be whole numbers")
+            starts = starts.astype(np.int64)
             positions = np.repeat(starts - self.q_indptr_host[:-1], q_lens) + np.arange(
                 self.num_tokens)
             if np.any(starts < 0) or (positions.size and positions.max() >= 2**31):

@@ -50,3 +50,9 @@ def test_prompt_rows_do_not_count():
 def test_marks():
     with pytest.raises(RuntimeError, match="decodes 2 tokens"):
         WeightsPlan([0, 2], [40], 4, 8, CPU, upload=False, decodes=[2])
+
+
+def test_marks_of_other_rows():
+    with pytest.raises(ValueError, match="3 rows but"):
+        plan([300, 700, 301], 8, 0, [True])
+    assert plan([], 8, 0).workspace_bytes() == 0

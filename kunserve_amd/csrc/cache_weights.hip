@@ -53,20 +53,6 @@ struct WeightsArgs {
   float scale_log2;
 };
 
-// Maximum and sum over the four 16-lane groups.
-__device__ __forceinline__ float across_groups_max(float x) {
-  const auto a = __builtin_amdgcn_permlane16_swap(f32_to_bits(x), f32_to_bits(x), false, false);
-  x = fmaxf(bits_to_f32(a[0]), bits_to_f32(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(f32_to_bits(x), f32_to_bits(x), false, false);
-  return fmaxf(bits_to_f32(b[0]), bits_to_f32(b[1]));
-}
-__device__ __forceinline__ float across_groups_sum(float x) {
-  const auto a = __builtin_amdgcn_permlane16_swap(f32_to_bits(x), f32_to_bits(x), false, false);
-  x = bits_to_f32(a[0]) + bits_to_f32(a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(f32_to_bits(x), f32_to_bits(x), false, false);
-  return bits_to_f32(b[0]) + bits_to_f32(b[1]);
-}
-
 // m and l of two disjoint sets of scores.
 __device__ __forceinline__ float2 join(float2 x, float2 y) {
   const float m = fmaxf(x.x, y.x);
@@ -224,13 +210,13 @@ __global__ __launch_bounds__(kThreads) void weights_scores_kernel(WeightsArgs a)
         for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
           for (int x = 0; x < 4; ++x) m = fmaxf(m, sc[sub][x]);
-        m = fmaxf(across_groups_max(m) * a.scale_log2, kNegBig);
+        m = fmaxf(groups_max(m) * a.scale_log2, kNegBig);
         float l = 0.f;
 #pragma unroll
         for (int sub = 0; sub < kSubs; ++sub)
 #pragma unroll
           for (int x = 0; x < 4; ++x) l += fast_exp2(fmaf(sc[sub][x], a.scale_log2, -m));
-        l = across_groups_sum(l);
+        l = groups_sum(l);
         if (tg == 0) s_stat[wave][c] = float2{m, l};
       }
     }

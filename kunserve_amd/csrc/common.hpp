@@ -184,6 +184,20 @@ __device__ __forceinline__ float group_sum(float x) {
   }
 }
 
+// Maximum and sum over the four 16-lane groups.
+__device__ __forceinline__ float groups_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(f32_to_bits(x), f32_to_bits(x), false, false);
+  x = fmaxf(bits_to_f32(a[0]), bits_to_f32(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(f32_to_bits(x), f32_to_bits(x), false, false);
+  return fmaxf(bits_to_f32(b[0]), bits_to_f32(b[1]));
+}
+__device__ __forceinline__ float groups_sum(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(f32_to_bits(x), f32_to_bits(x), false, false);
+  x = bits_to_f32(a[0]) + bits_to_f32(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(f32_to_bits(x), f32_to_bits(x), false, false);
+  return bits_to_f32(b[0]) + bits_to_f32(b[1]);
+}
+
 __device__ __forceinline__ float fast_exp2(float x) {
   return __builtin_amdgcn_exp2f(x);
 }

@@ -265,14 +265,6 @@ __device__ __forceinline__ float row_lse(const DecodeArgs& a, float m, float sum
   return sum > 0.f ? m + __log2f(sum) : a.lse && sum != sum ? sum : -INFINITY;
 }
 
-// Maximum and sum over the four 16-lane groups.
-__device__ __forceinline__ float groups_max(float x) {
-  const auto a = __builtin_amdgcn_permlane16_swap(f32_to_bits(x), f32_to_bits(x), false, false);
-  x = fmaxf(bits_to_f32(a[0]), bits_to_f32(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(f32_to_bits(x), f32_to_bits(x), false, false);
-  return fmaxf(bits_to_f32(b[0]), bits_to_f32(b[1]));
-}
-
 // One head's attention over the tokens of a wave's steps (from t0 on, every
 // `stride`), in fp32 on the vector
 // units and a load at a time: what the MFMA kernel falls back to for values

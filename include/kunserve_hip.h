@@ -489,7 +489,7 @@ typedef struct {
 
 typedef struct {
   int64_t num_columns;   /* observed (column, partition) entries              */
-  int64_t score_tokens;  /* cached tokens of the decode rows                  */
+  int64_t score_tokens;  /* cached tokens of the decode rows with scores      */
   int32_t num_items;     /* work records (row, partition)                     */
   int32_t num_combines;  /* records of the columns' combination               */
   int32_t num_score_items; /* records of the decode rows' tokens              */
@@ -521,7 +521,7 @@ int kunserve_weights_plan(const int32_t* q_indptr_host, const int32_t* kv_len_ho
 int64_t kunserve_weights_workspace_bytes(const kunserve_weights_plan_info* info);
 
 /* What a step's attention says of the cache: for every row b with new tokens
- * (but the plan's decode rows),
+ * (but the plan's decode rows that leave scores),
  * cached token t and KV head g,
  *   w := (t new ? 0 : w) + sum of softmax(q . K^T * sm_scale)[t]
  * over the last min(q_len[b], window) new tokens of the row that see t (their

@@ -5,16 +5,17 @@
 //   w[t] := (t new ? 0 : w[t]) + sum over observers i and the query heads h of
 //           the KV head of p[i, h, t]
 // for every cached token of the row and every KV head, in fp32. A new token's
-// weight starts at 0, so pages that are used again need no clearing.
+// weight starts at 0 (clear_weights_kernel: in steps that add none).
 //
-// Columns: the row's observers times the query heads of a KV head. Three
-// launches: the maximum and sum of every column over each partition of
-// kPartTokens tokens; their combination; and the scores once more, this time
-// as probabilities summed over the columns. The sums run in one order, with no
-// atomics, so results do not depend on timing. A step's decode rows need no second
-// look at K: their decode launch leaves its scores. Of the three launches a workgroup keeps its partition
-// of K in registers (64 tokens a wave, as MFMA operands) and takes the columns
-// 16 at a time, so K is read once by each of the two launches.
+// Columns: the row's observers times the query heads of a KV head. Two launches
+// read K: the maximum and sum of every column over each partition of kPartTokens
+// tokens, then the scores once more, this time as probabilities summed over the
+// columns. The second combines the partitions' statistics itself; from rows of more
+// than kMaxOwnParts partitions on, a launch between the two does. The sums run in one
+// order, with no atomics, so results do not depend on timing. A workgroup keeps its
+// partition of K in registers (64 tokens a wave, as MFMA operands) and takes the
+// columns 16 at a time, so K is read once by each of the two. A step's decode rows need
+// no second look at K: their decode launch leaves its scores.
 #include <algorithm>
 #include <cmath>
 #include <vector>

@@ -922,7 +922,8 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
   // (11 us) 21.1 against 26.8, 320 of 3000 (22 us) 31.4 against 32.1, 256 of 8000 (46 us)
   // 41.6 against 34.8.
   double narrow_work = 0.0;
-  const double narrow_us = 0.0115 * std::pow(head_dim / 128.0, 1.4);   // a token, of a workgroup
+  // A token, of a workgroup (grouped_part_tokens: 11.5 ns at head_dim 128, 30 at 256).
+  const double narrow_us = 0.0115 * std::pow(head_dim / 128.0, 1.4);
   int64_t tail_tokens = 0;
   for (int32_t b = 0; b < num_seqs; ++b) tail_tokens += kv_len[b];
   for (const Segment& s : segments) {
@@ -944,9 +945,13 @@ int shared_plan(const int32_t* indptr, const int32_t* indices, const int32_t* kv
     info->wide |= is_wide(s);
   }
   // A piece takes at most a CU's share of the segments' work (of a long one of narrow
-  // workgroups, which run two to a CU, 0.7 at head_dim 128: 24 rows behind 6000 tokens,
-  // 32 heads on 8, 21.2 us against 21.8 and, at 1.6, 24.4), or what ends behind the
-  // tails' bytes: fewer pieces are fewer partials. Wide, 128 rows behind 8192 tokens with
+  // workgroups, which run two to a CU, 0.7 at head_dim 128: a few per cent either way.
+  // 32 heads on 8 at 0.5, 0.7, 1.0 and 1.4 of a share: 24 rows behind 6000 tokens 24.5, 22.4,
+  // 22.9 and 25.0 us, 48 behind 4096 28.1, 26.1, 26.7 and 29.8, 12 behind 12000 23.7, 22.8,
+  // 22.5 and 25.5, 16 behind 4000 (6 us of share) 20.0, 17.5, 16.3 and 17.8; head_dim 64, 40
+  // behind 3000 21.0, 20.4, 19.5 and 19.2, 32 behind 8000 25.6, 21.6, 23.2 and 24.6; head_dim
+  // 256, 40 behind 3000 41.0, 36.3, 35.8 and 37.1), or what ends behind the tails' bytes:
+  // fewer pieces are fewer partials. Wide, 128 rows behind 8192 tokens with
   // tails of up to 2000, 64 heads on 8: 110 us in pieces of 2048, 119 in 2752, 124 in 1600,
   // 137 in 1024.
   const double tails_us = double(tail_tokens) * num_kv_heads * head_dim * 4 / (6.6e6 * cus / 256);

@@ -93,8 +93,8 @@ class WeightsPlan:
     """Work of add_weights for a step's rows, computed on the host once per step and
     shared by every layer (kunserve_weights_plan). decodes marks the rows whose
     decode launch leaves its scores for the weights (AttentionStep's) with 1;
-    add_weights passes over them, not over other decode rows, marked 2. The workspace is laid out by q_indptr, so the kernels read the
-    plan's copy of it."""
+    add_weights passes over them, not over other decode rows, marked 2. The workspace
+    is laid out by q_indptr, so the kernels read the plan's copy of it."""
 
     def __init__(self, q_indptr_host: Sequence[int], kv_len_host: Sequence[int],
                  num_qo_heads: int, window: int, device: torch.device, upload: bool = True,

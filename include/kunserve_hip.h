@@ -247,6 +247,30 @@ int kunserve_rotary_append_kv(const kunserve_kv_pool* pool, int32_t layer,
                               const int32_t* positions_dev,
                               kunserve_stream_t stream);
 
+/* Rotary positions on several axes (an image's time, height and width): pair j
+ * is turned by the position on axis axis_dev[j] (rotary_dim / 2 entries in [0,
+ * num_axes); others count as axis 0). Token i's position on axis x is
+ * positions_dev[x * position_stride + i]; position_stride 0: one position for
+ * every axis. */
+typedef struct {
+  const int32_t* axis_dev;
+  int32_t num_axes;
+  int64_t position_stride;
+} kunserve_rotary_axes;
+
+/* kunserve_rotary_append_kv with positions on several axes (axes NULL: on one). */
+int kunserve_rotary_axes_append_kv(const kunserve_kv_pool* pool, int32_t layer,
+                                   const kunserve_page_table* table,
+                                   const int32_t* q_indptr_dev, int32_t num_tokens,
+                                   const kunserve_tensor3* q, kunserve_tensor3* q_out,
+                                   int32_t num_qo_heads,
+                                   const kunserve_tensor3* k_new,
+                                   const kunserve_tensor3* v_new,
+                                   const kunserve_rotary* rotary,
+                                   const kunserve_rotary_axes* axes,
+                                   const int32_t* positions_dev,
+                                   kunserve_stream_t stream);
+
 /* ---------------------------------------------- decode attention (A4) */
 
 typedef struct {
@@ -475,6 +499,58 @@ int kunserve_paged_prefill(const kunserve_kv_pool* pool, int32_t layer,
                            void* workspace_dev, int64_t workspace_bytes,
                            kunserve_stream_t stream);
 
+/* ---------------------------- attention of drafted trees of tokens */
+
+typedef struct {
+  int32_t num_work;      /* work records (incl. padding)                      */
+  int32_t num_merge;     /* tokens whose row is split                         */
+  int32_t num_slots;     /* partial-result slots                              */
+  int32_t num_seqs;      /* what the plan was made for, from here on          */
+  int32_t head_dim;
+  int32_t page_size;
+  int32_t num_qo_heads;
+  int32_t num_kv_heads;
+  int32_t plan_ints;     /* int32 entries of the plan buffer in use           */
+} kunserve_tree_plan_info;
+
+/* Upper bound of the plan buffer length (int32 entries); -1 on a bad argument. */
+int64_t kunserve_tree_plan_bound(const int32_t* q_indptr_host,
+                                 const int32_t* kv_len_host, int32_t num_seqs,
+                                 int32_t num_qo_heads, int32_t num_kv_heads,
+                                 int32_t head_dim);
+
+/* Host-side plan of rows whose new tokens are the nodes of trees. Row b's are
+ * q_indptr[b+1] - q_indptr[b] tokens (q_indptr starts at 0), tokens q_first[b]
+ * onwards of q and out (NULL: q_indptr[b]), the last ones of its kv_len[b];
+ * parents[q_indptr[b] + i] is the place among them of token i's parent, below
+ * i, or -1: it follows the cached tokens. indptr is the page table's. Rows are
+ * cut into pieces of part_rounds rounds (256, 128 or 64 tokens at head_dim 64,
+ * 128 and 256; 0: chosen from num_cus). */
+int kunserve_tree_plan(const int32_t* indptr_host, const int32_t* q_indptr_host,
+                       const int32_t* q_first_host, const int32_t* kv_len_host,
+                       const int32_t* parents_host, int32_t num_seqs,
+                       int32_t num_qo_heads, int32_t num_kv_heads,
+                       int32_t page_size, int32_t head_dim, int32_t num_cus,
+                       int32_t part_rounds, int32_t* plan_host,
+                       int64_t plan_capacity, kunserve_tree_plan_info* info);
+
+/* Workspace bytes needed by kunserve_tree_attention for this plan. */
+int64_t kunserve_tree_workspace_bytes(const kunserve_tree_plan_info* info);
+
+/* Attention of the plan's new tokens: each sees its row's cached tokens before
+ * them, its ancestors and itself (their K and V are in the pages already).
+ * Otherwise as kunserve_paged_decode, on the table the plan was made from (its
+ * ids may be others, its lengths not). out may be q, and is 16-byte aligned
+ * with strides that are multiples of 8; so is the workspace. */
+int kunserve_tree_attention(const kunserve_kv_pool* pool, int32_t layer,
+                            const kunserve_page_table* table,
+                            const kunserve_tensor3* q, kunserve_tensor3* out,
+                            int32_t num_qo_heads, float sm_scale,
+                            const int32_t* plan_dev,
+                            const kunserve_tree_plan_info* info,
+                            void* workspace_dev, int64_t workspace_bytes,
+                            kunserve_stream_t stream);
+
 /* -------------------------- attention weights of the cache, eviction */
 
 /* Accumulated attention weight of every cached token and KV head (device,
@@ -564,6 +640,28 @@ int kunserve_evict(const kunserve_kv_pool* pool, const kunserve_kv_weights* weig
                    int32_t max_keep, int32_t max_len, int32_t sinks,
                    int32_t recent, int32_t* kept_dev, int64_t kept_stride,
                    kunserve_stream_t stream);
+
+/* ------------------------------- cached tokens that change their place */
+
+/* Of each row's cached tokens from place first[b] on, those at first[b] +
+ * kept[b * kept_stride + j], j < max_kept, come to first[b] + j: K, V and (if
+ * weights is not NULL) weights, in every layer and KV head, in place. An entry moves
+ * its token down: one that is negative, its own place j, below it, or past the row's
+ * end moves nothing, and the slot keeps what it has. What the other entries read is
+ * what the slots held before the call. Pages with tokens from first[b] on are in no
+ * other place of the table. Of pages outside the pool a source gives zeros, a
+ * destination is not written. */
+int kunserve_keep_tokens(const kunserve_kv_pool* pool, const kunserve_kv_weights* weights,
+                         const kunserve_page_table* table, const int32_t* first_dev,
+                         const int32_t* kept_dev, int64_t kept_stride, int32_t max_kept,
+                         kunserve_stream_t stream);
+
+/* For each move (source page, destination page, tokens; device int32 [n][3]) the
+ * page's first `tokens` slots are copied, K, V and weights (NULL: none), in every
+ * layer. No destination is a source or in two moves. A move with a page outside the
+ * pool is left out. */
+int kunserve_copy_pages(const kunserve_kv_pool* pool, const kunserve_kv_weights* weights,
+                        const int32_t* moves_dev, int64_t n, kunserve_stream_t stream);
 
 /* ------------------------------------------------ a step's layers */
 
@@ -662,6 +760,25 @@ typedef struct {
  * kunserve_rotary_append_kv, q in place, in place of io's frequencies. */
 int kunserve_attention_step_with(const kunserve_step* step,
                                  const kunserve_step_extras* extras, int32_t layer,
+                                 const kunserve_step_io* io,
+                                 const kunserve_rotary* rotary,
+                                 kunserve_stream_t stream);
+
+/* What else a step may have. tree_table.num_seqs > 0: rows whose new tokens are
+ * drafted trees, run by tree_plan_dev in the step's workspace (the weights of a step
+ * are not formed from them). axes.num_axes > 0: rotary turns by positions on several
+ * axes (kunserve_rotary_axes_append_kv). */
+typedef struct {
+  kunserve_page_table tree_table;
+  const int32_t* tree_plan_dev;
+  kunserve_tree_plan_info tree_info;
+  kunserve_rotary_axes axes;
+} kunserve_step_more;
+
+/* kunserve_attention_step_with with more (may be NULL). */
+int kunserve_attention_step_more(const kunserve_step* step,
+                                 const kunserve_step_extras* extras,
+                                 const kunserve_step_more* more, int32_t layer,
                                  const kunserve_step_io* io,
                                  const kunserve_rotary* rotary,
                                  kunserve_stream_t stream);

@@ -17,19 +17,21 @@ from . import _lib
 from .cache_weights import KVWeights, WeightsPlan, add_weights, evict
 from .llama_op import LlamaOp, kept_layers
 from .paged_kv import (AttentionStep, DecodePlan, KVPool, PageTable, PrefillPlan,
-                       SharedDecodePlan, append_kv, copy_blocks, csr_from_lists,
+                       SharedDecodePlan, TreePlan, append_kv, copy_blocks, csr_from_lists,
                        kv_lens_for_step, kv_pack, kv_scatter, paged_decode, paged_prefill,
-                       rope_append_kv, rope_inv_freq, rotary_append_kv, shared_decode, swap)
+                       rope_append_kv, rope_inv_freq, rotary_append_kv, shared_decode, swap,
+                       tree_attention, tree_depths)
 from .pmm import PmmPool
 from .rotary import Rotary, rotary_frequencies
+from .token_moves import fork_rows, keep_tokens
 
 __all__ = [
     "AttentionStep", "DecodePlan", "KVPool", "KVWeights", "LlamaOp", "PageTable", "PmmPool",
-    "PrefillPlan", "Rotary", "SharedDecodePlan", "WeightsPlan", "add_weights", "append_kv",
-    "copy_blocks", "csr_from_lists", "evict", "kv_lens_for_step", "kv_pack", "kept_layers",
-    "kv_scatter", "paged_decode", "paged_prefill", "rope_append_kv", "rope_inv_freq",
-    "rotary_append_kv", "rotary_frequencies", "shared_decode", "swap",
-    "library_path",
+    "PrefillPlan", "Rotary", "SharedDecodePlan", "TreePlan", "WeightsPlan", "add_weights",
+    "append_kv", "copy_blocks", "csr_from_lists", "evict", "fork_rows", "keep_tokens",
+    "kv_lens_for_step", "kv_pack", "kept_layers", "kv_scatter", "paged_decode", "paged_prefill",
+    "rope_append_kv", "rope_inv_freq", "rotary_append_kv", "rotary_frequencies", "shared_decode",
+    "swap", "tree_attention", "tree_depths", "library_path",
 ]
 
 

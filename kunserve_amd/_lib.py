@@ -100,6 +100,21 @@ class Rotary(Structure):
                 ("scale", c_float)]
 
 
+class RotaryAxes(Structure):
+    _fields_ = [("axis_dev", c_void_p), ("num_axes", c_int32), ("position_stride", c_int64)]
+
+
+class TreePlanInfo(Structure):
+    _fields_ = [("num_work", c_int32), ("num_merge", c_int32), ("num_slots", c_int32),
+                ("num_seqs", c_int32), ("head_dim", c_int32), ("page_size", c_int32),
+                ("num_qo_heads", c_int32), ("num_kv_heads", c_int32), ("plan_ints", c_int32)]
+
+
+class StepMore(Structure):
+    _fields_ = [("tree_table", PageTable), ("tree_plan_dev", c_void_p),
+                ("tree_info", TreePlanInfo), ("axes", RotaryAxes)]
+
+
 class StepExtras(Structure):
     _fields_ = [
         ("shared_plan_dev", c_void_p), ("shared_info", SharedPlanInfo), ("weights", KVWeights),
@@ -139,6 +154,25 @@ SIGNATURES = {
                                           c_int32, POINTER(Tensor3), POINTER(Tensor3), c_int32,
                                           POINTER(Tensor3), POINTER(Tensor3), POINTER(Rotary),
                                           c_void_p, c_void_p]),
+    "kunserve_rotary_axes_append_kv": (c_int, [POINTER(KVPool), c_int32, POINTER(PageTable),
+                                               c_void_p, c_int32, POINTER(Tensor3),
+                                               POINTER(Tensor3), c_int32, POINTER(Tensor3),
+                                               POINTER(Tensor3), POINTER(Rotary),
+                                               POINTER(RotaryAxes), c_void_p, c_void_p]),
+    "kunserve_tree_plan_bound": (c_int64, [c_void_p, c_void_p, c_int32, c_int32, c_int32,
+                                           c_int32]),
+    "kunserve_tree_plan": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32,
+                                   c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p,
+                                   c_int64, POINTER(TreePlanInfo)]),
+    "kunserve_tree_workspace_bytes": (c_int64, [POINTER(TreePlanInfo)]),
+    "kunserve_tree_attention": (c_int, [POINTER(KVPool), c_int32, POINTER(PageTable),
+                                        POINTER(Tensor3), POINTER(Tensor3), c_int32, c_float,
+                                        c_void_p, POINTER(TreePlanInfo), c_void_p, c_int64,
+                                        c_void_p]),
+    "kunserve_keep_tokens": (c_int, [POINTER(KVPool), POINTER(KVWeights), POINTER(PageTable),
+                                     c_void_p, c_void_p, c_int64, c_int32, c_void_p]),
+    "kunserve_copy_pages": (c_int, [POINTER(KVPool), POINTER(KVWeights), c_void_p, c_int64,
+                                    c_void_p]),
     "kunserve_shared_plan_bound": (c_int64, [c_void_p, c_int32, c_int32]),
     "kunserve_shared_plan": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,
                                      c_int32, c_int32, c_int32, c_int64, c_void_p, c_int64,
@@ -196,6 +230,9 @@ SIGNATURES = {
                                          c_int32, c_int32]),
     "kunserve_attention_step": (c_int, [POINTER(Step), c_int32, c_void_p, c_void_p]),
     "kunserve_attention_step_with": (c_int, [POINTER(Step), POINTER(StepExtras), c_int32, c_void_p,
+                                             POINTER(Rotary), c_void_p]),
+    "kunserve_attention_step_more": (c_int, [POINTER(Step), POINTER(StepExtras),
+                                             POINTER(StepMore), c_int32, c_void_p,
                                              POINTER(Rotary), c_void_p]),
     "kunserve_fused_pool": (c_int, [POINTER(KVPool), c_int64, c_int32, POINTER(KVPool)]),
     "kunserve_fused_page_ids": (c_int, [c_void_p, c_int64, c_int64, c_int32, c_int64,

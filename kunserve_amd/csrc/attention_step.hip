@@ -48,11 +48,20 @@ extern "C" int kunserve_tensors_overlap(const kunserve_tensor3* a, int32_t heads
 
 extern "C" int kunserve_attention_step(const kunserve_step* step, int32_t layer,
                                        const kunserve_step_io* io, kunserve_stream_t stream) {
-  return kunserve_attention_step_with(step, nullptr, layer, io, nullptr, stream);
+  return kunserve_attention_step_more(step, nullptr, nullptr, layer, io, nullptr, stream);
 }
 
 extern "C" int kunserve_attention_step_with(const kunserve_step* step,
                                             const kunserve_step_extras* extras, int32_t layer,
+                                            const kunserve_step_io* io,
+                                            const kunserve_rotary* rotary,
+                                            kunserve_stream_t stream) {
+  return kunserve_attention_step_more(step, extras, nullptr, layer, io, rotary, stream);
+}
+
+extern "C" int kunserve_attention_step_more(const kunserve_step* step,
+                                            const kunserve_step_extras* extras,
+                                            const kunserve_step_more* more, int32_t layer,
                                             const kunserve_step_io* io,
                                             const kunserve_rotary* rotary,
                                             kunserve_stream_t stream) {
@@ -61,8 +70,11 @@ extern "C" int kunserve_attention_step_with(const kunserve_step* step,
   KSV_CHECK_ARG(rotary || !io->inv_freq_dev || !extras || !extras->positions_dev,
                 "positions need a rotary: io's frequencies rotate at the tokens' places in the cache");
   const bool weighted = extras && extras->weights.w;
+  const bool trees = more && more->tree_table.num_seqs > 0;
+  KSV_CHECK_ARG(!weighted || !trees, "attention weights are not formed from drafted trees");
+  KSV_CHECK_ARG(rotary || !more || more->axes.num_axes == 0, "positions on axes need a rotary");
   kunserve_tensor3 q = io->q, out = io->out;
-  StepFusion decode, prefill;
+  StepFusion decode, prefill, tree;
   decode.counters = step->counters_dev;
   decode.num_counters = step->num_counters;
   prefill.counters = step->prefill_counters_dev;
@@ -109,16 +121,18 @@ extern "C" int kunserve_attention_step_with(const kunserve_step* step,
     }
   }
   if (rotary) {
-    rc = kunserve_rotary_append_kv(&step->pool, layer, &step->table, step->q_indptr_dev,
-                                   step->num_tokens, &q, &q, step->num_qo_heads, &io->k, &io->v,
-                                   rotary, extras ? extras->positions_dev : nullptr, stream);
+    rc = kunserve_rotary_axes_append_kv(&step->pool, layer, &step->table, step->q_indptr_dev,
+                                        step->num_tokens, &q, &q, step->num_qo_heads, &io->k,
+                                        &io->v, rotary,
+                                        more && more->axes.num_axes ? &more->axes : nullptr,
+                                        extras ? extras->positions_dev : nullptr, stream);
   } else if (io->inv_freq_dev) {
     rc = kunserve_rope_append_kv(&step->pool, layer, &step->table, step->q_indptr_dev,
                                  step->num_tokens, &q, step->num_qo_heads, &io->k, &io->v,
                                  io->inv_freq_dev, io->interleave, stream);
   } else if (step->appends && !out_overlaps_new()) {
-    decode.k_new = prefill.k_new = &io->k;
-    decode.v_new = prefill.v_new = &io->v;
+    decode.k_new = prefill.k_new = tree.k_new = &io->k;
+    decode.v_new = prefill.v_new = tree.v_new = &io->v;
   } else {
     rc = kunserve_append_kv(&step->pool, layer, &step->table, step->q_indptr_dev,
                             step->num_tokens, &io->k, &io->v, stream);
@@ -142,6 +156,12 @@ extern "C" int kunserve_attention_step_with(const kunserve_step* step,
                        step->prefill_q_start_dev, &q, &out, step->num_qo_heads, step->sm_scale,
                        step->prefill_plan_dev, &step->prefill_info, step->workspace_dev,
                        step->workspace_bytes, prefill, stream);
+    if (rc) return rc;
+  }
+  if (trees) {
+    rc = tree_attention(&step->pool, layer, &more->tree_table, &q, &out, step->num_qo_heads,
+                        step->sm_scale, more->tree_plan_dev, &more->tree_info,
+                        step->workspace_dev, step->workspace_bytes, tree, stream);
     if (rc) return rc;
   }
   if (weighted) {

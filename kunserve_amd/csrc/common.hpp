@@ -102,6 +102,13 @@ int shared_decode(const kunserve_kv_pool* pool, int32_t layer, const kunserve_pa
                   const kunserve_shared_plan_info* info, void* workspace_dev,
                   int64_t workspace_bytes, const StepFusion& fusion, kunserve_stream_t stream);
 
+// The same for a tree plan (kunserve_tree_attention); of `fusion` the append.
+int tree_attention(const kunserve_kv_pool* pool, int32_t layer, const kunserve_page_table* table,
+                   const kunserve_tensor3* q, kunserve_tensor3* out, int32_t num_qo_heads,
+                   float sm_scale, const int32_t* plan_dev, const kunserve_tree_plan_info* info,
+                   void* workspace_dev, int64_t workspace_bytes, const StepFusion& fusion,
+                   kunserve_stream_t stream);
+
 // The attention weights of a step's decode rows from the scores that their decode
 // launch left in the plan's workspace (weights_scores says where).
 void weights_scores(const kunserve_weights_plan_info* info, const int32_t* plan_dev,

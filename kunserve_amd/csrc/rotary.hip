@@ -3,7 +3,8 @@
 // 298-312; the append's slots kunserve/request.py:447-462).
 //
 // Token i of the step, at position p, has each rotated pair (a, b) of its q
-// and k heads turned by the angle p * freq[j] and scaled:
+// and k heads turned by the angle p * freq[j] (with axes, p its position on the
+// pair's axis) and scaled:
 //   a' = scale * (a cos - b sin),  b' = scale * (b cos + a sin).
 // The first rotary_dim dims of a head are rotated, pair j being dims (j, j +
 // rotary_dim / 2) or (2j, 2j + 1); the others pass. The angle is formed in 64
@@ -37,7 +38,10 @@ struct RotaryArgs {
   const int32_t* indices;
   const int32_t* kv_len;
   const int32_t* q_indptr;
-  const int32_t* positions;   // null, or [num_tokens]
+  const int32_t* positions;   // null, or [num_tokens]; with axes [num_axes][position_stride]
+  const int32_t* axis;        // null, or [rotary_dim / 2]: the axis of each pair
+  int32_t num_axes;
+  int64_t position_stride;
   const double* freq;         // [rotary_dim / 2], radians per position
   float scale;
   int32_t num_seqs;
@@ -65,7 +69,12 @@ __global__ __launch_bounds__(kThreads) void rotary_append_kernel(RotaryArgs a) {
   const int pos = a.positions ? a.positions[tok] : at;
   const int half = a.rotary_dim / 2;
   for (int j = threadIdx.x; j < half; j += kThreads) {
-    const double turns = double(pos) * a.freq[j] * 0.15915494309189535;   // 1 / 2 pi
+    int at_axis = pos;
+    if (a.axis) {
+      const int x = a.axis[j];
+      at_axis = a.positions[(x > 0 && x < a.num_axes ? x : 0) * a.position_stride + tok];
+    }
+    const double turns = double(at_axis) * a.freq[j] * 0.15915494309189535;   // 1 / 2 pi
     float s, c;
     sincospif(2.f * float(turns - rint(turns)), &s, &c);
     s_cos[j] = c * a.scale;
@@ -144,6 +153,22 @@ extern "C" int kunserve_rotary_append_kv(const kunserve_kv_pool* pool, int32_t l
                                          const kunserve_rotary* rotary,
                                          const int32_t* positions_dev,
                                          kunserve_stream_t stream) {
+  return kunserve_rotary_axes_append_kv(pool, layer, table, q_indptr_dev, num_tokens, q, q_out,
+                                        num_qo_heads, k_new, v_new, rotary, nullptr,
+                                        positions_dev, stream);
+}
+
+extern "C" int kunserve_rotary_axes_append_kv(const kunserve_kv_pool* pool, int32_t layer,
+                                              const kunserve_page_table* table,
+                                              const int32_t* q_indptr_dev, int32_t num_tokens,
+                                              const kunserve_tensor3* q, kunserve_tensor3* q_out,
+                                              int32_t num_qo_heads,
+                                              const kunserve_tensor3* k_new,
+                                              const kunserve_tensor3* v_new,
+                                              const kunserve_rotary* rotary,
+                                              const kunserve_rotary_axes* axes,
+                                              const int32_t* positions_dev,
+                                              kunserve_stream_t stream) {
   clear_error();
   int rc = check_pool(pool, true);
   if (rc) return rc;
@@ -160,7 +185,12 @@ extern "C" int kunserve_rotary_append_kv(const kunserve_kv_pool* pool, int32_t l
                 pool->head_dim);
   KSV_CHECK_ARG(std::isfinite(rotary->scale), "rotary scale %g is not finite",
                 double(rotary->scale));
+  KSV_CHECK_ARG(!axes || (axes->num_axes > 0 && (axes->position_stride == 0 ||
+                                                 axes->position_stride >= num_tokens)),
+                "%d axes with positions %lld apart", axes ? axes->num_axes : 0,
+                (long long)(axes ? axes->position_stride : 0));
   if (num_tokens == 0 || table->num_seqs == 0) return KUNSERVE_OK;
+  KSV_CHECK_ARG(!axes || (axes->axis_dev && positions_dev), "axes need the pairs' and positions");
   KSV_CHECK_ARG(q_indptr_dev && table->indptr_dev && table->indices_dev && table->kv_len_dev &&
                     rotary->freq_dev,
                 "null table array or frequencies");
@@ -211,6 +241,11 @@ extern "C" int kunserve_rotary_append_kv(const kunserve_kv_pool* pool, int32_t l
   a.kv_len = table->kv_len_dev;
   a.q_indptr = q_indptr_dev;
   a.positions = positions_dev;
+  if (axes) {
+    a.axis = axes->axis_dev;
+    a.num_axes = axes->num_axes;
+    a.position_stride = axes->position_stride;
+  }
   a.freq = rotary->freq_dev;
   a.scale = rotary->scale;
   a.num_seqs = table->num_seqs;

@@ -1,0 +1,279 @@
+// Cached tokens that change their place: of a row's tokens those that stay moved
+// together (kunserve_keep_tokens), and rows continued in pages of their own
+// (kunserve_copy_pages). The reference moves whole blocks alone
+// (LlamaOp.local_copy_blocks, kunserve/worker.py:818-823).
+//
+// Both are HBM-bound copies of 16-byte chunks: what moves is read and written once.
+#include "common.hpp"
+
+namespace kunserve {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kLoads = 8;   // 16-byte loads of a lane that are under way together
+
+struct KeepArgs {
+  f16* k;
+  f16* v;
+  int64_t page_stride, layer_stride, head_stride, token_stride;
+  float* w;   // null, or the tokens' weights
+  int64_t w_page, w_layer, w_head;
+  const int32_t* indptr;
+  const int32_t* indices;
+  const int32_t* kv_len;
+  const int32_t* first;
+  const int32_t* kept;
+  int64_t kept_stride;
+  int32_t max_kept;
+  int32_t num_pages;
+  int32_t page_shift;
+  int32_t num_layers;
+  int32_t num_heads;
+  int64_t num_slabs;   // rows x K and V x layers x heads
+};
+
+// A slab is a row's tokens of one layer, KV head and K or V. It moves chunk by chunk:
+// slots [c, c + n) are written after the tokens kept[c], .. kept[c + n - 1] have been
+// read, by one wave (W 1) or by a workgroup that meets between. A token moves down
+// (kept[j] > j), so what a later chunk reads no earlier one has written.
+template <int D, int W>
+__global__ __launch_bounds__(kThreads) void keep_tokens_kernel(KeepArgs a) {
+  constexpr int CH = D / 8;
+  constexpr int TPL = kWave / CH;                 // tokens of a load
+  constexpr int CHUNK = kLoads * TPL * W;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  const int64_t slab = W == 1 ? int64_t(blockIdx.x) * kWaves + wave : blockIdx.x;
+  if (slab >= a.num_slabs) return;   // uniform in a wave; no barrier where W is 1
+  const int head = int(slab % a.num_heads);
+  const int64_t rest = slab / a.num_heads;
+  const int layer = int(rest % a.num_layers);
+  const bool of_v = rest / a.num_layers & 1;
+  const int b = int(rest / a.num_layers >> 1);
+  const int lrow = lane / CH, lcol = lane % CH;
+
+  const int first = a.first[b], len = a.kv_len[b] - first;
+  if (first < 0 || len <= 1) return;   // uniform
+  const int32_t* pages = a.indices + a.indptr[b];
+  const int32_t* kept = a.kept + int64_t(b) * a.kept_stride;
+  const int mask = (1 << a.page_shift) - 1;
+  f16* base = (of_v ? a.v : a.k) + int64_t(layer) * a.layer_stride + int64_t(head) * a.head_stride +
+              8 * lcol;
+  float* weights = a.w && !of_v && lcol == 0
+                       ? a.w + int64_t(layer) * a.w_layer + int64_t(head) * a.w_head
+                       : nullptr;
+
+  const int n = min(a.max_kept, len);
+  for (int c = 0; c < n; c += CHUNK) {
+    int from[kLoads], src[kLoads], dst[kLoads];
+    f16x8 x[kLoads];
+    float w[kLoads];
+    auto place = [&](int i) { return c + ((W == 1 ? 0 : wave) + W * i) * TPL + lrow; };
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int j = place(i);
+      from[i] = j < n ? kept[j] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const bool moves = from[i] > place(i) && from[i] < len;
+      src[i] = moves ? pages[(first + from[i]) >> a.page_shift] : -1;
+      dst[i] = moves ? pages[(first + place(i)) >> a.page_shift] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const bool ok = src[i] >= 0 && src[i] < a.num_pages;
+      const int slot = (first + from[i]) & mask;
+      x[i] = ok ? load_f16x8(base + int64_t(src[i]) * a.page_stride + int64_t(slot) * a.token_stride)
+                : f16x8{};
+      if (a.w) w[i] = ok && weights ? weights[int64_t(src[i]) * a.w_page + slot] : 0.f;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // read before any of it is overwritten
+    if constexpr (W > 1) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      if (dst[i] < 0 || dst[i] >= a.num_pages) continue;
+      const int slot = (first + place(i)) & mask;
+      store_f16x8(base + int64_t(dst[i]) * a.page_stride + int64_t(slot) * a.token_stride, x[i]);
+      if (weights) weights[int64_t(dst[i]) * a.w_page + slot] = w[i];
+    }
+  }
+}
+
+struct CopyArgs {
+  f16* k;
+  f16* v;
+  int64_t page_stride, layer_stride, head_stride, token_stride;
+  float* w;
+  int64_t w_page, w_layer, w_head;
+  const int32_t* moves;   // [n][3]: source page, destination page, tokens
+  int32_t num_pages;
+  int32_t page_size;
+  int32_t num_heads;
+  int32_t heads;          // heads of a workgroup
+};
+
+// Workgroup (move, layer and K or V, head group): the waves take the loads of its heads'
+// tokens in turn.
+template <int D>
+__global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyArgs a) {
+  constexpr int CH = D / 8;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  const int32_t* m = a.moves + 3 * int64_t(blockIdx.x);
+  const int from = m[0], to = m[1], tokens = min(m[2], a.page_size);
+  if (from < 0 || from >= a.num_pages || to < 0 || to >= a.num_pages || tokens <= 0) return;
+  const int layer = int(blockIdx.y) >> 1;
+  const bool of_v = blockIdx.y & 1;
+  const int h0 = int(blockIdx.z) * a.heads, nh = min(a.heads, a.num_heads - h0);
+  f16* base = (of_v ? a.v : a.k) + int64_t(layer) * a.layer_stride;
+  const f16* src = base + int64_t(from) * a.page_stride;
+  f16* dst = base + int64_t(to) * a.page_stride;
+  const int per_head = (tokens * CH + kWave - 1) / kWave, total = per_head * nh;   // uniform
+  for (int at = wave; at < total; at += kWaves * kLoads) {
+    u32x4 x[kLoads];
+    int64_t off[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int l = at + i * kWaves, h = l / per_head;   // uniform
+      const int unit = (l - h * per_head) * kWave + lane;
+      const bool in = l < total && unit < tokens * CH;
+      off[i] = in ? int64_t(h0 + h) * a.head_stride + int64_t(unit / CH) * a.token_stride + 8 * (unit % CH)
+                  : -1;
+      if (in) x[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + off[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      if (off[i] >= 0) __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4*>(dst + off[i]));
+  }
+  if (a.w && !of_v) {
+    float* w = a.w + int64_t(layer) * a.w_layer;
+    for (int u = threadIdx.x; u < nh * a.page_size; u += kThreads) {
+      const int h = h0 + u / a.page_size, t = u % a.page_size;
+      if (t < tokens)
+        w[int64_t(to) * a.w_page + int64_t(h) * a.w_head + t] =
+            w[int64_t(from) * a.w_page + int64_t(h) * a.w_head + t];
+    }
+  }
+}
+
+}  // namespace
+}  // namespace kunserve
+
+using namespace kunserve;
+
+extern "C" int kunserve_keep_tokens(const kunserve_kv_pool* pool,
+                                    const kunserve_kv_weights* weights,
+                                    const kunserve_page_table* table, const int32_t* first_dev,
+                                    const int32_t* kept_dev, int64_t kept_stride,
+                                    int32_t max_kept, kunserve_stream_t stream) {
+  clear_error();
+  int rc = check_pool(pool, true);
+  if (rc) return rc;
+  if (weights) {
+    rc = check_weights(weights, pool);
+    if (rc) return rc;
+  }
+  KSV_CHECK_ARG(table && table->num_seqs >= 0, "null table or num_seqs < 0");
+  KSV_CHECK_ARG(max_kept >= 0 && kept_stride >= max_kept, "kept rows of %lld hold %d entries",
+                (long long)kept_stride, max_kept);
+  if (table->num_seqs == 0 || max_kept == 0) return KUNSERVE_OK;
+  KSV_CHECK_ARG(table->indptr_dev && table->indices_dev && table->kv_len_dev && first_dev && kept_dev,
+                "null table array, first or kept");
+  KeepArgs a{};
+  a.k = static_cast<f16*>(pool->k);
+  a.v = static_cast<f16*>(pool->v);
+  a.page_stride = pool->page_stride;
+  a.layer_stride = pool->layer_stride;
+  a.head_stride = pool->head_stride;
+  a.token_stride = pool->token_stride;
+  if (weights) {
+    a.w = weights->w;
+    a.w_page = weights->page_stride;
+    a.w_layer = weights->layer_stride;
+    a.w_head = weights->head_stride;
+  }
+  a.indptr = table->indptr_dev;
+  a.indices = table->indices_dev;
+  a.kv_len = table->kv_len_dev;
+  a.first = first_dev;
+  a.kept = kept_dev;
+  a.kept_stride = kept_stride;
+  a.max_kept = max_kept;
+  a.num_pages = int32_t(pool->num_pages);
+  a.page_shift = __builtin_ctz(pool->page_size);
+  a.num_layers = pool->num_layers;
+  a.num_heads = pool->num_kv_heads;
+  a.num_slabs = 2 * int64_t(table->num_seqs) * pool->num_layers * pool->num_kv_heads;
+  // A wave to a slab where its chunk holds the list: no barrier, and four slabs to a
+  // workgroup.
+  const int chunk = kLoads * kWave / (pool->head_dim / 8);
+  const bool small = max_kept <= chunk;
+  const int64_t blocks = small ? (a.num_slabs + kWaves - 1) / kWaves : a.num_slabs;
+  KSV_CHECK_ARG(blocks < (int64_t(1) << 31), "grid of %lld workgroups is too large",
+                (long long)blocks);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  switch (pool->head_dim) {
+    case 64:
+      if (small) keep_tokens_kernel<64, 1><<<grid, kThreads, 0, s>>>(a);
+      else keep_tokens_kernel<64, kWaves><<<grid, kThreads, 0, s>>>(a);
+      break;
+    case 128:
+      if (small) keep_tokens_kernel<128, 1><<<grid, kThreads, 0, s>>>(a);
+      else keep_tokens_kernel<128, kWaves><<<grid, kThreads, 0, s>>>(a);
+      break;
+    default:
+      if (small) keep_tokens_kernel<256, 1><<<grid, kThreads, 0, s>>>(a);
+      else keep_tokens_kernel<256, kWaves><<<grid, kThreads, 0, s>>>(a);
+  }
+  KSV_CHECK_LAUNCH();
+  return KUNSERVE_OK;
+}
+
+extern "C" int kunserve_copy_pages(const kunserve_kv_pool* pool, const kunserve_kv_weights* weights,
+                                   const int32_t* moves_dev, int64_t n, kunserve_stream_t stream) {
+  clear_error();
+  int rc = check_pool(pool, true);
+  if (rc) return rc;
+  if (weights) {
+    rc = check_weights(weights, pool);
+    if (rc) return rc;
+  }
+  KSV_CHECK_ARG(n >= 0 && n < (int64_t(1) << 31), "%lld moves", (long long)n);
+  if (n == 0) return KUNSERVE_OK;
+  KSV_CHECK_ARG(moves_dev, "null moves");
+  KSV_CHECK_ARG(pool->num_layers < 32768 && pool->num_kv_heads < 65536,
+                "%d layers of %d heads are too many", pool->num_layers, pool->num_kv_heads);
+  CopyArgs a{};
+  a.k = static_cast<f16*>(pool->k);
+  a.v = static_cast<f16*>(pool->v);
+  a.page_stride = pool->page_stride;
+  a.layer_stride = pool->layer_stride;
+  a.head_stride = pool->head_stride;
+  a.token_stride = pool->token_stride;
+  if (weights) {
+    a.w = weights->w;
+    a.w_page = weights->page_stride;
+    a.w_layer = weights->layer_stride;
+    a.w_head = weights->head_stride;
+  }
+  a.moves = moves_dev;
+  a.num_pages = int32_t(pool->num_pages);
+  a.page_size = pool->page_size;
+  a.num_heads = pool->num_kv_heads;
+  // Heads of a workgroup: about 64 loads, two rounds of its waves.
+  const int64_t per_head = (int64_t(pool->page_size) * (pool->head_dim / 8) + kWave - 1) / kWave;
+  a.heads = int32_t(per_head >= 64 ? 1 : 64 / per_head);
+  const dim3 grid(unsigned(n), unsigned(2 * pool->num_layers),
+                  unsigned((pool->num_kv_heads + a.heads - 1) / a.heads));
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  switch (pool->head_dim) {
+    case 64: copy_pages_kernel<64><<<grid, kThreads, 0, s>>>(a); break;
+    case 128: copy_pages_kernel<128><<<grid, kThreads, 0, s>>>(a); break;
+    default: copy_pages_kernel<256><<<grid, kThreads, 0, s>>>(a);
+  }
+  KSV_CHECK_LAUNCH();
+  return KUNSERVE_OK;
+}

@@ -1,0 +1,450 @@
+// Attention of drafted trees of tokens: a row's new tokens are the nodes of a tree
+// (guesses of what follows its cache, verified in one step), of which each sees the
+// row's cached tokens before them, its ancestors and itself. The reference decodes one
+// token of a row in a step (kunserve/request.py:654-670).
+//
+//   o[i, h] = sum_t p[i, h, t] V[t, g],  p = softmax over t of (q[i, h] . K[t, g]) * scale,
+//   t in the P cached tokens and {P + j : j an ancestor of i, or i}
+//
+// The (token, query head of a KV head) pairs of a row are the columns of a workgroup's
+// products: column c is token c / ratio, head g ratio + c % ratio. K and V of the cached
+// tokens are read once for all of them; the drafted tokens, whose mask is a bit per
+// (token, drafted token), follow in rounds of their own, and with the step's new k
+// and v their rows are read from there and written into their pages. Rows are split
+// into runs of rounds where there is less to do than CUs; the partials are joined
+// as those of decode rows are.
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "decode_tile.hpp"
+
+namespace kunserve {
+namespace {
+
+constexpr int kTreeRecord = 16;   // ints of a work record
+constexpr int kBlock = 32;        // tokens of a score tile
+
+// A round is what the four waves load at a time: a DecodeTile step each. Its tokens
+// are `BLOCKS` score tiles. Element x of half h of a tile's scores (32x32: lane
+// column, register x, lane half h) is token element e = x % 8 of lane group g =
+// 2 (x / 8) + h; a lane group's 8 tokens are those that one lane of a load has.
+template <int D>
+struct TreeTile : DecodeTile<D> {
+  static constexpr int ROUND = kWaves * DecodeTile<D>::STEP;
+  static constexpr int BLOCKS = ROUND / kBlock;
+};
+// The place of a round's token u among the bits of a mask: (tile, bit).
+inline void mask_bit(int head_dim, int u, int* tile, int* bit) {
+  const int tpl = kWave / (head_dim / 8), step = 8 * tpl;   // DecodeTile's
+  const int wave = u / step, v = u % step, e = v / tpl, l = v % tpl;   // l: lane row
+  const int group = head_dim == 64 ? l & 3 : head_dim == 128 ? l : 2 * (wave & 1) + l;
+  *tile = head_dim == 64 ? 2 * wave + (l >> 2) : head_dim == 128 ? wave : wave >> 1;
+  *bit = 16 * (group & 1) + 8 * (group >> 1) + e;
+}
+inline int round_tokens(int head_dim) { return 4 * 8 * kWave / (head_dim / 8); }
+
+struct TreeArgs {
+  DecodeArgs d;               // q, out, the pool, partials (work, group: unused)
+  const int32_t* records;     // [num_work][kTreeRecord], as TreeItem has them
+  const uint32_t* masks;      // [rows][T][rounds][BLOCKS]
+};
+
+// A work record: columns [c0, c0 + cols) of a row and KV head over rounds [rb, re) of
+// its tokens: `np` rounds of cached ones, then those of the drafted ones.
+struct TreeItem {
+  int tokens;    // drafted tokens of the row; 0: padding
+  int q_first;   // its first in q and out
+  int prefix;    // cached tokens before them
+  int page_at;   // where the row's pages start
+  int c0, cols, head;
+  int np, rb, re;
+  int slot, parts, part;   // slot of the row's first partial (-1: none), of how many, which
+  int mask_at, mask_words; // the row's masks, words of a token's
+};
+__device__ __forceinline__ TreeItem tree_item(const int32_t* r) {
+  return {r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7], r[8], r[9], r[10], r[11], r[12], r[13], r[14]};
+}
+
+// A column's attention over the tokens [lo, hi) of every round of the item, in fp32 on
+// the vector units, a load at a time (wave_rows, with the tree's mask). Masked tokens
+// leave nothing, whatever K and V hold there.
+template <typename T, int D>
+__device__ __forceinline__ void tree_column(const TreeArgs& ta, const TreeItem& it, int c, int lo,
+                                            int hi, float& m, float& l, float (&acc)[8]) {
+  typedef TreeTile<D> L;
+  const DecodeArgs& a = ta.d;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int lrow = lane / L::CH, lcol = lane % L::CH;
+  const int token = c / a.ratio, hq = it.head * a.ratio + c % a.ratio;
+  const auto q = load_v8<T>(a.q + int64_t(it.q_first + token) * a.q_tok + int64_t(hq) * a.q_head +
+                            8 * lcol);
+  const int64_t head = int64_t(it.head) * a.head_stride + 8 * lcol;
+  const uint32_t* mask = ta.masks + it.mask_at + int64_t(token) * it.mask_words;
+  m = kNegBig;
+  l = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  for (int r = it.rb; r < it.re; ++r) {
+    const bool drafted = r >= it.np;
+    const int t0 = (drafted ? r - it.np : r) * L::ROUND;
+    const int end = min(drafted ? it.tokens : it.prefix, t0 + hi);
+#pragma unroll 1
+    for (int u0 = t0 + lo; u0 < end; u0 += L::TPL) {
+      const int u = u0 + lrow, pos = drafted ? it.prefix + u : u;
+      bool seen = u < end;
+      if (seen && drafted) {
+        const int v = u - t0, wave = v / L::STEP, e = v % L::STEP / L::TPL, row = v % L::TPL;
+        const int group = D == 64 ? row & 3 : D == 128 ? row : 2 * (wave & 1) + row;
+        const int tile = D == 64 ? 2 * wave + (row >> 2) : D == 128 ? wave : wave >> 1;
+        seen = mask[(r - it.np) * L::BLOCKS + tile] >> (16 * (group & 1) + 8 * (group >> 1) + e) & 1;
+      }
+      int p = -1;
+      if (seen) {
+        p = a.indices[it.page_at + (pos >> a.page_shift)];
+        seen = p >= 0 && p < a.num_pages;
+      }
+      const f16* kp = g_zero_row + 8 * lcol;
+      const f16* vp = kp;
+      if (seen && drafted && a.k_new) {
+        kp = a.k_new + int64_t(it.q_first + u) * a.kn_tok + int64_t(it.head) * a.kn_head + 8 * lcol;
+        vp = a.v_new + int64_t(it.q_first + u) * a.vn_tok + int64_t(it.head) * a.vn_head + 8 * lcol;
+      } else if (seen) {
+        const int64_t off = head + int64_t(p) * a.page_stride +
+                            int64_t(pos & ((1 << a.page_shift) - 1)) * a.token_stride;
+        kp = a.k + off;
+        vp = a.v + off;
+      }
+      const auto k = load_v8<T>(kp);
+      const auto v = load_v8<T>(vp);
+      float s = group_sum<L::CH>(dot8(q, k, 0.f)) * a.scale_log2;
+      s = seen ? s : -INFINITY;
+      const float mx = fmaxf(m, s);
+      const float alpha = fast_exp2(m - mx), pr = fast_exp2(s - mx);
+      m = mx;
+      l = fmaf(l, alpha, pr);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = fmaf(pr, float(v[e]), acc[e] * alpha);
+    }
+  }
+#pragma unroll
+  for (int off = L::CH; off < kWave; off <<= 1) {
+    const float m2 = __shfl_xor(m, off), l2 = __shfl_xor(l, off);
+    const float mx = fmaxf(m, m2);
+    const float f1 = fast_exp2(m - mx), f2 = fast_exp2(m2 - mx);
+    m = mx;
+    l = l * f1 + l2 * f2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = acc[e] * f1 + __shfl_xor(acc[e], off) * f2;
+  }
+}
+
+// Where a column's result goes: a partial (fp32) or out.
+__device__ __forceinline__ int64_t part_row(const TreeArgs& ta, const TreeItem& it, int c) {
+  return int64_t(it.slot + c / ta.d.ratio * it.parts + it.part) * ta.d.num_qo_heads +
+         it.head * ta.d.ratio + c % ta.d.ratio;
+}
+
+// The drafted rows of the item's rounds whose first column is one of its own, into
+// their pages.
+template <int D>
+__device__ __forceinline__ void append_rows(const TreeArgs& ta, const TreeItem& it) {
+  typedef TreeTile<D> L;
+  const DecodeArgs& a = ta.d;
+  const int lo = max((max(it.rb, it.np) - it.np) * L::ROUND, (it.c0 + a.ratio - 1) / a.ratio);
+  const int hi = min(min(it.tokens, (it.re - it.np) * L::ROUND),
+                     (it.c0 + it.cols + a.ratio - 1) / a.ratio);
+  for (int i = threadIdx.x; i < (hi - lo) * 2 * L::CH; i += kThreads) {
+    const int u = lo + i / (2 * L::CH), of_v = i / L::CH & 1, c = i % L::CH;
+    const int pos = it.prefix + u;
+    const int p = a.indices[it.page_at + (pos >> a.page_shift)];
+    if (p < 0 || p >= a.num_pages) continue;
+    const f16* src = (of_v ? a.v_new + int64_t(it.q_first + u) * a.vn_tok + int64_t(it.head) * a.vn_head
+                           : a.k_new + int64_t(it.q_first + u) * a.kn_tok + int64_t(it.head) * a.kn_head);
+    f16* dst = const_cast<f16*>(of_v ? a.v : a.k) + int64_t(it.head) * a.head_stride +
+               int64_t(p) * a.page_stride + int64_t(pos & ((1 << a.page_shift) - 1)) * a.token_stride;
+    store_f16x8(dst + 8 * c, load_f16x8(src + 8 * c));
+  }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void tree_attention_kernel(TreeArgs ta) {
+  typedef TreeTile<D> L;
+  const DecodeArgs& a = ta.d;
+  const TreeItem it = tree_item(ta.records + kTreeRecord * int64_t(blockIdx.x));
+  if (it.tokens == 0) return;
+  if (a.k_new) append_rows<D>(ta, it);
+  const int lane = threadIdx.x & (kWave - 1);
+  const int lrow = lane / L::CH, lcol = lane % L::CH;
+  for (int i = int(threadIdx.x) >> 6; i < it.cols; i += kWaves) {
+    const int c = it.c0 + i;
+    float m, l, acc[8];
+    tree_column<T, D>(ta, it, c, 0, L::ROUND, m, l, acc);
+    if (lrow != 0) continue;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (it.slot < 0) {
+      T* op = reinterpret_cast<T*>(a.out) + int64_t(it.q_first + c / a.ratio) * a.o_tok +
+              int64_t(it.head * a.ratio + c % a.ratio) * a.o_head + 8 * lcol;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) op[e] = T(acc[e] * inv);
+    } else {
+      const int64_t row = part_row(ta, it, c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a.part_o[row * D + 8 * lcol + e] = acc[e] * inv;
+      if (lcol == 0) a.part_lse[row] = partial_lse(m, l);
+    }
+  }
+}
+
+template <typename T>
+int launch_tree(int head_dim, const TreeArgs& ta, unsigned blocks, hipStream_t s) {
+  switch (head_dim) {
+    case 64: tree_attention_kernel<T, 64><<<blocks, kThreads, 0, s>>>(ta); break;
+    case 128: tree_attention_kernel<T, 128><<<blocks, kThreads, 0, s>>>(ta); break;
+    default: tree_attention_kernel<T, 256><<<blocks, kThreads, 0, s>>>(ta);
+  }
+  KSV_CHECK_LAUNCH();
+  return KUNSERVE_OK;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Columns of a workgroup.
+constexpr int kMaxCols = 128;
+
+struct TreeRow {
+  int32_t tokens, q_first, prefix, page_at, mask_at, mask_words, np, rounds;
+};
+
+int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_first,
+              const int32_t* kv_len, const int32_t* parents, int32_t num_seqs,
+              int32_t num_qo_heads, int32_t num_kv_heads, int32_t page_size, int32_t head_dim,
+              int32_t num_cus, int32_t part_rounds, std::vector<int32_t>& plan,
+              kunserve_tree_plan_info* info) {
+  const int ratio = num_qo_heads / num_kv_heads;
+  const int round = round_tokens(head_dim), tiles = round / kBlock;
+  const int64_t cus = num_cus > 0 ? num_cus : 256;
+  std::vector<TreeRow> rows(num_seqs);
+  std::vector<uint32_t> masks;
+  int64_t work = 0;   // rounds of all workgroups
+  int32_t longest = 0;
+  for (int32_t b = 0; b < num_seqs; ++b) {
+    const int32_t n = q_indptr[b + 1] - q_indptr[b];
+    TreeRow& r = rows[b];
+    KSV_CHECK_ARG(n >= 0 && kv_len[b] >= n, "row %d: %d new tokens of %d", b, n, kv_len[b]);
+    KSV_CHECK_ARG(int64_t(indptr[b + 1]) - indptr[b] >= ceil_div(kv_len[b], page_size),
+                  "row %d: %lld pages for %d tokens", b, (long long)indptr[b + 1] - indptr[b],
+                  kv_len[b]);
+    r.tokens = n;
+    r.q_first = q_first ? q_first[b] : q_indptr[b];
+    r.prefix = kv_len[b] - n;
+    r.page_at = indptr[b];
+    r.np = int32_t(ceil_div(r.prefix, round));
+    r.rounds = r.np + int32_t(ceil_div(n, round));
+    r.mask_words = int32_t(ceil_div(n, round)) * tiles;
+    KSV_CHECK_ARG(int64_t(masks.size()) + int64_t(n) * r.mask_words < (int64_t(1) << 30),
+                  "trees of too many tokens");
+    r.mask_at = int32_t(masks.size());
+    masks.resize(masks.size() + size_t(n) * r.mask_words, 0u);
+    uint32_t* m = masks.data() + r.mask_at;
+    const int32_t* up = parents + q_indptr[b];
+    for (int32_t i = 0; i < n; ++i) {
+      KSV_CHECK_ARG(up[i] >= -1 && up[i] < i, "row %d: token %d has parent %d", b, i, up[i]);
+      uint32_t* own = m + size_t(i) * r.mask_words;
+      if (up[i] >= 0) std::copy_n(m + size_t(up[i]) * r.mask_words, r.mask_words, own);
+      int tile, bit;
+      mask_bit(head_dim, i % round, &tile, &bit);
+      own[i / round * tiles + tile] |= 1u << bit;
+    }
+    work += n ? int64_t(r.rounds) * ceil_div(int64_t(n) * ratio, kMaxCols) * num_kv_heads : 0;
+    if (n) longest = std::max(longest, r.rounds);
+  }
+  // A workgroup's run of rounds: what gives every CU two of them.
+  int64_t run = part_rounds > 0 ? part_rounds : std::max<int64_t>(1, ceil_div(work, 2 * cus));
+  run = std::min<int64_t>(run, std::max(longest, 1));
+
+  struct Piece {
+    int32_t row, part, rb, re;
+  };
+  std::vector<Piece> pieces;
+  std::vector<int32_t> merges, slot(num_seqs, -1), parts(num_seqs, 1);
+  int64_t slots = 0;
+  for (int32_t b = 0; b < num_seqs; ++b) {
+    const TreeRow& r = rows[b];
+    if (r.tokens == 0) continue;
+    parts[b] = int32_t(ceil_div(r.rounds, run));
+    const int32_t len = int32_t(ceil_div(r.rounds, parts[b]));
+    parts[b] = int32_t(ceil_div(r.rounds, len));
+    for (int32_t i = 0; i < parts[b]; ++i)
+      pieces.push_back({b, i, i * len, std::min(r.rounds, (i + 1) * len)});
+    if (parts[b] == 1) continue;
+    slot[b] = int32_t(slots);
+    for (int32_t i = 0; i < r.tokens; ++i, slots += parts[b])
+      merges.insert(merges.end(), {r.q_first + i, int32_t(slots), parts[b], 0});
+    KSV_CHECK_ARG(slots < (int64_t(1) << 31), "too many partial results");
+  }
+  // Longest first, to the XCD with least to do; the column tiles of a piece and KV
+  // head, which read the same K and V, one after the other on one XCD.
+  std::stable_sort(pieces.begin(), pieces.end(), [](const Piece& x, const Piece& y) {
+    return x.re - x.rb > y.re - y.rb;
+  });
+  std::vector<int32_t> lanes[kXcds];
+  int64_t load[kXcds] = {};
+  size_t depth = 0;
+  for (const Piece& p : pieces) {
+    const TreeRow& r = rows[p.row];
+    const int32_t cols = r.tokens * ratio;
+    for (int32_t h = 0; h < num_kv_heads; ++h) {
+      const int x = int(std::min_element(load, load + kXcds) - load);
+      for (int32_t c = 0; c < cols; c += kMaxCols) {
+        lanes[x].insert(lanes[x].end(),
+                        {r.tokens, r.q_first, r.prefix, r.page_at, c, std::min(kMaxCols, cols - c),
+                         h, r.np, p.rb, p.re, slot[p.row], parts[p.row], p.part, r.mask_at,
+                         r.mask_words, 0});
+        load[x] += p.re - p.rb;
+      }
+      depth = std::max(depth, lanes[x].size() / kTreeRecord);
+    }
+  }
+  for (size_t r = 0; r < depth; ++r)
+    for (int x = 0; x < kXcds; ++x)
+      for (int i = 0; i < kTreeRecord; ++i)
+        plan.push_back(kTreeRecord * r + i < lanes[x].size() ? lanes[x][kTreeRecord * r + i] : 0);
+  info->num_work = int32_t(kXcds * depth);
+  info->num_merge = int32_t(merges.size() / 4);
+  info->num_slots = int32_t(slots);
+  info->num_seqs = num_seqs;
+  info->head_dim = head_dim;
+  info->page_size = page_size;
+  info->num_qo_heads = num_qo_heads;
+  info->num_kv_heads = num_kv_heads;
+  plan.insert(plan.end(), merges.begin(), merges.end());
+  plan.insert(plan.end(), masks.begin(), masks.end());
+  KSV_CHECK_ARG(plan.size() < (size_t(1) << 31), "the plan is too long");
+  info->plan_ints = int32_t(plan.size());
+  return KUNSERVE_OK;
+}
+
+}  // namespace
+}  // namespace kunserve
+
+using namespace kunserve;
+
+extern "C" int64_t kunserve_tree_plan_bound(const int32_t* q_indptr_host,
+                                            const int32_t* kv_len_host, int32_t num_seqs,
+                                            int32_t num_qo_heads, int32_t num_kv_heads,
+                                            int32_t head_dim) {
+  if (num_seqs < 0 || num_qo_heads <= 0 || num_kv_heads <= 0 ||
+      (num_seqs > 0 && (!q_indptr_host || !kv_len_host)) ||
+      (head_dim != 64 && head_dim != 128 && head_dim != 256))
+    return -1;
+  const int64_t round = round_tokens(head_dim), ratio = ceil_div(num_qo_heads, num_kv_heads);
+  int64_t items = 0, rest = 0;
+  for (int32_t b = 0; b < num_seqs; ++b) {
+    const int64_t n = std::max<int64_t>(0, int64_t(q_indptr_host[b + 1]) - q_indptr_host[b]);
+    const int64_t rounds = ceil_div(std::max(kv_len_host[b], 0), round) + 1;
+    items += rounds * num_kv_heads * ceil_div(n * ratio, 32);
+    rest += n * (4 + ceil_div(n, round) * round / kBlock);
+  }
+  return kTreeRecord * kXcds * items + rest;
+}
+
+extern "C" int kunserve_tree_plan(const int32_t* indptr_host, const int32_t* q_indptr_host,
+                                  const int32_t* q_first_host, const int32_t* kv_len_host,
+                                  const int32_t* parents_host, int32_t num_seqs,
+                                  int32_t num_qo_heads, int32_t num_kv_heads, int32_t page_size,
+                                  int32_t head_dim, int32_t num_cus, int32_t part_rounds,
+                                  int32_t* plan_host, int64_t plan_capacity,
+                                  kunserve_tree_plan_info* info) {
+  clear_error();
+  KSV_CHECK_ARG(info && plan_host, "null plan buffer or info");
+  KSV_CHECK_ARG(num_seqs >= 0 && (num_seqs == 0 || (indptr_host && q_indptr_host && kv_len_host)),
+                "bad table or num_seqs");
+  KSV_CHECK_ARG(num_qo_heads > 0 && num_kv_heads > 0 && num_qo_heads % num_kv_heads == 0,
+                "num_qo_heads %d not a multiple of num_kv_heads %d", num_qo_heads, num_kv_heads);
+  KSV_CHECK_ARG(page_size >= kMinPageSize && (page_size & (page_size - 1)) == 0,
+                "page_size %d must be a power of two >= %d", page_size, kMinPageSize);
+  KSV_CHECK_ARG(part_rounds >= 0, "part_rounds %d is negative", part_rounds);
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) {
+    set_error("head_dim %d not compiled", head_dim);
+    return KUNSERVE_EUNSUPPORTED;
+  }
+  KSV_CHECK_ARG(num_seqs == 0 || q_indptr_host[0] == 0, "q_indptr starts at %d", q_indptr_host[0]);
+  KSV_CHECK_ARG(num_seqs == 0 || q_indptr_host[num_seqs] == 0 || parents_host, "null parents");
+  return no_throw([&] {
+    std::vector<int32_t> plan;
+    const int rc = tree_plan(indptr_host, q_indptr_host, q_first_host, kv_len_host, parents_host,
+                             num_seqs, num_qo_heads, num_kv_heads, page_size, head_dim, num_cus,
+                             part_rounds, plan, info);
+    if (rc) return rc;
+    if (int64_t(plan.size()) > plan_capacity) {
+      set_error("plan needs %lld ints, capacity %lld", (long long)plan.size(),
+                (long long)plan_capacity);
+      return int(KUNSERVE_ENOSPC);
+    }
+    std::copy(plan.begin(), plan.end(), plan_host);
+    return int(KUNSERVE_OK);
+  });
+}
+
+extern "C" int64_t kunserve_tree_workspace_bytes(const kunserve_tree_plan_info* info) {
+  if (!info) return -1;
+  return int64_t(info->num_slots) * info->num_qo_heads * (info->head_dim + 1) * 4;
+}
+
+int kunserve::tree_attention(const kunserve_kv_pool* pool, int32_t layer,
+                             const kunserve_page_table* table, const kunserve_tensor3* q,
+                             kunserve_tensor3* out, int32_t num_qo_heads, float sm_scale,
+                             const int32_t* plan_dev, const kunserve_tree_plan_info* info,
+                             void* workspace_dev, int64_t workspace_bytes,
+                             const StepFusion& fusion, kunserve_stream_t stream) {
+  clear_error();
+  KSV_CHECK_ARG(pool && table && q && out && info, "null argument");
+  KSV_CHECK_ARG(info->head_dim == pool->head_dim, "plan made for head_dim %d, pool has %d",
+                info->head_dim, pool->head_dim);
+  KSV_CHECK_ARG(info->page_size == pool->page_size, "plan made for pages of %d, pool has %d",
+                info->page_size, pool->page_size);
+  KSV_CHECK_ARG(info->num_qo_heads == num_qo_heads && info->num_kv_heads == pool->num_kv_heads,
+                "plan made for %d query heads on %d, not %d on %d", info->num_qo_heads,
+                info->num_kv_heads, num_qo_heads, pool->num_kv_heads);
+  KSV_CHECK_ARG(info->num_seqs == table->num_seqs, "plan made for %d rows, not %d", info->num_seqs,
+                table->num_seqs);
+  KSV_CHECK_ARG(num_qo_heads < 65536, "%d query heads: at most 65535", num_qo_heads);
+  // The launch's arguments and the joining of its partials are the decode launch's.
+  kunserve_decode_plan_info parts{};
+  parts.num_work = info->num_work;
+  parts.num_merge = info->num_merge;
+  parts.num_slots = info->num_slots;
+  parts.group_size = decode_group(num_qo_heads, std::max(pool->num_kv_heads, 1));
+  TreeArgs ta{};
+  StepFusion append;
+  append.k_new = fusion.k_new;
+  append.v_new = fusion.v_new;
+  const int rc = decode_args(pool, layer, table, nullptr, q, out, num_qo_heads, sm_scale, plan_dev,
+                             &parts, workspace_dev, workspace_bytes, append, &ta.d);
+  if (rc || info->num_work == 0) return rc;
+  KSV_CHECK_ARG(aligned16(workspace_dev), "workspace must be 16-byte aligned");
+  KSV_CHECK_ARG(aligned16(out->data) && out->token_stride % 8 == 0 && out->head_stride % 8 == 0,
+                "out must be 16-byte aligned with strides that are multiples of 8");
+  ta.records = plan_dev;
+  const int32_t* merges = plan_dev + kTreeRecord * int64_t(info->num_work);
+  ta.masks = reinterpret_cast<const uint32_t*>(merges + 4 * int64_t(info->num_merge));
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const int err = pool->dtype == KUNSERVE_DTYPE_BF16
+                      ? launch_tree<bf16>(pool->head_dim, ta, unsigned(info->num_work), s)
+                      : launch_tree<f16>(pool->head_dim, ta, unsigned(info->num_work), s);
+  if (err) return err;
+  parts.num_work = 0;   // the records behind which its merges are
+  return decode_merge(pool, ta.d, &parts, merges, s);
+}
+
+extern "C" int kunserve_tree_attention(const kunserve_kv_pool* pool, int32_t layer,
+                                       const kunserve_page_table* table,
+                                       const kunserve_tensor3* q, kunserve_tensor3* out,
+                                       int32_t num_qo_heads, float sm_scale,
+                                       const int32_t* plan_dev,
+                                       const kunserve_tree_plan_info* info, void* workspace_dev,
+                                       int64_t workspace_bytes, kunserve_stream_t stream) {
+  return kunserve::tree_attention(pool, layer, table, q, out, num_qo_heads, sm_scale, plan_dev,
+                                  info, workspace_dev, workspace_bytes, StepFusion{}, stream);
+}

@@ -105,7 +105,8 @@ class LlamaOp:
                  share_prefixes: bool = False, weights: Optional[KVWeights] = None,
                  window: int = 16,
                  rope_positions: Optional[List[int]] = None,
-                 learn: bool = True) -> AttentionStep:
+                 learn: bool = True,
+                 trees: Optional[List[Optional[List[int]]]] = None) -> AttentionStep:
         """Prepares the attention stage of one step (kunserve/worker.py:270-312).
 
         Argument meanings follow kunserve/flash_backend.py:2448-2469. A layer
@@ -118,8 +119,8 @@ class LlamaOp:
         num_restore_requests = 0 (kunserve/flash_backend.py:2465).
         is_context_stage (not in the reference signature) gives the rows'
         real stages when use_tensor_cores hides them (kv_lens_for_step).
-        share_prefixes, weights, window, rope_positions and learn (not in it either)
-        are AttentionStep's.
+        share_prefixes, weights, window, rope_positions, learn and trees (not in it
+        either) are AttentionStep's.
         """
         if len(input_tokens_batched) != num_requests or len(pages_of_reqs) != num_requests:
             raise ValueError("num_requests does not match the per-row argument lists")
@@ -154,7 +155,7 @@ class LlamaOp:
                              is_context_stage=is_context_stage, layer_offset=offset,
                              id_map=id_map, num_ids=min(max_num_pages, num_ids),
                              share_prefixes=share_prefixes, weights=weights, window=window,
-                             rope_positions=rope_positions, learn=learn)
+                             rope_positions=rope_positions, learn=learn, trees=trees)
         step.layer_range = (local_layer_start, local_layer_end)
         return step
 

@@ -530,6 +530,97 @@ class PrefillPlan:
         return int(_lib.lib().kunserve_prefill_workspace_bytes(ctypes.byref(self.info)))
 
 
+_TREE_PLAN_INTS = 1 << 20   # 4 MiB
+
+
+class TreePlan:
+    """Plan of rows whose new tokens are drafted trees (kunserve_tree_plan), computed
+    on the host once per step and shared by every layer.
+
+    Row b's new tokens are the last len(parents[b]) of its kv_len; parents[b][i] is
+    the place of token i's parent among them, below i, or -1 for one that follows the
+    cached tokens. They are tokens q_first[b] onwards of q and out (default: one row
+    after the other). part_rounds: rounds of a piece of a row, 0 to choose."""
+
+    def __init__(self, table: "PageTable", parents: Sequence[Sequence[int]], num_qo_heads: int,
+                 num_kv_heads: int, page_size: int, device: torch.device,
+                 num_cus: Optional[int] = None, upload: bool = True, head_dim: int = 128,
+                 q_first: Optional[Sequence[int]] = None, part_rounds: int = 0):
+        n = table.num_seqs
+        if len(parents) != n:
+            raise ValueError(f"{n} rows but {len(parents)} trees")
+        q_indptr = np.zeros(n + 1, dtype=np.int64)
+        np.cumsum([len(p) for p in parents], out=q_indptr[1:])
+        tokens = int(q_indptr[-1])
+        up = np.empty(tokens, dtype=np.int32)
+        for b, p in enumerate(parents):
+            up[q_indptr[b]:q_indptr[b + 1]] = _tree(p, b)
+        qi = _i32(q_indptr)
+        first = qi[:-1] if q_first is None else _i32(q_first)
+        if first.shape != (n,) or np.any(first < 0):
+            raise ValueError(f"{n} rows need as many first tokens, 0 at least")
+        if n and int(table.indptr_host[-1]) > table.indices_host.size:
+            raise ValueError("the table's indptr runs past its indices")
+        kv = table.kv_len_host
+        kv_ptr = kv.ctypes.data if n else None
+        cap = int(_lib.lib().kunserve_tree_plan_bound(qi.ctypes.data, kv_ptr, n, num_qo_heads,
+                                                      num_kv_heads, head_dim))
+        self.info = _lib.TreePlanInfo()
+        # The bound holds for pieces of one round and is far above what plans use.
+        for size in (min(cap, _TREE_PLAN_INTS), cap):
+            buf = np.empty(max(size, 4), dtype=np.int32)   # the plan writes what it uses
+            try:
+                _lib.call("kunserve_tree_plan", table.indptr_host.ctypes.data, qi.ctypes.data,
+                          np.ascontiguousarray(first).ctypes.data, kv_ptr, up.ctypes.data, n,
+                          num_qo_heads, num_kv_heads, page_size, head_dim,
+                          num_cus if num_cus is not None else _num_cus(device), part_rounds,
+                          buf.ctypes.data, buf.size, ctypes.byref(self.info))
+                break
+            except _lib.KunserveError as e:
+                if e.code != _lib.ENOSPC or size >= cap:
+                    raise
+        self.plan_host = buf[: self.info.plan_ints].copy()
+        self.end = int((first + np.diff(q_indptr)).max(initial=0))   # tokens that q and out have
+        self.plan = None
+        if upload:
+            self.bind(_upload_packed(self.host_arrays(), device))
+        self.num_qo_heads = num_qo_heads
+        self.table = table
+
+    def host_arrays(self) -> list:
+        return [self.plan_host]
+
+    def bind(self, dev: Sequence[torch.Tensor]) -> None:
+        self.plan = dev[0] if self.info.plan_ints else None
+
+    def workspace_bytes(self) -> int:
+        return int(_lib.lib().kunserve_tree_workspace_bytes(ctypes.byref(self.info)))
+
+
+def _tree(parents: Sequence[int], row: int) -> np.ndarray:
+    """A row's tree as int32, checked."""
+    p = np.asarray(parents)
+    if p.ndim != 1 or (p.size and p.dtype.kind not in "iu"):
+        raise ValueError(f"row {row}: a tree is a list of whole numbers")
+    bad = (p < -1) | (p >= np.arange(p.size))
+    if np.any(bad):
+        i = int(np.argmax(bad))
+        raise ValueError(f"row {row}: drafted token {i} has parent {int(p[i])}, which is neither "
+                         "-1 nor a token before it")
+    return p.astype(np.int32)
+
+
+def tree_depths(parents: Sequence[int]) -> np.ndarray:
+    """How many drafted ancestors each token of a tree has: a token's place in its
+    sequence is the cached tokens' number and this."""
+    up = _tree(parents, 0).astype(np.int64)
+    depth = (up >= 0).astype(np.int64)
+    while np.any(up >= 0):   # ancestors 1, 2, 4, .. away
+        depth += np.where(up >= 0, depth[up], 0)
+        up = np.where(up >= 0, up[up], -1)
+    return depth
+
+
 # ------------------------------------------------------------------ ops
 
 
@@ -666,8 +757,8 @@ def rotary_append_kv(pool: KVPool, layer: int, table: PageTable, q_indptr: torch
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The attention prologue of one layer with a Rotary: q and k_new rotated, the
     rotated k and v_new written into their pages. positions (device int32
-    [num_tokens]): the tokens' rotary positions, where they are not their places in
-    the cache. The rotated q goes to out (default: q, in place), which must be q
+    [num_tokens], or [axes, num_tokens] for a Rotary of several axes): the tokens'
+    rotary positions, where they are not their places in the cache. The rotated q goes to out (default: q, in place), which must be q
     or lie apart from q, k_new and v_new. Returns out."""
     q_shape, k_shape, device = q.shape, k_new.shape, pool.device
     tokens, dim, dtype = k_shape[0], pool.head_dim, pool.dtype
@@ -685,12 +776,25 @@ def rotary_append_kv(pool: KVPool, layer: int, table: PageTable, q_indptr: torch
         _check_reach(device, q=q, k_new=k_new, v_new=v_new, out=out)
     rotary.check(dim, device)
     _check_row_map(q_indptr, table.num_seqs + 1, device, "q_indptr")
-    _check_row_map(positions, tokens, device, "positions")
+    if positions is not None and positions.dim() == 2:
+        rotary.check_positions(positions)
+        _check_row_map(positions.view(-1) if positions.is_contiguous() else positions,
+                       rotary.num_axes * tokens, device, "positions")
+        if rotary.pair_axis is None:
+            positions = positions[0]
+    else:
+        _check_row_map(positions, tokens, device, "positions")
     if not q.dtype == k_new.dtype == v_new.dtype == out.dtype == dtype:
         pool.check_dtype(q, k_new, v_new, out)
     qd = _tensor3(q)
     od, kd, vd = qd if out is q else _tensor3(out), _tensor3(k_new), _tensor3(v_new)
     ref = ctypes.byref
+    axes = rotary.axes_desc(positions)
+    if axes is not None:
+        _lib.call("kunserve_rotary_axes_append_kv", pool.desc(), layer, table.desc(),
+                  q_indptr.data_ptr(), tokens, ref(qd), ref(od), q_shape[1], ref(kd), ref(vd),
+                  rotary.desc, ref(axes), positions.data_ptr(), _stream_ptr(device))
+        return out
     _lib.call("kunserve_rotary_append_kv", pool.desc(), layer, table.desc(), q_indptr.data_ptr(),
               tokens, ref(qd), ref(od), q_shape[1], ref(kd), ref(vd), rotary.desc,
               None if positions is None else positions.data_ptr(), _stream_ptr(device))
@@ -752,6 +856,40 @@ def _decode(entry: str, info, pool: KVPool, layer: int, table: PageTable, q: tor
     _lib.call(entry, pool.desc(), layer, table.desc(), _ptr(q_token),
               ctypes.byref(qd), ctypes.byref(od), hq, ctypes.c_float(scale),
               _ptr(plan.plan), ctypes.byref(info), _ptr(workspace),
+              0 if workspace is None else workspace.numel() * workspace.element_size(),
+              _stream_ptr(pool.device))
+    return out
+
+
+def tree_attention(pool: KVPool, layer: int, table: PageTable, q: torch.Tensor, plan: TreePlan,
+                   sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                   workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of drafted trees of tokens, on the plan made from their table: each
+    of the plan's tokens of q [num_tokens, Hq, D] sees its row's cached tokens before
+    them, its ancestors and itself, whose K and V are in the pages. Other tokens of
+    out are left as they are."""
+    if plan.table is not table:
+        raise ValueError("the plan was made from another table")
+    if q.shape[0] < plan.end:
+        raise ValueError(f"q has {q.shape[0]} tokens, the plan's rows end at {plan.end}")
+    if q.shape[2] != pool.head_dim:
+        raise ValueError(f"q shape {tuple(q.shape)} does not match head_dim {pool.head_dim}")
+    _check_reach(pool.device, q=q, out=out)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=pool.device)
+    if out.shape != q.shape:
+        raise ValueError(f"out shape {tuple(out.shape)} differs from q's {tuple(q.shape)}")
+    pool.check_dtype(q, out)
+    scale = sm_scale if sm_scale is not None else 1.0 / math.sqrt(pool.head_dim)
+    need = plan.workspace_bytes()
+    if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=pool.device)
+    if plan.info.plan_ints and plan.plan is None:
+        raise RuntimeError("tree plan used before its device array was bound")
+    qd, od = _tensor3(q), _tensor3(out)
+    _lib.call("kunserve_tree_attention", pool.desc(), layer, table.desc(), ctypes.byref(qd),
+              ctypes.byref(od), q.shape[1], ctypes.c_float(scale), _ptr(plan.plan),
+              ctypes.byref(plan.info), _ptr(workspace),
               0 if workspace is None else workspace.numel() * workspace.element_size(),
               _stream_ptr(pool.device))
     return out
@@ -826,8 +964,17 @@ class AttentionStep:
     (rows that share pages, in a pool whose weights others learn).
 
     rope_positions: for each row the rotary position of its first new token, where
-    that is not its place in the cache (rows shortened by evict). Only a Rotary
-    takes them.
+    that is not its place in the cache (rows shortened by evict), or an array [axes,
+    num_tokens] with every new token's position on each axis of a Rotary of several.
+    Only a Rotary takes them.
+
+    trees: for each row None, or the tree that its new tokens are (drafted tokens that
+    the step verifies): a list with the place of each token's parent among them, below
+    its own, or -1 for one that follows the row's cache. A token then sees the row's
+    cached tokens before them, its ancestors and itself, and is rotated behind its
+    ancestors, which only a Rotary does. Such a row is a prefill row: its first index
+    counts the tokens it has cached. keep_tokens keeps the accepted ones. Weights do
+    not learn from a step with trees (learn=False).
 
     All of the step's index arrays (tables, plans, row and token indices)
     reach the device in one copy on the current stream, with no host wait.
@@ -835,7 +982,10 @@ class AttentionStep:
 
     weights = None
     positions = None
+    tree = None
     _extras_ref = None
+    _more = None
+    _first = None
 
     def __init__(self, pool: KVPool, num_qo_heads: int, q_lens: Sequence[int],
                  first_token_indexes: Sequence[int], is_prefill_requests: Sequence[int],
@@ -845,7 +995,8 @@ class AttentionStep:
                  id_map: Optional[Callable[[np.ndarray], np.ndarray]] = None,
                  num_ids: Optional[int] = None, share_prefixes: bool = False,
                  share_min_bytes: Optional[int] = None, weights=None, window: int = 16,
-                 rope_positions: Optional[Sequence[int]] = None, learn: bool = True):
+                 rope_positions: Optional[Sequence[int]] = None, learn: bool = True,
+                 trees: Optional[Sequence[Optional[Sequence[int]]]] = None):
         self.pool = pool
         self.num_qo_heads = num_qo_heads
         self.layer_offset = layer_offset
@@ -856,9 +1007,12 @@ class AttentionStep:
         if np.any(q_lens < 1):
             raise ValueError("every row needs at least one input token")
         pages_per_row = [len(p) for p in pages_of_reqs]
-        is_decode = decode_rows(first_token_indexes, q_lens, is_prefill_requests,
-                                use_tensor_cores, is_context_stage, pages_per_row,
-                                pool.page_size)
+        drafted = _drafted_rows(trees, q_lens, is_prefill_requests, is_context_stage)
+        # (A tree says what its row is: not for decode_rows to find out.)
+        is_decode = decode_rows(first_token_indexes,
+                                q_lens if trees is None else np.where(drafted, 2, q_lens),
+                                is_prefill_requests, use_tensor_cores, is_context_stage,
+                                pages_per_row, pool.page_size)
         self.kv_len = _kv_lens(first_token_indexes, q_lens, is_decode)
         self.q_indptr_host = np.zeros(len(q_lens) + 1, dtype=np.int32)
         np.cumsum(q_lens, out=self.q_indptr_host[1:])
@@ -878,6 +1032,8 @@ class AttentionStep:
                 raise ValueError("learn=False is for a step with weights")
             weights, cleared = None, weights
         if weights is not None:
+            if drafted.any():
+                raise ValueError("weights do not learn from drafted trees: learn=False")
             if window < 1:
                 raise ValueError(f"window {window} must be positive")
             if not self.table.pages_private:
@@ -885,8 +1041,16 @@ class AttentionStep:
                                  "step's lists")
             self.weights = weights
         positions = None
-        if rope_positions is not None:
-            starts = np.asarray(rope_positions)
+        if np.ndim(rope_positions) == 2 and len(rope_positions) != 1:
+            positions = np.asarray(rope_positions)
+            if positions.shape[0] < 2 or positions.shape[1] != self.num_tokens:
+                raise ValueError(f"{self.num_tokens} tokens but {positions.shape} rope_positions")
+            if positions.size and positions.dtype.kind not in "iu":
+                raise ValueError("rope_positions must be whole numbers")
+            if positions.size and (positions.min() < 0 or positions.max() >= 2**31):
+                raise ValueError("rope_positions must lie in [0, 2^31)")
+        elif rope_positions is not None or drafted.any():
+            starts = np.asarray(self.kv_len - q_lens if rope_positions is None else rope_positions)
             if starts.shape != (n_rows,):
                 raise ValueError(f"{n_rows} rows but {starts.shape} rope_positions")
             if n_rows and starts.dtype.kind not in "iu":
@@ -894,6 +1058,9 @@ class AttentionStep:
             starts = starts.astype(np.int64)
             positions = np.repeat(starts - self.q_indptr_host[:-1], q_lens) + np.arange(
                 self.num_tokens)
+            for b in np.flatnonzero(drafted):
+                at = self.q_indptr_host[b]
+                positions[at:at + q_lens[b]] = starts[b] + tree_depths(trees[b])
             if np.any(starts < 0) or (positions.size and positions.max() >= 2**31):
                 raise ValueError("rope_positions must lie in [0, 2^31)")
 
@@ -901,7 +1068,8 @@ class AttentionStep:
         uploads = [[self.q_indptr_host], self.table]
         self.decode = self.prefill = None
         all_rows = np.arange(n_rows)
-        dec_rows, pre_rows = all_rows[is_decode], all_rows[~is_decode]
+        dec_rows, pre_rows = all_rows[is_decode], all_rows[~is_decode & ~drafted]
+        tree_rows = all_rows[drafted]
         # Row subsets take their rows from the step's CSR arrays (ids already
         # checked and mapped), not from the lists again.
         def sub_table(rows):
@@ -940,6 +1108,15 @@ class AttentionStep:
                                upload=False, head_dim=pool.head_dim)
             self.prefill = _Subset(pre_rows, tokens, table, None, plan)
             uploads += ([] if whole else [table, [tokens], [qi]]) + [plan]
+
+        if tree_rows.size:
+            table = self.table if tree_rows.size == n_rows else sub_table(tree_rows)
+            plan = TreePlan(table, [trees[b] for b in tree_rows], num_qo_heads, pool.num_kv_heads,
+                            pool.page_size, dev, upload=False, head_dim=pool.head_dim,
+                            q_first=self.q_indptr_host[tree_rows])
+            self.tree = _Subset(tree_rows, None, table, None, plan)
+            uploads += ([] if tree_rows.size == n_rows else [table]) + [plan]
+            uploads.append([self.kv_len - q_lens])   # keep_tokens' first places
 
         if positions is not None:
             uploads.append([positions])
@@ -989,11 +1166,14 @@ class AttentionStep:
                 self.prefill.q_indptr = next(rest)[0]
             else:
                 self.prefill.q_indptr = self.q_indptr
+        if tree_rows.size:
+            self._first = next(rest)[0]
         if positions is not None:
-            self.positions = next(rest)[0]
+            self.positions = next(rest)[0].view(positions.shape)
         # Scratch shared by every layer of the step (launches are serialised on one stream).
         ws = max(self.decode.plan.workspace_bytes(pool.head_dim) if self.decode else 0,
-                 self.prefill.plan.workspace_bytes() if self.prefill else 0)
+                 self.prefill.plan.workspace_bytes() if self.prefill else 0,
+                 self.tree.plan.workspace_bytes() if self.tree else 0)
         self.workspace = torch.empty(ws, dtype=torch.uint8, device=dev) if ws > 0 else None
         if weights is not None:
             self._weights_workspace = torch.empty(self._weights_plan.workspace_bytes(),
@@ -1006,6 +1186,7 @@ class AttentionStep:
         """The step as kunserve_attention_step takes it (every array it names
         is held by this object)."""
         d, p, t = self.decode, self.prefill, self.table
+        self._private = bool(appends)   # the new tokens' pages are in one place each
         n_dec, n_pre = self._num_counters
         counters = 0 if self.counters is None else self.counters.data_ptr()
         self._step = _lib.Step(
@@ -1034,6 +1215,9 @@ class AttentionStep:
                 self._extras.weights_workspace_bytes = self._weights_workspace.numel()
             self._extras.positions_dev = _ptr(self.positions)
             self._extras_ref = ctypes.byref(self._extras)
+        if self.tree is not None:
+            self._more = _lib.StepMore(self.tree.table._desc, _ptr(self.tree.plan.plan),
+                                       self.tree.plan.info)
         self._device = self.pool.device
         self._device_index = self._device.index   # a device tensor's is never None
         self._q_shape = (self.num_tokens, self.num_qo_heads, self.pool.head_dim)
@@ -1062,7 +1246,7 @@ class AttentionStep:
             inv_freq, interleave = rope   # exactly two
             interleave = int(bool(interleave))
             if self.positions is not None:
-                raise ValueError("rope_positions need a Rotary")
+                raise ValueError("trees and rope_positions need a Rotary")
         if out is None:
             out = torch.empty_like(q)
         qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
@@ -1077,13 +1261,20 @@ class AttentionStep:
                          and inv_freq.is_contiguous()))):
             # One native call for the layer.
             self.pool.desc()
+            more = self._more
             if rotary is not None:
                 rotary.check(self.pool.head_dim, self._device)
+                if rotary.num_axes > 1 or self.positions is not None:
+                    more = self._rotary_more(rotary)
             io = _lib.STEP_IO.pack(
                 q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
                 vs[1], out.data_ptr(), os[0], os[1],
                 0 if inv_freq is None else inv_freq.data_ptr(), interleave)
-            if rotary is None and self._extras_ref is None:
+            if more is not None:
+                _lib.call("kunserve_attention_step_more", self._step_ref, self._extras_ref,
+                          ctypes.byref(more), local, io, None if rotary is None else rotary.desc,
+                          _stream_ptr(self._device))
+            elif rotary is None and self._extras_ref is None:
                 _lib.call("kunserve_attention_step", self._step_ref, local, io,
                           _stream_ptr(self._device))
             else:
@@ -1119,6 +1310,9 @@ class AttentionStep:
             p = self.prefill
             paged_prefill(self.pool, local, p.table, p.q_indptr, q, p.plan, self.scale,
                           out=out, workspace=self.workspace, q_start=p.tokens)
+        if self.tree is not None:
+            tree_attention(self.pool, local, self.tree.table, q, self.tree.plan, self.scale,
+                           out=out, workspace=self.workspace)
         if self.weights is not None:
             # Every row through add_weights: these launches left no scores.
             plan = self.weights.plan(self.q_indptr_host, self.kv_len, self.num_qo_heads,
@@ -1126,3 +1320,54 @@ class AttentionStep:
             plan.bind(_upload_packed(plan.host_arrays(), self._device))
             self.weights.add(self.pool, local, self.table, self.q_indptr, q, plan, self.scale)
         return out
+
+    def _rotary_more(self, rotary: Rotary) -> Optional[_lib.StepMore]:
+        """What a layer with this rotary has beside the step: its axes, where the step
+        has positions on them."""
+        rotary.check_positions(self.positions)
+        axes = rotary.axes_desc(self.positions)
+        if axes is None:
+            return self._more
+        more = _lib.StepMore(axes=axes)
+        if self._more is not None:
+            more = _lib.StepMore(self._more.tree_table, self._more.tree_plan_dev,
+                                 self._more.tree_info, axes)
+        return more
+
+    def keep_tokens(self, kept, weights=None) -> None:
+        """Of each row's new tokens those at kept[b] stay, moved to the places behind
+        what the row had cached, in every layer and KV head of the pool: the accepted
+        path of a drafted tree. kept counts from the row's first new token, rising
+        (lists, or a device int32 tensor [rows, most kept] with -1 behind a row's last:
+        no host wait, and a graph capture takes it). weights (a KVWeights of the pool)
+        move along. The row goes on with its cached tokens and those kept. The pages of
+        new tokens must be in one place of the step's lists (ValueError)."""
+        from .token_moves import move_tokens
+
+        if not self._private:
+            raise ValueError("tokens move in place: their pages must be in one place of the "
+                             "step's lists")
+        first = self.kv_len - np.diff(self.q_indptr_host)
+        if self._first is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a step without trees uploads its rows' first places: not "
+                                   "under a capture")
+            self._first = _upload(_i32(first), self.pool.device)
+        move_tokens(self.pool, self.table, self._first, first, kept, weights)
+
+
+def _drafted_rows(trees, q_lens: np.ndarray, is_prefill_requests, is_context_stage) -> np.ndarray:
+    """Which rows have a tree, checked against their lengths and stages."""
+    if trees is None:
+        return np.zeros(len(q_lens), dtype=bool)
+    if len(trees) != len(q_lens):
+        raise ValueError(f"{len(q_lens)} rows but {len(trees)} trees")
+    drafted = np.array([t is not None for t in trees], dtype=bool)
+    for b in np.flatnonzero(drafted):
+        if len(trees[b]) != q_lens[b]:
+            raise ValueError(f"row {b}: {q_lens[b]} new tokens but a tree of {len(trees[b])}")
+        for stage in (is_prefill_requests, is_context_stage):
+            if stage is not None and not stage[b]:
+                raise ValueError(f"row {b}: a row with a tree is a prefill row, whose first index "
+                                 "counts its cached tokens")
+    return drafted

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Mapping, Optional
+from typing import Mapping, Optional, Sequence
 
 import numpy as np
 import torch
@@ -119,17 +119,44 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0,
     return f * (1.0 - slowed) + f / factor * slowed, scale
 
 
+def _pair_axes(pairs: int, sections: Optional[Sequence[int]],
+               axes: Optional[Sequence[int]]) -> Optional[np.ndarray]:
+    """The axis of every pair (int32), None where there is one."""
+    if sections is None and axes is None:
+        return None
+    if sections is not None and axes is not None:
+        raise ValueError("give sections or axes")
+    given = np.asarray(sections if axes is None else axes)
+    if given.ndim != 1 or given.size == 0 or given.dtype.kind not in "iu" or given.min() < 0:
+        raise ValueError("sections and axes are lists of whole numbers, 0 at least")
+    if axes is None:
+        if int(given.sum()) != pairs:
+            raise ValueError(f"sections of {int(given.sum())} pairs, the rotary has {pairs}")
+        return np.repeat(np.arange(given.size), given).astype(np.int32)
+    if given.size != pairs:
+        raise ValueError(f"the axes of {given.size} pairs, the rotary has {pairs}")
+    if int(given.max()) >= 1024:
+        raise ValueError("1024 axes at most")
+    return given.astype(np.int32)
+
+
 class Rotary:
     """Rotary embedding of the first rotary_dim dims of every head (a multiple of
     16): pairs (j, j + rotary_dim / 2), or (2j, 2j + 1) with interleave. Angles are
     formed in 64 bits, so they are exact at positions of any length.
 
     frequencies and scale replace those of rotary_frequencies(rotary_dim, theta,
-    scaling). Use: AttentionStep.run(rope=rotary), rotary_append_kv."""
+    scaling). Use: AttentionStep.run(rope=rotary), rotary_append_kv.
+
+    sections or axes: the tokens have a position on each of several axes (time, height
+    and width of an image), and a pair turns by that on its own. sections: how many
+    pairs each axis has, one axis' pairs after the other's; axes: the axis of every
+    pair."""
 
     def __init__(self, rotary_dim: int, theta: float = 10000.0, interleave: bool = False,
                  scaling: Optional[Mapping] = None, device="cuda", frequencies=None,
-                 scale: Optional[float] = None):
+                 scale: Optional[float] = None, sections: Optional[Sequence[int]] = None,
+                 axes: Optional[Sequence[int]] = None):
         if rotary_dim < 16 or rotary_dim % 16:
             raise ValueError(f"rotary_dim {rotary_dim} must be a positive multiple of 16")
         if frequencies is None:
@@ -145,11 +172,29 @@ class Rotary:
         self.scale = float(factor if scale is None else scale)
         if not math.isfinite(self.scale):
             raise ValueError(f"scale {self.scale} is not finite")
+        pair_axis = _pair_axes(rotary_dim // 2, sections, axes)
+        self.num_axes = 1 if pair_axis is None else int(pair_axis.max()) + 1
+        if sections is not None:
+            self.num_axes = len(sections)
+        self.pair_axis = None if pair_axis is None else torch.from_numpy(pair_axis).to(device)
         self.frequencies = torch.from_numpy(f).to(device)
         self.device = self.frequencies.device
         self._desc = _lib.Rotary(self.frequencies.data_ptr(), rotary_dim, int(self.interleave),
                                  self.scale)
         self.desc = ctypes.byref(self._desc)   # as the C entries take it
+
+    def axes_desc(self, positions: Optional[torch.Tensor]) -> Optional[_lib.RotaryAxes]:
+        """The axes as the C entries take them, for positions [tokens] (one for every
+        axis) or [axes, tokens]; None where there is one axis, or no positions."""
+        if self.pair_axis is None or positions is None:
+            return None
+        stride = positions.shape[1] if positions.dim() == 2 else 0
+        return _lib.RotaryAxes(self.pair_axis.data_ptr(), self.num_axes, stride)
+
+    def check_positions(self, positions: Optional[torch.Tensor]) -> None:
+        if positions is not None and positions.dim() == 2 and positions.shape[0] != self.num_axes:
+            raise ValueError(f"positions on {positions.shape[0]} axes, the rotary has "
+                             f"{self.num_axes}")
 
     def check(self, head_dim: int, device: torch.device) -> None:
         if self.rotary_dim > head_dim:

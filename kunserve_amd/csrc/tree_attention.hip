@@ -145,6 +145,21 @@ __device__ __forceinline__ int64_t part_row(const TreeArgs& ta, const TreeItem& 
          it.head * ta.d.ratio + c % ta.d.ratio;
 }
 
+// vt[e]: dim 8 chunk + e of the lane's 8 tokens.
+template <typename V8>
+__device__ __forceinline__ void tree_transpose8(const V8 (&v)[8], V8 (&vt)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    u32x4 d;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      d[x] = __builtin_amdgcn_perm(__builtin_bit_cast(u32x4, v[2 * x + 1])[e >> 1],
+                                   __builtin_bit_cast(u32x4, v[2 * x])[e >> 1],
+                                   (e & 1) ? 0x07060302u : 0x05040100u);
+    vt[e] = __builtin_bit_cast(V8, d);
+  }
+}
+
 // The drafted rows of the item's rounds whose first column is one of its own, into
 // their pages.
 template <int D>
@@ -167,50 +182,356 @@ __device__ __forceinline__ void append_rows(const TreeArgs& ta, const TreeItem& 
   }
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void tree_attention_kernel(TreeArgs ta) {
+// A workgroup has 32 WC columns: wave w takes those of tile w % WC and, of each round,
+// the tokens of its share w / WC of 4 / WC. All waves load: K goes to LDS by token rows, V
+// as the 8 tokens of a lane for each dim. S^T = K Q^T and O^T = V^T P^T on 32x32 tiles,
+// so that a column's scores are in the registers of its two lanes, where its
+// probabilities are the second product's operand.
+template <typename T, int D, int WC>
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_kernel(TreeArgs ta) {
+  typedef typename Vec<T>::v8 V8;
   typedef TreeTile<D> L;
+  constexpr int STEP = L::STEP, TPL = L::TPL, LOADS = L::LOADS, CH = L::CH;
+  constexpr int KS = D / 16;           // products of a score tile
+  constexpr int OT = D / 32;           // output tiles of a column tile
+  constexpr int WT = kWaves / WC;      // shares of a round's tokens
+  constexpr int GB = L::BLOCKS / WT;   // score tiles of a share
+  static_assert(GB >= 1, "a share has a tile at least");
+  constexpr int KBYTES = L::ROUND * D * 2;
   const DecodeArgs& a = ta.d;
+  __shared__ __attribute__((aligned(16))) char s_raw[2 * KBYTES];   // K, V; in the end O
+  __shared__ uint32_t s_drop[2 * kWaves];   // tokens of the round's tiles that nobody sees
+  __shared__ float s_ml[kWaves][2][kWave];
+
   const TreeItem it = tree_item(ta.records + kTreeRecord * int64_t(blockIdx.x));
   if (it.tokens == 0) return;
-  if (a.k_new) append_rows<D>(ta, it);
   const int lane = threadIdx.x & (kWave - 1);
-  const int lrow = lane / L::CH, lcol = lane % L::CH;
-  for (int i = int(threadIdx.x) >> 6; i < it.cols; i += kWaves) {
-    const int c = it.c0 + i;
-    float m, l, acc[8];
-    tree_column<T, D>(ta, it, c, 0, L::ROUND, m, l, acc);
-    if (lrow != 0) continue;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (it.slot < 0) {
-      T* op = reinterpret_cast<T*>(a.out) + int64_t(it.q_first + c / a.ratio) * a.o_tok +
-              int64_t(it.head * a.ratio + c % a.ratio) * a.o_head + 8 * lcol;
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  const int col = lane & 31, h = lane >> 5;   // column of a tile, half of its rows
+  const int lrow = lane / CH, lcol = lane % CH;
+  const int wc = wave % WC, wt = wave / WC;
+  const bool active = 32 * wc < it.cols;      // uniform
+  const int c = it.c0 + min(32 * wc + col, it.cols - 1);
+  const int token = int(uint32_t(c) / uint32_t(a.ratio));
+  const int hq = it.head * a.ratio + c - token * a.ratio;
+  const int page_mask = (1 << a.page_shift) - 1;
+
+  // ---- loads. A round's tokens of a wave are STEP; cached ones lie in pages whose ids a
+  // register's lanes hold, one for `granule` tokens, a round ahead of the loads.
+  const int gshift = min(a.page_shift, 4);
+  const bool two = TPL > 4 && a.page_shift < 3;   // a load's rows in two pages
+  const int last_page = max(it.prefix - 1, 0) >> a.page_shift;
+  auto ids_of = [&](int r) {
+    const int t = r * L::ROUND + wave * STEP + (lane << gshift);
+    return r < it.np ? a.indices[it.page_at + min(t >> a.page_shift, last_page)] : 0;
+  };
+  const int64_t head_at = int64_t(it.head) * a.head_stride;
+  const char* const kb = reinterpret_cast<const char*>(a.k + head_at);
+  const char* const vb = reinterpret_cast<const char*>(a.v + head_at);
+  const uint32_t lane_at =
+      2 * (uint32_t(two ? lrow & 3 : lrow) * uint32_t(a.token_stride) + 8 * uint32_t(lcol));
+  V8 k[LOADS], v[LOADS];
+  uint32_t bad = 0;   // bit i: the lane's row of load i is no token that anybody sees
+  auto load_round = [&](int r, int ids) {
+    if (r < it.np) {   // uniform
+      const int t0 = r * L::ROUND + wave * STEP;
+      bad = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) op[e] = T(acc[e] * inv);
+      for (int i = 0; i < LOADS; ++i) {
+        const int t = t0 + i * TPL;
+        auto place = [&](int t, int& ok) {   // bytes from the head's base
+          const int p = __builtin_amdgcn_readlane(ids, (t - t0) >> gshift);
+          ok = t < it.prefix && p >= 0 && p < a.num_pages;
+          return ok ? 2 * (int64_t(p) * a.page_stride + int64_t(t & page_mask) * a.token_stride) : 0;
+        };
+        int ok;
+        int64_t at = place(t, ok);
+        if (two) {
+          int ok2;
+          const int64_t at2 = place(t + 4, ok2);
+          at = lrow & 4 ? at2 : at;
+          ok = lrow & 4 ? ok2 : ok;
+        }
+        k[i] = load_v8<T>(kb + at + lane_at);
+        v[i] = load_v8<T>(vb + at + lane_at);
+        bad |= ok ? 0u : 1u << i;
+      }
+      if (t0 + STEP > it.prefix) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) bad |= t0 + i * TPL + lrow >= it.prefix ? 1u << i : 0u;
+      }
     } else {
-      const int64_t row = part_row(ta, it, c);
+      const int u0 = (r - it.np) * L::ROUND + wave * STEP;
+      bad = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a.part_o[row * D + 8 * lcol + e] = acc[e] * inv;
-      if (lcol == 0) a.part_lse[row] = partial_lse(m, l);
+      for (int i = 0; i < LOADS; ++i) {
+        const int u = u0 + i * TPL + lrow, pos = it.prefix + u;
+        const int p = u < it.tokens ? a.indices[it.page_at + (pos >> a.page_shift)] : -1;
+        const bool ok = p >= 0 && p < a.num_pages;
+        const f16* kp = g_zero_row;
+        const f16* vp = g_zero_row;
+        if (ok && a.k_new) {
+          kp = a.k_new + int64_t(it.q_first + u) * a.kn_tok + int64_t(it.head) * a.kn_head;
+          vp = a.v_new + int64_t(it.q_first + u) * a.vn_tok + int64_t(it.head) * a.vn_head;
+        } else if (ok) {
+          const int64_t at = head_at + int64_t(p) * a.page_stride + int64_t(pos & page_mask) * a.token_stride;
+          kp = a.k + at;
+          vp = a.v + at;
+        }
+        k[i] = load_v8<T>(kp + 8 * lcol);
+        v[i] = load_v8<T>(vp + 8 * lcol);
+        bad |= ok ? 0u : 1u << i;
+      }
+    }
+  };
+
+  int ids = it.rb < it.re ? ids_of(it.rb) : 0;
+  V8 q[KS];
+  {
+    const f16* qp = a.q + int64_t(it.q_first + token) * a.q_tok + int64_t(hq) * a.q_head + 8 * h;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[s] = load_v8<T>(qp + 16 * s);
+  }
+  if (it.rb < it.re) load_round(it.rb, ids);
+  ids = it.rb + 1 < it.re ? ids_of(it.rb + 1) : 0;
+  if (a.k_new && it.re > it.np) append_rows<D>(ta, it);
+
+  f32x16 o[OT];
+#pragma unroll
+  for (int d = 0; d < OT; ++d) o[d] = f32x16{};
+  float m = kNegBig, lsum = 0.f;   // m the same in a column's two lanes
+
+  // Row `col` of a score tile is element e of lane group g (TreeTile).
+  const int e = ((col >> 3) & 1) * 4 + (col & 3), g = 2 * (col >> 4) + ((col >> 2) & 1);
+  // Chunk c of token row (e, g) lies at c ^ swz: the 16 rows that 16 lanes read differ in
+  // it, and so do those of a load, whose rows have e = i.
+  auto swz = [](int e, int g) { return D == 64 ? e : 2 * e + (g & 1); };
+  const int k_row = (D == 64 ? 8 * e + g : D == 128 ? 4 * e + g : 16 * (g >> 1) + 2 * e + (g & 1)) * CH;
+  auto tile_row0 = [](int blk) { return D == 64 ? 64 * (blk >> 1) + 4 * (blk & 1) : 32 * blk; };
+  T* const sk = reinterpret_cast<T*>(s_raw);
+  V8* const sv = reinterpret_cast<V8*>(s_raw + KBYTES);
+  const int own_g = D == 64 ? lrow & 3 : D == 128 ? lrow : 2 * (wave & 1) + lrow;
+  const int own_blk = D == 64 ? 2 * wave + (lrow >> 2) : D == 128 ? wave : wave >> 1;
+  auto v_chunk = [](int g, int l) { return D == 64 ? l ^ ((g & 1) << 3) : l; };   // two groups to 16 lanes
+
+  auto sync = [&] {
+    // Where a share's tokens are those that its only wave has loaded, LDS order will do.
+    if constexpr (WC == 1 && WT == kWaves)
+      __builtin_amdgcn_wave_barrier();
+    else
+      __syncthreads();
+  };
+
+  for (int r = it.rb; r < it.re; ++r) {
+    const bool drafted = r >= it.np;   // uniform
+    uint32_t hide[GB];
+    if (drafted && active) {
+      const uint32_t* mask = ta.masks + it.mask_at + int64_t(token) * it.mask_words +
+                             (r - it.np) * L::BLOCKS + wt * GB;
+#pragma unroll
+      for (int b = 0; b < GB; ++b) hide[b] = ~mask[b];
+    }
+    // K and V to LDS. V of a token that nobody sees has to be 0: 0 x V is.
+    const bool any_bad = __any(bad != 0);
+    if (any_bad) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+        if (bad >> i & 1) v[i] = V8{};
+    }
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+      *reinterpret_cast<V8*>(&sk[(wave * STEP + i * TPL + lrow) * D + 8 * (lcol ^ swz(i, own_g))]) = k[i];
+    V8 vt[8];
+    tree_transpose8(v, vt);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) sv[(own_blk * 4 + own_g) * D + v_chunk(own_g, x * CH + lcol)] = vt[x];
+    {
+      // Bit 16 h + 8 s + e of a tile's word: element e of lane group 2 s + h.
+      uint32_t word[2] = {0u, 0u};   // at head_dim 64 a wave's two tiles
+      if (any_bad) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const uint64_t rows = __ballot(bad >> i & 1);
+#pragma unroll
+          for (int l = 0; l < TPL; ++l) {
+            const int gr = D == 64 ? l & 3 : D == 128 ? l : l + 2 * (wave & 1);
+            word[D == 64 ? l >> 2 : 0] |= uint32_t(rows >> (l * CH) & 1) << (16 * (gr & 1) + 8 * (gr >> 1) + i);
+          }
+        }
+      }
+      if (lane == 0) {
+        s_drop[D == 64 ? 2 * wave : wave] = word[0];
+        if (D == 64) s_drop[2 * wave + 1] = word[1];
+      }
+    }
+    if (r + 1 < it.re) {
+      load_round(r + 1, ids);
+      ids = r + 2 < it.re ? ids_of(r + 2) : 0;
+    }
+    sync();
+    if (active) {
+      const int left = drafted ? it.tokens - (r - it.np) * L::ROUND : it.prefix - r * L::ROUND;
+#pragma unroll
+      for (int b = 0; b < GB; ++b) {
+        const int blk = wt * GB + b;
+        if ((tile_row0(blk) & ~31) >= left) break;   // uniform: no tokens from here on
+        f32x16 sc = {};
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+          sc = mfma32(*reinterpret_cast<const V8*>(
+                          &sk[(tile_row0(blk) * CH + k_row + ((2 * s + h) ^ swz(e, g))) * 8]),
+                      q[s], sc);
+        uint32_t gone = D == 256 ? s_drop[2 * blk] | s_drop[2 * blk + 1] : s_drop[blk];
+        gone = __builtin_amdgcn_readfirstlane(gone);
+        if (drafted || gone) {   // uniform
+          const uint32_t w = (drafted ? hide[b] | gone : gone) >> (16 * h);
+#pragma unroll
+          for (int x = 0; x < 16; ++x) sc[x] = w >> x & 1 ? -INFINITY : sc[x];
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) mx = fmaxf(mx, sc[x]);
+        if (__any(mx * a.scale_log2 > m + 8.f)) {
+          mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.scale_log2;
+          const float m_new = mx > m + 8.f ? mx : m;
+          const float alpha = fast_exp2(m - m_new);
+          m = m_new;
+          lsum *= alpha;
+#pragma unroll
+          for (int d = 0; d < OT; ++d)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) o[d][x] *= alpha;
+        }
+        // Probabilities in two 16-bit terms, as in every decode launch.
+        V8 ph[2], pl[2];
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const float p = fast_exp2(fmaf(sc[x], a.scale_log2, -m));
+          lsum += p;
+          const T hi = T(p);
+          ph[x >> 3][x & 7] = hi;
+          pl[x >> 3][x & 7] = T(p - float(hi));
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int d = 0; d < OT; ++d) {
+            const V8 va = sv[(blk * 4 + 2 * s + h) * D + v_chunk(h, 32 * d + col)];
+            o[d] = mfma32(va, ph[s], o[d]);
+            o[d] = mfma32(va, pl[s], o[d]);
+          }
+      }
+    }
+    sync();
+  }
+
+  // Values that the products do not carry (0 x infinity of a token that a column does not
+  // see, infinity in two terms): those columns once more on the vector units.
+  float z = 0.f;
+#pragma unroll
+  for (int d = 0; d < OT; ++d)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) z = fmaf(o[d][x], 0.f, z);
+  if (active && __any(!(z == 0.f))) {
+    const int n = min(32, it.cols - 32 * wc);
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      float m1, l1, acc[8];
+      tree_column<T, D>(ta, it, it.c0 + 32 * wc + j, wt * GB * kBlock, (wt + 1) * GB * kBlock, m1, l1, acc);
+      const bool mine = col == j;
+      if (mine) {
+        m = m1;
+        lsum = h ? 0.f : l1;
+      }
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const float y = __shfl(acc[(32 * d + 8 * (x >> 2)) / CH], (8 * (x >> 2) + 4 * h + (x & 3)) % CH);
+          o[d][x] = mine ? y : o[d][x];
+        }
     }
   }
+  lsum += __shfl_xor(lsum, 32);
+
+  // The shares of a column tile joined, the upper half of them into the lower.
+  float* const s_o = reinterpret_cast<float*>(s_raw);
+#pragma unroll
+  for (int half = WT / 2; half >= 1; half /= 2) {
+    __syncthreads();
+    if (active && wt >= half && wt < 2 * half) {
+      float* to = s_o + ((wt - half) * WC + wc) * OT * 16 * kWave + lane;
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) to[(16 * d + x) * kWave] = o[d][x];
+      s_ml[(wt - half) * WC + wc][0][lane] = m;
+      s_ml[(wt - half) * WC + wc][1][lane] = lsum;
+    }
+    __syncthreads();
+    if (active && wt < half) {
+      const float* from = s_o + (wt * WC + wc) * OT * 16 * kWave + lane;
+      const float m2 = s_ml[wt * WC + wc][0][lane], l2 = s_ml[wt * WC + wc][1][lane];
+      const float mx = fmaxf(m, m2);
+      const float f1 = fast_exp2(m - mx), f2 = fast_exp2(m2 - mx);
+      m = mx;
+      lsum = lsum * f1 + l2 * f2;
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[d][x] = o[d][x] * f1 + from[(16 * d + x) * kWave] * f2;
+    }
+  }
+  if (!active || wt > 0 || 32 * wc + col >= it.cols) return;
+  const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+  // A lane has D / 16 chunks of 8 dims: chunk 8 (j / 4) + 4 h + j % 4.
+  constexpr int NCH = D / 16;
+  f16* op = a.out + int64_t(it.q_first + token) * a.o_tok + int64_t(hq) * a.o_head;
+  const int64_t prow = it.slot < 0 ? 0 : part_row(ta, it, c);
+#pragma unroll
+  for (int j = 0; j < NCH; ++j) {
+    const int d0 = 8 * (8 * (j >> 2) + 4 * h + (j & 3));
+    float y[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) y[x] = o[(x * NCH + j) / 16][(x * NCH + j) % 16] * inv;
+    if (it.slot < 0) {   // uniform
+      V8 w;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) w[x] = T(y[x]);
+      *reinterpret_cast<V8*>(op + d0) = w;
+    } else {
+      float* po = a.part_o + prow * D + d0;
+      *reinterpret_cast<f32x4*>(po) = f32x4{y[0], y[1], y[2], y[3]};
+      *reinterpret_cast<f32x4*>(po + 4) = f32x4{y[4], y[5], y[6], y[7]};
+    }
+  }
+  if (it.slot >= 0 && h == 0) a.part_lse[prow] = partial_lse(m, lsum);
 }
 
-template <typename T>
-int launch_tree(int head_dim, const TreeArgs& ta, unsigned blocks, hipStream_t s) {
-  switch (head_dim) {
-    case 64: tree_attention_kernel<T, 64><<<blocks, kThreads, 0, s>>>(ta); break;
-    case 128: tree_attention_kernel<T, 128><<<blocks, kThreads, 0, s>>>(ta); break;
-    default: tree_attention_kernel<T, 256><<<blocks, kThreads, 0, s>>>(ta);
+template <typename T, int D>
+int launch_tree_dim(int col_waves, const TreeArgs& ta, unsigned blocks, hipStream_t s) {
+  constexpr int kLeast = D == 256 ? 2 : 1;   // (a round has two score tiles there)
+  switch (col_waves) {
+    case 1: tree_attention_kernel<T, D, kLeast><<<blocks, kThreads, 0, s>>>(ta); break;
+    case 2: tree_attention_kernel<T, D, 2><<<blocks, kThreads, 0, s>>>(ta); break;
+    default: tree_attention_kernel<T, D, 4><<<blocks, kThreads, 0, s>>>(ta);
   }
   KSV_CHECK_LAUNCH();
   return KUNSERVE_OK;
 }
 
+template <typename T>
+int launch_tree(int head_dim, int col_waves, const TreeArgs& ta, unsigned blocks, hipStream_t s) {
+  switch (head_dim) {
+    case 64: return launch_tree_dim<T, 64>(col_waves, ta, blocks, s);
+    case 128: return launch_tree_dim<T, 128>(col_waves, ta, blocks, s);
+    default: return launch_tree_dim<T, 256>(col_waves, ta, blocks, s);
+  }
+}
+
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Columns of a workgroup.
-constexpr int kMaxCols = 128;
+constexpr int kTileCols = 32;   // columns of a wave
 
 struct TreeRow {
   int32_t tokens, q_first, prefix, page_at, mask_at, mask_words, np, rounds;
@@ -226,6 +547,12 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
   const int64_t cus = num_cus > 0 ? num_cus : 256;
   std::vector<TreeRow> rows(num_seqs);
   std::vector<uint32_t> masks;
+  // Waves along the columns: as few as hold the widest row's.
+  int32_t widest = 0;
+  for (int32_t b = 0; b < num_seqs; ++b)
+    widest = std::max(widest, std::min(q_indptr[b + 1] - q_indptr[b], 128) * ratio);
+  const int col_waves = widest <= kTileCols && head_dim != 256 ? 1 : widest <= 2 * kTileCols ? 2 : 4;
+  const int max_cols = kTileCols * col_waves;
   int64_t work = 0;   // rounds of all workgroups
   int32_t longest = 0;
   for (int32_t b = 0; b < num_seqs; ++b) {
@@ -256,7 +583,7 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
       mask_bit(head_dim, i % round, &tile, &bit);
       own[i / round * tiles + tile] |= 1u << bit;
     }
-    work += n ? int64_t(r.rounds) * ceil_div(int64_t(n) * ratio, kMaxCols) * num_kv_heads : 0;
+    work += n ? int64_t(r.rounds) * ceil_div(int64_t(n) * ratio, max_cols) * num_kv_heads : 0;
     if (n) longest = std::max(longest, r.rounds);
   }
   // A workgroup's run of rounds: what gives every CU two of them.
@@ -296,9 +623,9 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
     const int32_t cols = r.tokens * ratio;
     for (int32_t h = 0; h < num_kv_heads; ++h) {
       const int x = int(std::min_element(load, load + kXcds) - load);
-      for (int32_t c = 0; c < cols; c += kMaxCols) {
+      for (int32_t c = 0; c < cols; c += max_cols) {
         lanes[x].insert(lanes[x].end(),
-                        {r.tokens, r.q_first, r.prefix, r.page_at, c, std::min(kMaxCols, cols - c),
+                        {r.tokens, r.q_first, r.prefix, r.page_at, c, std::min(max_cols, cols - c),
                          h, r.np, p.rb, p.re, slot[p.row], parts[p.row], p.part, r.mask_at,
                          r.mask_words, 0});
         load[x] += p.re - p.rb;
@@ -313,6 +640,7 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
   info->num_work = int32_t(kXcds * depth);
   info->num_merge = int32_t(merges.size() / 4);
   info->num_slots = int32_t(slots);
+  info->col_waves = col_waves;
   info->num_seqs = num_seqs;
   info->head_dim = head_dim;
   info->page_size = page_size;
@@ -409,6 +737,10 @@ int kunserve::tree_attention(const kunserve_kv_pool* pool, int32_t layer,
                 info->num_kv_heads, num_qo_heads, pool->num_kv_heads);
   KSV_CHECK_ARG(info->num_seqs == table->num_seqs, "plan made for %d rows, not %d", info->num_seqs,
                 table->num_seqs);
+  KSV_CHECK_ARG(info->col_waves == 1 || info->col_waves == 2 || info->col_waves == 4,
+                "plan of %d waves along the columns", info->col_waves);
+  KSV_CHECK_ARG(pool->token_stride < (int64_t(1) << 28),
+                "tokens %lld elements apart: less than 2^28 here", (long long)pool->token_stride);
   KSV_CHECK_ARG(num_qo_heads < 65536, "%d query heads: at most 65535", num_qo_heads);
   // The launch's arguments and the joining of its partials are the decode launch's.
   kunserve_decode_plan_info parts{};
@@ -431,8 +763,8 @@ int kunserve::tree_attention(const kunserve_kv_pool* pool, int32_t layer,
   ta.masks = reinterpret_cast<const uint32_t*>(merges + 4 * int64_t(info->num_merge));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int err = pool->dtype == KUNSERVE_DTYPE_BF16
-                      ? launch_tree<bf16>(pool->head_dim, ta, unsigned(info->num_work), s)
-                      : launch_tree<f16>(pool->head_dim, ta, unsigned(info->num_work), s);
+                      ? launch_tree<bf16>(pool->head_dim, info->col_waves, ta, unsigned(info->num_work), s)
+                      : launch_tree<f16>(pool->head_dim, info->col_waves, ta, unsigned(info->num_work), s);
   if (err) return err;
   parts.num_work = 0;   // the records behind which its merges are
   return decode_merge(pool, ta.d, &parts, merges, s);

@@ -158,4 +158,4 @@ def test_bound_holds():
 
 
 def test_info_is_that_of_the_header():
-    assert ctypes.sizeof(_lib.TreePlanInfo) == 36 and ctypes.sizeof(_lib.RotaryAxes) == 24
+    assert ctypes.sizeof(_lib.TreePlanInfo) == 40 and ctypes.sizeof(_lib.RotaryAxes) == 24

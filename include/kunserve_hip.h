@@ -505,7 +505,7 @@ typedef struct {
   int32_t num_work;      /* work records (incl. padding)                      */
   int32_t num_merge;     /* tokens whose row is split                         */
   int32_t num_slots;     /* partial-result slots                              */
-  int32_t col_waves;     /* waves of a workgroup along its columns, 32 to each */
+  int32_t columns;       /* (token, query head) pairs of a workgroup at most  */
   int32_t num_seqs;      /* what the plan was made for, from here on          */
   int32_t head_dim;
   int32_t page_size;

@@ -106,7 +106,7 @@ class RotaryAxes(Structure):
 
 class TreePlanInfo(Structure):
     _fields_ = [("num_work", c_int32), ("num_merge", c_int32), ("num_slots", c_int32),
-                ("col_waves", c_int32), ("num_seqs", c_int32), ("head_dim", c_int32),
+                ("columns", c_int32), ("num_seqs", c_int32), ("head_dim", c_int32),
                 ("page_size", c_int32), ("num_qo_heads", c_int32), ("num_kv_heads", c_int32),
                 ("plan_ints", c_int32)]
 

@@ -15,6 +15,7 @@
 // as those of decode rows are.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 #include "decode_tile.hpp"
@@ -139,6 +140,24 @@ __device__ __forceinline__ void tree_column(const TreeArgs& ta, const TreeItem& 
   }
 }
 
+// Two probabilities x, y as the sum of two 16-bit terms each: the first cut off, not
+// rounded, so that it costs a byte move (bf16) or one conversion (fp16) for both; the second
+// is the difference, rounded (2^-17 and 2^-22 of the value).
+template <typename T>
+__device__ __forceinline__ void two_terms(float x, float y, uint32_t& hi, uint32_t& lo) {
+  if constexpr (std::is_same<T, bf16>::value) {
+    const uint32_t a = f32_to_bits(x), b = f32_to_bits(y);
+    hi = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const b2 l = {__bf16(x - bits_to_f32(int(a & 0xffff0000u))), __bf16(y - bits_to_f32(int(b & 0xffff0000u)))};
+    lo = __builtin_bit_cast(uint32_t, l);
+  } else {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - float(h[0]), y - float(h[1])));
+  }
+}
+
 // Where a column's result goes: a partial (fp32) or out.
 __device__ __forceinline__ int64_t part_row(const TreeArgs& ta, const TreeItem& it, int c) {
   return int64_t(it.slot + c / ta.d.ratio * it.parts + it.part) * ta.d.num_qo_heads +
@@ -157,28 +176,6 @@ __device__ __forceinline__ void tree_transpose8(const V8 (&v)[8], V8 (&vt)[8]) {
                                    __builtin_bit_cast(u32x4, v[2 * x])[e >> 1],
                                    (e & 1) ? 0x07060302u : 0x05040100u);
     vt[e] = __builtin_bit_cast(V8, d);
-  }
-}
-
-// The drafted rows of the item's rounds whose first column is one of its own, into
-// their pages.
-template <int D>
-__device__ __forceinline__ void append_rows(const TreeArgs& ta, const TreeItem& it) {
-  typedef TreeTile<D> L;
-  const DecodeArgs& a = ta.d;
-  const int lo = max((max(it.rb, it.np) - it.np) * L::ROUND, (it.c0 + a.ratio - 1) / a.ratio);
-  const int hi = min(min(it.tokens, (it.re - it.np) * L::ROUND),
-                     (it.c0 + it.cols + a.ratio - 1) / a.ratio);
-  for (int i = threadIdx.x; i < (hi - lo) * 2 * L::CH; i += kThreads) {
-    const int u = lo + i / (2 * L::CH), of_v = i / L::CH & 1, c = i % L::CH;
-    const int pos = it.prefix + u;
-    const int p = a.indices[it.page_at + (pos >> a.page_shift)];
-    if (p < 0 || p >= a.num_pages) continue;
-    const f16* src = (of_v ? a.v_new + int64_t(it.q_first + u) * a.vn_tok + int64_t(it.head) * a.vn_head
-                           : a.k_new + int64_t(it.q_first + u) * a.kn_tok + int64_t(it.head) * a.kn_head);
-    f16* dst = const_cast<f16*>(of_v ? a.v : a.k) + int64_t(it.head) * a.head_stride +
-               int64_t(p) * a.page_stride + int64_t(pos & ((1 << a.page_shift) - 1)) * a.token_stride;
-    store_f16x8(dst + 8 * c, load_f16x8(src + 8 * c));
   }
 }
 
@@ -219,11 +216,17 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
   // ---- loads. A round's tokens of a wave are STEP; cached ones lie in pages whose ids a
   // register's lanes hold, one for `granule` tokens, a round ahead of the loads.
   const int gshift = min(a.page_shift, 4);
-  const bool two = TPL > 4 && a.page_shift < 3;   // a load's rows in two pages
+  const bool two = TPL == 8 && a.page_shift == 2;   // a load's rows in two pages
   const int last_page = max(it.prefix - 1, 0) >> a.page_shift;
   auto ids_of = [&](int r) {
-    const int t = r * L::ROUND + wave * STEP + (lane << gshift);
-    return r < it.np ? a.indices[it.page_at + min(t >> a.page_shift, last_page)] : 0;
+    if (r < it.np) {   // uniform
+      const int t = r * L::ROUND + wave * STEP + (lane << gshift);
+      return a.indices[it.page_at + min(t >> a.page_shift, last_page)];
+    }
+    // Of drafted tokens page by page, from that of the wave's first.
+    const int at = it.prefix + min((r - it.np) * L::ROUND + wave * STEP, it.tokens - 1);
+    return a.indices[it.page_at + min((at >> a.page_shift) + lane,
+                                      (it.prefix + it.tokens - 1) >> a.page_shift)];
   };
   const int64_t head_at = int64_t(it.head) * a.head_stride;
   const char* const kb = reinterpret_cast<const char*>(a.k + head_at);
@@ -232,42 +235,61 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
       2 * (uint32_t(two ? lrow & 3 : lrow) * uint32_t(a.token_stride) + 8 * uint32_t(lcol));
   V8 k[LOADS], v[LOADS];
   uint32_t bad = 0;   // bit i: the lane's row of load i is no token that anybody sees
-  auto load_round = [&](int r, int ids) {
-    if (r < it.np) {   // uniform
-      const int t0 = r * L::ROUND + wave * STEP;
-      bad = 0;
+  // Page ids outside the pool, and tokens behind the cached ones, read page 0.
+  auto load_cached = [&](int r, int ids, auto loads_per_page) {
+    constexpr int P = decltype(loads_per_page)::value;   // 0: two pages to a load
+    constexpr int N = P ? LOADS / P : 2 * LOADS;         // granules
+    const int t0 = r * L::ROUND + wave * STEP;
+    bad = 0;
+    int64_t at[N];   // bytes from the head's base
+    uint32_t gone = 0;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int t = t0 + (P ? n * P * TPL : n * (TPL / 2));
+      const int p = __builtin_amdgcn_readlane(ids, n);
+      const bool ok = t < it.prefix && p >= 0 && p < a.num_pages;
+      at[n] = ok ? 2 * (int64_t(p) * a.page_stride + int64_t(t & page_mask) * a.token_stride) : 0;
+      gone |= ok ? 0u : 1u << n;
+    }
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      int64_t from;
+      if constexpr (P)
+        from = at[i / P] + i % P * (2 * TPL * a.token_stride);
+      else
+        from = at[2 * i] + (lrow & 4 ? at[2 * i + 1] - at[2 * i] : 0);
+      // (Past the caches: 64 rows of 4096, 32 columns, 179 us a layer against 198; where four
+      // workgroups read the same K and V 280 against 277.)
+      k[i] = load_v8_nt<T>(kb + from + lane_at);
+      v[i] = load_v8_nt<T>(vb + from + lane_at);
+    }
+    if (gone || t0 + STEP > it.prefix) {   // uniform
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int t = t0 + i * TPL;
-        auto place = [&](int t, int& ok) {   // bytes from the head's base
-          const int p = __builtin_amdgcn_readlane(ids, (t - t0) >> gshift);
-          ok = t < it.prefix && p >= 0 && p < a.num_pages;
-          return ok ? 2 * (int64_t(p) * a.page_stride + int64_t(t & page_mask) * a.token_stride) : 0;
-        };
-        int ok;
-        int64_t at = place(t, ok);
-        if (two) {
-          int ok2;
-          const int64_t at2 = place(t + 4, ok2);
-          at = lrow & 4 ? at2 : at;
-          ok = lrow & 4 ? ok2 : ok;
-        }
-        k[i] = load_v8<T>(kb + at + lane_at);
-        v[i] = load_v8<T>(vb + at + lane_at);
-        bad |= ok ? 0u : 1u << i;
+        const int n = P ? i / (P ? P : 1) : 2 * i + (lrow >> 2);
+        bad |= (gone >> n & 1) || t0 + i * TPL + lrow >= it.prefix ? 1u << i : 0u;
       }
-      if (t0 + STEP > it.prefix) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) bad |= t0 + i * TPL + lrow >= it.prefix ? 1u << i : 0u;
-      }
+    }
+  };
+  typedef std::integral_constant<int, 16 / TPL> Pages16;
+  typedef std::integral_constant<int, TPL == 8 ? 0 : 4 / TPL> Pages4;
+  typedef std::integral_constant<int, TPL == 8 ? 1 : 8 / TPL> Pages8;
+  auto load_round = [&](int r, int ids) {
+    if (r < it.np) {   // uniform
+      if (a.page_shift >= 4)
+        load_cached(r, ids, Pages16{});
+      else if (a.page_shift == 3)
+        load_cached(r, ids, Pages8{});
+      else
+        load_cached(r, ids, Pages4{});
     } else {
       const int u0 = (r - it.np) * L::ROUND + wave * STEP;
       bad = 0;
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int u = u0 + i * TPL + lrow, pos = it.prefix + u;
-        const int p = u < it.tokens ? a.indices[it.page_at + (pos >> a.page_shift)] : -1;
-        const bool ok = p >= 0 && p < a.num_pages;
+        const int p = __shfl(ids, (pos >> a.page_shift) - ((it.prefix + u0) >> a.page_shift));
+        const bool ok = u < it.tokens && p >= 0 && p < a.num_pages;
         const f16* kp = g_zero_row;
         const f16* vp = g_zero_row;
         if (ok && a.k_new) {
@@ -285,6 +307,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
     }
   };
 
+  // (The next round's ids are read without a branch, behind which the compiler would wait
+  // for them, and so for the loads before them.)
   int ids = it.rb < it.re ? ids_of(it.rb) : 0;
   V8 q[KS];
   {
@@ -292,27 +316,38 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
 #pragma unroll
     for (int s = 0; s < KS; ++s) q[s] = load_v8<T>(qp + 16 * s);
   }
-  if (it.rb < it.re) load_round(it.rb, ids);
-  ids = it.rb + 1 < it.re ? ids_of(it.rb + 1) : 0;
-  if (a.k_new && it.re > it.np) append_rows<D>(ta, it);
+  if (it.rb < it.re) {
+    load_round(it.rb, ids);
+    ids = ids_of(min(it.rb + 1, it.re - 1));
+  }
 
   f32x16 o[OT];
 #pragma unroll
   for (int d = 0; d < OT; ++d) o[d] = f32x16{};
   float m = kNegBig, lsum = 0.f;   // m the same in a column's two lanes
 
+  // LDS addresses as one register each and constants: with one for each chunk they were
+  // spilled, and their reloads waited for the loads on their way.
   // Row `col` of a score tile is element e of lane group g (TreeTile).
   const int e = ((col >> 3) & 1) * 4 + (col & 3), g = 2 * (col >> 4) + ((col >> 2) & 1);
   // Chunk c of token row (e, g) lies at c ^ swz: the 16 rows that 16 lanes read differ in
   // it, and so do those of a load, whose rows have e = i.
   auto swz = [](int e, int g) { return D == 64 ? e : 2 * e + (g & 1); };
+  auto swz_of = [](int i) { return D == 64 ? i : 2 * i; };   // of load i, but for its group
   const int k_row = (D == 64 ? 8 * e + g : D == 128 ? 4 * e + g : 16 * (g >> 1) + 2 * e + (g & 1)) * CH;
   auto tile_row0 = [](int blk) { return D == 64 ? 64 * (blk >> 1) + 4 * (blk & 1) : 32 * blk; };
-  T* const sk = reinterpret_cast<T*>(s_raw);
-  V8* const sv = reinterpret_cast<V8*>(s_raw + KBYTES);
+  auto moved = [](int base, int bits) {   // base ^ bits, made at each use
+    asm volatile("v_xor_b32 %0, %1, %2" : "=v"(base) : "n"(bits), "v"(base));
+    return base;
+  };
   const int own_g = D == 64 ? lrow & 3 : D == 128 ? lrow : 2 * (wave & 1) + lrow;
   const int own_blk = D == 64 ? 2 * wave + (lrow >> 2) : D == 128 ? wave : wave >> 1;
-  auto v_chunk = [](int g, int l) { return D == 64 ? l ^ ((g & 1) << 3) : l; };   // two groups to 16 lanes
+  // Chunk l of a lane group's V: at head_dim 64 two groups fill 16 lanes, apart by an XOR.
+  auto v_chunk = [](int g, int l) { return D == 64 ? l ^ ((g & 1) << 3) : l; };
+  const int k_read = 16 * (k_row + (h ^ swz(e, g)));
+  const int v_read = KBYTES + 16 * (h * D + v_chunk(h, col));
+  const int k_park = 16 * ((wave * STEP + lrow) * CH + (lcol ^ (D == 64 ? 0 : own_g & 1)));
+  const int v_park = KBYTES + 16 * ((own_blk * 4 + own_g) * D + v_chunk(own_g, lcol));
 
   auto sync = [&] {
     // Where a share's tokens are those that its only wave has loaded, LDS order will do.
@@ -324,12 +359,19 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
 
   for (int r = it.rb; r < it.re; ++r) {
     const bool drafted = r >= it.np;   // uniform
-    uint32_t hide[GB];
-    if (drafted && active) {
-      const uint32_t* mask = ta.masks + it.mask_at + int64_t(token) * it.mask_words +
-                             (r - it.np) * L::BLOCKS + wt * GB;
+    if (drafted && a.k_new) {   // uniform: rows whose first column is the workgroup's, to their pages
+      const int lo = (it.c0 + a.ratio - 1) / a.ratio;
+      const int hi = min(it.tokens, (it.c0 + it.cols + a.ratio - 1) / a.ratio);
 #pragma unroll
-      for (int b = 0; b < GB; ++b) hide[b] = ~mask[b];
+      for (int i = 0; i < LOADS; ++i) {
+        const int u = (r - it.np) * L::ROUND + wave * STEP + i * TPL + lrow, pos = it.prefix + u;
+        if (u < lo || u >= hi || (bad >> i & 1)) continue;
+        const int64_t at = head_at +
+                           int64_t(a.indices[it.page_at + (pos >> a.page_shift)]) * a.page_stride +
+                           int64_t(pos & page_mask) * a.token_stride + 8 * lcol;
+        *reinterpret_cast<V8*>(const_cast<f16*>(a.k) + at) = k[i];
+        *reinterpret_cast<V8*>(const_cast<f16*>(a.v) + at) = v[i];
+      }
     }
     // K and V to LDS. V of a token that nobody sees has to be 0: 0 x V is.
     const bool any_bad = __any(bad != 0);
@@ -340,11 +382,12 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
     }
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
-      *reinterpret_cast<V8*>(&sk[(wave * STEP + i * TPL + lrow) * D + 8 * (lcol ^ swz(i, own_g))]) = k[i];
+      *reinterpret_cast<V8*>(s_raw + moved(k_park, 16 * swz_of(i)) + 16 * i * TPL * CH) = k[i];
     V8 vt[8];
     tree_transpose8(v, vt);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) sv[(own_blk * 4 + own_g) * D + v_chunk(own_g, x * CH + lcol)] = vt[x];
+    for (int x = 0; x < 8; ++x)   // (an XOR of 8 chunks is one of rows of 8)
+      *reinterpret_cast<V8*>(s_raw + (D == 64 ? moved(v_park, 16 * x * CH) : v_park + 16 * x * CH)) = vt[x];
     {
       // Bit 16 h + 8 s + e of a tile's word: element e of lane group 2 s + h.
       uint32_t word[2] = {0u, 0u};   // at head_dim 64 a wave's two tiles
@@ -366,25 +409,36 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
     }
     if (r + 1 < it.re) {
       load_round(r + 1, ids);
-      ids = r + 2 < it.re ? ids_of(r + 2) : 0;
+      ids = ids_of(min(r + 2, it.re - 1));
     }
     sync();
     if (active) {
+      const uint32_t* mask = ta.masks + it.mask_at + int64_t(token) * it.mask_words +
+                             (r - it.np) * L::BLOCKS + wt * GB;
       const int left = drafted ? it.tokens - (r - it.np) * L::ROUND : it.prefix - r * L::ROUND;
-#pragma unroll
+#pragma unroll 1
       for (int b = 0; b < GB; ++b) {
         const int blk = wt * GB + b;
         if ((tile_row0(blk) & ~31) >= left) break;   // uniform: no tokens from here on
+        const int k_at = k_read + 16 * tile_row0(blk) * CH, v_at = v_read + 16 * 4 * D * blk;
+        // Operands are read together, V's while the scores become probabilities: read one
+        // by one before its product, each waited for LDS.
+        V8 ka[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) ka[s] = *reinterpret_cast<const V8*>(s_raw + moved(k_at, 32 * s));
+        __builtin_amdgcn_sched_barrier(0);
         f32x16 sc = {};
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
-          sc = mfma32(*reinterpret_cast<const V8*>(
-                          &sk[(tile_row0(blk) * CH + k_row + ((2 * s + h) ^ swz(e, g))) * 8]),
-                      q[s], sc);
+        for (int s = 0; s < KS; ++s) sc = mfma32(ka[s], q[s], sc);
+        V8 va[2][OT];
+#pragma unroll
+        for (int d = 0; d < OT; ++d)
+          va[0][d] = *reinterpret_cast<const V8*>(s_raw + v_at + 16 * 32 * d);
+        __builtin_amdgcn_sched_barrier(0);
         uint32_t gone = D == 256 ? s_drop[2 * blk] | s_drop[2 * blk + 1] : s_drop[blk];
         gone = __builtin_amdgcn_readfirstlane(gone);
         if (drafted || gone) {   // uniform
-          const uint32_t w = (drafted ? hide[b] | gone : gone) >> (16 * h);
+          const uint32_t w = (drafted ? ~mask[b] | gone : gone) >> (16 * h);
 #pragma unroll
           for (int x = 0; x < 16; ++x) sc[x] = w >> x & 1 ? -INFINITY : sc[x];
         }
@@ -403,23 +457,31 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
             for (int x = 0; x < 16; ++x) o[d][x] *= alpha;
         }
         // Probabilities in two 16-bit terms, as in every decode launch.
-        V8 ph[2], pl[2];
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const float p = fast_exp2(fmaf(sc[x], a.scale_log2, -m));
-          lsum += p;
-          const T hi = T(p);
-          ph[x >> 3][x & 7] = hi;
-          pl[x >> 3][x & 7] = T(p - float(hi));
-        }
+        for (int s = 0; s < 2; ++s) {
+          u32x4 h4, l4;
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int d = 0; d < OT; ++d) {
-            const V8 va = sv[(blk * 4 + 2 * s + h) * D + v_chunk(h, 32 * d + col)];
-            o[d] = mfma32(va, ph[s], o[d]);
-            o[d] = mfma32(va, pl[s], o[d]);
+          for (int x = 0; x < 8; x += 2) {
+            const float p0 = fast_exp2(fmaf(sc[8 * s + x], a.scale_log2, -m));
+            const float p1 = fast_exp2(fmaf(sc[8 * s + x + 1], a.scale_log2, -m));
+            lsum += p0 + p1;
+            uint32_t hi, lo;
+            two_terms<T>(p0, p1, hi, lo);
+            h4[x / 2] = hi;
+            l4[x / 2] = lo;
           }
+          const V8 ph = __builtin_bit_cast(V8, h4), pl = __builtin_bit_cast(V8, l4);
+          if (s == 0) {
+#pragma unroll
+            for (int d = 0; d < OT; ++d)
+              va[1][d] = *reinterpret_cast<const V8*>(s_raw + v_at + 16 * (2 * D + 32 * d));
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int d = 0; d < OT; ++d) o[d] = mfma32(va[s][d], ph, o[d]);
+#pragma unroll
+          for (int d = 0; d < OT; ++d) o[d] = mfma32(va[s][d], pl, o[d]);
+        }
       }
     }
     sync();
@@ -640,7 +702,7 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
   info->num_work = int32_t(kXcds * depth);
   info->num_merge = int32_t(merges.size() / 4);
   info->num_slots = int32_t(slots);
-  info->col_waves = col_waves;
+  info->columns = col_waves;
   info->num_seqs = num_seqs;
   info->head_dim = head_dim;
   info->page_size = page_size;
@@ -737,8 +799,8 @@ int kunserve::tree_attention(const kunserve_kv_pool* pool, int32_t layer,
                 info->num_kv_heads, num_qo_heads, pool->num_kv_heads);
   KSV_CHECK_ARG(info->num_seqs == table->num_seqs, "plan made for %d rows, not %d", info->num_seqs,
                 table->num_seqs);
-  KSV_CHECK_ARG(info->col_waves == 1 || info->col_waves == 2 || info->col_waves == 4,
-                "plan of %d waves along the columns", info->col_waves);
+  KSV_CHECK_ARG(info->columns == 1 || info->columns == 2 || info->columns == 4,
+                "plan of %d waves along the columns", info->columns);
   KSV_CHECK_ARG(pool->token_stride < (int64_t(1) << 28),
                 "tokens %lld elements apart: less than 2^28 here", (long long)pool->token_stride);
   KSV_CHECK_ARG(num_qo_heads < 65536, "%d query heads: at most 65535", num_qo_heads);
@@ -763,8 +825,8 @@ int kunserve::tree_attention(const kunserve_kv_pool* pool, int32_t layer,
   ta.masks = reinterpret_cast<const uint32_t*>(merges + 4 * int64_t(info->num_merge));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int err = pool->dtype == KUNSERVE_DTYPE_BF16
-                      ? launch_tree<bf16>(pool->head_dim, info->col_waves, ta, unsigned(info->num_work), s)
-                      : launch_tree<f16>(pool->head_dim, info->col_waves, ta, unsigned(info->num_work), s);
+                      ? launch_tree<bf16>(pool->head_dim, info->columns, ta, unsigned(info->num_work), s)
+                      : launch_tree<f16>(pool->head_dim, info->columns, ta, unsigned(info->num_work), s);
   if (err) return err;
   parts.num_work = 0;   // the records behind which its merges are
   return decode_merge(pool, ta.d, &parts, merges, s);

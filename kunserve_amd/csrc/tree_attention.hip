@@ -15,6 +15,7 @@
 // as those of decode rows are.
 #include <algorithm>
 #include <cmath>
+#include <map>
 #include <type_traits>
 #include <vector>
 
@@ -26,24 +27,34 @@ namespace {
 constexpr int kTreeRecord = 16;   // ints of a work record
 constexpr int kBlock = 32;        // tokens of a score tile
 
-// A round is what the four waves load at a time: a DecodeTile step each. Its tokens
-// are `BLOCKS` score tiles. Element x of half h of a tile's scores (32x32: lane
-// column, register x, lane half h) is token element e = x % 8 of lane group g =
-// 2 (x / 8) + h; a lane group's 8 tokens are those that one lane of a load has.
-template <int D>
-struct TreeTile : DecodeTile<D> {
-  static constexpr int ROUND = kWaves * DecodeTile<D>::STEP;
+// A round is what the waves load at a time, LOADS loads of TPL token rows each, and its
+// tokens are score tiles of 32. Element x of half h of a tile's scores (32x32: lane
+// column, register x, lane half h) is token element e = x % 8 of lane group g = 2 (x / 8)
+// + h: the 8 tokens of a group are those that one lane has of one wave's loads, or of two
+// waves' (eight waves with 4 loads), so that V is transposed within a lane.
+template <int D, int WC>
+struct TreeTile {
+  static constexpr int WAVES = WC > kWaves ? WC : kWaves;
+  static constexpr int LOADS = 8 * kWaves / WAVES;
+  static constexpr int CH = D / 8;              // 16-byte chunks of a token row
+  static constexpr int TPL = kWave / CH;
+  static constexpr int STEP = TPL * LOADS;      // tokens of a wave
+  static constexpr int ROUND = WAVES * STEP;
   static constexpr int BLOCKS = ROUND / kBlock;
 };
-// The place of a round's token u among the bits of a mask: (tile, bit).
-inline void mask_bit(int head_dim, int u, int* tile, int* bit) {
-  const int tpl = kWave / (head_dim / 8), step = 8 * tpl;   // DecodeTile's
-  const int wave = u / step, v = u % step, e = v / tpl, l = v % tpl;   // l: lane row
-  const int group = head_dim == 64 ? l & 3 : head_dim == 128 ? l : 2 * (wave & 1) + l;
-  *tile = head_dim == 64 ? 2 * wave + (l >> 2) : head_dim == 128 ? wave : wave >> 1;
-  *bit = 16 * (group & 1) + 8 * (group >> 1) + e;
+// Tile, element and lane group of a round's token u.
+struct TilePlace {
+  int tile, e, g;
+};
+__host__ __device__ __forceinline__ TilePlace tile_place(int head_dim, int u) {
+  const int w = u & 31;
+  if (head_dim == 64) return {2 * (u >> 6) + (u >> 2 & 1), u >> 3 & 7, u & 3};
+  if (head_dim == 128) return {u >> 5, w >> 2, w & 3};
+  return {u >> 5, w >> 1 & 7, 2 * (w >> 4) + (w & 1)};
 }
-inline int round_tokens(int head_dim) { return 4 * 8 * kWave / (head_dim / 8); }
+__host__ __device__ __forceinline__ int mask_bit(const TilePlace& p) {
+  return 16 * (p.g & 1) + 8 * (p.g >> 1) + p.e;
+}
 
 struct TreeArgs {
   DecodeArgs d;               // q, out, the pool, partials (work, group: unused)
@@ -70,10 +81,10 @@ __device__ __forceinline__ TreeItem tree_item(const int32_t* r) {
 // A column's attention over the tokens [lo, hi) of every round of the item, in fp32 on
 // the vector units, a load at a time (wave_rows, with the tree's mask). Masked tokens
 // leave nothing, whatever K and V hold there.
-template <typename T, int D>
+template <typename T, int D, int WC>
 __device__ __forceinline__ void tree_column(const TreeArgs& ta, const TreeItem& it, int c, int lo,
                                             int hi, float& m, float& l, float (&acc)[8]) {
-  typedef TreeTile<D> L;
+  typedef TreeTile<D, WC> L;
   const DecodeArgs& a = ta.d;
   const int lane = threadIdx.x & (kWave - 1);
   const int lrow = lane / L::CH, lcol = lane % L::CH;
@@ -95,10 +106,8 @@ __device__ __forceinline__ void tree_column(const TreeArgs& ta, const TreeItem& 
       const int u = u0 + lrow, pos = drafted ? it.prefix + u : u;
       bool seen = u < end;
       if (seen && drafted) {
-        const int v = u - t0, wave = v / L::STEP, e = v % L::STEP / L::TPL, row = v % L::TPL;
-        const int group = D == 64 ? row & 3 : D == 128 ? row : 2 * (wave & 1) + row;
-        const int tile = D == 64 ? 2 * wave + (row >> 2) : D == 128 ? wave : wave >> 1;
-        seen = mask[(r - it.np) * L::BLOCKS + tile] >> (16 * (group & 1) + 8 * (group >> 1) + e) & 1;
+        const TilePlace at = tile_place(D, u);
+        seen = mask[at.tile] >> mask_bit(at) & 1;
       }
       int p = -1;
       if (seen) {
@@ -164,19 +173,9 @@ __device__ __forceinline__ int64_t part_row(const TreeArgs& ta, const TreeItem& 
          it.head * ta.d.ratio + c % ta.d.ratio;
 }
 
-// vt[e]: dim 8 chunk + e of the lane's 8 tokens.
-template <typename V8>
-__device__ __forceinline__ void tree_transpose8(const V8 (&v)[8], V8 (&vt)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    u32x4 d;
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-      d[x] = __builtin_amdgcn_perm(__builtin_bit_cast(u32x4, v[2 * x + 1])[e >> 1],
-                                   __builtin_bit_cast(u32x4, v[2 * x])[e >> 1],
-                                   (e & 1) ? 0x07060302u : 0x05040100u);
-    vt[e] = __builtin_bit_cast(V8, d);
-  }
+// The tokens' dwords x and y (2 dims each) to those of dim 2 d + odd.
+__device__ __forceinline__ uint32_t dim_pair(uint32_t x, uint32_t y, int odd) {
+  return __builtin_amdgcn_perm(y, x, odd ? 0x07060302u : 0x05040100u);
 }
 
 // A workgroup has 32 WC columns: wave w takes those of tile w % WC and, of each round,
@@ -184,21 +183,27 @@ __device__ __forceinline__ void tree_transpose8(const V8 (&v)[8], V8 (&vt)[8]) {
 // as the 8 tokens of a lane for each dim. S^T = K Q^T and O^T = V^T P^T on 32x32 tiles,
 // so that a column's scores are in the registers of its two lanes, where its
 // probabilities are the second product's operand.
+// Of the 24 products of a tile at head_dim 128 eight are the second terms of the
+// probabilities. 64 rows of 4096 tokens (bf16, 32/8 heads of 128): 8 tokens each 172 us a
+// layer, 6.25 TB/s, as fast as single tokens; 32 each 272 us, of which the products take
+// 165 at a large product's rate; 64 each 446 us and 335.
 template <typename T, int D, int WC>
-__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_kernel(TreeArgs ta) {
+__global__ __launch_bounds__((TreeTile<D, WC>::WAVES * kWave), D == 256 ? 1 : 2) void tree_attention_kernel(TreeArgs ta) {
   typedef typename Vec<T>::v8 V8;
-  typedef TreeTile<D> L;
+  typedef TreeTile<D, WC> L;
   constexpr int STEP = L::STEP, TPL = L::TPL, LOADS = L::LOADS, CH = L::CH;
   constexpr int KS = D / 16;           // products of a score tile
   constexpr int OT = D / 32;           // output tiles of a column tile
-  constexpr int WT = kWaves / WC;      // shares of a round's tokens
+  constexpr int WAVES = L::WAVES;
+  constexpr int WT = WAVES / WC;      // shares of a round's tokens
   constexpr int GB = L::BLOCKS / WT;   // score tiles of a share
   static_assert(GB >= 1, "a share has a tile at least");
   constexpr int KBYTES = L::ROUND * D * 2;
+  constexpr int BUFS = WAVES > kWaves ? 2 : 1;
   const DecodeArgs& a = ta.d;
-  __shared__ __attribute__((aligned(16))) char s_raw[2 * KBYTES];   // K, V; in the end O
-  __shared__ uint32_t s_drop[2 * kWaves];   // tokens of the round's tiles that nobody sees
-  __shared__ float s_ml[kWaves][2][kWave];
+  __shared__ __attribute__((aligned(16))) char s_raw[BUFS * 2 * KBYTES];   // K, V; in the end O
+  __shared__ uint32_t s_drop[BUFS][2 * WAVES];   // tokens of a round that nobody sees, by wave
+  __shared__ float s_ml[WAVES][2][kWave];
 
   const TreeItem it = tree_item(ta.records + kTreeRecord * int64_t(blockIdx.x));
   if (it.tokens == 0) return;
@@ -213,6 +218,12 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
   const int hq = it.head * a.ratio + c - token * a.ratio;
   const int page_mask = (1 << a.page_shift) - 1;
 
+  // (A copy of a lane's number that keeps what is made from it where it is made: what
+  // seldom runs has its addresses to itself.)
+  auto here = [](int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+  };
   // ---- loads. A round's tokens of a wave are STEP; cached ones lie in pages whose ids a
   // register's lanes hold, one for `granule` tokens, a round ahead of the loads.
   const int gshift = min(a.page_shift, 4);
@@ -236,15 +247,15 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
   V8 k[LOADS], v[LOADS];
   uint32_t bad = 0;   // bit i: the lane's row of load i is no token that anybody sees
   // Page ids outside the pool, and tokens behind the cached ones, read page 0.
-  auto load_cached = [&](int r, int ids, auto loads_per_page) {
+  auto load_cached = [&](int r, int ids, auto loads_per_page) __attribute__((always_inline)) {
     constexpr int P = decltype(loads_per_page)::value;   // 0: two pages to a load
-    constexpr int N = P ? LOADS / P : 2 * LOADS;         // granules
+    constexpr int G = P ? LOADS / P : 2 * LOADS;         // granules
     const int t0 = r * L::ROUND + wave * STEP;
     bad = 0;
-    int64_t at[N];   // bytes from the head's base
+    int64_t at[G];   // bytes from the head's base
     uint32_t gone = 0;
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
+    for (int n = 0; n < G; ++n) {
       const int t = t0 + (P ? n * P * TPL : n * (TPL / 2));
       const int p = __builtin_amdgcn_readlane(ids, n);
       const bool ok = t < it.prefix && p >= 0 && p < a.num_pages;
@@ -274,7 +285,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
   typedef std::integral_constant<int, 16 / TPL> Pages16;
   typedef std::integral_constant<int, TPL == 8 ? 0 : 4 / TPL> Pages4;
   typedef std::integral_constant<int, TPL == 8 ? 1 : 8 / TPL> Pages8;
-  auto load_round = [&](int r, int ids) {
+  auto load_round = [&](int r, int ids) __attribute__((always_inline)) {
     if (r < it.np) {   // uniform
       if (a.page_shift >= 4)
         load_cached(r, ids, Pages16{});
@@ -328,43 +339,44 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
 
   // LDS addresses as one register each and constants: with one for each chunk they were
   // spilled, and their reloads waited for the loads on their way.
-  // Row `col` of a score tile is element e of lane group g (TreeTile).
+  // Row `col` of a score tile is element e of lane group g; its token's row in the round:
   const int e = ((col >> 3) & 1) * 4 + (col & 3), g = 2 * (col >> 4) + ((col >> 2) & 1);
-  // Chunk c of token row (e, g) lies at c ^ swz: the 16 rows that 16 lanes read differ in
-  // it, and so do those of a load, whose rows have e = i.
-  auto swz = [](int e, int g) { return D == 64 ? e : 2 * e + (g & 1); };
-  auto swz_of = [](int i) { return D == 64 ? i : 2 * i; };   // of load i, but for its group
-  const int k_row = (D == 64 ? 8 * e + g : D == 128 ? 4 * e + g : 16 * (g >> 1) + 2 * e + (g & 1)) * CH;
+  const int k_row = D == 64 ? 8 * e + g : D == 128 ? 4 * e + g : 16 * (g >> 1) + 2 * e + (g & 1);
   auto tile_row0 = [](int blk) { return D == 64 ? 64 * (blk >> 1) + 4 * (blk & 1) : 32 * blk; };
+  // Chunk c of token row (e, g) lies at c ^ swz: the 16 rows that 16 lanes read differ in
+  // it. A load's rows have one e.
+  auto swz = [](int e, int g) { return D == 64 ? e : 2 * e + (g & 1); };
   auto moved = [](int base, int bits) {   // base ^ bits, made at each use
     asm volatile("v_xor_b32 %0, %1, %2" : "=v"(base) : "n"(bits), "v"(base));
     return base;
   };
-  const int own_g = D == 64 ? lrow & 3 : D == 128 ? lrow : 2 * (wave & 1) + lrow;
-  const int own_blk = D == 64 ? 2 * wave + (lrow >> 2) : D == 128 ? wave : wave >> 1;
+  // What a lane loads: element own.e + i of lane group own.g of tile own.tile.
+  const TilePlace own = tile_place(D, wave * STEP + lrow);
   // Chunk l of a lane group's V: at head_dim 64 two groups fill 16 lanes, apart by an XOR.
   auto v_chunk = [](int g, int l) { return D == 64 ? l ^ ((g & 1) << 3) : l; };
-  const int k_read = 16 * (k_row + (h ^ swz(e, g)));
+  const int k_read = 16 * (k_row * CH + (h ^ swz(e, g)));
   const int v_read = KBYTES + 16 * (h * D + v_chunk(h, col));
-  const int k_park = 16 * ((wave * STEP + lrow) * CH + (lcol ^ (D == 64 ? 0 : own_g & 1)));
-  const int v_park = KBYTES + 16 * ((own_blk * 4 + own_g) * D + v_chunk(own_g, lcol));
+  const int k_park = 16 * ((wave * STEP + lrow) * CH + (lcol ^ swz(own.e, own.g)));
+  const int v_park = KBYTES + 16 * ((own.tile * 4 + own.g) * D + v_chunk(own.g, lcol)) + 2 * own.e;
 
   auto sync = [&] {
     // Where a share's tokens are those that its only wave has loaded, LDS order will do.
-    if constexpr (WC == 1 && WT == kWaves)
+    if constexpr (WC == 1 && WT == WAVES)
       __builtin_amdgcn_wave_barrier();
     else
       __syncthreads();
   };
 
-  for (int r = it.rb; r < it.re; ++r) {
+  // The loaded round r to LDS.
+  auto stage = [&](int r, int buf) __attribute__((always_inline)) {
     const bool drafted = r >= it.np;   // uniform
-    if (drafted && a.k_new) {   // uniform: rows whose first column is the workgroup's, to their pages
+    if (drafted && a.k_new) {   // rows whose first column is the workgroup's, to their pages
       const int lo = (it.c0 + a.ratio - 1) / a.ratio;
       const int hi = min(it.tokens, (it.c0 + it.cols + a.ratio - 1) / a.ratio);
+      const int lr = here(lrow);
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int u = (r - it.np) * L::ROUND + wave * STEP + i * TPL + lrow, pos = it.prefix + u;
+        const int u = (r - it.np) * L::ROUND + wave * STEP + i * TPL + lr, pos = it.prefix + u;
         if (u < lo || u >= hi || (bad >> i & 1)) continue;
         const int64_t at = head_at +
                            int64_t(a.indices[it.page_at + (pos >> a.page_shift)]) * a.page_stride +
@@ -373,118 +385,154 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
         *reinterpret_cast<V8*>(const_cast<f16*>(a.v) + at) = v[i];
       }
     }
-    // K and V to LDS. V of a token that nobody sees has to be 0: 0 x V is.
+    // V of a token that nobody sees has to be 0: 0 x V is.
     const bool any_bad = __any(bad != 0);
     if (any_bad) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i)
         if (bad >> i & 1) v[i] = V8{};
     }
+    char* const to = s_raw + buf * 2 * KBYTES;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
-      *reinterpret_cast<V8*>(s_raw + moved(k_park, 16 * swz_of(i)) + 16 * i * TPL * CH) = k[i];
-    V8 vt[8];
-    tree_transpose8(v, vt);
+      *reinterpret_cast<V8*>(to + moved(k_park, 16 * (D == 64 ? i : 2 * i)) + 16 * i * TPL * CH) = k[i];
 #pragma unroll
-    for (int x = 0; x < 8; ++x)   // (an XOR of 8 chunks is one of rows of 8)
-      *reinterpret_cast<V8*>(s_raw + (D == 64 ? moved(v_park, 16 * x * CH) : v_park + 16 * x * CH)) = vt[x];
-    {
-      // Bit 16 h + 8 s + e of a tile's word: element e of lane group 2 s + h.
-      uint32_t word[2] = {0u, 0u};   // at head_dim 64 a wave's two tiles
-      if (any_bad) {
+    for (int x = 0; x < 8; ++x) {   // dim 8 lcol + x of the lane's tokens
+      // (at head_dim 64 rows of 8 chunks, their XOR is one of rows)
+      char* const at = to + (D == 64 ? moved(v_park, 16 * x * CH) : v_park + 16 * x * CH);
+      uint32_t d[LOADS / 2];
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-          const uint64_t rows = __ballot(bad >> i & 1);
+      for (int y = 0; y < LOADS / 2; ++y)
+        d[y] = dim_pair(__builtin_bit_cast(u32x4, v[2 * y])[x >> 1],
+                        __builtin_bit_cast(u32x4, v[2 * y + 1])[x >> 1], x & 1);
+      if constexpr (LOADS == 8)
+        *reinterpret_cast<u32x4*>(at) = u32x4{d[0], d[1], d[2], d[3]};
+      else
+        *reinterpret_cast<uint64_t*>(at) = uint64_t(d[0]) | uint64_t(d[1]) << 32;
+    }
+    uint32_t word[2] = {0u, 0u};   // at head_dim 64 a wave's two tiles
+    if (any_bad) {
+      const uint32_t bits = bad << mask_bit(own);   // (elements own.e + i)
 #pragma unroll
-          for (int l = 0; l < TPL; ++l) {
-            const int gr = D == 64 ? l & 3 : D == 128 ? l : l + 2 * (wave & 1);
-            word[D == 64 ? l >> 2 : 0] |= uint32_t(rows >> (l * CH) & 1) << (16 * (gr & 1) + 8 * (gr >> 1) + i);
-          }
-        }
+      for (int l = 0; l < TPL; ++l)
+        word[D == 64 ? l >> 2 : 0] |= uint32_t(__builtin_amdgcn_readlane(int(bits), l * CH));
+    }
+    if (lane < 2) s_drop[buf][2 * wave + lane] = lane ? word[1] : word[0];
+  };
+  // Tokens of tile blk that nobody sees.
+  auto dropped = [&](int buf, int blk) {
+    constexpr int PER = 32 / (D == 64 ? STEP / 2 : STEP);   // waves that load a tile
+    const int w0 = D == 64 ? (blk >> 1) * PER : blk * PER;
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) w |= s_drop[buf][2 * (w0 + i) + (D == 64 ? blk & 1 : 0)];
+    return w;
+  };
+
+  // This wave's tiles of round r.
+  auto compute = [&](int r, int buf) __attribute__((always_inline)) {
+    const bool drafted = r >= it.np;   // uniform
+    const uint32_t* mask = ta.masks + it.mask_at + int64_t(token) * it.mask_words +
+                           (r - it.np) * L::BLOCKS + wt * GB;
+    const int left = drafted ? it.tokens - (r - it.np) * L::ROUND : it.prefix - r * L::ROUND;
+#pragma unroll 1
+    for (int b = 0; b < GB; ++b) {
+      const int blk = wt * GB + b;
+      if ((tile_row0(blk) & ~31) >= left) break;   // uniform: no tokens from here on
+      const int k_at = k_read + buf * 2 * KBYTES + 16 * tile_row0(blk) * CH;
+      const int v_at = v_read + buf * 2 * KBYTES + 16 * 4 * D * blk;
+      // Operands are read together, V's while the scores become probabilities: read one
+      // by one before its product, each waited for LDS.
+      V8 ka[KS];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) ka[s] = *reinterpret_cast<const V8*>(s_raw + moved(k_at, 32 * s));
+      __builtin_amdgcn_sched_barrier(0);
+      f32x16 sc = {};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) sc = mfma32(ka[s], q[s], sc);
+      V8 va[2][OT];
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+        va[0][d] = *reinterpret_cast<const V8*>(s_raw + v_at + 16 * 32 * d);
+      __builtin_amdgcn_sched_barrier(0);
+      const uint32_t gone = __builtin_amdgcn_readfirstlane(dropped(buf, blk));
+      if (drafted || gone) {   // uniform
+        const uint32_t w = (drafted ? ~mask[b] | gone : gone) >> (16 * h);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) sc[x] = w >> x & 1 ? -INFINITY : sc[x];
       }
-      if (lane == 0) {
-        s_drop[D == 64 ? 2 * wave : wave] = word[0];
-        if (D == 64) s_drop[2 * wave + 1] = word[1];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) mx = fmaxf(mx, sc[x]);
+      if (__any(mx * a.scale_log2 > m + 8.f)) {
+        mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.scale_log2;
+        const float m_new = mx > m + 8.f ? mx : m;
+        const float alpha = fast_exp2(m - m_new);
+        m = m_new;
+        lsum *= alpha;
+#pragma unroll
+        for (int d = 0; d < OT; ++d)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[d][x] *= alpha;
+      }
+      // Probabilities in two 16-bit terms, as in every decode launch.
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        u32x4 h4, l4;
+#pragma unroll
+        for (int x = 0; x < 8; x += 2) {
+          const float p0 = fast_exp2(fmaf(sc[8 * s + x], a.scale_log2, -m));
+          const float p1 = fast_exp2(fmaf(sc[8 * s + x + 1], a.scale_log2, -m));
+          lsum += p0 + p1;
+          uint32_t hi, lo;
+          two_terms<T>(p0, p1, hi, lo);
+          h4[x / 2] = hi;
+          l4[x / 2] = lo;
+        }
+        const V8 ph = __builtin_bit_cast(V8, h4), pl = __builtin_bit_cast(V8, l4);
+        if (s == 0) {
+#pragma unroll
+          for (int d = 0; d < OT; ++d)
+            va[1][d] = *reinterpret_cast<const V8*>(s_raw + v_at + 16 * (2 * D + 32 * d));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d = 0; d < OT; ++d) o[d] = mfma32(va[s][d], ph, o[d]);
+#pragma unroll
+        for (int d = 0; d < OT; ++d) o[d] = mfma32(va[s][d], pl, o[d]);
       }
     }
+  };
+
+  auto next_round = [&](int r, int buf) __attribute__((always_inline)) {
+    if (r >= it.re) return;
+    stage(r, buf);
     if (r + 1 < it.re) {
       load_round(r + 1, ids);
       ids = ids_of(min(r + 2, it.re - 1));
     }
-    sync();
-    if (active) {
-      const uint32_t* mask = ta.masks + it.mask_at + int64_t(token) * it.mask_words +
-                             (r - it.np) * L::BLOCKS + wt * GB;
-      const int left = drafted ? it.tokens - (r - it.np) * L::ROUND : it.prefix - r * L::ROUND;
-#pragma unroll 1
-      for (int b = 0; b < GB; ++b) {
-        const int blk = wt * GB + b;
-        if ((tile_row0(blk) & ~31) >= left) break;   // uniform: no tokens from here on
-        const int k_at = k_read + 16 * tile_row0(blk) * CH, v_at = v_read + 16 * 4 * D * blk;
-        // Operands are read together, V's while the scores become probabilities: read one
-        // by one before its product, each waited for LDS.
-        V8 ka[KS];
-#pragma unroll
-        for (int s = 0; s < KS; ++s) ka[s] = *reinterpret_cast<const V8*>(s_raw + moved(k_at, 32 * s));
-        __builtin_amdgcn_sched_barrier(0);
-        f32x16 sc = {};
-#pragma unroll
-        for (int s = 0; s < KS; ++s) sc = mfma32(ka[s], q[s], sc);
-        V8 va[2][OT];
-#pragma unroll
-        for (int d = 0; d < OT; ++d)
-          va[0][d] = *reinterpret_cast<const V8*>(s_raw + v_at + 16 * 32 * d);
-        __builtin_amdgcn_sched_barrier(0);
-        uint32_t gone = D == 256 ? s_drop[2 * blk] | s_drop[2 * blk + 1] : s_drop[blk];
-        gone = __builtin_amdgcn_readfirstlane(gone);
-        if (drafted || gone) {   // uniform
-          const uint32_t w = (drafted ? ~mask[b] | gone : gone) >> (16 * h);
-#pragma unroll
-          for (int x = 0; x < 16; ++x) sc[x] = w >> x & 1 ? -INFINITY : sc[x];
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int x = 0; x < 16; ++x) mx = fmaxf(mx, sc[x]);
-        if (__any(mx * a.scale_log2 > m + 8.f)) {
-          mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.scale_log2;
-          const float m_new = mx > m + 8.f ? mx : m;
-          const float alpha = fast_exp2(m - m_new);
-          m = m_new;
-          lsum *= alpha;
-#pragma unroll
-          for (int d = 0; d < OT; ++d)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) o[d][x] *= alpha;
-        }
-        // Probabilities in two 16-bit terms, as in every decode launch.
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          u32x4 h4, l4;
-#pragma unroll
-          for (int x = 0; x < 8; x += 2) {
-            const float p0 = fast_exp2(fmaf(sc[8 * s + x], a.scale_log2, -m));
-            const float p1 = fast_exp2(fmaf(sc[8 * s + x + 1], a.scale_log2, -m));
-            lsum += p0 + p1;
-            uint32_t hi, lo;
-            two_terms<T>(p0, p1, hi, lo);
-            h4[x / 2] = hi;
-            l4[x / 2] = lo;
-          }
-          const V8 ph = __builtin_bit_cast(V8, h4), pl = __builtin_bit_cast(V8, l4);
-          if (s == 0) {
-#pragma unroll
-            for (int d = 0; d < OT; ++d)
-              va[1][d] = *reinterpret_cast<const V8*>(s_raw + v_at + 16 * (2 * D + 32 * d));
-          }
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int d = 0; d < OT; ++d) o[d] = mfma32(va[s][d], ph, o[d]);
-#pragma unroll
-          for (int d = 0; d < OT; ++d) o[d] = mfma32(va[s][d], pl, o[d]);
-        }
-      }
+  };
+  if constexpr (BUFS == 2) {
+    // Eight waves are alone on their CU: half of them stage the next round, in the other
+    // buffer, while the others compute, and the other way round. (Four waves leave that to
+    // the CU's second workgroup: with two buffers they took as long.)
+    const bool late = wave >= L::WAVES / 2;   // uniform
+    next_round(it.rb, 0);
+    __syncthreads();
+    for (int r = it.rb; r < it.re; ++r) {
+      const int buf = (r - it.rb) & 1;
+      if (late && active) compute(r, buf);
+      next_round(r + 1, buf ^ 1);
+      if (!late && active) compute(r, buf);
+      __syncthreads();
     }
-    sync();
+  } else {
+    for (int r = it.rb; r < it.re; ++r) {
+      next_round(r, 0);
+      sync();
+      if (active) compute(r, 0);
+      sync();
+    }
   }
 
   // Values that the products do not carry (0 x infinity of a token that a column does not
@@ -499,7 +547,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
       float m1, l1, acc[8];
-      tree_column<T, D>(ta, it, it.c0 + 32 * wc + j, wt * GB * kBlock, (wt + 1) * GB * kBlock, m1, l1, acc);
+      tree_column<T, D, WC>(ta, it, it.c0 + 32 * wc + j, wt * GB * kBlock, (wt + 1) * GB * kBlock, m1, l1, acc);
       const bool mine = col == j;
       if (mine) {
         m = m1;
@@ -570,34 +618,117 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void tree_attention_ker
   if (it.slot >= 0 && h == 0) a.part_lse[prow] = partial_lse(m, lsum);
 }
 
+// Columns of a workgroup for rows of up to `widest`: as few as hold them, four waves' up to
+// 128. More share what loads and stages K and V with eight waves at head_dim 128: 64 rows of
+// 4096 tokens, 256 columns, 446 us against 490; at 64 both take as long (16 rows, 88 us),
+// and at 256 a wave's registers are two waves'.
+int tree_columns(int head_dim, int64_t widest) {
+  if (head_dim == 256) return widest <= 64 ? 64 : 128;
+  if (widest <= 128 || head_dim == 64) return widest <= 32 ? 32 : widest <= 64 ? 64 : 128;
+  return 256;
+}
+int round_tokens(int head_dim) { return kWaves * 8 * kWave / (head_dim / 8); }
+
 template <typename T, int D>
-int launch_tree_dim(int col_waves, const TreeArgs& ta, unsigned blocks, hipStream_t s) {
-  constexpr int kLeast = D == 256 ? 2 : 1;   // (a round has two score tiles there)
-  switch (col_waves) {
-    case 1: tree_attention_kernel<T, D, kLeast><<<blocks, kThreads, 0, s>>>(ta); break;
-    case 2: tree_attention_kernel<T, D, 2><<<blocks, kThreads, 0, s>>>(ta); break;
-    default: tree_attention_kernel<T, D, 4><<<blocks, kThreads, 0, s>>>(ta);
+int launch_tree_dim(int columns, const TreeArgs& ta, unsigned blocks, hipStream_t s) {
+  if constexpr (D == 256) {
+    if (columns == 64)
+      tree_attention_kernel<T, D, 2><<<blocks, kThreads, 0, s>>>(ta);
+    else
+      tree_attention_kernel<T, D, 4><<<blocks, kThreads, 0, s>>>(ta);
+  } else {
+    if constexpr (D == 128) {
+      if (columns == 256) tree_attention_kernel<T, D, 8><<<blocks, 2 * kThreads, 0, s>>>(ta);
+    }
+    switch (columns) {
+      case 32: tree_attention_kernel<T, D, 1><<<blocks, kThreads, 0, s>>>(ta); break;
+      case 64: tree_attention_kernel<T, D, 2><<<blocks, kThreads, 0, s>>>(ta); break;
+      case 128: tree_attention_kernel<T, D, 4><<<blocks, kThreads, 0, s>>>(ta); break;
+    }
   }
   KSV_CHECK_LAUNCH();
   return KUNSERVE_OK;
 }
 
 template <typename T>
-int launch_tree(int head_dim, int col_waves, const TreeArgs& ta, unsigned blocks, hipStream_t s) {
+int launch_tree(int head_dim, int columns, const TreeArgs& ta, unsigned blocks, hipStream_t s) {
   switch (head_dim) {
-    case 64: return launch_tree_dim<T, 64>(col_waves, ta, blocks, s);
-    case 128: return launch_tree_dim<T, 128>(col_waves, ta, blocks, s);
-    default: return launch_tree_dim<T, 256>(col_waves, ta, blocks, s);
+    case 64: return launch_tree_dim<T, 64>(columns, ta, blocks, s);
+    case 128: return launch_tree_dim<T, 128>(columns, ta, blocks, s);
+    default: return launch_tree_dim<T, 256>(columns, ta, blocks, s);
   }
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-constexpr int kTileCols = 32;   // columns of a wave
-
 struct TreeRow {
   int32_t tokens, q_first, prefix, page_at, mask_at, mask_words, np, rounds;
 };
+
+// Rounds [rb, re) of a row to a workgroup for each KV head and column tile: of parts as
+// long as one another, none longer than `run`.
+int32_t part_rounds_of(const TreeRow& r, int64_t run) {
+  return int32_t(ceil_div(r.rounds, ceil_div(r.rounds, run)));
+}
+
+// The run of rounds that ends first: workgroups go, longest first, to the place that is
+// free first, of `places` on the device, and cost a round more than they have; joining
+// partials costs a round and the time that their bytes take at the rate of a round's.
+// (Against the time of every run, 13 shapes: the run taken 4% from the best at most, on
+// average 0.5%; with work / places to each, as far as 20% off: 32 rows of 256 to 6000 tokens
+// 115 us against 130, 4 of 4096 at head_dim 256 67 against 86, 21 whole rows of 40 to 1800 44
+// against 50.)
+int64_t best_run(const std::vector<TreeRow>& rows, int32_t longest, int64_t work, int cols, int ratio,
+                 int32_t num_kv_heads, int round, int64_t places) {
+  const int64_t even = std::max<int64_t>(1, ceil_div(work, places));
+  int64_t best = std::max(longest, 1);
+  double least = 0;
+  auto attempt = [&](int64_t run) {
+    std::map<int64_t, int64_t> items, load;   // workgroups by cost; places by when they are free
+    int64_t slots = 0;
+    for (const TreeRow& r : rows) {
+      if (r.tokens == 0) continue;
+      const int64_t len = part_rounds_of(r, run), parts = ceil_div(r.rounds, len);
+      const int64_t each = num_kv_heads * ceil_div(int64_t(r.tokens) * ratio, cols);
+      if (parts > 1) {
+        items[len + 1] += (parts - 1) * each;
+        slots += parts * r.tokens;
+      }
+      items[r.rounds - (parts - 1) * len + 1] += each;
+    }
+    load[0] = places;
+    for (auto i = items.rbegin(); i != items.rend(); ++i) {
+      for (int64_t left = i->second; left > 0;) {
+        const auto first = load.begin();
+        const int64_t at = first->first, n = std::min(left, first->second);
+        if (n == first->second)
+          load.erase(first);
+        else
+          first->second -= n;
+        load[at + i->first] += n;
+        left -= n;
+      }
+    }
+    // (A partial of a head is 4 bytes a dim, written and read; a round's token 4 bytes a dim.)
+    const double end = double(load.rbegin()->first) + (slots ? 1 : 0) +
+                       2.0 * double(slots) * ratio * num_kv_heads / (double(places) * round);
+    if (least == 0 || end < least) {
+      least = end;
+      best = run;
+    }
+  };
+  attempt(best);
+  // Equal parts of the longest row, down to half an even share.
+  for (int64_t parts = 2, last = best; parts <= 64; ++parts) {
+    const int64_t run = ceil_div(longest, parts);
+    if (2 * run < even || run == last) break;
+    last = run;
+    attempt(run);
+  }
+  for (int64_t run : {even, even + (even + 3) / 4, even + (even + 1) / 2})
+    if (run < longest) attempt(run);
+  return best;
+}
 
 int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_first,
               const int32_t* kv_len, const int32_t* parents, int32_t num_seqs,
@@ -605,16 +736,14 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
               int32_t num_cus, int32_t part_rounds, std::vector<int32_t>& plan,
               kunserve_tree_plan_info* info) {
   const int ratio = num_qo_heads / num_kv_heads;
+  int64_t widest = 0;
+  for (int32_t b = 0; b < num_seqs; ++b)
+    widest = std::max(widest, (int64_t(q_indptr[b + 1]) - q_indptr[b]) * ratio);
+  const int max_cols = tree_columns(head_dim, widest);
   const int round = round_tokens(head_dim), tiles = round / kBlock;
   const int64_t cus = num_cus > 0 ? num_cus : 256;
   std::vector<TreeRow> rows(num_seqs);
   std::vector<uint32_t> masks;
-  // Waves along the columns: as few as hold the widest row's.
-  int32_t widest = 0;
-  for (int32_t b = 0; b < num_seqs; ++b)
-    widest = std::max(widest, std::min(q_indptr[b + 1] - q_indptr[b], 128) * ratio);
-  const int col_waves = widest <= kTileCols && head_dim != 256 ? 1 : widest <= 2 * kTileCols ? 2 : 4;
-  const int max_cols = kTileCols * col_waves;
   int64_t work = 0;   // rounds of all workgroups
   int32_t longest = 0;
   for (int32_t b = 0; b < num_seqs; ++b) {
@@ -641,16 +770,16 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
       KSV_CHECK_ARG(up[i] >= -1 && up[i] < i, "row %d: token %d has parent %d", b, i, up[i]);
       uint32_t* own = m + size_t(i) * r.mask_words;
       if (up[i] >= 0) std::copy_n(m + size_t(up[i]) * r.mask_words, r.mask_words, own);
-      int tile, bit;
-      mask_bit(head_dim, i % round, &tile, &bit);
-      own[i / round * tiles + tile] |= 1u << bit;
+      const TilePlace at = tile_place(head_dim, i);
+      own[at.tile] |= 1u << mask_bit(at);
     }
     work += n ? int64_t(r.rounds) * ceil_div(int64_t(n) * ratio, max_cols) * num_kv_heads : 0;
     if (n) longest = std::max(longest, r.rounds);
   }
-  // A workgroup's run of rounds: what gives every CU two of them.
-  int64_t run = part_rounds > 0 ? part_rounds : std::max<int64_t>(1, ceil_div(work, 2 * cus));
-  run = std::min<int64_t>(run, std::max(longest, 1));
+  const int64_t slots_at_once = (head_dim == 256 || max_cols == 256 ? 1 : 2) * cus;
+  const int64_t run = part_rounds > 0
+                          ? std::min<int64_t>(part_rounds, std::max(longest, 1))
+                          : best_run(rows, longest, work, max_cols, ratio, num_kv_heads, round, slots_at_once);
 
   struct Piece {
     int32_t row, part, rb, re;
@@ -661,8 +790,7 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
   for (int32_t b = 0; b < num_seqs; ++b) {
     const TreeRow& r = rows[b];
     if (r.tokens == 0) continue;
-    parts[b] = int32_t(ceil_div(r.rounds, run));
-    const int32_t len = int32_t(ceil_div(r.rounds, parts[b]));
+    const int32_t len = part_rounds_of(r, run);
     parts[b] = int32_t(ceil_div(r.rounds, len));
     for (int32_t i = 0; i < parts[b]; ++i)
       pieces.push_back({b, i, i * len, std::min(r.rounds, (i + 1) * len)});
@@ -690,7 +818,7 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
                         {r.tokens, r.q_first, r.prefix, r.page_at, c, std::min(max_cols, cols - c),
                          h, r.np, p.rb, p.re, slot[p.row], parts[p.row], p.part, r.mask_at,
                          r.mask_words, 0});
-        load[x] += p.re - p.rb;
+        load[x] += p.re - p.rb + 1;
       }
       depth = std::max(depth, lanes[x].size() / kTreeRecord);
     }
@@ -702,7 +830,7 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
   info->num_work = int32_t(kXcds * depth);
   info->num_merge = int32_t(merges.size() / 4);
   info->num_slots = int32_t(slots);
-  info->columns = col_waves;
+  info->columns = max_cols;
   info->num_seqs = num_seqs;
   info->head_dim = head_dim;
   info->page_size = page_size;
@@ -728,13 +856,14 @@ extern "C" int64_t kunserve_tree_plan_bound(const int32_t* q_indptr_host,
       (num_seqs > 0 && (!q_indptr_host || !kv_len_host)) ||
       (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return -1;
+  // (The fewest columns to a workgroup of any plan.)
   const int64_t round = round_tokens(head_dim), ratio = ceil_div(num_qo_heads, num_kv_heads);
   int64_t items = 0, rest = 0;
   for (int32_t b = 0; b < num_seqs; ++b) {
     const int64_t n = std::max<int64_t>(0, int64_t(q_indptr_host[b + 1]) - q_indptr_host[b]);
     const int64_t rounds = ceil_div(std::max(kv_len_host[b], 0), round) + 1;
     items += rounds * num_kv_heads * ceil_div(n * ratio, 32);
-    rest += n * (4 + ceil_div(n, round) * round / kBlock);
+    rest += n * (4 + ceil_div(n, 256) * (256 / kBlock));
   }
   return kTreeRecord * kXcds * items + rest;
 }
@@ -799,8 +928,8 @@ int kunserve::tree_attention(const kunserve_kv_pool* pool, int32_t layer,
                 info->num_kv_heads, num_qo_heads, pool->num_kv_heads);
   KSV_CHECK_ARG(info->num_seqs == table->num_seqs, "plan made for %d rows, not %d", info->num_seqs,
                 table->num_seqs);
-  KSV_CHECK_ARG(info->columns == 1 || info->columns == 2 || info->columns == 4,
-                "plan of %d waves along the columns", info->columns);
+  KSV_CHECK_ARG(tree_columns(info->head_dim, info->columns) == info->columns,
+                "plan of %d columns to a workgroup", info->columns);
   KSV_CHECK_ARG(pool->token_stride < (int64_t(1) << 28),
                 "tokens %lld elements apart: less than 2^28 here", (long long)pool->token_stride);
   KSV_CHECK_ARG(num_qo_heads < 65536, "%d query heads: at most 65535", num_qo_heads);

@@ -51,7 +51,7 @@ def test_records_cover_every_column_and_round_once(dim, part_rounds, ratio, hkv)
         b = [i for i in range(len(sizes)) if first[i] == q0 and sizes[i] == tokens][0]
         assert prefix == lens[b] - sizes[b] and np_ == -(-prefix // ROUND[dim])
         assert 0 <= rb < re <= np_ + -(-tokens // ROUND[dim])
-        assert 0 < cols <= 128 and c0 + cols <= tokens * ratio
+        assert 0 < cols <= plan.info.columns <= (256 if dim == 128 else 128) and c0 + cols <= tokens * ratio
         assert (slot < 0) == (n == 1) and 0 <= part < n
         for c in range(c0, c0 + cols):
             for i in range(rb, re):
@@ -69,6 +69,22 @@ def test_records_cover_every_column_and_round_once(dim, part_rounds, ratio, hkv)
         b = [i for i in range(len(sizes)) if first[i] <= token < first[i + 1]][0]
         assert {v[0] + (token - first[b]) * v[1] for k, v in seen.items() if k[0] == b} == {s0}
     assert used == set(range(plan.info.num_slots))
+
+
+@pytest.mark.parametrize("lens,tokens,hkv,dim,split,workgroups", [
+    ([1508], 8, 8, 128, True, 104),             # one row: a round to a workgroup
+    ([4104] * 64, 8, 8, 128, False, 512),       # two whole rows and heads to a CU
+    ([4104] * 16, 8, 8, 128, True, 512),        # a quarter of a row
+    ([1000] * 21, 16, 32, 64, False, 672),      # whole rows end before halves would
+    ([4160] * 4, 64, 4, 256, True, 256),        # one workgroup to a CU
+], ids=["one", "filled", "quarters", "nearly", "dim256"])
+def test_runs_fill_the_device(lens, tokens, hkv, dim, split, workgroups):
+    trees = [list(range(-1, tokens - 1))] * len(lens)
+    plan = make(np.array(lens), trees, hkv * (1 if dim == 64 else 4), hkv, dim, cus=256)
+    rec, _, _ = parts(plan)
+    rec = rec[rec[:, 0] > 0]
+    assert (plan.info.num_slots > 0) == split
+    assert abs(len(rec) - workgroups) <= workgroups // 8, len(rec)
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256])

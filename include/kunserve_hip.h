@@ -657,12 +657,26 @@ int kunserve_keep_tokens(const kunserve_kv_pool* pool, const kunserve_kv_weights
                          const int32_t* kept_dev, int64_t kept_stride, int32_t max_kept,
                          kunserve_stream_t stream);
 
-/* For each move (source page, destination page, tokens; device int32 [n][3]) the
- * page's first `tokens` slots are copied, K, V and weights (NULL: none), in every
- * layer. No destination is a source or in two moves. A move with a page outside the
- * pool is left out. */
+/* The moves (kunserve_copy_pages) after which rows go on in page lists of their own.
+ * Host arrays: list b of 2 num_seqs is indices_host[indptr_host[b] .. indptr_host[b + 1]),
+ * row b's those of b and of num_seqs + b, ceil(kv_len_host[b] / page_size) pages each.
+ * Where a row's two pages differ the first one's tokens in use move to the second. Writes
+ * up to `capacity` moves (int32 [capacity][3], the lists' pages / 2 are enough) and
+ * returns their number, negative on a bad argument; so is a page that is moved to and
+ * in the first list of a row or moved to twice. */
+int64_t kunserve_fork_moves(const int32_t* indptr_host, const int32_t* indices_host,
+                            const int32_t* kv_len_host, int32_t num_seqs, int32_t page_size,
+                            int64_t num_pages, int32_t* moves_host, int64_t capacity);
+
+/* For each move (source page, destination page, tokens; int32 [n][3]) the page's first
+ * `tokens` slots are copied, K, V and weights (NULL: none), in every layer. The moves are
+ * at moves_dev or, up to KUNSERVE_MOVES_BY_VALUE of them, at moves_host (the other is
+ * NULL): they go with the launch, and the array is the caller's again. No destination is
+ * a source or in two moves. A move with a page outside the pool is left out. */
+#define KUNSERVE_MOVES_BY_VALUE 256
 int kunserve_copy_pages(const kunserve_kv_pool* pool, const kunserve_kv_weights* weights,
-                        const int32_t* moves_dev, int64_t n, kunserve_stream_t stream);
+                        const int32_t* moves_host, const int32_t* moves_dev, int64_t n,
+                        kunserve_stream_t stream);
 
 /* ------------------------------------------------ a step's layers */
 

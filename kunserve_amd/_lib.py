@@ -19,6 +19,7 @@ ERANGE = -2
 ENOSPC = -3
 EUNSUPPORTED = -4
 EHIP = -5
+MOVES_BY_VALUE = 256
 _CODE_NAMES = {EINVAL: "EINVAL", ERANGE: "ERANGE", ENOSPC: "ENOSPC",
                EUNSUPPORTED: "EUNSUPPORTED", EHIP: "EHIP"}
 
@@ -172,8 +173,10 @@ SIGNATURES = {
                                         c_void_p]),
     "kunserve_keep_tokens": (c_int, [POINTER(KVPool), POINTER(KVWeights), POINTER(PageTable),
                                      c_void_p, c_void_p, c_int64, c_int32, c_void_p]),
-    "kunserve_copy_pages": (c_int, [POINTER(KVPool), POINTER(KVWeights), c_void_p, c_int64,
-                                    c_void_p]),
+    "kunserve_fork_moves": (c_int64, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int64,
+                                      c_void_p, c_int64]),
+    "kunserve_copy_pages": (c_int, [POINTER(KVPool), POINTER(KVWeights), c_void_p, c_void_p,
+                                    c_int64, c_void_p]),
     "kunserve_shared_plan_bound": (c_int64, [c_void_p, c_int32, c_int32]),
     "kunserve_shared_plan": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,
                                      c_int32, c_int32, c_int32, c_int64, c_void_p, c_int64,
@@ -257,6 +260,7 @@ class KunserveError(RuntimeError):
     def __init__(self, func: str, code: int, message: str):
         super().__init__(f"{func} failed ({_CODE_NAMES.get(code, code)}): {message}")
         self.code = code
+        self.detail = message
 
 
 def lib() -> ctypes.CDLL:

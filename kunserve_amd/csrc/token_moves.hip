@@ -4,6 +4,9 @@
 // (LlamaOp.local_copy_blocks, kunserve/worker.py:818-823).
 //
 // Both are HBM-bound copies of 16-byte chunks: what moves is read and written once.
+#include <algorithm>
+#include <vector>
+
 #include "common.hpp"
 
 namespace kunserve {
@@ -107,22 +110,31 @@ struct CopyArgs {
   int64_t page_stride, layer_stride, head_stride, token_stride;
   float* w;
   int64_t w_page, w_layer, w_head;
-  const int32_t* moves;   // [n][3]: source page, destination page, tokens
   int32_t num_pages;
   int32_t page_size;
   int32_t num_heads;
   int32_t heads;          // heads of a workgroup
 };
 
+// [n][3]: source page, destination page, tokens. Few of them go with the launch's
+// arguments: an upload of their own takes longer than they do (8 samples' last pages, with
+// building the table: 34 us against 40).
+struct MovesThere {
+  const int32_t* m;
+};
+struct MovesHere {
+  int32_t m[3 * KUNSERVE_MOVES_BY_VALUE];
+};
+
 // Workgroup (move, layer and K or V, head group): the waves take the loads of its heads'
 // tokens in turn.
-template <int D>
-__global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyArgs a) {
+template <int D, typename Moves>
+__global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyArgs a, Moves moves) {
   constexpr int CH = D / 8;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
-  const int32_t* m = a.moves + 3 * int64_t(blockIdx.x);
-  const int from = m[0], to = m[1], tokens = min(m[2], a.page_size);
+  const int64_t at3 = 3 * int64_t(blockIdx.x);
+  const int from = moves.m[at3], to = moves.m[at3 + 1], tokens = min(moves.m[at3 + 2], a.page_size);
   if (from < 0 || from >= a.num_pages || to < 0 || to >= a.num_pages || tokens <= 0) return;
   const int layer = int(blockIdx.y) >> 1;
   const bool of_v = blockIdx.y & 1;
@@ -155,6 +167,18 @@ __global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyArgs a) {
         w[int64_t(to) * a.w_page + int64_t(h) * a.w_head + t] =
             w[int64_t(from) * a.w_page + int64_t(h) * a.w_head + t];
     }
+  }
+}
+
+template <int D>
+void copy_pages(dim3 grid, const CopyArgs& a, const int32_t* moves_host, const int32_t* moves_dev,
+                int64_t n, hipStream_t s) {
+  if (moves_host) {
+    MovesHere here;
+    std::copy_n(moves_host, 3 * n, here.m);
+    copy_pages_kernel<D><<<grid, kThreads, 0, s>>>(a, here);
+  } else {
+    copy_pages_kernel<D><<<grid, kThreads, 0, s>>>(a, MovesThere{moves_dev});
   }
 }
 
@@ -232,8 +256,55 @@ extern "C" int kunserve_keep_tokens(const kunserve_kv_pool* pool,
   return KUNSERVE_OK;
 }
 
+extern "C" int64_t kunserve_fork_moves(const int32_t* indptr_host, const int32_t* indices_host,
+                                       const int32_t* kv_len_host, int32_t num_seqs,
+                                       int32_t page_size, int64_t num_pages, int32_t* moves_host,
+                                       int64_t capacity) {
+  clear_error();
+  KSV_CHECK_ARG(num_seqs >= 0 && page_size > 0 && num_pages >= 0 && num_pages < (int64_t(1) << 31),
+                "bad num_seqs, page_size or num_pages");
+  if (num_seqs == 0) return 0;
+  KSV_CHECK_ARG(indptr_host && kv_len_host && indices_host && (moves_host || capacity == 0),
+                "null table or moves");
+  int64_t n = 0;
+  const int rc = no_throw([&]() -> int {
+    enum : uint8_t { kFree, kHeld, kTaken };
+    std::vector<uint8_t> use(static_cast<size_t>(num_pages), kFree);
+    auto pages = [&](int32_t b) { return indices_host + indptr_host[b]; };
+    auto count = [&](int32_t b) { return (int64_t(kv_len_host[b]) + page_size - 1) / page_size; };
+    for (int32_t b = 0; b < num_seqs; ++b) {
+      KSV_CHECK_ARG(kv_len_host[b] >= 0, "row %d: %d tokens", b, kv_len_host[b]);
+      for (int32_t list : {b, num_seqs + b}) {
+        KSV_CHECK_ARG(indptr_host[list + 1] - int64_t(indptr_host[list]) >= count(b),
+                      "row %d: %lld pages for %d tokens", b,
+                      (long long)indptr_host[list + 1] - indptr_host[list], kv_len_host[b]);
+        for (int64_t i = 0; i < count(b); ++i)
+          KSV_CHECK_ARG(pages(list)[i] >= 0 && pages(list)[i] < num_pages,
+                        "page id %d outside the pool [0, %lld)", pages(list)[i], (long long)num_pages);
+      }
+      for (int64_t i = 0; i < count(b); ++i) use[pages(b)[i]] = kHeld;   // (the kept ones too)
+    }
+    for (int32_t b = 0; b < num_seqs; ++b)
+      for (int64_t i = 0; i < count(b); ++i) {
+        const int32_t from = pages(b)[i], to = pages(num_seqs + b)[i];
+        if (from == to) continue;
+        KSV_CHECK_ARG(use[to] != kHeld, "page %d of pages_out holds tokens of the rows", to);
+        KSV_CHECK_ARG(use[to] != kTaken, "page %d of pages_out is copied to twice", to);
+        use[to] = kTaken;
+        KSV_CHECK_ARG(n < capacity, "more than %lld moves", (long long)capacity);
+        int32_t* m = moves_host + 3 * n++;
+        m[0] = from;
+        m[1] = to;
+        m[2] = int32_t(std::min<int64_t>(page_size, kv_len_host[b] - i * page_size));
+      }
+    return KUNSERVE_OK;
+  });
+  return rc ? rc : n;
+}
+
 extern "C" int kunserve_copy_pages(const kunserve_kv_pool* pool, const kunserve_kv_weights* weights,
-                                   const int32_t* moves_dev, int64_t n, kunserve_stream_t stream) {
+                                   const int32_t* moves_host, const int32_t* moves_dev, int64_t n,
+                                   kunserve_stream_t stream) {
   clear_error();
   int rc = check_pool(pool, true);
   if (rc) return rc;
@@ -243,7 +314,9 @@ extern "C" int kunserve_copy_pages(const kunserve_kv_pool* pool, const kunserve_
   }
   KSV_CHECK_ARG(n >= 0 && n < (int64_t(1) << 31), "%lld moves", (long long)n);
   if (n == 0) return KUNSERVE_OK;
-  KSV_CHECK_ARG(moves_dev, "null moves");
+  KSV_CHECK_ARG(!moves_host != !moves_dev, "moves are either on the host or on the device");
+  KSV_CHECK_ARG(!moves_host || n <= KUNSERVE_MOVES_BY_VALUE, "%lld moves on the host: %d at most",
+                (long long)n, KUNSERVE_MOVES_BY_VALUE);
   KSV_CHECK_ARG(pool->num_layers < 32768 && pool->num_kv_heads < 65536,
                 "%d layers of %d heads are too many", pool->num_layers, pool->num_kv_heads);
   CopyArgs a{};
@@ -259,7 +332,6 @@ extern "C" int kunserve_copy_pages(const kunserve_kv_pool* pool, const kunserve_
     a.w_layer = weights->layer_stride;
     a.w_head = weights->head_stride;
   }
-  a.moves = moves_dev;
   a.num_pages = int32_t(pool->num_pages);
   a.page_size = pool->page_size;
   a.num_heads = pool->num_kv_heads;
@@ -270,9 +342,9 @@ extern "C" int kunserve_copy_pages(const kunserve_kv_pool* pool, const kunserve_
                   unsigned((pool->num_kv_heads + a.heads - 1) / a.heads));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   switch (pool->head_dim) {
-    case 64: copy_pages_kernel<64><<<grid, kThreads, 0, s>>>(a); break;
-    case 128: copy_pages_kernel<128><<<grid, kThreads, 0, s>>>(a); break;
-    default: copy_pages_kernel<256><<<grid, kThreads, 0, s>>>(a);
+    case 64: copy_pages<64>(grid, a, moves_host, moves_dev, n, s); break;
+    case 128: copy_pages<128>(grid, a, moves_host, moves_dev, n, s); break;
+    default: copy_pages<256>(grid, a, moves_host, moves_dev, n, s);
   }
   KSV_CHECK_LAUNCH();
   return KUNSERVE_OK;

@@ -758,8 +758,9 @@ def rotary_append_kv(pool: KVPool, layer: int, table: PageTable, q_indptr: torch
     """The attention prologue of one layer with a Rotary: q and k_new rotated, the
     rotated k and v_new written into their pages. positions (device int32
     [num_tokens], or [axes, num_tokens] for a Rotary of several axes): the tokens'
-    rotary positions, where they are not their places in the cache. The rotated q goes to out (default: q, in place), which must be q
-    or lie apart from q, k_new and v_new. Returns out."""
+    rotary positions, where they are not their places in the cache. The rotated q goes to
+    out (default: q, in place), which must be q or lie apart from q, k_new and v_new.
+    Returns out."""
     q_shape, k_shape, device = q.shape, k_new.shape, pool.device
     tokens, dim, dtype = k_shape[0], pool.head_dim, pool.dtype
     if k_shape != v_new.shape or k_shape[1:] != (pool.num_kv_heads, dim):
@@ -778,8 +779,7 @@ def rotary_append_kv(pool: KVPool, layer: int, table: PageTable, q_indptr: torch
     _check_row_map(q_indptr, table.num_seqs + 1, device, "q_indptr")
     if positions is not None and positions.dim() == 2:
         rotary.check_positions(positions)
-        _check_row_map(positions.view(-1) if positions.is_contiguous() else positions,
-                       rotary.num_axes * tokens, device, "positions")
+        _check_row_map(positions, tokens, device, "positions", rotary.num_axes)
         if rotary.pair_axis is None:
             positions = positions[0]
     else:
@@ -801,10 +801,12 @@ def rotary_append_kv(pool: KVPool, layer: int, table: PageTable, q_indptr: torch
     return out
 
 
-def _check_row_map(m: Optional[torch.Tensor], n: int, device: torch.device, what: str) -> None:
-    if m is not None and (m.dtype != torch.int32 or m.shape != (n,) or m.device != device
-                          or not m.is_contiguous()):
-        raise ValueError(f"{what} must be a contiguous int32 tensor of {n} entries on {device}")
+def _check_row_map(m: Optional[torch.Tensor], n: int, device: torch.device, what: str,
+                   axes: int = 0) -> None:
+    if m is not None and (m.dtype != torch.int32 or m.shape != ((axes, n) if axes else (n,))
+                          or m.device != device or not m.is_contiguous()):
+        raise ValueError(f"{what} must be a contiguous int32 tensor of {f'{axes} x ' if axes else ''}"
+                         f"{n} entries on {device}")
 
 
 def paged_decode(pool: KVPool, layer: int, table: PageTable, q: torch.Tensor, plan: DecodePlan,

@@ -176,6 +176,7 @@ class Rotary:
         self.num_axes = 1 if pair_axis is None else int(pair_axis.max()) + 1
         if sections is not None:
             self.num_axes = len(sections)
+        self._axes = None
         self.pair_axis = None if pair_axis is None else torch.from_numpy(pair_axis).to(device)
         self.frequencies = torch.from_numpy(f).to(device)
         self.device = self.frequencies.device
@@ -189,7 +190,10 @@ class Rotary:
         if self.pair_axis is None or positions is None:
             return None
         stride = positions.shape[1] if positions.dim() == 2 else 0
-        return _lib.RotaryAxes(self.pair_axis.data_ptr(), self.num_axes, stride)
+        axes = self._axes   # the last call's serves most
+        if axes is None or axes.position_stride != stride:
+            self._axes = axes = _lib.RotaryAxes(self.pair_axis.data_ptr(), self.num_axes, stride)
+        return axes
 
     def check_positions(self, positions: Optional[torch.Tensor]) -> None:
         if positions is not None and positions.dim() == 2 and positions.shape[0] != self.num_axes:

@@ -125,23 +125,24 @@ def fork_rows(pool: KVPool, pages_of_reqs: Sequence[Sequence[int]], kv_lens: Seq
     lens = lens.astype(np.int64)
     indptr, indices = csr_from_lists([*pages_of_reqs, *pages_out], np.concatenate([lens, lens]),
                                      pool.page_size, pool.num_pages)
-    src, dst = indices[:indptr[n]], indices[indptr[n]:]
-    copied = src != dst
-    if not copied.any():
+    moves = np.empty((indices.size // 2, 3), dtype=np.int32)
+    lens = _i32(lens)
+    try:
+        count = _lib.call("kunserve_fork_moves", indptr.ctypes.data, indices.ctypes.data,
+                          lens.ctypes.data, n, pool.page_size, pool.num_pages,
+                          moves.ctypes.data, len(moves))
+    except _lib.KunserveError as e:
+        if e.code != _lib.EINVAL:
+            raise
+        raise ValueError(e.detail) from None
+    if count == 0:
         return
-    tokens = np.full(src.size, pool.page_size, dtype=np.int32)
-    ends = indptr[1:n + 1][lens > 0] - 1     # the rows' last pages
-    tokens[ends] = (lens[lens > 0] - 1) % pool.page_size + 1
-    to = dst[copied]
-    use = np.zeros(pool.num_pages, dtype=np.int8)
-    use[src] = 1
-    use[dst[~copied]] = 1
-    if use[to].any():
-        raise ValueError(f"page {int(to[use[to] != 0][0])} of pages_out holds tokens of the rows")
-    use[to] = 2
-    if np.count_nonzero(use == 2) != to.size:
-        raise ValueError("a page is copied to twice")
-    moves = _upload(np.stack([src[copied], to, tokens[copied]], axis=1), pool.device)
+    here = there = None
+    if count <= _lib.MOVES_BY_VALUE:
+        here = moves.ctypes.data
+    else:
+        on_device = _upload(moves[:count], pool.device)
+        there = on_device.data_ptr()
     _lib.call("kunserve_copy_pages", pool.desc(),
-              None if weights is None else ctypes.byref(weights._desc), moves.data_ptr(),
-              len(to), _stream_ptr(pool.device))
+              None if weights is None else ctypes.byref(weights._desc), here, there, count,
+              _stream_ptr(pool.device))

@@ -114,6 +114,28 @@ def test_fork_rows(device, dim, page, dtype):
         assert torch.equal(t, want)
 
 
+@pytest.mark.parametrize("pages", [255, 256, 257])
+def test_fork_rows_of_many_pages(device, pages):
+    """Up to 256 moves go with the launch, more by a copy of their own."""
+    n, rng = 2 * pages, np.random.default_rng(pages)
+    pool = random_pool(n, 1, 1, 4, 64, device, 1)
+    ids = rng.permutation(n).tolist()
+    src, dst = ids[:pages], ids[pages:]
+    old = [pool.k.clone(), pool.v.clone()]
+    lens, rows, out = [], [], []
+    for at in range(0, pages, 50):
+        rows.append(src[at:at + 50])
+        out.append(dst[at:at + 50])
+        lens.append(4 * len(rows[-1]) - at % 4)
+    fork_rows(pool, rows, lens, out)
+    for t, was in zip((pool.k, pool.v), old):
+        want = was.clone()
+        for a, b, l in zip(rows, out, lens):
+            for at in range(l):
+                want[b[at // 4], :, :, at % 4] = was[a[at // 4], :, :, at % 4]
+        assert torch.equal(t, want)
+
+
 def test_fork_rows_strides(device):
     big = torch.randn(12, 2, 2, 6, 16, 128, device=device).to(F16)
     pool = KVPool(big[:, :, 0, 1:4], big[:, :, 1, 1:4])

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from kunserve_amd import KVPool, KVWeights, PageTable, Rotary, fork_rows, keep_tokens
+from kunserve_amd import KVPool, KVWeights, PageTable, Rotary, _lib, fork_rows, keep_tokens
 
 CPU = torch.device("cpu")
 
@@ -72,6 +72,58 @@ def test_tensors_and_weights_of_others():
 def test_fork_refusals(lists, lens, out, why):
     with pytest.raises(ValueError, match=why):
         fork_rows(pool(), lists, lens, out)
+
+
+def fork_moves(lists, lens, page, num_pages, capacity=None):
+    indptr = np.cumsum([0] + [len(x) for x in lists]).astype(np.int32)
+    ids = np.array([i for x in lists for i in x] + [0], dtype=np.int32)
+    lens = np.array(lens, dtype=np.int32)
+    out = np.full((len(ids), 3), -7, dtype=np.int32)
+    n = _lib.call("kunserve_fork_moves", indptr.ctypes.data, ids.ctypes.data, lens.ctypes.data,
+                  len(lens), page, num_pages, out.ctypes.data,
+                  len(out) if capacity is None else capacity)
+    assert (out[n:] == -7).all()
+    return out[:n].tolist()
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_fork_moves(seed):
+    rng = np.random.default_rng(seed)
+    page = int(rng.choice([4, 16]))
+    lens = rng.integers(0, 5 * page, size=int(rng.integers(1, 7)))
+    need = -(-lens // page)
+    ids = iter(rng.permutation(80).tolist())
+    rows = [[next(ids) for _ in range(n)] for n in need]
+    out = [[i if rng.integers(2) else next(ids) for i in r] for r in rows]
+    want = [[a, b, int(min(page, lens[r] - i * page))] for r in range(len(lens))
+            for i, (a, b) in enumerate(zip(rows[r], out[r])) if a != b]
+    # (pages behind the tokens in use are not looked at)
+    assert fork_moves([x + [99] for x in rows] + [x + [rows[0][0] if rows[0] else 3] for x in out],
+                      lens, page, 80) == want
+    if want:
+        with pytest.raises(_lib.KunserveError, match="moves"):
+            fork_moves(rows + out, lens, page, 80, capacity=len(want) - 1)
+
+
+@pytest.mark.parametrize("lists,lens,why", [
+    ([[0], []], [4], "0 pages for 4"),
+    ([[80], [1]], [4], "page id 80 outside"),
+    ([[0], [-1]], [4], "page id -1 outside"),
+    ([[0], [1]], [-4], "-4 tokens"),
+])
+def test_fork_moves_refusals(lists, lens, why):
+    with pytest.raises(_lib.KunserveError, match=why):
+        fork_moves(lists, lens, 4, 80)
+
+
+def test_copy_pages_refusals():
+    p, moves = pool(), np.zeros((300, 3), np.int32)
+    for host, dev, n, why in ((None, None, 1, "either"), (moves, moves, 1, "either"),
+                              (moves, None, 257, "256 at most"), (None, moves, -1, "-1 moves")):
+        with pytest.raises(_lib.KunserveError, match=why):
+            _lib.call("kunserve_copy_pages", p.desc(), None, None if host is None else host.ctypes.data,
+                      None if dev is None else dev.ctypes.data, n, None)
+    assert _lib.call("kunserve_copy_pages", p.desc(), None, None, None, 0, None) == 0
 
 
 def test_fork_pages_outside():

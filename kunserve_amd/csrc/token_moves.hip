@@ -113,12 +113,13 @@ struct CopyArgs {
   int32_t num_pages;
   int32_t page_size;
   int32_t num_heads;
-  int32_t heads;          // heads of a workgroup
+  int32_t heads, parts;   // heads of a workgroup, workgroups of all
+  uint32_t slabs;         // workgroups of a move
 };
 
 // [n][3]: source page, destination page, tokens. Few of them go with the launch's
 // arguments: an upload of their own takes longer than they do (8 samples' last pages, with
-// building the table: 34 us against 40).
+// building the table: 22 us against 30).
 struct MovesThere {
   const int32_t* m;
 };
@@ -127,18 +128,22 @@ struct MovesHere {
 };
 
 // Workgroup (move, layer and K or V, head group): the waves take the loads of its heads'
-// tokens in turn.
+// tokens in turn. Moves are the slowest: those of one source read the same rows on one XCD
+// where the groups are a multiple of eight, and neighbours in time are pages apart (eight
+// pages of 76 tokens, 32 layers of 8 heads: 14 us from one source and 20 from eight; with the
+// moves fastest 41 and 36). Past the caches only the writes: reads too 26 and 28.
 template <int D, typename Moves>
 __global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyArgs a, Moves moves) {
   constexpr int CH = D / 8;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
-  const int64_t at3 = 3 * int64_t(blockIdx.x);
+  const int slab = int(blockIdx.x % a.slabs);
+  const int64_t at3 = 3 * int64_t(blockIdx.x / a.slabs);
   const int from = moves.m[at3], to = moves.m[at3 + 1], tokens = min(moves.m[at3 + 2], a.page_size);
   if (from < 0 || from >= a.num_pages || to < 0 || to >= a.num_pages || tokens <= 0) return;
-  const int layer = int(blockIdx.y) >> 1;
-  const bool of_v = blockIdx.y & 1;
-  const int h0 = int(blockIdx.z) * a.heads, nh = min(a.heads, a.num_heads - h0);
+  const int h0 = slab % a.parts * a.heads, layer = slab / a.parts >> 1;
+  const bool of_v = slab / a.parts & 1;
+  const int nh = min(a.heads, a.num_heads - h0);
   f16* base = (of_v ? a.v : a.k) + int64_t(layer) * a.layer_stride;
   const f16* src = base + int64_t(from) * a.page_stride;
   f16* dst = base + int64_t(to) * a.page_stride;
@@ -153,7 +158,7 @@ __global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyArgs a, Moves 
       const bool in = l < total && unit < tokens * CH;
       off[i] = in ? int64_t(h0 + h) * a.head_stride + int64_t(unit / CH) * a.token_stride + 8 * (unit % CH)
                   : -1;
-      if (in) x[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + off[i]));
+      if (in) x[i] = *reinterpret_cast<const u32x4*>(src + off[i]);
     }
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
@@ -338,8 +343,10 @@ extern "C" int kunserve_copy_pages(const kunserve_kv_pool* pool, const kunserve_
   // Heads of a workgroup: about 64 loads, two rounds of its waves.
   const int64_t per_head = (int64_t(pool->page_size) * (pool->head_dim / 8) + kWave - 1) / kWave;
   a.heads = int32_t(per_head >= 64 ? 1 : 64 / per_head);
-  const dim3 grid(unsigned(n), unsigned(2 * pool->num_layers),
-                  unsigned((pool->num_kv_heads + a.heads - 1) / a.heads));
+  a.parts = (pool->num_kv_heads + a.heads - 1) / a.heads;
+  a.slabs = uint32_t(2 * pool->num_layers) * uint32_t(a.parts);
+  KSV_CHECK_ARG(n * a.slabs < (int64_t(1) << 31), "%lld moves of %u workgroups", (long long)n, a.slabs);
+  const dim3 grid(static_cast<unsigned>(n * a.slabs));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   switch (pool->head_dim) {
     case 64: copy_pages<64>(grid, a, moves_host, moves_dev, n, s); break;

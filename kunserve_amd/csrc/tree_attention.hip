@@ -249,7 +249,7 @@ __global__ __launch_bounds__((TreeTile<D, WC>::WAVES * kWave), D == 256 ? 1 : 2)
   // Page ids outside the pool, and tokens behind the cached ones, read page 0.
   auto load_cached = [&](int r, int ids, auto loads_per_page) __attribute__((always_inline)) {
     constexpr int P = decltype(loads_per_page)::value;   // 0: two pages to a load
-    constexpr int G = P ? LOADS / P : 2 * LOADS;         // granules
+    constexpr int G = P ? LOADS / (P ? P : 1) : 2 * LOADS;   // granules
     const int t0 = r * L::ROUND + wave * STEP;
     bad = 0;
     int64_t at[G];   // bytes from the head's base

@@ -278,3 +278,27 @@ def test_a_request_drafts_keeps_forks_and_goes_on(device, dtype, dim):
         got = tokens_of(pool.k, layer, pages, n).double()
         h = history[layer][0].transpose(0, 1)
         assert ((got - h).abs() <= h.abs() * tol / 2 + 2.0 ** -18).all()
+
+
+@pytest.mark.parametrize("rows,dim,page", [(1, 64, 4), (7, 128, 16), (9, 256, 16), (37, 64, 32)])
+def test_fork_rows_of_one_prompt(device, rows, dim, page):
+    """Samples of one prompt, some of them shorter than it, and a row of its own."""
+    rng = np.random.default_rng(rows)
+    prompt, lens = [3, 0, 5], [int(2 * page + rng.integers(1, page + 1)) for _ in range(rows)]
+    other = [6, 7]
+    ids = iter(range(8, 8 + 3 * rows + 2))
+    out = [[3, next(ids), next(ids)] if b % 3 == 1 else [3, 0, next(ids)] for b in range(rows)]
+    lists, lens = [prompt] * rows + [other], lens + [page + 1]
+    out.append([next(ids), next(ids)])
+    pool = random_pool(8 + 3 * rows + 2, 2, 3, page, dim, device, 1)
+    w = KVWeights(pool)
+    w.w.uniform_()
+    before = [t.clone() for t in (pool.k, pool.v, w.w)]
+    fork_rows(pool, lists, lens, out, weights=w)
+    for t, old in zip((pool.k, pool.v, w.w), before):
+        want = old.clone()
+        for a, b, n in zip(lists, out, lens):
+            for at in range(n):
+                if a[at // page] != b[at // page]:
+                    want[b[at // page], :, :, at % page] = old[a[at // page], :, :, at % page]
+        assert torch.equal(t, want)

@@ -549,12 +549,8 @@ class TreePlan:
         n = table.num_seqs
         if len(parents) != n:
             raise ValueError(f"{n} rows but {len(parents)} trees")
-        q_indptr = np.zeros(n + 1, dtype=np.int64)
-        np.cumsum([len(p) for p in parents], out=q_indptr[1:])
-        tokens = int(q_indptr[-1])
-        up = np.empty(tokens, dtype=np.int32)
-        for b, p in enumerate(parents):
-            up[q_indptr[b]:q_indptr[b + 1]] = _tree(p, b)
+        trees = parents if isinstance(parents, _Trees) else _Trees(parents, range(n))
+        q_indptr, up = trees.indptr, _i32(trees.up)
         qi = _i32(q_indptr)
         first = qi[:-1] if q_first is None else _i32(q_first)
         if first.shape != (n,) or np.any(first < 0):
@@ -597,28 +593,46 @@ class TreePlan:
         return int(_lib.lib().kunserve_tree_workspace_bytes(ctypes.byref(self.info)))
 
 
-def _tree(parents: Sequence[int], row: int) -> np.ndarray:
-    """A row's tree as int32, checked."""
-    p = np.asarray(parents)
-    if p.ndim != 1 or (p.size and p.dtype.kind not in "iu"):
-        raise ValueError(f"row {row}: a tree is a list of whole numbers")
-    bad = (p < -1) | (p >= np.arange(p.size))
-    if np.any(bad):
-        i = int(np.argmax(bad))
-        raise ValueError(f"row {row}: drafted token {i} has parent {int(p[i])}, which is neither "
-                         "-1 nor a token before it")
-    return p.astype(np.int32)
+class _Trees:
+    """Rows' trees one after the other, checked: tokens of row b are
+    [indptr[b], indptr[b + 1]), up their parents among the row's."""
+
+    def __init__(self, parents: Sequence[Sequence[int]], rows: Sequence[int]):
+        self.indptr = np.zeros(len(parents) + 1, dtype=np.int64)
+        np.cumsum([len(p) for p in parents], out=self.indptr[1:])
+        up = _flat_ids(parents)
+        if up is None:
+            kept = [np.asarray(p) for p in parents]
+            for b, p in zip(rows, kept):
+                if p.ndim != 1 or (p.size and p.dtype.kind not in "iu"):
+                    raise ValueError(f"row {b}: a tree is a list of whole numbers")
+            up = np.concatenate([p.astype(np.int64) for p in kept] or [np.zeros(0, np.int64)])
+        self.first = np.repeat(self.indptr[:-1], np.diff(self.indptr))   # of each token's row
+        place = np.arange(up.size) - self.first
+        bad = (up < -1) | (up >= place)
+        if bad.any():
+            i = int(np.argmax(bad))
+            b = int(np.searchsorted(self.indptr, i, side="right")) - 1
+            raise ValueError(f"row {rows[b]}: drafted token {place[i]} has parent {up[i]}, which is "
+                             "neither -1 nor a token before it")
+        self.up = up
+
+    def __len__(self) -> int:
+        return len(self.indptr) - 1
+
+    def depths(self) -> np.ndarray:
+        up = np.where(self.up >= 0, self.up + self.first, -1)
+        depth = (up >= 0).astype(np.int64)
+        while (up >= 0).any():   # ancestors 1, 2, 4, .. away
+            depth += np.where(up >= 0, depth[up], 0)
+            up = np.where(up >= 0, up[up], -1)
+        return depth
 
 
 def tree_depths(parents: Sequence[int]) -> np.ndarray:
     """How many drafted ancestors each token of a tree has: a token's place in its
     sequence is the cached tokens' number and this."""
-    up = _tree(parents, 0).astype(np.int64)
-    depth = (up >= 0).astype(np.int64)
-    while np.any(up >= 0):   # ancestors 1, 2, 4, .. away
-        depth += np.where(up >= 0, depth[up], 0)
-        up = np.where(up >= 0, up[up], -1)
-    return depth
+    return _Trees([parents], [0]).depths()
 
 
 # ------------------------------------------------------------------ ops
@@ -1042,6 +1056,8 @@ class AttentionStep:
                 raise ValueError("attention weights need pages that are in one place of the "
                                  "step's lists")
             self.weights = weights
+        tree_rows = np.flatnonzero(drafted)
+        drafts = _Trees([trees[b] for b in tree_rows], tree_rows) if tree_rows.size else None
         positions = None
         if np.ndim(rope_positions) == 2 and len(rope_positions) != 1:
             positions = np.asarray(rope_positions)
@@ -1060,9 +1076,9 @@ class AttentionStep:
             starts = starts.astype(np.int64)
             positions = np.repeat(starts - self.q_indptr_host[:-1], q_lens) + np.arange(
                 self.num_tokens)
-            for b in np.flatnonzero(drafted):
-                at = self.q_indptr_host[b]
-                positions[at:at + q_lens[b]] = starts[b] + tree_depths(trees[b])
+            if drafted.any():
+                positions[np.repeat(drafted, q_lens)] = (
+                    np.repeat(starts[drafted], q_lens[drafted]) + drafts.depths())
             if np.any(starts < 0) or (positions.size and positions.max() >= 2**31):
                 raise ValueError("rope_positions must lie in [0, 2^31)")
 
@@ -1071,7 +1087,6 @@ class AttentionStep:
         self.decode = self.prefill = None
         all_rows = np.arange(n_rows)
         dec_rows, pre_rows = all_rows[is_decode], all_rows[~is_decode & ~drafted]
-        tree_rows = all_rows[drafted]
         # Row subsets take their rows from the step's CSR arrays (ids already
         # checked and mapped), not from the lists again.
         def sub_table(rows):
@@ -1113,7 +1128,7 @@ class AttentionStep:
 
         if tree_rows.size:
             table = self.table if tree_rows.size == n_rows else sub_table(tree_rows)
-            plan = TreePlan(table, [trees[b] for b in tree_rows], num_qo_heads, pool.num_kv_heads,
+            plan = TreePlan(table, drafts, num_qo_heads, pool.num_kv_heads,
                             pool.page_size, dev, upload=False, head_dim=pool.head_dim,
                             q_first=self.q_indptr_host[tree_rows])
             self.tree = _Subset(tree_rows, None, table, None, plan)

@@ -1365,11 +1365,9 @@ class AttentionStep:
             raise ValueError("tokens move in place: their pages must be in one place of the "
                              "step's lists")
         first = self.kv_len - np.diff(self.q_indptr_host)
-        if self._first is None:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("a step without trees uploads its rows' first places: not "
-                                   "under a capture")
-            self._first = _upload(_i32(first), self.pool.device)
+        if self._first is None and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a step without trees uploads its rows' first places: not under a "
+                               "capture")
         move_tokens(self.pool, self.table, self._first, first, kept, weights)
 
 

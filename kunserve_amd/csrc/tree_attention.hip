@@ -335,6 +335,9 @@ __global__ __launch_bounds__((TreeTile<D, WC>::WAVES * kWave), D == 256 ? 1 : 2)
   f32x16 o[OT];
 #pragma unroll
   for (int d = 0; d < OT; ++d) o[d] = f32x16{};
+  // Probabilities are 2^(s - m): m is the maximum, or up to 8 below it, and `lift` lower in
+  // fp16, whose least value is 2^-24: many tokens far below the maximum do not vanish together.
+  constexpr float lift = std::is_same<T, bf16>::value ? 0.f : 7.f;
   float m = kNegBig, lsum = 0.f;   // m the same in a column's two lanes
 
   // LDS addresses as one register each and constants: with one for each chunk they were
@@ -466,9 +469,9 @@ __global__ __launch_bounds__((TreeTile<D, WC>::WAVES * kWave), D == 256 ? 1 : 2)
       float mx = -INFINITY;
 #pragma unroll
       for (int x = 0; x < 16; ++x) mx = fmaxf(mx, sc[x]);
-      if (__any(mx * a.scale_log2 > m + 8.f)) {
+      if (__any(mx * a.scale_log2 > m + (8.f + lift))) {
         mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.scale_log2;
-        const float m_new = mx > m + 8.f ? mx : m;
+        const float m_new = mx > m + (8.f + lift) ? mx - lift : m;
         const float alpha = fast_exp2(m - m_new);
         m = m_new;
         lsum *= alpha;
@@ -571,7 +574,8 @@ __global__ __launch_bounds__((TreeTile<D, WC>::WAVES * kWave), D == 256 ? 1 : 2)
   // lane's values), the others' of which it reads from LDS, and writes them out. (As little
   // code as can be: a workgroup runs it once, and waits for most of it to be fetched. Halves
   // joined step by step, as single values in LDS, and written by one share's waves: one row of
-  // 1500 12.4 us a layer against 11.8, 16 of 4096 at head_dim 256 82 against 73.)
+  // 1500 12.4 us a layer against 11.8, 4 of 4096 with 256 columns at head_dim 256 67
+  // against 64.)
   constexpr int U = 2 * OT, OWN = U / WT;
   float y[8 * OWN];
   if constexpr (WT > 1) {
@@ -785,6 +789,9 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
                   kv_len[b]);
     r.tokens = n;
     r.q_first = q_first ? q_first[b] : q_indptr[b];
+    KSV_CHECK_ARG(r.q_first >= 0, "row %d: its first token is %d", b, r.q_first);
+    KSV_CHECK_ARG(int64_t(n) * ratio < (int64_t(1) << 31) - max_cols, "row %d: %d tokens of %d heads",
+                  b, n, ratio);
     r.prefix = kv_len[b] - n;
     r.page_at = indptr[b];
     r.np = int32_t(ceil_div(r.prefix, round));

@@ -167,6 +167,30 @@ def test_prefix_values_that_are_not_finite(device, dim, dtype):
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("tokens", [1, 70])
+def test_a_long_tail_far_below_the_maximum(device, dim, dtype, tokens):
+    """One token with a score 17.5 above 20000 others, which together have 5e-4 of its
+    probability, each 2^-25.2 (less than a step of fp16 at 0)."""
+    n, page = 20000, 16
+    rng = np.random.default_rng(dim + tokens)
+    lists, pages = random_pages(rng, [n + tokens], page)
+    pool = random_pool(pages, 1, 1, page, dim, device, 1, dtype=dtype)
+    pool.k.zero_()
+    pool.v.fill_(-3.0)
+    at = 12345
+    pool.k[lists[0][at // page], 0, 0, at % page] = 17.5 / math.sqrt(dim)
+    pool.v[lists[0][at // page], 0, 0, at % page] = 1.0
+    q = torch.ones(tokens, 2, dim, device=device, dtype=dtype)
+    k = torch.zeros(tokens, 1, dim, device=device, dtype=dtype)
+    v = torch.full((tokens, 1, dim), -3.0, device=device, dtype=dtype)
+    tree = random_tree(rng, tokens, 4)
+    step = AttentionStep(pool, 2, [tokens], [n], [1], lists, trees=[tree])
+    out = step.run(0, q, k, v)
+    check_step(pool, 0, lists, [n + tokens], [tree], q, k, v, out, 1 / math.sqrt(dim))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
 def test_slots_behind_a_row_do_not_matter(device, dim):
     """Neither NaN behind the row's last token nor what its new slots held before."""
     pool, lists, lens, trees, q, k, v = make(device, [10, 3], [90, 6], 4, 2, dim, 16, F16)

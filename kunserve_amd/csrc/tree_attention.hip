@@ -652,15 +652,20 @@ __global__ __launch_bounds__((TreeTile<D, WC>::WAVES * kWave), D == 256 ? 1 : 2)
   }
 }
 
-// Columns of a workgroup for rows of up to `widest`: as few as hold them, four waves' up to
-// 128. More share what loads and stages K and V with eight waves at head_dim 128: 64 rows of
-// 4096 tokens, 256 columns, 446 us against 490; at 64 both take as long (16 rows, 88 us),
-// and at 256 a wave's registers are two waves'.
-int tree_columns(int head_dim, int64_t widest) {
-  if (head_dim == 256) return widest <= 64 ? 64 : 128;
-  if (widest <= 128 || head_dim == 64) return widest <= 32 ? 32 : widest <= 64 ? 64 : 128;
-  return 256;
-}
+// What a plan's workgroups can be: their columns, how many to a CU, and the time of a round
+// where every place is taken, base + tile for each column tile (of 64 rows of 4096 tokens of
+// 4 to 64, within a tenth; us). Four waves up to 128 columns; eight at head_dim 128 (at 64
+// they gained nothing, at 256 a wave's registers are two waves').
+struct TreeKind {
+  int columns, per_cu;
+  float base, tile;
+};
+constexpr TreeKind kKinds[3][4] = {
+    {{32, 2, 4.0f, 0.8f}, {64, 2, 4.7f, 1.0f}, {128, 2, 6.0f, 1.0f}, {}},
+    {{32, 2, 3.8f, 0.6f}, {64, 2, 4.6f, 0.6f}, {128, 2, 4.7f, 1.0f}, {256, 1, 4.1f, 0.36f}},
+    {{64, 1, 3.6f, 0.1f}, {128, 1, 4.6f, 0.1f}, {}, {}},
+};
+const TreeKind* kinds_of(int head_dim) { return kKinds[head_dim / 128]; }
 int round_tokens(int head_dim) { return kWaves * 8 * kWave / (head_dim / 8); }
 
 template <typename T, int D>
@@ -698,6 +703,32 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct TreeRow {
   int32_t tokens, q_first, prefix, page_at, mask_at, mask_words, np, rounds;
 };
+
+// The kind of workgroups that takes least time for all rows: the narrowest that hold a row's
+// columns are its own best, but few rows wider than the others pay for several workgroups
+// sooner than all for wider ones (63 rows of 8 tokens and one of 33, 4 heads: XX us a layer,
+// 322 in workgroups of 256 columns).
+const TreeKind& best_kind(const int32_t* q_indptr, const int32_t* kv_len, int32_t num_seqs, int ratio,
+                          int head_dim) {
+  const TreeKind* const kinds = kinds_of(head_dim);
+  int best = 0;
+  double least = 0;
+  for (int k = 0; k < 4 && kinds[k].columns; ++k) {
+    double time = 0;
+    for (int32_t b = 0; b < num_seqs; ++b) {
+      const int64_t cols = (int64_t(q_indptr[b + 1]) - q_indptr[b]) * ratio;
+      const double each = double(ceil_div(cols, kinds[k].columns)) * kinds[k].base +
+                          double(ceil_div(cols, 32)) * kinds[k].tile;
+      time += each * double(ceil_div(kv_len[b], round_tokens(head_dim)) + 1);
+    }
+    time /= kinds[k].per_cu;
+    if (k == 0 || time < least) {
+      best = k;
+      least = time;
+    }
+  }
+  return kinds[best];
+}
 
 // Rounds [rb, re) of a row to a workgroup for each KV head and column tile: of parts as
 // long as one another, none longer than `run`.
@@ -770,10 +801,8 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
               int32_t num_cus, int32_t part_rounds, std::vector<int32_t>& plan,
               kunserve_tree_plan_info* info) {
   const int ratio = num_qo_heads / num_kv_heads;
-  int64_t widest = 0;
-  for (int32_t b = 0; b < num_seqs; ++b)
-    widest = std::max(widest, (int64_t(q_indptr[b + 1]) - q_indptr[b]) * ratio);
-  const int max_cols = tree_columns(head_dim, widest);
+  const TreeKind& kind = best_kind(q_indptr, kv_len, num_seqs, ratio, head_dim);
+  const int max_cols = kind.columns;
   const int round = round_tokens(head_dim), tiles = round / kBlock;
   const int64_t cus = num_cus > 0 ? num_cus : 256;
   std::vector<TreeRow> rows(num_seqs);
@@ -813,7 +842,7 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
     work += n ? int64_t(r.rounds) * ceil_div(int64_t(n) * ratio, max_cols) * num_kv_heads : 0;
     if (n) longest = std::max(longest, r.rounds);
   }
-  const int64_t slots_at_once = (head_dim == 256 || max_cols == 256 ? 1 : 2) * cus;
+  const int64_t slots_at_once = kind.per_cu * cus;
   const int64_t run = part_rounds > 0
                           ? std::min<int64_t>(part_rounds, std::max(longest, 1))
                           : best_run(rows, longest, work, max_cols, ratio, num_kv_heads, round, slots_at_once);
@@ -965,8 +994,9 @@ int kunserve::tree_attention(const kunserve_kv_pool* pool, int32_t layer,
                 info->num_kv_heads, num_qo_heads, pool->num_kv_heads);
   KSV_CHECK_ARG(info->num_seqs == table->num_seqs, "plan made for %d rows, not %d", info->num_seqs,
                 table->num_seqs);
-  KSV_CHECK_ARG(tree_columns(info->head_dim, info->columns) == info->columns,
-                "plan of %d columns to a workgroup", info->columns);
+  bool known = false;
+  for (int k = 0; k < 4; ++k) known = known || (info->columns && kinds_of(info->head_dim)[k].columns == info->columns);
+  KSV_CHECK_ARG(known, "plan of %d columns to a workgroup", info->columns);
   KSV_CHECK_ARG(pool->token_stride < (int64_t(1) << 28),
                 "tokens %lld elements apart: less than 2^28 here", (long long)pool->token_stride);
   KSV_CHECK_ARG(num_qo_heads < 65536, "%d query heads: at most 65535", num_qo_heads);

@@ -651,11 +651,14 @@ int kunserve_evict(const kunserve_kv_pool* pool, const kunserve_kv_weights* weig
  * end moves nothing, and the slot keeps what it has. What the other entries read is
  * what the slots held before the call. Pages with tokens from first[b] on are in no
  * other place of the table. Of pages outside the pool a source gives zeros, a
- * destination is not written. */
+ * destination is not written. first is at first_dev or, for up to
+ * KUNSERVE_FIRST_BY_VALUE rows, at first_host (the other is NULL): it goes with the
+ * launch, and the array is the caller's again. */
+#define KUNSERVE_FIRST_BY_VALUE 256
 int kunserve_keep_tokens(const kunserve_kv_pool* pool, const kunserve_kv_weights* weights,
-                         const kunserve_page_table* table, const int32_t* first_dev,
-                         const int32_t* kept_dev, int64_t kept_stride, int32_t max_kept,
-                         kunserve_stream_t stream);
+                         const kunserve_page_table* table, const int32_t* first_host,
+                         const int32_t* first_dev, const int32_t* kept_dev, int64_t kept_stride,
+                         int32_t max_kept, kunserve_stream_t stream);
 
 /* The moves (kunserve_copy_pages) after which rows go on in page lists of their own.
  * Host arrays: list b of 2 num_seqs is indices_host[indptr_host[b] .. indptr_host[b + 1]),

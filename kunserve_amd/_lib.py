@@ -20,6 +20,7 @@ ENOSPC = -3
 EUNSUPPORTED = -4
 EHIP = -5
 MOVES_BY_VALUE = 256
+FIRST_BY_VALUE = 256
 _CODE_NAMES = {EINVAL: "EINVAL", ERANGE: "ERANGE", ENOSPC: "ENOSPC",
                EUNSUPPORTED: "EUNSUPPORTED", EHIP: "EHIP"}
 
@@ -172,7 +173,7 @@ SIGNATURES = {
                                         c_void_p, POINTER(TreePlanInfo), c_void_p, c_int64,
                                         c_void_p]),
     "kunserve_keep_tokens": (c_int, [POINTER(KVPool), POINTER(KVWeights), POINTER(PageTable),
-                                     c_void_p, c_void_p, c_int64, c_int32, c_void_p]),
+                                     c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p]),
     "kunserve_fork_moves": (c_int64, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int64,
                                       c_void_p, c_int64]),
     "kunserve_copy_pages": (c_int, [POINTER(KVPool), POINTER(KVWeights), c_void_p, c_void_p,

@@ -5,6 +5,7 @@
 //
 // Both are HBM-bound copies of 16-byte chunks: what moves is read and written once.
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 #include "common.hpp"
@@ -25,7 +26,6 @@ struct KeepArgs {
   const int32_t* indptr;
   const int32_t* indices;
   const int32_t* kv_len;
-  const int32_t* first;
   const int32_t* kept;
   int64_t kept_stride;
   int32_t max_kept;
@@ -36,12 +36,21 @@ struct KeepArgs {
   int64_t num_slabs;   // rows x K and V x layers x heads
 };
 
+// [rows]: the rows' first places, which for few rows go with the launch's arguments (small rows
+// cut short 15 us a call with the host's work, 29 with an upload and more of that).
+struct FirstThere {
+  const int32_t* at;
+};
+struct FirstHere {
+  int32_t at[KUNSERVE_FIRST_BY_VALUE];
+};
+
 // A slab is a row's tokens of one layer, KV head and K or V. It moves chunk by chunk:
 // slots [c, c + n) are written after the tokens kept[c], .. kept[c + n - 1] have been
 // read, by one wave (W 1) or by a workgroup that meets between. A token moves down
 // (kept[j] > j), so what a later chunk reads no earlier one has written.
-template <int D, int W>
-__global__ __launch_bounds__(kThreads) void keep_tokens_kernel(KeepArgs a) {
+template <int D, int W, typename First>
+__global__ __launch_bounds__(kThreads) void keep_tokens_kernel(KeepArgs a, First from_place) {
   constexpr int CH = D / 8;
   constexpr int TPL = kWave / CH;                 // tokens of a load
   constexpr int CHUNK = kLoads * TPL * W;
@@ -56,7 +65,7 @@ __global__ __launch_bounds__(kThreads) void keep_tokens_kernel(KeepArgs a) {
   const int b = int(rest / a.num_layers >> 1);
   const int lrow = lane / CH, lcol = lane % CH;
 
-  const int first = a.first[b], len = a.kv_len[b] - first;
+  const int first = from_place.at[b], len = a.kv_len[b] - first;
   if (first < 0 || len <= 1) return;   // uniform
   const int32_t* pages = a.indices + a.indptr[b];
   const int32_t* kept = a.kept + int64_t(b) * a.kept_stride;
@@ -176,6 +185,25 @@ __global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyArgs a, Moves 
 }
 
 template <int D>
+void keep_tokens(dim3 grid, bool small, const KeepArgs& a, const int32_t* first_host,
+                 const int32_t* first_dev, int32_t rows, hipStream_t s) {
+  auto launch = [&](const auto& first) {
+    typedef std::decay_t<decltype(first)> First;
+    if (small)
+      keep_tokens_kernel<D, 1, First><<<grid, kThreads, 0, s>>>(a, first);
+    else
+      keep_tokens_kernel<D, kWaves, First><<<grid, kThreads, 0, s>>>(a, first);
+  };
+  if (first_host) {
+    FirstHere here;
+    std::copy_n(first_host, rows, here.at);
+    launch(here);
+  } else {
+    launch(FirstThere{first_dev});
+  }
+}
+
+template <int D>
 void copy_pages(dim3 grid, const CopyArgs& a, const int32_t* moves_host, const int32_t* moves_dev,
                 int64_t n, hipStream_t s) {
   if (moves_host) {
@@ -194,9 +222,10 @@ using namespace kunserve;
 
 extern "C" int kunserve_keep_tokens(const kunserve_kv_pool* pool,
                                     const kunserve_kv_weights* weights,
-                                    const kunserve_page_table* table, const int32_t* first_dev,
-                                    const int32_t* kept_dev, int64_t kept_stride,
-                                    int32_t max_kept, kunserve_stream_t stream) {
+                                    const kunserve_page_table* table, const int32_t* first_host,
+                                    const int32_t* first_dev, const int32_t* kept_dev,
+                                    int64_t kept_stride, int32_t max_kept,
+                                    kunserve_stream_t stream) {
   clear_error();
   int rc = check_pool(pool, true);
   if (rc) return rc;
@@ -208,8 +237,12 @@ extern "C" int kunserve_keep_tokens(const kunserve_kv_pool* pool,
   KSV_CHECK_ARG(max_kept >= 0 && kept_stride >= max_kept, "kept rows of %lld hold %d entries",
                 (long long)kept_stride, max_kept);
   if (table->num_seqs == 0 || max_kept == 0) return KUNSERVE_OK;
-  KSV_CHECK_ARG(table->indptr_dev && table->indices_dev && table->kv_len_dev && first_dev && kept_dev,
-                "null table array, first or kept");
+  KSV_CHECK_ARG(table->indptr_dev && table->indices_dev && table->kv_len_dev && kept_dev,
+                "null table array or kept");
+  KSV_CHECK_ARG(!first_host != !first_dev, "first places are either on the host or on the device");
+  KSV_CHECK_ARG(!first_host || table->num_seqs <= KUNSERVE_FIRST_BY_VALUE,
+                "first places of %d rows on the host: %d at most", table->num_seqs,
+                KUNSERVE_FIRST_BY_VALUE);
   KeepArgs a{};
   a.k = static_cast<f16*>(pool->k);
   a.v = static_cast<f16*>(pool->v);
@@ -226,7 +259,6 @@ extern "C" int kunserve_keep_tokens(const kunserve_kv_pool* pool,
   a.indptr = table->indptr_dev;
   a.indices = table->indices_dev;
   a.kv_len = table->kv_len_dev;
-  a.first = first_dev;
   a.kept = kept_dev;
   a.kept_stride = kept_stride;
   a.max_kept = max_kept;
@@ -245,17 +277,9 @@ extern "C" int kunserve_keep_tokens(const kunserve_kv_pool* pool,
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(blocks));
   switch (pool->head_dim) {
-    case 64:
-      if (small) keep_tokens_kernel<64, 1><<<grid, kThreads, 0, s>>>(a);
-      else keep_tokens_kernel<64, kWaves><<<grid, kThreads, 0, s>>>(a);
-      break;
-    case 128:
-      if (small) keep_tokens_kernel<128, 1><<<grid, kThreads, 0, s>>>(a);
-      else keep_tokens_kernel<128, kWaves><<<grid, kThreads, 0, s>>>(a);
-      break;
-    default:
-      if (small) keep_tokens_kernel<256, 1><<<grid, kThreads, 0, s>>>(a);
-      else keep_tokens_kernel<256, kWaves><<<grid, kThreads, 0, s>>>(a);
+    case 64: keep_tokens<64>(grid, small, a, first_host, first_dev, table->num_seqs, s); break;
+    case 128: keep_tokens<128>(grid, small, a, first_host, first_dev, table->num_seqs, s); break;
+    default: keep_tokens<256>(grid, small, a, first_host, first_dev, table->num_seqs, s);
   }
   KSV_CHECK_LAUNCH();
   return KUNSERVE_OK;

@@ -33,17 +33,20 @@ def keep_tokens(pool: KVPool, table: PageTable, first: Union[int, Sequence[int]]
     given = np.asarray(first)
     if given.dtype.kind not in "iu" or given.shape not in ((), (n,)):
         raise ValueError(f"first must be a whole number, or one per row ({n})")
-    starts = np.broadcast_to(given.astype(np.int64), (n,))
-    lens = table.kv_len_host.astype(np.int64)
-    if np.any(starts < 0) or np.any(starts > lens):
-        bad = int(np.argmax((starts < 0) | (starts > lens)))
-        raise ValueError(f"row {bad}: first place {int(starts[bad])} of {int(lens[bad])} tokens")
+    lens = table.kv_len_host
+    out = (given < 0) | (given > lens)
+    if out.any():
+        bad = int(np.argmax(out))
+        raise ValueError(f"row {bad}: first place {int(given.reshape(-1)[bad % given.size])} of "
+                         f"{int(lens[bad])} tokens")
+    starts = np.empty(n, dtype=np.int32)
+    starts[:] = given
     if pool.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("keep_tokens cannot be captured: its first places are uploaded; "
                            "AttentionStep.keep_tokens can")
     moving = np.zeros(n + 1, dtype=np.int32)
     np.cumsum(lens - starts, out=moving[1:])
-    ids = np.concatenate([table.indices_host, np.zeros(1, np.int32)])   # (never empty)
+    ids = table.indices_host if table.indices_host.size else moving   # (there is one)
     if not _lib.call("kunserve_new_pages_private", table.indptr_host.ctypes.data,
                      ids.ctypes.data, moving.ctypes.data, table.kv_len_host.ctypes.data, n,
                      pool.page_size, pool.num_pages):
@@ -72,7 +75,13 @@ def move_tokens(pool: KVPool, table: PageTable, first: Optional[torch.Tensor],
         width = stride = kept.shape[1]
     if n == 0 or width == 0:
         return
-    if not isinstance(kept, torch.Tensor) and first is None:
+    here = None
+    if first is None and n <= _lib.FIRST_BY_VALUE:
+        first_host = _i32(first_host)
+        here = first_host.ctypes.data
+        if not isinstance(kept, torch.Tensor):
+            kept = _upload(kept, device)
+    elif not isinstance(kept, torch.Tensor) and first is None:
         both = _upload(np.concatenate([_i32(first_host), kept.reshape(-1)]), device)
         first, kept = both[:n], both[n:]
     elif first is None:
@@ -80,8 +89,9 @@ def move_tokens(pool: KVPool, table: PageTable, first: Optional[torch.Tensor],
     elif not isinstance(kept, torch.Tensor):
         kept = _upload(kept, device)
     _lib.call("kunserve_keep_tokens", pool.desc(),
-              None if weights is None else ctypes.byref(weights._desc), table.desc(),
-              first.data_ptr(), kept.data_ptr(), stride, width, _stream_ptr(device))
+              None if weights is None else ctypes.byref(weights._desc), table.desc(), here,
+              None if here is not None else first.data_ptr(), kept.data_ptr(), stride, width,
+              _stream_ptr(device))
 
 
 def _kept_rows(kept: Sequence[Sequence[int]], lens: np.ndarray) -> np.ndarray:

@@ -46,6 +46,26 @@ def test_keep_tokens(device, dim, page, dtype):
     assert torch.equal(w.w, want_w)
 
 
+@pytest.mark.parametrize("rows", [255, 256, 257])
+def test_keep_tokens_of_many_rows(device, rows):
+    """First places of up to 256 rows go with the launch, of more by a copy of their own."""
+    rng = np.random.default_rng(rows)
+    lens = [4 + b % 9 for b in range(rows)]
+    lists, pages = random_pages(rng, lens, 4)
+    pool = random_pool(pages, 1, 1, 4, 64, device, 1)
+    first = [b % 3 for b in range(rows)]
+    kept = [sorted(rng.permutation(n - f)[:(n - f) // 2].tolist()) for n, f in zip(lens, first)]
+    want = [moved(t, lists, first, kept, 4) for t in (pool.k, pool.v)]
+    table = PageTable.from_lists(lists, lens, pool)
+    if rows == 256:   # entries on the device too
+        dev = torch.full((rows, max(map(len, kept))), -1, dtype=torch.int32)
+        for b, x in enumerate(kept):
+            dev[b, :len(x)] = torch.tensor(x, dtype=torch.int32)
+        kept = dev.to(device)
+    keep_tokens(pool, table, first, kept)
+    assert torch.equal(pool.k, want[0]) and torch.equal(pool.v, want[1])
+
+
 def test_keep_tokens_short_lists_and_device_entries(device):
     """Lists that one wave moves; entries that move nothing; a tensor's rows apart."""
     rng = np.random.default_rng(4)

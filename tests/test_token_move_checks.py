@@ -1,4 +1,6 @@
 """Refusals of keep_tokens, fork_rows and rotaries of several axes, on the host (CPU only)."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -124,6 +126,16 @@ def test_copy_pages_refusals():
             _lib.call("kunserve_copy_pages", p.desc(), None, None if host is None else host.ctypes.data,
                       None if dev is None else dev.ctypes.data, n, None)
     assert _lib.call("kunserve_copy_pages", p.desc(), None, None, None, 0, None) == 0
+
+
+def test_keep_tokens_refuses_first_places():
+    p = pool()
+    zeros = np.zeros(300, np.int32)
+    n = zeros.ctypes.data
+    t = _lib.PageTable(indptr_dev=n, indices_dev=n, kv_len_dev=n, num_seqs=300)   # (refused unread)
+    for host, dev, why in ((None, None, "either"), (n, n, "either"), (n, None, "256 at most")):
+        with pytest.raises(_lib.KunserveError, match=why):
+            _lib.call("kunserve_keep_tokens", p.desc(), None, ctypes.byref(t), host, dev, n, 1, 1, None)
 
 
 def test_fork_pages_outside():

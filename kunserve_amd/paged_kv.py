@@ -370,11 +370,12 @@ class PageTable:
 
 
 def _tensor3(t: torch.Tensor) -> _lib.Tensor3:
-    if t.dim() != 3 or t.stride(-1) != 1:
+    s = t.stride()
+    if len(s) != 3 or s[2] != 1:
         raise ValueError("expected a [tokens, heads, head_dim] tensor with head_dim contiguous")
     if t.dtype not in _DTYPES:
         raise ValueError("expected float16 or bfloat16")
-    return _lib.Tensor3(t.data_ptr(), t.stride(0), t.stride(1))
+    return _lib.Tensor3(t.data_ptr(), s[0], s[1])
 
 
 def _check_reach(device: torch.device, **tensors: Optional[torch.Tensor]) -> None:

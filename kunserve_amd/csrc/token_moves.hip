@@ -33,7 +33,7 @@ struct KeepArgs {
   int32_t page_shift;
   int32_t num_layers;
   int32_t num_heads;
-  int64_t num_slabs;   // rows x K and V x layers x heads
+  int64_t num_slabs;   // rows x layers x heads, x K and V where they are a workgroup's each
 };
 
 // [rows]: the rows' first places, which for few rows go with the launch's arguments (small rows
@@ -45,15 +45,19 @@ struct FirstHere {
   int32_t at[KUNSERVE_FIRST_BY_VALUE];
 };
 
-// A slab is a row's tokens of one layer, KV head and K or V. It moves chunk by chunk:
-// slots [c, c + n) are written after the tokens kept[c], .. kept[c + n - 1] have been
-// read, by one wave (W 1) or by a workgroup that meets between. A token moves down
-// (kept[j] > j), so what a later chunk reads no earlier one has written.
+// A slab is a row's tokens of one layer and KV head, K and V for a wave (W 1), one of them
+// for a workgroup. It moves chunk by chunk: slots [c, c + n) are written after the tokens
+// kept[c], .. kept[c + n - 1] have been read, by the wave or by the workgroup, which meets
+// between. A token moves down (kept[j] > j), so what a later chunk reads no earlier one has
+// written. Accepted paths are short, and a wave waits for what it reads: rows, lists, page
+// ids, tokens (64 rows, 32 layers of 8 heads: 17 us, 20 with a wave each for K and V).
 template <int D, int W, typename First>
 __global__ __launch_bounds__(kThreads) void keep_tokens_kernel(KeepArgs a, First from_place) {
   constexpr int CH = D / 8;
   constexpr int TPL = kWave / CH;                 // tokens of a load
-  constexpr int CHUNK = kLoads * TPL * W;
+  constexpr int KV = W == 1 ? 2 : 1;              // K and V of a wave's tokens, or one of them
+  constexpr int N = kLoads / KV;                  // loads of either
+  constexpr int CHUNK = N * TPL * W;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
   const int64_t slab = W == 1 ? int64_t(blockIdx.x) * kWaves + wave : blockIdx.x;
@@ -61,8 +65,8 @@ __global__ __launch_bounds__(kThreads) void keep_tokens_kernel(KeepArgs a, First
   const int head = int(slab % a.num_heads);
   const int64_t rest = slab / a.num_heads;
   const int layer = int(rest % a.num_layers);
-  const bool of_v = rest / a.num_layers & 1;
-  const int b = int(rest / a.num_layers >> 1);
+  const bool of_v = KV == 1 && (rest / a.num_layers & 1);
+  const int b = int(rest / a.num_layers / (KV == 1 ? 2 : 1));
   const int lrow = lane / CH, lcol = lane % CH;
 
   const int first = from_place.at[b], len = a.kv_len[b] - first;
@@ -70,44 +74,48 @@ __global__ __launch_bounds__(kThreads) void keep_tokens_kernel(KeepArgs a, First
   const int32_t* pages = a.indices + a.indptr[b];
   const int32_t* kept = a.kept + int64_t(b) * a.kept_stride;
   const int mask = (1 << a.page_shift) - 1;
-  f16* base = (of_v ? a.v : a.k) + int64_t(layer) * a.layer_stride + int64_t(head) * a.head_stride +
-              8 * lcol;
+  const int64_t at = int64_t(layer) * a.layer_stride + int64_t(head) * a.head_stride + 8 * lcol;
+  f16* const base[2] = {(of_v ? a.v : a.k) + at, a.v + at};
   float* weights = a.w && !of_v && lcol == 0
                        ? a.w + int64_t(layer) * a.w_layer + int64_t(head) * a.w_head
                        : nullptr;
 
   const int n = min(a.max_kept, len);
   for (int c = 0; c < n; c += CHUNK) {
-    int from[kLoads], src[kLoads], dst[kLoads];
-    f16x8 x[kLoads];
-    float w[kLoads];
+    int from[N], src[N], dst[N];
+    f16x8 x[KV][N];
+    float w[N];
     auto place = [&](int i) { return c + ((W == 1 ? 0 : wave) + W * i) * TPL + lrow; };
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
+    for (int i = 0; i < N; ++i) {
       const int j = place(i);
       from[i] = j < n ? kept[j] : -1;
     }
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
+    for (int i = 0; i < N; ++i) {
       const bool moves = from[i] > place(i) && from[i] < len;
       src[i] = moves ? pages[(first + from[i]) >> a.page_shift] : -1;
       dst[i] = moves ? pages[(first + place(i)) >> a.page_shift] : -1;
     }
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
+    for (int i = 0; i < N; ++i) {
       const bool ok = src[i] >= 0 && src[i] < a.num_pages;
       const int slot = (first + from[i]) & mask;
-      x[i] = ok ? load_f16x8(base + int64_t(src[i]) * a.page_stride + int64_t(slot) * a.token_stride)
-                : f16x8{};
+#pragma unroll
+      for (int z = 0; z < KV; ++z)
+        x[z][i] = ok ? load_f16x8(base[z] + int64_t(src[i]) * a.page_stride + int64_t(slot) * a.token_stride)
+                     : f16x8{};
       if (a.w) w[i] = ok && weights ? weights[int64_t(src[i]) * a.w_page + slot] : 0.f;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // read before any of it is overwritten
     if constexpr (W > 1) __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
+    for (int i = 0; i < N; ++i) {
       if (dst[i] < 0 || dst[i] >= a.num_pages) continue;
       const int slot = (first + place(i)) & mask;
-      store_f16x8(base + int64_t(dst[i]) * a.page_stride + int64_t(slot) * a.token_stride, x[i]);
+#pragma unroll
+      for (int z = 0; z < KV; ++z)
+        store_f16x8(base[z] + int64_t(dst[i]) * a.page_stride + int64_t(slot) * a.token_stride, x[z][i]);
       if (weights) weights[int64_t(dst[i]) * a.w_page + slot] = w[i];
     }
   }
@@ -266,11 +274,11 @@ extern "C" int kunserve_keep_tokens(const kunserve_kv_pool* pool,
   a.page_shift = __builtin_ctz(pool->page_size);
   a.num_layers = pool->num_layers;
   a.num_heads = pool->num_kv_heads;
-  a.num_slabs = 2 * int64_t(table->num_seqs) * pool->num_layers * pool->num_kv_heads;
-  // A wave to a slab where its chunk holds the list: no barrier, and four slabs to a
+  // A wave to a slab where two of its chunks hold the list: no barrier, and four slabs to a
   // workgroup.
   const int chunk = kLoads * kWave / (pool->head_dim / 8);
   const bool small = max_kept <= chunk;
+  a.num_slabs = (small ? 1 : 2) * int64_t(table->num_seqs) * pool->num_layers * pool->num_kv_heads;
   const int64_t blocks = small ? (a.num_slabs + kWaves - 1) / kWaves : a.num_slabs;
   KSV_CHECK_ARG(blocks < (int64_t(1) << 31), "grid of %lld workgroups is too large",
                 (long long)blocks);

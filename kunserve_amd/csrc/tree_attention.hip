@@ -158,7 +158,8 @@ __device__ __forceinline__ void two_terms(float x, float y, uint32_t& hi, uint32
     const uint32_t a = f32_to_bits(x), b = f32_to_bits(y);
     hi = __builtin_amdgcn_perm(b, a, 0x07060302u);
     typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    const b2 l = {__bf16(x - bits_to_f32(int(a & 0xffff0000u))), __bf16(y - bits_to_f32(int(b & 0xffff0000u)))};
+    const b2 l = {__bf16(x - bits_to_f32(int(a & 0xffff0000u))),
+                  __bf16(y - bits_to_f32(int(b & 0xffff0000u)))};
     lo = __builtin_bit_cast(uint32_t, l);
   } else {
     const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
@@ -188,7 +189,8 @@ __device__ __forceinline__ uint32_t dim_pair(uint32_t x, uint32_t y, int odd) {
 // layer, 6.25 TB/s, as fast as single tokens; 32 each 272 us, of which the products take
 // 165 at a large product's rate; 64 each 446 us and 335.
 template <typename T, int D, int WC>
-__global__ __launch_bounds__((TreeTile<D, WC>::WAVES * kWave), D == 256 ? 1 : 2) void tree_attention_kernel(TreeArgs ta) {
+__global__ __launch_bounds__((TreeTile<D, WC>::WAVES * kWave), D == 256 ? 1 : 2)
+void tree_attention_kernel(TreeArgs ta) {
   typedef typename Vec<T>::v8 V8;
   typedef TreeTile<D, WC> L;
   constexpr int STEP = L::STEP, TPL = L::TPL, LOADS = L::LOADS, CH = L::CH;
@@ -848,7 +850,8 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
   const int64_t slots_at_once = kind.per_cu * cus;
   const int64_t run = part_rounds > 0
                           ? std::min<int64_t>(part_rounds, std::max(longest, 1))
-                          : best_run(rows, longest, work, max_cols, ratio, num_kv_heads, round, slots_at_once);
+                          : best_run(rows, longest, work, max_cols, ratio, num_kv_heads, round,
+                                     slots_at_once);
 
   struct Piece {
     int32_t row, part, rb, re;
@@ -997,9 +1000,6 @@ int kunserve::tree_attention(const kunserve_kv_pool* pool, int32_t layer,
                 info->num_kv_heads, num_qo_heads, pool->num_kv_heads);
   KSV_CHECK_ARG(info->num_seqs == table->num_seqs, "plan made for %d rows, not %d", info->num_seqs,
                 table->num_seqs);
-  bool known = false;
-  for (int k = 0; k < 4; ++k) known = known || (info->columns && kinds_of(info->head_dim)[k].columns == info->columns);
-  KSV_CHECK_ARG(known, "plan of %d columns to a workgroup", info->columns);
   KSV_CHECK_ARG(pool->token_stride < (int64_t(1) << 28),
                 "tokens %lld elements apart: less than 2^28 here", (long long)pool->token_stride);
   KSV_CHECK_ARG(num_qo_heads < 65536, "%d query heads: at most 65535", num_qo_heads);
@@ -1016,6 +1016,10 @@ int kunserve::tree_attention(const kunserve_kv_pool* pool, int32_t layer,
   const int rc = decode_args(pool, layer, table, nullptr, q, out, num_qo_heads, sm_scale, plan_dev,
                              &parts, workspace_dev, workspace_bytes, append, &ta.d);
   if (rc || info->num_work == 0) return rc;
+  bool known = false;   // (the pool's head_dim is one of three here)
+  for (int k = 0; k < 4 && info->columns; ++k)
+    known = known || kinds_of(info->head_dim)[k].columns == info->columns;
+  KSV_CHECK_ARG(known, "plan of %d columns to a workgroup", info->columns);
   KSV_CHECK_ARG(aligned16(workspace_dev), "workspace must be 16-byte aligned");
   KSV_CHECK_ARG(aligned16(out->data) && out->token_stride % 8 == 0 && out->head_stride % 8 == 0,
                 "out must be 16-byte aligned with strides that are multiples of 8");

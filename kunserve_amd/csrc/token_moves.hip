@@ -16,6 +16,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kLoads = 8;   // 16-byte loads of a lane that are under way together
+constexpr int64_t kMaxBlocks = (int64_t(1) << 32) / kThreads;   // a launch's threads fit 32 bits
 
 struct KeepArgs {
   f16* k;
@@ -131,7 +132,6 @@ struct CopyArgs {
   int32_t page_size;
   int32_t num_heads;
   int32_t heads, parts;   // heads of a workgroup, workgroups of all
-  uint32_t slabs;         // workgroups of a move
 };
 
 // [n][3]: source page, destination page, tokens. Few of them go with the launch's
@@ -154,8 +154,8 @@ __global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyArgs a, Moves 
   constexpr int CH = D / 8;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
-  const int slab = int(blockIdx.x % a.slabs);
-  const int64_t at3 = 3 * int64_t(blockIdx.x / a.slabs);
+  const int slab = int(blockIdx.x);
+  const int64_t at3 = 3 * int64_t(blockIdx.y);
   const int from = moves.m[at3], to = moves.m[at3 + 1], tokens = min(moves.m[at3 + 2], a.page_size);
   if (from < 0 || from >= a.num_pages || to < 0 || to >= a.num_pages || tokens <= 0) return;
   const int h0 = slab % a.parts * a.heads, layer = slab / a.parts >> 1;
@@ -213,10 +213,10 @@ void keep_tokens(dim3 grid, bool small, const KeepArgs& a, const int32_t* first_
 
 template <int D>
 void copy_pages(dim3 grid, const CopyArgs& a, const int32_t* moves_host, const int32_t* moves_dev,
-                int64_t n, hipStream_t s) {
+                hipStream_t s) {
   if (moves_host) {
     MovesHere here;
-    std::copy_n(moves_host, 3 * n, here.m);
+    std::copy_n(moves_host, 3 * grid.y, here.m);
     copy_pages_kernel<D><<<grid, kThreads, 0, s>>>(a, here);
   } else {
     copy_pages_kernel<D><<<grid, kThreads, 0, s>>>(a, MovesThere{moves_dev});
@@ -280,7 +280,7 @@ extern "C" int kunserve_keep_tokens(const kunserve_kv_pool* pool,
   const bool small = max_kept <= chunk;
   a.num_slabs = (small ? 1 : 2) * int64_t(table->num_seqs) * pool->num_layers * pool->num_kv_heads;
   const int64_t blocks = small ? (a.num_slabs + kWaves - 1) / kWaves : a.num_slabs;
-  KSV_CHECK_ARG(blocks < (int64_t(1) << 31), "grid of %lld workgroups is too large",
+  KSV_CHECK_ARG(blocks < kMaxBlocks, "grid of %lld workgroups is too large",
                 (long long)blocks);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(blocks));
@@ -376,14 +376,18 @@ extern "C" int kunserve_copy_pages(const kunserve_kv_pool* pool, const kunserve_
   const int64_t per_head = (int64_t(pool->page_size) * (pool->head_dim / 8) + kWave - 1) / kWave;
   a.heads = int32_t(per_head >= 64 ? 1 : 64 / per_head);
   a.parts = (pool->num_kv_heads + a.heads - 1) / a.heads;
-  a.slabs = uint32_t(2 * pool->num_layers) * uint32_t(a.parts);
-  KSV_CHECK_ARG(n * a.slabs < (int64_t(1) << 31), "%lld moves of %u workgroups", (long long)n, a.slabs);
-  const dim3 grid(static_cast<unsigned>(n * a.slabs));
+  const int64_t slabs = 2 * int64_t(pool->num_layers) * a.parts;   // workgroups of a move
+  KSV_CHECK_ARG(slabs < kMaxBlocks, "moves of %lld workgroups", (long long)slabs);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  switch (pool->head_dim) {
-    case 64: copy_pages<64>(grid, a, moves_host, moves_dev, n, s); break;
-    case 128: copy_pages<128>(grid, a, moves_host, moves_dev, n, s); break;
-    default: copy_pages<256>(grid, a, moves_host, moves_dev, n, s);
+  constexpr int64_t kMoves = 65535;   // of a launch
+  for (int64_t from = 0; from < n; from += kMoves) {
+    const dim3 grid(unsigned(slabs), unsigned(std::min(kMoves, n - from)));
+    const int32_t* dev = moves_dev ? moves_dev + 3 * from : nullptr;
+    switch (pool->head_dim) {
+      case 64: copy_pages<64>(grid, a, moves_host, dev, s); break;
+      case 128: copy_pages<128>(grid, a, moves_host, dev, s); break;
+      default: copy_pages<256>(grid, a, moves_host, dev, s);
+    }
   }
   KSV_CHECK_LAUNCH();
   return KUNSERVE_OK;

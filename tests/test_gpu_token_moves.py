@@ -156,6 +156,19 @@ def test_fork_rows_of_many_pages(device, pages):
         assert torch.equal(t, want)
 
 
+def test_fork_rows_of_more_pages_than_a_launch_takes(device):
+    pages = 70001
+    pool = random_pool(2 * pages, 1, 1, 4, 64, device, 1)
+    ids = torch.randperm(2 * pages, generator=torch.Generator().manual_seed(1))
+    src, dst = ids[:pages], ids[pages:]
+    want = [t.clone() for t in (pool.k, pool.v)]
+    for t in want:
+        t[dst[:-1].to(device)] = t[src[:-1].to(device)]
+        t[dst[-1], :, :, :3] = t[src[-1], :, :, :3]
+    fork_rows(pool, [src.tolist()], [4 * pages - 1], [dst.tolist()])
+    assert torch.equal(pool.k, want[0]) and torch.equal(pool.v, want[1])
+
+
 def test_fork_rows_strides(device):
     big = torch.randn(12, 2, 2, 6, 16, 128, device=device).to(F16)
     pool = KVPool(big[:, :, 0, 1:4], big[:, :, 1, 1:4])

@@ -274,8 +274,10 @@ extern "C" int kunserve_keep_tokens(const kunserve_kv_pool* pool,
   a.page_shift = __builtin_ctz(pool->page_size);
   a.num_layers = pool->num_layers;
   a.num_heads = pool->num_kv_heads;
-  // A wave to a slab where two of its chunks hold the list: no barrier, and four slabs to a
-  // workgroup.
+  // A wave to a slab where two of its chunks hold the longest list: no barrier, and four slabs
+  // to a workgroup. (8 layers of 8 heads of 128; 64 rows, all lists full: of 16 10 us against 19,
+  // of 32 20 each, of 64 42 against 41; 4 rows: of 16 3.6 against 3.7, of 32 5.0 against 4.0, of
+  // 64 8 against 5. Most lists are shorter than the longest.)
   const int chunk = kLoads * kWave / (pool->head_dim / 8);
   const bool small = max_kept <= chunk;
   a.num_slabs = (small ? 1 : 2) * int64_t(table->num_seqs) * pool->num_layers * pool->num_kv_heads;

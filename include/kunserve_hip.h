@@ -541,8 +541,8 @@ int64_t kunserve_tree_workspace_bytes(const kunserve_tree_plan_info* info);
 /* Attention of the plan's new tokens: each sees its row's cached tokens before
  * them, its ancestors and itself (their K and V are in the pages already).
  * Otherwise as kunserve_paged_decode, on the table the plan was made from (its
- * ids may be others, its lengths not). out may be q, and is 16-byte aligned
- * with strides that are multiples of 8; so is the workspace. */
+ * ids may be others, its lengths not). out may be q, and is 8-byte aligned with
+ * strides that are multiples of 4; the workspace is 16-byte aligned. */
 int kunserve_tree_attention(const kunserve_kv_pool* pool, int32_t layer,
                             const kunserve_page_table* table,
                             const kunserve_tensor3* q, kunserve_tensor3* out,

@@ -120,6 +120,12 @@ extern "C" int kunserve_attention_step_more(const kunserve_step* step,
       weights_scores(&info, extras->weights_plan_dev, extras->weights_workspace_dev, &decode);
     }
   }
+  if (trees) {   // before q is rotated in place, or a page written
+    rc = tree_check(&step->pool, layer, &more->tree_table, &q, &out, step->num_qo_heads,
+                    step->sm_scale, more->tree_plan_dev, &more->tree_info, step->workspace_dev,
+                    step->workspace_bytes);
+    if (rc) return rc;
+  }
   if (rotary) {
     rc = kunserve_rotary_axes_append_kv(&step->pool, layer, &step->table, step->q_indptr_dev,
                                         step->num_tokens, &q, &q, step->num_qo_heads, &io->k,

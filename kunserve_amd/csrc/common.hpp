@@ -108,6 +108,11 @@ int tree_attention(const kunserve_kv_pool* pool, int32_t layer, const kunserve_p
                    float sm_scale, const int32_t* plan_dev, const kunserve_tree_plan_info* info,
                    void* workspace_dev, int64_t workspace_bytes, const StepFusion& fusion,
                    kunserve_stream_t stream);
+// What it refuses, for a step that launches others before it.
+int tree_check(const kunserve_kv_pool* pool, int32_t layer, const kunserve_page_table* table,
+               const kunserve_tensor3* q, kunserve_tensor3* out, int32_t num_qo_heads,
+               float sm_scale, const int32_t* plan_dev, const kunserve_tree_plan_info* info,
+               void* workspace_dev, int64_t workspace_bytes);
 
 // The attention weights of a step's decode rows from the scores that their decode
 // launch left in the plan's workspace (weights_scores says where).

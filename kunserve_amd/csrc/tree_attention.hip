@@ -983,12 +983,13 @@ extern "C" int64_t kunserve_tree_workspace_bytes(const kunserve_tree_plan_info* 
   return int64_t(info->num_slots) * info->num_qo_heads * (info->head_dim + 1) * 4;
 }
 
-int kunserve::tree_attention(const kunserve_kv_pool* pool, int32_t layer,
-                             const kunserve_page_table* table, const kunserve_tensor3* q,
-                             kunserve_tensor3* out, int32_t num_qo_heads, float sm_scale,
-                             const int32_t* plan_dev, const kunserve_tree_plan_info* info,
-                             void* workspace_dev, int64_t workspace_bytes,
-                             const StepFusion& fusion, kunserve_stream_t stream) {
+// The arguments of the launch and of the joining of its partials, which are the decode
+// launch's; ta stays empty where there is no work.
+static int tree_args(const kunserve_kv_pool* pool, int32_t layer, const kunserve_page_table* table,
+                     const kunserve_tensor3* q, kunserve_tensor3* out, int32_t num_qo_heads,
+                     float sm_scale, const int32_t* plan_dev, const kunserve_tree_plan_info* info,
+                     void* workspace_dev, int64_t workspace_bytes, const StepFusion& fusion,
+                     kunserve_decode_plan_info* parts, TreeArgs* ta) {
   clear_error();
   KSV_CHECK_ARG(pool && table && q && out && info, "null argument");
   KSV_CHECK_ARG(info->head_dim == pool->head_dim, "plan made for head_dim %d, pool has %d",
@@ -1003,36 +1004,62 @@ int kunserve::tree_attention(const kunserve_kv_pool* pool, int32_t layer,
   KSV_CHECK_ARG(pool->token_stride < (int64_t(1) << 28),
                 "tokens %lld elements apart: less than 2^28 here", (long long)pool->token_stride);
   KSV_CHECK_ARG(num_qo_heads < 65536, "%d query heads: at most 65535", num_qo_heads);
-  // The launch's arguments and the joining of its partials are the decode launch's.
-  kunserve_decode_plan_info parts{};
-  parts.num_work = info->num_work;
-  parts.num_merge = info->num_merge;
-  parts.num_slots = info->num_slots;
-  parts.group_size = decode_group(num_qo_heads, std::max(pool->num_kv_heads, 1));
-  TreeArgs ta{};
+  *parts = kunserve_decode_plan_info{};
+  parts->num_work = info->num_work;
+  parts->num_merge = info->num_merge;
+  parts->num_slots = info->num_slots;
+  parts->group_size = decode_group(num_qo_heads, std::max(pool->num_kv_heads, 1));
+  *ta = TreeArgs{};
   StepFusion append;
   append.k_new = fusion.k_new;
   append.v_new = fusion.v_new;
   const int rc = decode_args(pool, layer, table, nullptr, q, out, num_qo_heads, sm_scale, plan_dev,
-                             &parts, workspace_dev, workspace_bytes, append, &ta.d);
+                             parts, workspace_dev, workspace_bytes, append, &ta->d);
   if (rc || info->num_work == 0) return rc;
   bool known = false;   // (the pool's head_dim is one of three here)
   for (int k = 0; k < 4 && info->columns; ++k)
     known = known || kinds_of(info->head_dim)[k].columns == info->columns;
   KSV_CHECK_ARG(known, "plan of %d columns to a workgroup", info->columns);
   KSV_CHECK_ARG(aligned16(workspace_dev), "workspace must be 16-byte aligned");
-  KSV_CHECK_ARG(aligned16(out->data) && out->token_stride % 8 == 0 && out->head_stride % 8 == 0,
-                "out must be 16-byte aligned with strides that are multiples of 8");
-  ta.records = plan_dev;
-  const int32_t* merges = plan_dev + kTreeRecord * int64_t(info->num_work);
-  ta.masks = reinterpret_cast<const uint32_t*>(merges + 4 * int64_t(info->num_merge));
+  KSV_CHECK_ARG((reinterpret_cast<uintptr_t>(out->data) & 7) == 0 && out->token_stride % 4 == 0 &&
+                    out->head_stride % 4 == 0,
+                "q must be 16-byte aligned with strides that are multiples of 8, out 8-byte "
+                "aligned with multiples of 4");
+  ta->records = plan_dev;
+  ta->masks = reinterpret_cast<const uint32_t*>(plan_dev + kTreeRecord * int64_t(info->num_work) +
+                                                4 * int64_t(info->num_merge));
+  return KUNSERVE_OK;
+}
+
+int kunserve::tree_check(const kunserve_kv_pool* pool, int32_t layer,
+                         const kunserve_page_table* table, const kunserve_tensor3* q,
+                         kunserve_tensor3* out, int32_t num_qo_heads, float sm_scale,
+                         const int32_t* plan_dev, const kunserve_tree_plan_info* info,
+                         void* workspace_dev, int64_t workspace_bytes) {
+  kunserve_decode_plan_info parts;
+  TreeArgs ta;
+  return tree_args(pool, layer, table, q, out, num_qo_heads, sm_scale, plan_dev, info,
+                   workspace_dev, workspace_bytes, StepFusion{}, &parts, &ta);
+}
+
+int kunserve::tree_attention(const kunserve_kv_pool* pool, int32_t layer,
+                             const kunserve_page_table* table, const kunserve_tensor3* q,
+                             kunserve_tensor3* out, int32_t num_qo_heads, float sm_scale,
+                             const int32_t* plan_dev, const kunserve_tree_plan_info* info,
+                             void* workspace_dev, int64_t workspace_bytes,
+                             const StepFusion& fusion, kunserve_stream_t stream) {
+  kunserve_decode_plan_info parts;
+  TreeArgs ta;
+  const int rc = tree_args(pool, layer, table, q, out, num_qo_heads, sm_scale, plan_dev, info,
+                           workspace_dev, workspace_bytes, fusion, &parts, &ta);
+  if (rc || info->num_work == 0) return rc;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int err = pool->dtype == KUNSERVE_DTYPE_BF16
                       ? launch_tree<bf16>(pool->head_dim, info->columns, ta, unsigned(info->num_work), s)
                       : launch_tree<f16>(pool->head_dim, info->columns, ta, unsigned(info->num_work), s);
   if (err) return err;
   parts.num_work = 0;   // the records behind which its merges are
-  return decode_merge(pool, ta.d, &parts, merges, s);
+  return decode_merge(pool, ta.d, &parts, plan_dev + kTreeRecord * int64_t(info->num_work), s);
 }
 
 extern "C" int kunserve_tree_attention(const kunserve_kv_pool* pool, int32_t layer,

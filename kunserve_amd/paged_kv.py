@@ -772,10 +772,10 @@ def rotary_append_kv(pool: KVPool, layer: int, table: PageTable, q_indptr: torch
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The attention prologue of one layer with a Rotary: q and k_new rotated, the
     rotated k and v_new written into their pages. positions (device int32
-    [num_tokens], or [axes, num_tokens] for a Rotary of several axes): the tokens'
-    rotary positions, where they are not their places in the cache. The rotated q goes to
-    out (default: q, in place), which must be q or lie apart from q, k_new and v_new.
-    Returns out."""
+    [num_tokens], or [axes, num_tokens] with one on each axis of the Rotary): the
+    tokens' rotary positions, where they are not their places in the cache. The rotated q
+    goes to out (default: q, in place), which must be q or lie apart from q, k_new and
+    v_new. Returns out."""
     q_shape, k_shape, device = q.shape, k_new.shape, pool.device
     tokens, dim, dtype = k_shape[0], pool.head_dim, pool.dtype
     if k_shape != v_new.shape or k_shape[1:] != (pool.num_kv_heads, dim):
@@ -982,8 +982,8 @@ class AttentionStep:
 
     rope_positions: for each row the rotary position of its first new token, where
     that is not its place in the cache (rows shortened by evict), or an array [axes,
-    num_tokens] with every new token's position on each axis of a Rotary of several.
-    Only a Rotary takes them.
+    num_tokens] with every new token's position on each axis of the Rotary ([1,
+    num_tokens] for one of a single axis). Only a Rotary takes them.
 
     trees: for each row None, or the tree that its new tokens are (drafted tokens that
     the step verifies): a list with the place of each token's parent among them, below
@@ -1060,9 +1060,9 @@ class AttentionStep:
         tree_rows = np.flatnonzero(drafted)
         drafts = _Trees([trees[b] for b in tree_rows], tree_rows) if tree_rows.size else None
         positions = None
-        if np.ndim(rope_positions) == 2 and len(rope_positions) != 1:
+        if np.ndim(rope_positions) == 2:
             positions = np.asarray(rope_positions)
-            if positions.shape[0] < 2 or positions.shape[1] != self.num_tokens:
+            if positions.shape[0] < 1 or positions.shape[1] != self.num_tokens:
                 raise ValueError(f"{self.num_tokens} tokens but {positions.shape} rope_positions")
             if positions.size and positions.dtype.kind not in "iu":
                 raise ValueError("rope_positions must be whole numbers")

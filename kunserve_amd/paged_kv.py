@@ -1359,18 +1359,20 @@ class AttentionStep:
         what the row had cached, in every layer and KV head of the pool: the accepted
         path of a drafted tree. kept counts from the row's first new token, rising
         (lists, or a device int32 tensor [rows, most kept] with -1 behind a row's last:
-        no host wait, and a graph capture takes it). weights (a KVWeights of the pool)
-        move along. The row goes on with its cached tokens and those kept. The pages of
-        new tokens must be in one place of the step's lists (ValueError)."""
+        no host wait, and a graph capture takes it, of a step without trees up to 256
+        rows). weights (a KVWeights of the pool) move along. The row goes on with its
+        cached tokens and those kept. The pages of new tokens must be in one place of the
+        step's lists (ValueError)."""
         from .token_moves import move_tokens
 
         if not self._private:
             raise ValueError("tokens move in place: their pages must be in one place of the "
                              "step's lists")
         first = self.kv_len - np.diff(self.q_indptr_host)
-        if self._first is None and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("a step without trees uploads its rows' first places: not under a "
-                               "capture")
+        if (self._first is None and len(first) > _lib.FIRST_BY_VALUE
+                and torch.cuda.is_current_stream_capturing()):
+            raise RuntimeError(f"a step of {len(first)} rows without trees uploads their first places: "
+                               "not under a capture")
         move_tokens(self.pool, self.table, self._first, first, kept, weights)
 
 

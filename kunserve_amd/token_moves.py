@@ -28,7 +28,7 @@ def keep_tokens(pool: KVPool, table: PageTable, first: Union[int, Sequence[int]]
     behind a row's last. An entry of a tensor that is not above its own place j or
     lies past the row's end moves nothing. weights (a KVWeights of the pool) move
     along. The pages from first[b] on must be in one place of the table
-    (ValueError)."""
+    (ValueError). Not for a graph capture, which takes AttentionStep.keep_tokens."""
     n = table.num_seqs
     given = np.asarray(first)
     if given.dtype.kind not in "iu" or given.shape not in ((), (n,)):
@@ -42,8 +42,8 @@ def keep_tokens(pool: KVPool, table: PageTable, first: Union[int, Sequence[int]]
     starts = np.empty(n, dtype=np.int32)
     starts[:] = given
     if pool.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("keep_tokens cannot be captured: its first places are uploaded; "
-                           "AttentionStep.keep_tokens can")
+        raise RuntimeError("not under a capture, which takes AttentionStep.keep_tokens: a step's rows "
+                           "and places")
     moving = np.zeros(n + 1, dtype=np.int32)
     np.cumsum(lens - starts, out=moving[1:])
     ids = table.indices_host if table.indices_host.size else moving   # (there is one)

@@ -891,7 +891,11 @@ def tree_attention(pool: KVPool, layer: int, table: PageTable, q: torch.Tensor, 
         raise ValueError(f"q has {q.shape[0]} tokens, the plan's rows end at {plan.end}")
     if q.shape[2] != pool.head_dim:
         raise ValueError(f"q shape {tuple(q.shape)} does not match head_dim {pool.head_dim}")
-    _check_reach(pool.device, q=q, out=out)
+    rows = table.desc()   # (bound, so that it has device arrays)
+    _check_reach(pool.device, q=q, out=out, workspace=workspace, plan=plan.plan,
+                 table=table.indices)
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=pool.device)
     if out.shape != q.shape:
@@ -904,7 +908,7 @@ def tree_attention(pool: KVPool, layer: int, table: PageTable, q: torch.Tensor, 
     if plan.info.plan_ints and plan.plan is None:
         raise RuntimeError("tree plan used before its device array was bound")
     qd, od = _tensor3(q), _tensor3(out)
-    _lib.call("kunserve_tree_attention", pool.desc(), layer, table.desc(), ctypes.byref(qd),
+    _lib.call("kunserve_tree_attention", pool.desc(), layer, rows, ctypes.byref(qd),
               ctypes.byref(od), q.shape[1], ctypes.c_float(scale), _ptr(plan.plan),
               ctypes.byref(plan.info), _ptr(workspace),
               0 if workspace is None else workspace.numel() * workspace.element_size(),

@@ -823,7 +823,8 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
                   kv_len[b]);
     r.tokens = n;
     r.q_first = q_first ? q_first[b] : q_indptr[b];
-    KSV_CHECK_ARG(r.q_first >= 0, "row %d: its first token is %d", b, r.q_first);
+    KSV_CHECK_ARG(r.q_first >= 0 && int64_t(r.q_first) + n <= int64_t(1) << 31,
+                  "row %d of %d tokens: its first token is %d", b, n, r.q_first);
     KSV_CHECK_ARG(int64_t(n) * ratio < (int64_t(1) << 31) - max_cols, "row %d: %d tokens of %d heads",
                   b, n, ratio);
     r.prefix = kv_len[b] - n;
@@ -846,6 +847,19 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
     }
     work += n ? int64_t(r.rounds) * ceil_div(int64_t(n) * ratio, max_cols) * num_kv_heads : 0;
     if (n) longest = std::max(longest, r.rounds);
+  }
+  if (q_first) {   // rows write their tokens of out
+    std::vector<int32_t> by_first;
+    for (int32_t b = 0; b < num_seqs; ++b)
+      if (rows[b].tokens) by_first.push_back(b);
+    const auto before = [&](int32_t x, int32_t y) { return rows[x].q_first < rows[y].q_first; };
+    if (!std::is_sorted(by_first.begin(), by_first.end(), before))
+      std::sort(by_first.begin(), by_first.end(), before);
+    for (size_t i = 1; i < by_first.size(); ++i) {
+      const TreeRow &x = rows[by_first[i - 1]], &y = rows[by_first[i]];
+      KSV_CHECK_ARG(int64_t(x.q_first) + x.tokens <= y.q_first, "rows %d and %d both have token %d",
+                    by_first[i - 1], by_first[i], y.q_first);
+    }
   }
   const int64_t slots_at_once = kind.per_cu * cus;
   const int64_t run = part_rounds > 0

@@ -541,7 +541,7 @@ class TreePlan:
     Row b's new tokens are the last len(parents[b]) of its kv_len; parents[b][i] is
     the place of token i's parent among them, below i, or -1 for one that follows the
     cached tokens. They are tokens q_first[b] onwards of q and out (default: one row
-    after the other). part_rounds: rounds of a piece of a row, 0 to choose."""
+    after the other), each in one row. part_rounds: rounds of a piece of a row, 0 to choose."""
 
     def __init__(self, table: "PageTable", parents: Sequence[Sequence[int]], num_qo_heads: int,
                  num_kv_heads: int, page_size: int, device: torch.device,

@@ -99,3 +99,22 @@ def test_refused_before_anything_changes(device, pinned):
     for t, old in zip((m.pool.k, m.pool.v, m.q), before):
         assert torch.equal(t, old)
     assert not big.any()
+
+
+@pytest.mark.parametrize("dim,hq,hkv,tokens,columns", [(64, 8, 2, 17, None), (128, 8, 2, 17, None),
+                                                       (128, 16, 4, 64, 256), (256, 8, 2, 64, None)])
+@pytest.mark.parametrize("page", [4, 8, 16])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_rows_append_within_their_launches(device, dim, hq, hkv, tokens, columns, page, dtype):
+    """Decode, prefill and tree launches that each take their rows' k and v from the step."""
+    m = Mixed(device, dim, dtype, page, hq, hkv, tokens)
+    before = [t.clone() for t in (m.pool.k, m.pool.v)]
+    step = m.step()
+    assert step._private and (columns is None or step.tree.plan.info.columns == columns)
+    out = step.run(0, m.q, m.k, m.v)
+    m.check_pool(before)
+    m.check(out)
+    for t in (m.pool.k, m.pool.v):   # and again, from pages without them
+        t.copy_(before[0] if t is m.pool.k else before[1])
+    assert torch.equal(step.run(0, m.q, m.k, m.v), out)
+    m.check_pool(before)

@@ -818,6 +818,7 @@ int tree_plan(const int32_t* indptr, const int32_t* q_indptr, const int32_t* q_f
     const int32_t n = q_indptr[b + 1] - q_indptr[b];
     TreeRow& r = rows[b];
     KSV_CHECK_ARG(n >= 0 && kv_len[b] >= n, "row %d: %d new tokens of %d", b, n, kv_len[b]);
+    KSV_CHECK_ARG(indptr[b] >= 0, "row %d: its pages start at %d", b, indptr[b]);
     KSV_CHECK_ARG(int64_t(indptr[b + 1]) - indptr[b] >= ceil_div(kv_len[b], page_size),
                   "row %d: %lld pages for %d tokens", b, (long long)indptr[b + 1] - indptr[b],
                   kv_len[b]);

@@ -1,4 +1,5 @@
-"""Which tokens of q and out a tree plan's rows may have (CPU only)."""
+"""Which tokens of q and out, and which of a table's pages, a tree plan's rows may have (CPU
+only)."""
 import ctypes
 
 import numpy as np
@@ -46,3 +47,10 @@ def test_tokens_past_32_bits():
     first[0] = 2**31 - 1
     with pytest.raises(_lib.KunserveError, match="first token is 2147483647"):
         make()
+
+
+def test_pages_before_the_table():
+    """A row's page ids are read from where the plan says."""
+    table = PageTable(np.array([-2, 2]), np.arange(2), [20], CPU, upload=False)
+    with pytest.raises(_lib.KunserveError, match="pages start at -2"):
+        TreePlan(table, [[-1, 0]], 4, 2, 16, CPU, num_cus=256, head_dim=64, upload=False)

@@ -521,9 +521,9 @@ int64_t kunserve_tree_plan_bound(const int32_t* q_indptr_host,
                                  int32_t head_dim);
 
 /* Host-side plan of rows whose new tokens are the nodes of trees. Row b's are
- * q_indptr[b+1] - q_indptr[b] tokens (q_indptr starts at 0), tokens q_first[b]
- * onwards of q and out (NULL: q_indptr[b]; in one row each), the last of its kv_len[b];
- * parents[q_indptr[b] + i] is the place among them of token i's parent, below
+ * q_indptr[b+1] - q_indptr[b] tokens (q_indptr starts at 0), the last ones of its
+ * kv_len[b]: tokens q_first[b] onwards of q and out (NULL: q_indptr[b]), each in one
+ * row. parents[q_indptr[b] + i] is the place among them of token i's parent, below
  * i, or -1: it follows the cached tokens. indptr is the page table's. Rows are
  * cut into pieces of part_rounds rounds (256, 128 or 64 tokens at head_dim 64,
  * 128 and 256; 0: chosen from num_cus). */

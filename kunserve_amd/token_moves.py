@@ -118,7 +118,7 @@ def fork_rows(pool: KVPool, pages_of_reqs: Sequence[Sequence[int]], kv_lens: Seq
     last tokens; a request that moves: other pages throughout.
 
     Both lists hold ceil(kv_lens[b] / page_size) pages at least; further ones are not
-    touched. A page that is copied to is none of pages_of_reqs' and in one place of
+    touched. A page that is copied to holds no row's cached tokens and is in one place of
     pages_out (ValueError). weights (a KVWeights of the pool) are copied along. Its table
     is built on the host: not for a graph capture."""
     n = len(kv_lens)

@@ -1031,7 +1031,7 @@ class AttentionStep:
         drafted = _drafted_rows(trees, q_lens, is_prefill_requests, is_context_stage)
         # (A tree says what its row is: not for decode_rows to find out.)
         is_decode = decode_rows(first_token_indexes,
-                                q_lens if trees is None else np.where(drafted, 2, q_lens),
+                                q_lens if drafted is None else np.where(drafted, 2, q_lens),
                                 is_prefill_requests, use_tensor_cores, is_context_stage,
                                 pages_per_row, pool.page_size)
         self.kv_len = _kv_lens(first_token_indexes, q_lens, is_decode)
@@ -1053,7 +1053,7 @@ class AttentionStep:
                 raise ValueError("learn=False is for a step with weights")
             weights, cleared = None, weights
         if weights is not None:
-            if drafted.any():
+            if drafted is not None:
                 raise ValueError("weights do not learn from drafted trees: learn=False")
             if window < 1:
                 raise ValueError(f"window {window} must be positive")
@@ -1061,19 +1061,19 @@ class AttentionStep:
                 raise ValueError("attention weights need pages that are in one place of the "
                                  "step's lists")
             self.weights = weights
-        tree_rows = np.flatnonzero(drafted)
-        drafts = _Trees([trees[b] for b in tree_rows], tree_rows) if tree_rows.size else None
-        positions = None
-        if np.ndim(rope_positions) == 2:
-            positions = np.asarray(rope_positions)
+        if drafted is not None:
+            tree_rows = np.flatnonzero(drafted)
+            drafts = _Trees([trees[b] for b in tree_rows], tree_rows)
+        positions = None if rope_positions is None else np.asarray(rope_positions)
+        if positions is not None and positions.ndim == 2:
             if positions.shape[0] < 1 or positions.shape[1] != self.num_tokens:
                 raise ValueError(f"{self.num_tokens} tokens but {positions.shape} rope_positions")
             if positions.size and positions.dtype.kind not in "iu":
                 raise ValueError("rope_positions must be whole numbers")
             if positions.size and (positions.min() < 0 or positions.max() >= 2**31):
                 raise ValueError("rope_positions must lie in [0, 2^31)")
-        elif rope_positions is not None or drafted.any():
-            starts = np.asarray(self.kv_len - q_lens if rope_positions is None else rope_positions)
+        elif positions is not None or drafted is not None:
+            starts = self.kv_len - q_lens if positions is None else positions
             if starts.shape != (n_rows,):
                 raise ValueError(f"{n_rows} rows but {starts.shape} rope_positions")
             if n_rows and starts.dtype.kind not in "iu":
@@ -1081,7 +1081,7 @@ class AttentionStep:
             starts = starts.astype(np.int64)
             positions = np.repeat(starts - self.q_indptr_host[:-1], q_lens) + np.arange(
                 self.num_tokens)
-            if drafted.any():
+            if drafted is not None:
                 positions[np.repeat(drafted, q_lens)] = (
                     np.repeat(starts[drafted], q_lens[drafted]) + drafts.depths())
             if np.any(starts < 0) or (positions.size and positions.max() >= 2**31):
@@ -1091,7 +1091,8 @@ class AttentionStep:
         uploads = [[self.q_indptr_host], self.table]
         self.decode = self.prefill = None
         all_rows = np.arange(n_rows)
-        dec_rows, pre_rows = all_rows[is_decode], all_rows[~is_decode & ~drafted]
+        dec_rows = all_rows[is_decode]
+        pre_rows = all_rows[~is_decode if drafted is None else ~is_decode & ~drafted]
         # Row subsets take their rows from the step's CSR arrays (ids already
         # checked and mapped), not from the lists again.
         def sub_table(rows):
@@ -1131,7 +1132,7 @@ class AttentionStep:
             self.prefill = _Subset(pre_rows, tokens, table, None, plan)
             uploads += ([] if whole else [table, [tokens], [qi]]) + [plan]
 
-        if tree_rows.size:
+        if drafted is not None:
             table = self.table if tree_rows.size == n_rows else sub_table(tree_rows)
             plan = TreePlan(table, drafts, num_qo_heads, pool.num_kv_heads,
                             pool.page_size, dev, upload=False, head_dim=pool.head_dim,
@@ -1188,7 +1189,7 @@ class AttentionStep:
                 self.prefill.q_indptr = next(rest)[0]
             else:
                 self.prefill.q_indptr = self.q_indptr
-        if tree_rows.size:
+        if drafted is not None:
             self._first = next(rest)[0]
         if positions is not None:
             self.positions = next(rest)[0].view(positions.shape)
@@ -1380,10 +1381,11 @@ class AttentionStep:
         move_tokens(self.pool, self.table, self._first, first, kept, weights)
 
 
-def _drafted_rows(trees, q_lens: np.ndarray, is_prefill_requests, is_context_stage) -> np.ndarray:
-    """Which rows have a tree, checked against their lengths and stages."""
+def _drafted_rows(trees, q_lens: np.ndarray, is_prefill_requests,
+                  is_context_stage) -> Optional[np.ndarray]:
+    """Which rows have a tree, checked against their lengths and stages; None: no row."""
     if trees is None:
-        return np.zeros(len(q_lens), dtype=bool)
+        return None
     if len(trees) != len(q_lens):
         raise ValueError(f"{len(q_lens)} rows but {len(trees)} trees")
     drafted = np.array([t is not None for t in trees], dtype=bool)
@@ -1394,4 +1396,4 @@ def _drafted_rows(trees, q_lens: np.ndarray, is_prefill_requests, is_context_sta
             if stage is not None and not stage[b]:
                 raise ValueError(f"row {b}: a row with a tree is a prefill row, whose first index "
                                  "counts its cached tokens")
-    return drafted
+    return drafted if drafted.any() else None

@@ -1314,8 +1314,11 @@ class AttentionStep:
                 "kunserve_tensors_overlap", ctypes.byref(_tensor3(out)), out.shape[1],
                 ctypes.byref(_tensor3(q)), q.shape[1], self.num_tokens, self.pool.head_dim):
             raise ValueError("out overlaps q, which the attention weights are formed from")
-        if self.tree is not None and (out.data_ptr() % 8 or os[0] % 4 or os[1] % 4):
-            raise ValueError("out must be 8-byte aligned with strides that are multiples of 4")
+        if self.tree is not None:   # (which comes last)
+            if out.shape != q_shape:
+                raise ValueError(f"out shape {tuple(out.shape)} differs from q's {tuple(q_shape)}")
+            if out.data_ptr() % 8 or os[0] % 4 or os[1] % 4:
+                raise ValueError("out must be 8-byte aligned with strides that are multiples of 4")
         if rotary is not None:
             rotary_append_kv(self.pool, local, self.table, self.q_indptr, q, k, v, rotary,
                              positions=self.positions)

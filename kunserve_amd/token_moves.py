@@ -42,8 +42,7 @@ def keep_tokens(pool: KVPool, table: PageTable, first: Union[int, Sequence[int]]
     starts = np.empty(n, dtype=np.int32)
     starts[:] = given
     if pool.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("not under a capture, which takes AttentionStep.keep_tokens: a step's rows "
-                           "and places")
+        raise RuntimeError("keep_tokens is not for a graph capture: AttentionStep.keep_tokens is")
     moving = np.zeros(n + 1, dtype=np.int32)
     np.cumsum(lens - starts, out=moving[1:])
     ids = table.indices_host if table.indices_host.size else moving   # (there is one)

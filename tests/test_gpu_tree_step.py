@@ -96,6 +96,11 @@ def test_refused_before_anything_changes(device, pinned):
     with pytest.raises((ValueError, _lib.KunserveError), match="8-byte aligned"):
         m.step().run(0, m.q, m.k, m.v, out=big[..., 2:130], rope=Rotary(128, device=device))
     torch.cuda.synchronize()
+    for shape in ((total,), (total, m.hq), (total - 1, m.hq, 128)):
+        with pytest.raises(ValueError, match="out shape"):
+            m.step().run(0, m.q, m.k, m.v, out=torch.empty(shape, dtype=BF16, device=device),
+                         rope=Rotary(128, device=device))
+    torch.cuda.synchronize()
     for t, old in zip((m.pool.k, m.pool.v, m.q), before):
         assert torch.equal(t, old)
     assert not big.any()

@@ -986,8 +986,9 @@ class AttentionStep:
 
     rope_positions: for each row the rotary position of its first new token, where
     that is not its place in the cache (rows shortened by evict), or an array [axes,
-    num_tokens] with every new token's position on each axis of the Rotary ([1,
-    num_tokens] for one of a single axis). Only a Rotary takes them.
+    num_tokens] with every new token's position on each axis of the Rotary (for one
+    of a single axis an array [1, num_tokens], not one list in a list). Only a Rotary
+    takes them.
 
     trees: for each row None, or the tree that its new tokens are (drafted tokens that
     the step verifies): a list with the place of each token's parent among them, below
@@ -1065,7 +1066,9 @@ class AttentionStep:
             tree_rows = np.flatnonzero(drafted)
             drafts = _Trees([trees[b] for b in tree_rows], tree_rows)
         positions = None if rope_positions is None else np.asarray(rope_positions)
-        if positions is not None and positions.ndim == 2:
+        # (One list in a list is more likely the rows' starts than an array of one axis.)
+        nested = isinstance(rope_positions, (list, tuple)) and len(rope_positions) == 1
+        if positions is not None and positions.ndim == 2 and not nested:
             if positions.shape[0] < 1 or positions.shape[1] != self.num_tokens:
                 raise ValueError(f"{self.num_tokens} tokens but {positions.shape} rope_positions")
             if positions.size and positions.dtype.kind not in "iu":

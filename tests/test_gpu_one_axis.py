@@ -104,6 +104,9 @@ def test_refusals(device):
                      (pos - 1000, "lie in"), (pos + 2**31, "lie in")):
         with pytest.raises(ValueError, match=why):
             new(bad)
+    for nested in (pos.tolist(), (pos[0],), [[7, 100, 3]]):   # one list in a list: no array of an axis
+        with pytest.raises(ValueError, match="3 rows but"):
+            new(nested)
     step = new(pos)
     with pytest.raises(ValueError, match="positions on 1 axes"):
         step.run(0, q.clone(), k, v, rope=Rotary(128, device=device, sections=[16, 24, 24]))
